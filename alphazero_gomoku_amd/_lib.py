@@ -22,7 +22,8 @@ SYMBOLS = ["azg_create", "azg_destroy", "azg_last_error", "azg_set_weights", "az
            "azg_stream", "azg_selfplay_begin", "azg_selfplay_step", "azg_selfplay_fetch",
            "azg_selfplay_end", "azg_equi_data", "azg_pure_search", "azg_host_timing", "azg_arena_stats", "azg_reroot_stats", "azg_selfplay_fetch_packed", "azg_unpack_states", "azg_playout_begin", "azg_playout_end",
            "azg_board_step_batch_static", "azg_gate_stats", "azg_gate_poke",
-           "azg_train_param_count", "azg_train_forward", "azg_train_backward", "azg_train_adam", "azg_train_step", "azg_train_epoch"]
+           "azg_train_param_count", "azg_train_forward", "azg_train_backward", "azg_train_adam", "azg_train_step", "azg_train_epoch",
+           "azg_dropout", "azg_linear_ce", "azg_linear_ce_workspace"]
 
 
 class AzgError(RuntimeError):
@@ -36,6 +37,27 @@ class Config(C.Structure):
                 ("n_games", C.c_int32), ("c_puct", C.c_double), ("device", C.c_int32),
                 ("prior_mode", C.c_int32), ("arena_nodes", C.c_int32), ("cnn_mode", C.c_int32),
                 ("big_arenas", C.c_int32)]
+
+
+F32, BF16, F16 = 0, 1, 2
+REDUCE_NONE, REDUCE_SUM, REDUCE_MEAN = 0, 1, 2
+
+
+class DropoutArgs(C.Structure):
+    _fields_ = [("device", C.c_int32), ("dtype", C.c_int32), ("rows", C.c_int64), ("cols", C.c_int64),
+                ("x", C.c_void_p), ("x_stride", C.c_int64), ("residual", C.c_void_p), ("residual_stride", C.c_int64),
+                ("out", C.c_void_p), ("out_stride", C.c_int64), ("p", C.c_double), ("seed", C.c_uint64), ("offset", C.c_uint64),
+                ("offset_dev", C.c_void_p), ("first_row", C.c_uint64), ("row_step", C.c_uint64), ("stream", C.c_void_p)]
+
+
+class LinearCeArgs(C.Structure):
+    _fields_ = [("device", C.c_int32), ("dtype", C.c_int32), ("reduction", C.c_int32), ("reserved", C.c_int32),
+                ("n", C.c_int64), ("hidden", C.c_int64), ("classes", C.c_int64), ("x", C.c_void_p), ("x_stride", C.c_int64),
+                ("w", C.c_void_p), ("w_stride", C.c_int64), ("bias", C.c_void_p), ("target", C.c_void_p), ("ignore_index", C.c_int64),
+                ("probs", C.c_void_p), ("probs_stride", C.c_int64), ("loss", C.c_void_p), ("entropy", C.c_void_p), ("stats", C.c_void_p),
+                ("dloss", C.c_void_p), ("grad_scale", C.c_double), ("dx", C.c_void_p), ("dx_stride", C.c_int64),
+                ("dw", C.c_void_p), ("dw_stride", C.c_int64), ("db", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("stream", C.c_void_p)]
 
 
 _lib = None
@@ -126,9 +148,13 @@ def load():
     L.azg_set_search_parts.argtypes = [vp, C.c_int]
     L.azg_stream.argtypes = [vp]
     L.azg_stream.restype = vp
+    L.azg_dropout.argtypes = [C.POINTER(DropoutArgs)]
+    L.azg_linear_ce.argtypes = [C.POINTER(LinearCeArgs)]
+    L.azg_linear_ce_workspace.argtypes = [C.POINTER(LinearCeArgs)]
     for name in SYMBOLS:
-        if name not in ("azg_destroy", "azg_last_error", "azg_stream"):
+        if name not in ("azg_destroy", "azg_last_error", "azg_stream", "azg_linear_ce_workspace"):
             getattr(L, name).restype = C.c_int
+    L.azg_linear_ce_workspace.restype = C.c_int64
     _lib = L
     return L
 

@@ -1,0 +1,712 @@
+// Softmax cross entropy of a projection, l = X W^T + b, with its gradient, in pieces of the classes: the logits
+// live in the accumulators of a matrix-core tile and leave it as softmax statistics (forward) or as the gradient
+// at the logits, 16 bits an element and one piece of the classes at a time (backward).
+//
+//   lse_i  = log sum_v exp l_iv, from the tiles' running (maximum, sum) pairs
+//   loss_i = lse_i - l_{i,t}   or   lse_i sum_v pi_iv - sum_v pi_iv l_iv
+//   D_iv   = g_i (p_iv sum_v pi_iv - pi_iv);   dX = D W;   dW = D^T X;   db = sum_i D_i
+//
+// All three products are one kernel core: C[m][n] = sum_k A[m][k] B[n][k] with both operands contiguous along k.
+// Operands that are not laid out so (transposes, float32, odd sizes) are copied once into such an "image".
+//
+// float32 runs on the 16-bit matrix cores too: x 2^s = hi + lo with hi, lo in half precision (s a power of two
+// from the tensor's largest magnitude, so that nothing overflows and what underflows is 2^-38 of the largest
+// element), and a product takes three instructions, hi hi + hi lo + lo hi.  hi carries 11 bits and lo 11 more, so
+// an operand is off by at most 2^-22 of itself and the dropped lo lo is at most 2^-22 of the product; sums are
+// float32.  An image row holds blocks of 64: 32 hi, then the 32 lo of the same k.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include <type_traits>
+
+namespace azgops {
+
+typedef float fx4 __attribute__((ext_vector_type(4)));
+typedef _Float16 hx8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bx8 __attribute__((ext_vector_type(8)));
+
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
+constexpr float kDScale = 16384.0f;      // images of D hold D 2^14: |D| <= 2 then ends below half precision's 65504 and
+                                         // probabilities down to 2^-28 keep all their bits
+
+// Operand element types: what an image holds and how many products a pair of image elements takes.
+struct OpF32 { using In = float; using Img = _Float16; static constexpr bool split = true; };
+struct OpF16 { using In = _Float16; using Img = _Float16; static constexpr bool split = false; };
+struct OpBF16 { using In = __bf16; using Img = __bf16; static constexpr bool split = false; };
+
+__device__ __align__(256) unsigned char g_zero_page[256];
+
+template <typename Img> struct Frag;
+template <> struct Frag<_Float16> {
+    using V = hx8;
+    static __device__ inline fx4 mfma(V a, V b, fx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Frag<__bf16> {
+    using V = bx8;
+    static __device__ inline fx4 mfma(V a, V b, fx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+
+// ---------------------------------------------------------------- the tile product
+// TM x TN output tile, 64 image elements of k per stage, WM x WN waves, 16x16x32 matrix instructions.
+// LDS rows are 128 bytes = eight 16-byte chunks; chunk c of row r sits at c ^ (r & 7), so the sixteen rows that a
+// fragment read touches spread over all banks.  Stages are double-buffered and filled by loads that go from global
+// memory straight to LDS.
+struct Operand {
+    const void *p;       // image, or the caller's 16-bit tensor
+    long long ld;        // elements
+    long long rows;
+};
+
+template <int TM, int TN, int WM, int WN>
+struct TileShape {
+    static constexpr int waves = WM * WN, threads = waves * 64;
+    static constexpr int MT = TM / WM / 16, NT = TN / WN / 16;
+    static constexpr int stage_bytes = (TM + TN) * 128, lds_bytes = 2 * stage_bytes;
+};
+
+typedef __attribute__((address_space(3))) void *lds_ptr;
+typedef const __attribute__((address_space(1))) void *glb_ptr;
+
+__device__ inline void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+template <typename Op, int TM, int TN, int WM, int WN>
+struct TileProduct {
+    using S = TileShape<TM, TN, WM, WN>;
+    using F = Frag<typename Op::Img>;
+    static constexpr int kA = TM / 8, kAll = (TM + TN) / 8;                     // groups of eight rows a stage
+
+    // acc[mt][nt][i]: row wm*(TM/WM) + 16 mt + 4 (lane >> 4) + i of A, row wn*(TN/WN) + 16 nt + (lane & 15) of B.
+    // Stages k0 .. k1 - 1; kvalid (a multiple of 8) image elements of k exist.
+    static __device__ inline void run(fx4 (&acc)[S::MT][S::NT], const Operand &A, long long m0, const Operand &B, long long n0,
+                                      long long kvalid, int k0, int k1, char *lds)
+    {
+        const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const int wm = wave / WN, wn = wave % WN;
+        constexpr int kLoads = (kAll + S::waves - 1) / S::waves;
+        const char *src[kLoads];
+        const int chunk = (lane & 7) ^ (lane >> 3);
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) {
+            const int g = i * S::waves + wave;                                  // wave-uniform
+            const bool is_a = g < kA;
+            const Operand &O = is_a ? A : B;
+            long long r = (is_a ? m0 + g * 8 : n0 + (g - kA) * 8) + (lane >> 3);
+            r = r < O.rows ? r : O.rows - 1;                                    // rows past the end: any finite place, never stored
+            src[i] = static_cast<const char *>(O.p) + (r * O.ld + (long long)k0 * 64 + chunk * 8) * 2;
+        }
+        auto load = [&](int kt, int buf) {
+            const bool past = (long long)kt * 64 + chunk * 8 >= kvalid;          // only in the last stage of an odd k
+#pragma unroll
+            for (int i = 0; i < kLoads; i++) {
+                const int g = i * S::waves + wave;
+                if (kAll % S::waves == 0 || g < kAll) {
+                    const char *p = past ? reinterpret_cast<const char *>(g_zero_page) : src[i];
+                    __builtin_amdgcn_global_load_lds((glb_ptr)p, (lds_ptr)(lds + buf * S::stage_bytes + g * 1024), 16, 0, 0);
+                    src[i] += 128;
+                }
+            }
+        };
+        const int fr = (lane & 15) * 128, fc = ((lane >> 4) ^ (lane & 7)) * 16;
+        const char *fa = lds + wm * (TM / WM) * 128 + fr, *fb = lds + TM * 128 + wn * (TN / WN) * 128 + fr;
+        if (k0 >= k1) return;
+        // (the barrier alone does not wait for loads that write LDS)
+        load(k0, 0);
+        wait_loads();
+        __syncthreads();
+        for (int kt = k0; kt < k1; kt++) {
+            const int buf = (kt - k0) & 1;
+            if (kt + 1 < k1) load(kt + 1, buf ^ 1);
+            const char *pa = fa + buf * S::stage_bytes, *pb = fb + buf * S::stage_bytes;
+            typename F::V a[2][S::MT], b[2][S::NT];
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++) {
+#pragma unroll
+                for (int t = 0; t < S::NT; t++) b[ks][t] = *reinterpret_cast<const typename F::V *>(pb + t * 2048 + (fc ^ (ks * 64)));
+#pragma unroll
+                for (int t = 0; t < S::MT; t++) a[ks][t] = *reinterpret_cast<const typename F::V *>(pa + t * 2048 + (fc ^ (ks * 64)));
+                if (!Op::split)
+#pragma unroll
+                    for (int mt = 0; mt < S::MT; mt++)
+#pragma unroll
+                        for (int nt = 0; nt < S::NT; nt++) acc[mt][nt] = F::mfma(a[ks][mt], b[ks][nt], acc[mt][nt]);
+            }
+            if (Op::split) {
+#pragma unroll
+                for (int mt = 0; mt < S::MT; mt++)
+#pragma unroll
+                    for (int nt = 0; nt < S::NT; nt++) {
+                        acc[mt][nt] = F::mfma(a[1][mt], b[0][nt], acc[mt][nt]);
+                        acc[mt][nt] = F::mfma(a[0][mt], b[1][nt], acc[mt][nt]);
+                        acc[mt][nt] = F::mfma(a[0][mt], b[0][nt], acc[mt][nt]);
+                    }
+            }
+            wait_loads();
+            __syncthreads();
+        }
+    }
+};
+
+// Workgroup number -> tile.  Consecutive workgroups go to the eight XCDs in turn, each with an L2 of its own: an XCD
+// gets a contiguous run of tiles, walked in strips of kStrip tiles of m so that the tiles in flight on it share rows
+// of both operands.
+constexpr int kStrip = 8;
+__device__ inline void tile_of(unsigned wg, int mt, int nt, int *m, int *n)
+{
+    const unsigned total = (unsigned)mt * (unsigned)nt, per = total / 8, rest = total % 8, x = wg % 8, j = wg / 8;
+    const unsigned t = x * per + (x < rest ? x : rest) + j;
+    const unsigned strip = t / (unsigned)(kStrip * nt), first = strip * kStrip;
+    const unsigned h = min((unsigned)kStrip, (unsigned)mt - first), in = t - strip * kStrip * nt;
+    *m = (int)(first + in % h);
+    *n = (int)(in / h);
+}
+
+// ---------------------------------------------------------------- images
+struct PackArgs {
+    const void *src;              // [rows][cols], stride ld
+    long long ld, rows, cols;
+    void *img;                    // [rows][ldi] or null
+    long long ldi;                // padded columns (image elements)
+    void *imgt;                   // [cols][ldt] or null: the transpose
+    long long ldt;                // padded rows (image elements)
+    const long long *target;      // not null: rows whose target is ignore_index are read as zero
+    long long ignore;
+    const float *maxpart;         // float32: kMaxParts partial maxima of the tensor
+    long long r_first;            // first row of this launch
+};
+constexpr int kMaxParts = 256;
+
+// power of two that brings the largest magnitude into [2^13, 2^14); 1 for an all-zero tensor
+__device__ inline float split_scale(float mx)
+{
+    if (!(mx > 0.f)) return 1.f;
+    int e = 14 - (int)((__builtin_bit_cast(uint32_t, mx) >> 23) & 255) + 126;    // mx = f 2^(E-126), f in [1/2, 1)
+    e = e > 126 ? 126 : (e < -126 ? -126 : e);
+    return __builtin_bit_cast(float, (uint32_t)((e + 127) << 23));
+}
+__device__ inline float max_of_parts(const float *parts)                        // every thread of a wave calls it
+{
+    const int lane = threadIdx.x & 63;
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMaxParts / 64; i++) m = fmaxf(m, parts[i * 64 + lane]);
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
+    return m;
+}
+
+// partial maxima of the finite magnitudes of a float32 tensor (rows whose target is ignore_index left out)
+__global__ __launch_bounds__(256) void absmax_kernel(PackArgs a, float *parts)
+{
+    __shared__ float red[4];
+    const float *src = static_cast<const float *>(a.src);
+    float m = 0.f;
+    const long long per_row = (a.cols + 1023) / 1024, total = a.rows * per_row;
+    for (long long u = blockIdx.x; u < total; u += gridDim.x) {
+        const long long row = u / per_row, c0 = (u - row * per_row) * 1024 + threadIdx.x * 4;
+        if (a.target && a.target[row] == a.ignore) continue;
+        const float *p = src + row * a.ld;
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+            if (c0 + q < a.cols) { const float v = fabsf(p[c0 + q]); m = v < INFINITY ? fmaxf(m, v) : m; }
+    }
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) parts[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
+template <typename Op>
+__device__ inline void store_image(typename Op::Img *row, long long k, float v)
+{
+    if constexpr (Op::split) {
+        const _Float16 hi = (_Float16)v;
+        const float r = v - (float)hi;
+        const long long at = (k >> 5) * 64 + (k & 31);
+        row[at] = hi;
+        row[at + 32] = fabsf((float)hi) < INFINITY ? (_Float16)r : (_Float16)0.f;
+    } else {
+        row[k] = (typename Op::Img)v;
+    }
+}
+
+// 64 x 64 elements per workgroup: the image of the rows and / or of their transpose, zeros in the padding
+template <typename Op>
+__global__ __launch_bounds__(256) void pack_kernel(PackArgs a)
+{
+    __shared__ float tile[64][65];
+    const long long c0 = (long long)blockIdx.x * 64, r0 = a.r_first + (long long)blockIdx.y * 64;
+    const typename Op::In *src = static_cast<const typename Op::In *>(a.src);
+    const float scale = Op::split ? split_scale(max_of_parts(a.maxpart)) : 1.f;
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        const int r = i * 4 + (tid >> 6), c = tid & 63;
+        float v = 0.f;
+        if (r0 + r < a.rows && c0 + c < a.cols && !(a.target && a.target[r0 + r] == a.ignore)) v = (float)src[(r0 + r) * a.ld + c0 + c] * scale;
+        tile[r][c] = v;
+    }
+    __syncthreads();
+    const int per = Op::split ? 2 : 1;
+    if (a.img) {
+        typename Op::Img *img = static_cast<typename Op::Img *>(a.img);
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int r = i * 4 + (tid >> 6), c = tid & 63;
+            if (r0 + r < a.rows && (c0 + c) * per < a.ldi) store_image<Op>(img + (r0 + r) * a.ldi, c0 + c, tile[r][c]);
+        }
+    }
+    if (a.imgt) {
+        typename Op::Img *img = static_cast<typename Op::Img *>(a.imgt);
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int c = i * 4 + (tid >> 6), r = tid & 63;
+            if (c0 + c < a.cols && (r0 + r) * per < a.ldt) store_image<Op>(img + (c0 + c) * a.ldt, r0 + r, tile[r][c]);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- logits: statistics or gradient
+struct CeArgs {
+    Operand w, x;                 // classes (of this piece) x k, rows x k
+    long long kvalid;
+    int ktiles, mtiles, ntiles;
+    long long n, classes, v0;     // classes of this piece; v0 = first class of the piece
+    const void *bias;             // this piece's, operand type, or null
+    const float *xmax, *wmax;     // float32: partial maxima
+    const long long *target;
+    long long ignore;
+    const float *probs;           // [n][ldp], already offset to the piece's first class
+    long long ldp;
+    // statistics
+    float2 *part;                 // [tiles of classes][n]: maximum, sum of exp(l - maximum)
+    float *part_e;                // [tiles of classes][n]: sum of exp(l - maximum) l, or null
+    float4 *part_t;               // probabilities: sum pi l, sum pi, sum |pi|, -
+    float *tlogit;                // index: [n]
+    // gradient
+    const float4 *stats;          // [n]: m, sum pi / s, ... (RowArgs)
+    const float *rowg;            // [n]
+    void *d, *dt;                 // images of D [n][ldd] and of its transpose [classes][ldt]
+    long long ldd, ldt;
+    float *dbpart;                // [ntiles][classes] or null
+};
+
+template <typename T> __device__ inline float as_float(T v) { return (float)v; }
+
+template <typename Op, int TM, int TN, int WM, int WN, bool GRAD>
+__global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
+{
+    using S = TileShape<TM, TN, WM, WN>;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    int tm, tn;
+    tile_of(blockIdx.x, a.mtiles, a.ntiles, &tm, &tn);
+    const long long m0 = (long long)tm * TM, n0 = (long long)tn * TN;
+    fx4 acc[S::MT][S::NT];
+#pragma unroll
+    for (int i = 0; i < S::MT; i++)
+#pragma unroll
+        for (int j = 0; j < S::NT; j++) acc[i][j] = fx4{0.f, 0.f, 0.f, 0.f};
+    TileProduct<Op, TM, TN, WM, WN>::run(acc, a.w, m0, a.x, n0, a.kvalid, 0, a.ktiles, lds);
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
+    const float ux = Op::split ? 1.f / split_scale(max_of_parts(a.xmax)) : 1.f, uw = Op::split ? 1.f / split_scale(max_of_parts(a.wmax)) : 1.f;
+    const typename Op::In *bias = static_cast<const typename Op::In *>(a.bias);
+    const long long vw = m0 + wm * (TM / WM) + 4 * (lane >> 4);                  // this lane's first class of the piece
+#pragma unroll
+    for (int mt = 0; mt < S::MT; mt++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const long long v = vw + mt * 16 + i;
+            const float b = bias && v < a.classes ? (float)bias[v] : 0.f;
+#pragma unroll
+            for (int nt = 0; nt < S::NT; nt++) acc[mt][nt][i] = v < a.classes ? acc[mt][nt][i] * ux * uw + b : -INFINITY;
+        }
+    const long long nw = n0 + wn * (TN / WN) + (lane & 15);
+    if constexpr (!GRAD) {
+        // per row: maximum and sum over this tile's classes; lanes 16 and 32 apart, then the WM waves, share a row
+        constexpr int kCol = TN;
+        float *sm = reinterpret_cast<float *>(lds);                             // [WM][6][TN]; the stages are done with
+#pragma unroll
+        for (int nt = 0; nt < S::NT; nt++) {
+            const long long row = nw + nt * 16;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int mt = 0; mt < S::MT; mt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) mx = fmaxf(mx, acc[mt][nt][i]);
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            // (a NaN is passed over by fmaxf: it comes back through the sum; a maximum of -inf leaves every term exp(-inf))
+            const float base = mx == -INFINITY ? 0.f : mx;
+            float s = 0.f, e = 0.f, tl = 0.f, ts = 0.f, ta = 0.f;
+#pragma unroll
+            for (int mt = 0; mt < S::MT; mt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float l = acc[mt][nt][i], x = __builtin_amdgcn_exp2f((l - base) * kLog2e);
+                    s += x;
+                    if (a.part_e) e += x != 0.f ? x * l : 0.f;
+                }
+            if (a.probs && row < a.n) {
+                const float *pr = a.probs + row * a.ldp;
+#pragma unroll
+                for (int mt = 0; mt < S::MT; mt++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const long long v = vw + mt * 16 + i;
+                        if (v < a.classes) {
+                            const float p = pr[v];
+                            ts += p; ta += fabsf(p);
+                            tl += p != 0.f ? p * acc[mt][nt][i] : 0.f;
+                        }
+                    }
+            }
+            if (a.target && row < a.n) {
+                const long long t = a.target[row] - a.v0 - vw;
+                if (t >= 0 && t < TM)
+#pragma unroll
+                    for (int mt = 0; mt < S::MT; mt++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (t == mt * 16 + i && vw + t < a.classes) a.tlogit[row] = acc[mt][nt][i];
+            }
+            const int col = wn * (TN / WN) + nt * 16 + (lane & 15);
+#define AZG_PAIR(v) v += __shfl_xor(v, 16, 64); v += __shfl_xor(v, 32, 64)
+            AZG_PAIR(s);
+            if (a.part_e) { AZG_PAIR(e); }
+            if (a.probs) { AZG_PAIR(tl); AZG_PAIR(ts); AZG_PAIR(ta); }
+#undef AZG_PAIR
+            if (lane < 16) {
+                float *q = sm + (wm * 6) * kCol + col;
+                q[0] = mx; q[kCol] = s; q[2 * kCol] = e; q[3 * kCol] = tl; q[4 * kCol] = ts; q[5 * kCol] = ta;
+            }
+        }
+        __syncthreads();
+        for (int col = tid; col < TN; col += S::threads) {
+            const long long row = n0 + col;
+            if (row >= a.n) continue;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < WM; w++) mx = fmaxf(mx, sm[w * 6 * kCol + col]);
+            float s = 0.f, e = 0.f, tl = 0.f, ts = 0.f, ta = 0.f;
+#pragma unroll
+            for (int w = 0; w < WM; w++) {
+                const float *q = sm + w * 6 * kCol + col;
+                const float f = q[0] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((q[0] - mx) * kLog2e);
+                s += q[kCol] * f; e += q[2 * kCol] * f; tl += q[3 * kCol]; ts += q[4 * kCol]; ta += q[5 * kCol];
+            }
+            const long long at = (long long)tm * a.n + row;
+            a.part[at] = make_float2(mx, s);
+            if (a.part_e) a.part_e[at] = e;
+            if (a.probs) a.part_t[at] = make_float4(tl, ts, ta, 0.f);
+        }
+    } else {
+        typename Op::Img *d = static_cast<typename Op::Img *>(a.d), *dt = static_cast<typename Op::Img *>(a.dt);
+        const long long dpad = Op::split ? a.ldd / 2 : a.ldd, tpad = Op::split ? a.ldt / 2 : a.ldt;
+        float db[S::MT][4];
+#pragma unroll
+        for (int mt = 0; mt < S::MT; mt++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) db[mt][i] = 0.f;
+#pragma unroll
+        for (int nt = 0; nt < S::NT; nt++) {
+            const long long row = nw + nt * 16;
+            const bool live = row < a.n;
+            const float4 st = live ? a.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float g = live ? a.rowg[row] : 0.f;
+            const long long t = live && a.target ? a.target[row] - a.v0 - vw : -1;
+            const float *pr = a.probs ? a.probs + row * a.ldp : nullptr;
+#pragma unroll
+            for (int mt = 0; mt < S::MT; mt++) {
+                float v[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const long long cls = vw + mt * 16 + i;
+                    float q = __builtin_amdgcn_exp2f((acc[mt][nt][i] - st.x) * kLog2e) * st.y;
+                    if (pr) { if (live && cls < a.classes) q -= pr[cls]; }
+                    else if (t == mt * 16 + i) q -= 1.f;
+                    v[i] = g == 0.f || cls >= a.classes ? 0.f : q * g;          // a row that counts for nothing: zero whatever it holds
+                    db[mt][i] += v[i];
+                    v[i] *= kDScale;
+                }
+                // D: four classes of one row;  D^T: a 4 x 4 transpose among four neighbouring lanes, then four rows of one class
+                const long long cls = vw + mt * 16;
+                if (a.d && live && cls < dpad) {
+                    typename Op::Img h[4], l[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        h[i] = (typename Op::Img)v[i];
+                        if (Op::split) l[i] = (typename Op::Img)(v[i] - (float)h[i]);
+                    }
+                    typename Op::Img *o = d + row * a.ldd + (Op::split ? (cls >> 5) * 64 + (cls & 31) : cls);
+                    *reinterpret_cast<uint64_t *>(o) = *reinterpret_cast<uint64_t *>(h);
+                    if (Op::split) *reinterpret_cast<uint64_t *>(o + 32) = *reinterpret_cast<uint64_t *>(l);
+                }
+                if (a.dt) {
+                    const bool b0 = lane & 1, b1 = lane & 2;
+                    float w[4];
+                    {
+                        const float r01 = __shfl_xor(b0 ? v[0] : v[1], 1, 64), r23 = __shfl_xor(b0 ? v[2] : v[3], 1, 64);
+                        const float x0 = b0 ? r01 : v[0], x1 = b0 ? v[1] : r01, y0 = b0 ? r23 : v[2], y1 = b0 ? v[3] : r23;
+                        // even lanes: classes 0, 2 of rows (t, t+1); odd lanes: classes 1, 3
+                        const float p0 = __shfl_xor(b1 ? x0 : y0, 2, 64), p1 = __shfl_xor(b1 ? x1 : y1, 2, 64);
+                        w[0] = b1 ? p0 : x0; w[1] = b1 ? p1 : x1; w[2] = b1 ? y0 : p0; w[3] = b1 ? y1 : p1;
+                    }
+                    const long long c = cls + (lane & 3), r4 = row - (lane & 3);
+                    if (c < a.classes && r4 < tpad) {
+                        typename Op::Img h[4], l[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            h[i] = (typename Op::Img)w[i];
+                            if (Op::split) l[i] = (typename Op::Img)(w[i] - (float)h[i]);
+                        }
+                        typename Op::Img *o = dt + c * a.ldt + (Op::split ? (r4 >> 5) * 64 + (r4 & 31) : r4);
+                        *reinterpret_cast<uint64_t *>(o) = *reinterpret_cast<uint64_t *>(h);
+                        if (Op::split) *reinterpret_cast<uint64_t *>(o + 32) = *reinterpret_cast<uint64_t *>(l);
+                    }
+                }
+            }
+        }
+        if (a.dbpart) {
+            float *sm = reinterpret_cast<float *>(lds);                         // [WN][TM]
+#pragma unroll
+            for (int mt = 0; mt < S::MT; mt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float s = db[mt][i];
+                    s += __shfl_xor(s, 1, 64); s += __shfl_xor(s, 2, 64); s += __shfl_xor(s, 4, 64); s += __shfl_xor(s, 8, 64);
+                    if ((lane & 15) == 0) sm[wn * TM + wm * (TM / WM) + mt * 16 + 4 * (lane >> 4) + i] = s;
+                }
+            __syncthreads();
+            for (int v = tid; v < TM; v += S::threads)
+                if (m0 + v < a.classes) {
+                    float s = 0.f;
+#pragma unroll
+                    for (int w = 0; w < WN; w++) s += sm[w * TM + v];
+                    a.dbpart[(long long)tn * a.classes + m0 + v] = s;
+                }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- rows and totals
+struct RowArgs {
+    long long n, classes;
+    int tiles;
+    const float2 *part; const float *part_e; const float4 *part_t; const float *tlogit;
+    const long long *target; long long ignore;
+    float4 *stats;                // [n]: m, sum pi / s, sum |pi|, loss with lse = m + log s (so that p takes no rounding of lse)
+    float *ent;                   // [n] or null
+};
+// one wave per row: join the tiles' (maximum, sum) pairs in a fixed order
+__global__ __launch_bounds__(256) void rows_kernel(RowArgs a)
+{
+    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (row >= a.n) return;
+    float mx = -INFINITY, s = 0.f, e = 0.f, tl = 0.f, ts = 0.f, ta = 0.f;
+    for (int t = lane; t < a.tiles; t += 64) {
+        const float2 p = a.part[(long long)t * a.n + row];
+        const float m = fmaxf(mx, p.x), base = m == -INFINITY ? 0.f : m;
+        const float f0 = __builtin_amdgcn_exp2f((mx - base) * kLog2e), f1 = __builtin_amdgcn_exp2f((p.x - base) * kLog2e);
+        // (a pair without a class adds nothing; a NaN sum stays NaN)
+        s = (mx == -INFINITY ? s : s * f0) + (p.x == -INFINITY ? p.y : p.y * f1);
+        if (a.part_e) {
+            const float q = a.part_e[(long long)t * a.n + row];
+            e = (mx == -INFINITY ? e : e * f0) + (p.x == -INFINITY ? q : q * f1);
+        }
+        mx = m;
+        if (a.part_t) { const float4 q = a.part_t[(long long)t * a.n + row]; tl += q.x; ts += q.y; ta += q.z; }
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const float om = __shfl_xor(mx, d, 64), os = __shfl_xor(s, d, 64), oe = __shfl_xor(e, d, 64);
+        const float m = fmaxf(mx, om), base = m == -INFINITY ? 0.f : m;
+        const float f0 = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mx - base) * kLog2e);
+        const float f1 = om == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((om - base) * kLog2e);
+        s = s * f0 + os * f1; e = e * f0 + oe * f1; mx = m;
+        if (a.part_t) { tl += __shfl_xor(tl, d, 64); ts += __shfl_xor(ts, d, 64); ta += __shfl_xor(ta, d, 64); }
+    }
+    if (lane) return;
+    const float ls = logf(s), lse = (mx == -INFINITY ? 0.f : mx) + ls;
+    float loss, ent = lse - e / s;
+    if (a.target) {
+        const long long t = a.target[row];
+        ts = ta = 1.f;
+        if (t == a.ignore) { loss = 0.f; ent = 0.f; ts = ta = 0.f; }
+        else if (t < 0 || t >= a.classes) { loss = ent = NAN; ts = ta = NAN; }
+        else loss = (mx - a.tlogit[row]) + ls;
+    } else {
+        loss = lse * ts - tl;
+    }
+    a.stats[row] = make_float4(mx, ts / s, ta, loss);
+    if (a.ent) a.ent[row] = ent;
+}
+
+struct TotalArgs {
+    long long n;
+    int reduction;                // 0 none, 1 sum, 2 mean
+    const float4 *stats; const float *ent;
+    const long long *target; long long ignore;
+    float *loss, *ent_out;        // [n] or [1]; null: not asked for
+    const float *dloss;           // [n], [1] or null
+    float grad_scale;
+    float *rowg;                  // [n]: g_i / 2^e, or null without a backward pass
+    float *factor;                // [1]: 2^e (times the common g)
+};
+// totals of the rows in a fixed order, in double; the rows' gradient factors, scaled so that the largest |D| fits an image
+__global__ __launch_bounds__(1024) void totals_kernel(TotalArgs a)
+{
+    __shared__ double red[3][16];
+    __shared__ float redm[16];
+    const int tid = threadIdx.x;
+    double sl = 0.0, se = 0.0, cnt = 0.0;
+    float mx = 0.f;
+    for (long long i = tid; i < a.n; i += 1024) {
+        const float4 st = a.stats[i];
+        const bool used = !(a.target && a.target[i] == a.ignore);
+        sl += st.w; cnt += used ? 1.0 : 0.0;
+        if (a.ent) se += a.ent[i];
+        float g = 1.f;
+        if (a.reduction == 0) {
+            if (a.loss) a.loss[i] = st.w;
+            if (a.ent_out) a.ent_out[i] = a.ent[i];
+            if (a.rowg) g = (a.dloss ? a.dloss[i] : 1.f) * a.grad_scale;
+        }
+        const float m = fabsf(g) * st.z;
+        if (used && m < INFINITY) mx = fmaxf(mx, m);
+    }
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+        sl += __shfl_xor(sl, s, 64); se += __shfl_xor(se, s, 64); cnt += __shfl_xor(cnt, s, 64);
+        mx = fmaxf(mx, __shfl_xor(mx, s, 64));
+    }
+    if ((tid & 63) == 0) { red[0][tid >> 6] = sl; red[1][tid >> 6] = se; red[2][tid >> 6] = cnt; redm[tid >> 6] = mx; }
+    __syncthreads();
+    sl = se = cnt = 0.0; mx = 0.f;
+    for (int i = 0; i < 16; i++) { sl += red[0][i]; se += red[1][i]; cnt += red[2][i]; mx = fmaxf(mx, redm[i]); }
+    const double by = a.reduction == 2 ? (cnt > 0.0 ? 1.0 / cnt : 0.0) : 1.0;
+    if (a.reduction && tid == 0) {
+        if (a.loss) a.loss[0] = (float)(sl * by);
+        if (a.ent_out) a.ent_out[0] = (float)(se * by);
+    }
+    if (!a.rowg) return;
+    // 2^e >= the largest g_i sum|pi_i| (1 for an index target and a common g)
+    float up = 1.f;
+    if (mx > 0.f) {
+        int E = (int)((__builtin_bit_cast(uint32_t, mx) >> 23) & 255) - 126;     // mx <= 2^E
+        if ((__builtin_bit_cast(uint32_t, mx) & 0x7FFFFFu) == 0) E--;
+        E = E > 126 ? 126 : (E < -120 ? -120 : E);
+        up = __builtin_bit_cast(float, (uint32_t)((E + 127) << 23));
+    }
+    for (long long i = tid; i < a.n; i += 1024) {
+        const bool used = !(a.target && a.target[i] == a.ignore);
+        const float g = a.reduction == 0 ? (a.dloss ? a.dloss[i] : 1.f) * a.grad_scale : 1.f;
+        a.rowg[i] = used ? g / up : 0.f;
+    }
+    if (tid == 0) {
+        const float common = a.reduction ? (a.dloss ? a.dloss[0] : 1.f) * a.grad_scale * (float)by : 1.f;
+        a.factor[0] = up * common;
+    }
+}
+
+// ---------------------------------------------------------------- the gradients' products
+struct GradArgs {
+    Operand a, b;                 // a: the output's contiguous dimension, b: its rows
+    long long kvalid;
+    int ktiles, mtiles, ntiles, kper;   // stages per split
+    long long m, n;
+    void *out; long long ldo;     // [n][ldo], operand type (one split), or
+    float *acc;                   // float32 [splits][n][m]
+    bool add;                     // one split: add to acc instead of starting it
+    bool vec;                     // out can be stored four elements at a time
+    const float *amax;            // float32: partial maxima of the operand that is not D
+    const float *factor;
+};
+
+template <typename T, int N> struct __attribute__((packed)) Pack { T v[N]; };
+
+template <typename Op, int TM, int TN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64) void grad_kernel(GradArgs a)
+{
+    using S = TileShape<TM, TN, WM, WN>;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    int tm, tn;
+    tile_of(blockIdx.x, a.mtiles, a.ntiles, &tm, &tn);
+    const long long m0 = (long long)tm * TM, n0 = (long long)tn * TN;
+    const int k0 = blockIdx.y * a.kper, k1 = min(a.ktiles, k0 + a.kper);
+    fx4 acc[S::MT][S::NT];
+#pragma unroll
+    for (int i = 0; i < S::MT; i++)
+#pragma unroll
+        for (int j = 0; j < S::NT; j++) acc[i][j] = fx4{0.f, 0.f, 0.f, 0.f};
+    TileProduct<Op, TM, TN, WM, WN>::run(acc, a.a, m0, a.b, n0, a.kvalid, k0, k1, lds);
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
+    float f = *a.factor / kDScale;
+    if (Op::split) f /= split_scale(max_of_parts(a.amax));
+    const long long mw = m0 + wm * (TM / WM) + 4 * (lane >> 4), nw = n0 + wn * (TN / WN) + (lane & 15);
+#pragma unroll
+    for (int nt = 0; nt < S::NT; nt++) {
+        const long long n = nw + nt * 16;
+        if (n >= a.n) continue;
+#pragma unroll
+        for (int mt = 0; mt < S::MT; mt++) {
+            const long long m = mw + mt * 16;
+            if (m >= a.m) continue;
+            fx4 v = acc[mt][nt];
+            if (a.acc) {
+                float *o = a.acc + ((long long)blockIdx.y * a.n + n) * a.m + m;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (m + i < a.m) o[i] = a.add ? o[i] + v[i] : v[i];
+            } else {
+                typename Op::In *o = static_cast<typename Op::In *>(a.out) + n * a.ldo + m;
+                if (a.vec && m + 4 <= a.m) {
+                    Pack<typename Op::In, 4> q;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) q.v[i] = (typename Op::In)(v[i] * f);
+                    *reinterpret_cast<Pack<typename Op::In, 4> *>(o) = q;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (m + i < a.m) o[i] = (typename Op::In)(v[i] * f);
+                }
+            }
+        }
+    }
+}
+
+struct JoinArgs {
+    const float *acc;             // [splits][n][m]
+    int splits;
+    long long n, m;
+    void *out; long long ldo;
+    const float *amax, *factor;   // amax null: no image scale
+    float extra;                  // kDScale for products of D images, 1 for sums of unscaled D
+};
+// out[n][m] = factor * sum over splits, in their order; rows of the batch a thread each four columns apart
+template <typename Op>
+__global__ __launch_bounds__(256) void join_kernel(JoinArgs a)
+{
+    float f = *a.factor / a.extra;
+    if (Op::split && a.amax) f /= split_scale(max_of_parts(a.amax));
+    const long long total = a.n * a.m;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        float s = 0.f;
+        for (int z = 0; z < a.splits; z++) s += a.acc[(long long)z * total + i];
+        const long long r = i / a.m, c = i - r * a.m;
+        static_cast<typename Op::In *>(a.out)[r * a.ldo + c] = (typename Op::In)(s * f);
+    }
+}
+
+// zeros for gradients of an empty batch
+template <typename T>
+__global__ __launch_bounds__(256) void zero_rows_kernel(T *out, long long rows, long long cols, long long ld)
+{
+    const long long total = rows * cols;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256)
+        out[i / cols * ld + i % cols] = (T)0.f;
+}
+
+}  // namespace azgops

@@ -1,0 +1,465 @@
+// C entry points of the training-head operators (include/azgomoku.h): argument checks, plans, launches.
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+#include <hip/hip_runtime.h>
+
+#include "../../include/azgomoku.h"
+#include "azg_dropout.hpp"
+#include "azg_linear_ce.hpp"
+
+using namespace azgops;
+
+extern "C" void azg_set_error_text(const char *text);        // azgomoku.hip: what azg_last_error(NULL) returns
+
+namespace {
+
+int fail(int code, const char *fmt, ...)
+{
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    azg_set_error_text(buf);
+    return code;
+}
+
+#define OPS_HIP(call)                                                                                   \
+    do {                                                                                                \
+        hipError_t e_ = (call);                                                                         \
+        if (e_ != hipSuccess) return fail(AZG_EHIP, "%s failed: %s (%s:%d)", #call, hipGetErrorString(e_), __FILE__, __LINE__); \
+    } while (0)
+#define OPS_TRY(call) do { const int rc_ = (call); if (rc_) return rc_; } while (0)
+
+// makes a device current for the time of a call
+struct DeviceScope {
+    int before = -1;
+    bool changed = false;
+    int enter(int device)
+    {
+        OPS_HIP(hipGetDevice(&before));
+        if (before != device) { OPS_HIP(hipSetDevice(device)); changed = true; }
+        return AZG_OK;
+    }
+    ~DeviceScope() { if (changed) (void)hipSetDevice(before); }
+};
+
+long long up_to(long long v, long long m) { return (v + m - 1) / m * m; }
+
+bool bad_matrix(long long rows, long long cols, long long stride) { return rows > 1 && stride < cols; }
+
+}  // namespace
+
+// ---------------------------------------------------------------- dropout
+extern "C" int azg_dropout(const azg_dropout_args *a)
+{
+    if (!a) return fail(AZG_EINVAL, "null argument");
+    if (a->dtype != AZG_F32 && a->dtype != AZG_BF16 && a->dtype != AZG_F16) return fail(AZG_EINVAL, "azg_dropout: unknown dtype %d", a->dtype);
+    if (!(a->p >= 0.0 && a->p <= 1.0)) return fail(AZG_EINVAL, "azg_dropout: p must lie in [0, 1]");
+    if (a->rows < 0 || a->cols < 0) return fail(AZG_EINVAL, "azg_dropout: negative size");
+    if (a->rows == 0 || a->cols == 0) return AZG_OK;
+    if (a->rows > (1LL << 46) / a->cols) return fail(AZG_EINVAL, "azg_dropout: too many elements");
+    if (!a->x || !a->out) return fail(AZG_EINVAL, "null argument");
+    if (bad_matrix(a->rows, a->cols, a->x_stride) || bad_matrix(a->rows, a->cols, a->out_stride) || (a->residual && bad_matrix(a->rows, a->cols, a->residual_stride)))
+        return fail(AZG_EINVAL, "azg_dropout: a row stride is smaller than a row");
+    DeviceScope scope;
+    OPS_TRY(scope.enter(a->device));
+    DropoutArgs d{};
+    d.x = a->x; d.res = a->residual; d.out = a->out;
+    d.rows = a->rows; d.cols = a->cols; d.xs = a->x_stride; d.rs = a->residual_stride; d.os = a->out_stride;
+    d.seed = a->seed; d.offset = a->offset;
+    d.first = (unsigned long long)a->first_row * (unsigned long long)a->cols;
+    d.step = (unsigned long long)a->row_step * (unsigned long long)a->cols;
+    d.offset_dev = reinterpret_cast<const long long *>(a->offset_dev);
+    const long T = std::lround(a->p * 65536.0);
+    d.threshold = (unsigned)T;
+    d.scale = T < 65536 ? (float)(65536.0 / (double)(65536 - T)) : 0.f;
+    if (a->row_step == 1 && a->x_stride == a->cols && a->out_stride == a->cols && (!a->residual || a->residual_stride == a->cols)) {
+        d.cols = a->rows * a->cols;                           // one long row: element numbers run on from row to row
+        d.rows = 1;
+    }
+    const long long blocks_per_row = d.cols / 8 + 2;          // a row that starts inside a block touches one more
+    const long long grid = std::min<long long>((d.rows * blocks_per_row + 255) / 256, 1 << 20);
+    hipStream_t s = static_cast<hipStream_t>(a->stream);
+    if (a->dtype == AZG_F32) hipLaunchKernelGGL((dropout_kernel<float>), dim3(grid), dim3(256), 0, s, d, blocks_per_row);
+    else if (a->dtype == AZG_F16) hipLaunchKernelGGL((dropout_kernel<_Float16>), dim3(grid), dim3(256), 0, s, d, blocks_per_row);
+    else hipLaunchKernelGGL((dropout_kernel<__bf16>), dim3(grid), dim3(256), 0, s, d, blocks_per_row);
+    OPS_HIP(hipGetLastError());
+    return AZG_OK;
+}
+
+// ---------------------------------------------------------------- projection + softmax cross entropy
+namespace {
+
+// Room that the images of D, of W and of its transpose may take together before the classes are cut into pieces.
+constexpr long long kPieceBytes = 1LL << 30;
+
+struct Take {                                                 // offsets into the caller's workspace
+    size_t off = 0;
+    size_t operator()(size_t bytes) { const size_t at = off; off += (bytes + 255) / 256 * 256; return at; }
+};
+
+enum Shape { T256, T128, T64, TROW };
+struct ShapeDim { int tm, tn; };
+constexpr ShapeDim kDims[4] = {{256, 256}, {128, 128}, {64, 64}, {128, 16}};
+
+long long tiles_of(Shape s, long long m, long long n) { return ((m + kDims[s].tm - 1) / kDims[s].tm) * ((n + kDims[s].tn - 1) / kDims[s].tn); }
+
+Shape pick_logits(long long m, long long n, bool grad)
+{
+    if (!grad && n <= 16) return TROW;
+    if (tiles_of(T256, m, n) >= 200) return T256;
+    if (tiles_of(T128, m, n) >= 200) return T128;
+    return T64;
+}
+// tile and number of splits of k of a gradient's product
+struct GradPick { Shape shape; int splits, kper; };
+GradPick pick_grad(long long m, long long n, long long ktiles)
+{
+    GradPick g{T64, 1, (int)ktiles};
+    const long long most = std::max<long long>(1, ktiles / 8);
+    if (m > 128 && n > 128 && tiles_of(T256, m, n) * std::min<long long>(most, 32) >= 200) g.shape = T256;
+    else if (m > 64 && n > 64 && tiles_of(T128, m, n) * std::min<long long>(most, 32) >= 200) g.shape = T128;
+    const long long tiles = tiles_of(g.shape, m, n);
+    long long s = std::max<long long>(1, std::min<long long>({256 / std::max<long long>(tiles, 1), most, 32}));
+    g.kper = (int)((ktiles + s - 1) / s);
+    g.splits = (int)((ktiles + g.kper - 1) / g.kper);
+    return g;
+}
+
+struct Plan {
+    bool split, forward, backward, pack_w, pack_x;
+    int isz;                                                  // bytes of an image element
+    long long n, H, V, vp, pieces;
+    long long kimg, ldx, ldw;                                 // image elements along the features
+    long long ldd, ldt;                                       // images of D and of its transpose, elements
+    Shape lshape;
+    GradPick gx, gw;
+    size_t xmax, wmax, ximg, xt, wimg, wt, part, part_e, part_t, tlogit, stats, ent, rowg, factor, d, dt, dbpart, dxacc, dwacc, total;
+};
+
+bool aligned16(const void *p, long long stride, long long cols, long long rows)
+{
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && cols % 8 == 0 && (rows <= 1 || stride % 8 == 0);
+}
+
+int make_plan(const azg_linear_ce_args *a, Plan *p)
+{
+    p->split = a->dtype == AZG_F32;
+    p->isz = 2;
+    p->forward = a->loss != nullptr;
+    p->backward = a->dx || a->dw || a->db;
+    p->n = a->n; p->H = a->hidden; p->V = a->classes;
+    p->kimg = p->split ? up_to(p->H, 32) * 2 : up_to(p->H, 64);
+    p->pack_x = p->split || !aligned16(a->x, a->x_stride, a->hidden, a->n);
+    p->pack_w = p->split || !aligned16(a->w, a->w_stride, a->hidden, a->classes);
+    const long long np = p->split ? up_to(p->n, 32) * 2 : up_to(p->n, 64);
+    const long long per = (p->split ? 2 : 1);
+    // bytes a class of a piece costs
+    long long cost = p->pack_w ? p->kimg * 2 : 0;
+    if (p->backward) cost += p->n * per * 2 + np * 2 + (a->dx ? p->H * per * 2 : 0);
+    p->vp = p->V;
+    if (cost) p->vp = std::min<long long>(p->V, std::max<long long>(1024, kPieceBytes / cost / 256 * 256));
+    p->pieces = (p->V + p->vp - 1) / p->vp;
+    if (p->pieces > 1) {                                      // even pieces
+        p->vp = std::min<long long>(p->V, up_to((p->V + p->pieces - 1) / p->pieces, 256));
+        p->pieces = (p->V + p->vp - 1) / p->vp;
+    }
+    p->ldd = p->split ? up_to(p->vp, 32) * 2 : up_to(p->vp, 64);
+    p->ldt = np;
+    p->lshape = pick_logits(p->vp, p->n, p->backward);
+    if (p->lshape == TROW && p->backward) p->lshape = T64;
+    p->gx = pick_grad(p->H, p->n, (p->ldd + 63) / 64);
+    p->gw = pick_grad(p->H, p->vp, (p->ldt + 63) / 64);
+    const long long ltiles_m = (p->vp + kDims[p->lshape].tm - 1) / kDims[p->lshape].tm, ltiles_n = (p->n + kDims[p->lshape].tn - 1) / kDims[p->lshape].tn;
+    if (ltiles_m * ltiles_n > INT_MAX / 2 || tiles_of(p->gx.shape, p->H, p->n) > INT_MAX / 2 || tiles_of(p->gw.shape, p->H, p->vp) > INT_MAX / 2)
+        return fail(AZG_EINVAL, "azg_linear_ce: the problem is too large");
+    Take t;
+    p->xmax = t(p->split ? kMaxParts * 4 : 0);
+    p->wmax = t(p->split ? kMaxParts * 4 : 0);
+    p->ximg = t(p->pack_x ? (size_t)p->n * p->kimg * 2 : 0);
+    p->xt = t(p->backward && a->dw ? (size_t)p->H * p->ldt * 2 : 0);
+    p->wimg = t(p->pack_w ? (size_t)p->vp * p->kimg * 2 : 0);
+    p->wt = t(p->backward && a->dx ? (size_t)p->H * p->ldd * 2 : 0);
+    const long long ptiles = p->pieces * ltiles_m;
+    p->part = t(p->forward ? (size_t)ptiles * p->n * 8 : 0);
+    p->part_e = t(p->forward && a->entropy ? (size_t)ptiles * p->n * 4 : 0);
+    p->part_t = t(p->forward && a->probs ? (size_t)ptiles * p->n * 16 : 0);
+    p->tlogit = t((size_t)p->n * 4);
+    p->stats = t((size_t)p->n * 16);
+    p->ent = t((size_t)p->n * 4);
+    p->rowg = t((size_t)p->n * 4);
+    p->factor = t(4);
+    p->d = t(p->backward && a->dx ? (size_t)p->n * p->ldd * 2 : 0);
+    p->dt = t(p->backward && a->dw ? (size_t)p->vp * p->ldt * 2 : 0);
+    p->dbpart = t(p->backward && a->db ? (size_t)ltiles_n * p->vp * 4 : 0);
+    p->dxacc = t(p->backward && a->dx && (p->gx.splits > 1 || p->pieces > 1) ? (size_t)p->gx.splits * p->n * p->H * 4 : 0);
+    p->dwacc = t(p->backward && a->dw && p->gw.splits > 1 ? (size_t)p->gw.splits * p->vp * p->H * 4 : 0);
+    p->total = t.off;
+    return AZG_OK;
+}
+
+int check(const azg_linear_ce_args *a)
+{
+    if (!a) return fail(AZG_EINVAL, "null argument");
+    if (a->dtype != AZG_F32 && a->dtype != AZG_BF16 && a->dtype != AZG_F16) return fail(AZG_EINVAL, "azg_linear_ce: unknown dtype %d", a->dtype);
+    if (a->n < 0 || a->hidden < 1 || a->classes < 1) return fail(AZG_EINVAL, "azg_linear_ce: sizes must be n >= 0, hidden >= 1, classes >= 1");
+    if (a->n > INT_MAX || a->classes > INT_MAX || a->hidden > (1 << 22)) return fail(AZG_EINVAL, "azg_linear_ce: a size is too large");
+    if (a->reduction < AZG_REDUCE_NONE || a->reduction > AZG_REDUCE_MEAN) return fail(AZG_EINVAL, "azg_linear_ce: unknown reduction %d", a->reduction);
+    if (bad_matrix(a->n, a->hidden, a->x_stride) || bad_matrix(a->classes, a->hidden, a->w_stride)) return fail(AZG_EINVAL, "azg_linear_ce: a row stride is smaller than a row");
+    if (a->x_stride > (1 << 22) * 64LL || a->w_stride > (1 << 22) * 64LL) return fail(AZG_EINVAL, "azg_linear_ce: a row stride is too large");
+    return AZG_OK;
+}
+
+template <typename K> int allow_lds(K kernel, int bytes)
+{
+    if (bytes > 65536) OPS_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    return AZG_OK;
+}
+
+template <typename Op, int TM, int TN, int WM, int WN, bool GRAD>
+int launch_logits_shape(CeArgs c, hipStream_t s)
+{
+    using S = TileShape<TM, TN, WM, WN>;
+    c.mtiles = (int)((c.classes + TM - 1) / TM);
+    c.ntiles = (int)((c.n + TN - 1) / TN);
+    const int lds = std::max(S::lds_bytes, WM * 6 * TN * 4);
+    OPS_TRY(allow_lds(logits_kernel<Op, TM, TN, WM, WN, GRAD>, lds));
+    hipLaunchKernelGGL((logits_kernel<Op, TM, TN, WM, WN, GRAD>), dim3((unsigned)c.mtiles * c.ntiles), dim3(S::threads), lds, s, c);
+    OPS_HIP(hipGetLastError());
+    return AZG_OK;
+}
+template <typename Op, bool GRAD>
+int launch_logits(Shape shape, const CeArgs &c, hipStream_t s)
+{
+    switch (shape) {
+    case T256: return launch_logits_shape<Op, 256, 256, 2, 4, GRAD>(c, s);
+    case T128: return launch_logits_shape<Op, 128, 128, 2, 2, GRAD>(c, s);
+    case T64: return launch_logits_shape<Op, 64, 64, 2, 2, GRAD>(c, s);
+    default:
+        if constexpr (!GRAD) return launch_logits_shape<Op, 128, 16, 4, 1, false>(c, s);
+        return fail(AZG_EINVAL, "azg_linear_ce: internal: no such tile");
+    }
+}
+
+template <typename Op, int TM, int TN, int WM, int WN>
+int launch_grad_shape(GradArgs g, int splits, hipStream_t s)
+{
+    using S = TileShape<TM, TN, WM, WN>;
+    g.mtiles = (int)((g.m + TM - 1) / TM);
+    g.ntiles = (int)((g.n + TN - 1) / TN);
+    OPS_TRY(allow_lds(grad_kernel<Op, TM, TN, WM, WN>, S::lds_bytes));
+    hipLaunchKernelGGL((grad_kernel<Op, TM, TN, WM, WN>), dim3((unsigned)g.mtiles * g.ntiles, splits), dim3(S::threads), S::lds_bytes, s, g);
+    OPS_HIP(hipGetLastError());
+    return AZG_OK;
+}
+template <typename Op>
+int launch_grad(const GradPick &pick, GradArgs g, hipStream_t s)
+{
+    g.kper = pick.kper;
+    switch (pick.shape) {
+    case T256: return launch_grad_shape<Op, 256, 256, 2, 4>(g, pick.splits, s);
+    case T128: return launch_grad_shape<Op, 128, 128, 2, 2>(g, pick.splits, s);
+    default: return launch_grad_shape<Op, 64, 64, 2, 2>(g, pick.splits, s);
+    }
+}
+template <typename Op>
+int launch_join(const JoinArgs &j, hipStream_t s)
+{
+    const long long grid = std::min<long long>((j.n * j.m + 255) / 256, 1 << 16);
+    hipLaunchKernelGGL((join_kernel<Op>), dim3((unsigned)grid), dim3(256), 0, s, j);
+    OPS_HIP(hipGetLastError());
+    return AZG_OK;
+}
+template <typename Op>
+int launch_pack(const PackArgs &p, hipStream_t s)
+{
+    // (the padding of an image of the rows may reach into one more block of columns than the tensor has, and likewise)
+    const int per = Op::split ? 2 : 1;
+    const long long cols = std::max(p.cols, p.img ? p.ldi / per : 0), rows = std::max(p.rows, p.imgt ? p.ldt / per : 0);
+    const long long gx = (cols + 63) / 64, gy = (rows + 63) / 64;
+    for (long long y = 0; y < gy; y += 32768) {               // a grid has at most 65535 rows of workgroups
+        PackArgs q = p;
+        q.r_first = y * 64;
+        hipLaunchKernelGGL((pack_kernel<Op>), dim3((unsigned)gx, (unsigned)std::min<long long>(32768, gy - y)), dim3(256), 0, s, q);
+    }
+    OPS_HIP(hipGetLastError());
+    return AZG_OK;
+}
+
+template <typename Op>
+int run_ce(const azg_linear_ce_args *a, const Plan &p)
+{
+    using In = typename Op::In;
+    hipStream_t s = static_cast<hipStream_t>(a->stream);
+    char *ws = static_cast<char *>(a->workspace);
+    auto f32 = [&](size_t o) { return reinterpret_cast<float *>(ws + o); };
+    const long long *target = reinterpret_cast<const long long *>(a->target);
+    float4 *stats = a->stats ? static_cast<float4 *>(a->stats) : reinterpret_cast<float4 *>(ws + p.stats);
+    const In *W = static_cast<const In *>(a->w);
+
+    // images of the rows
+    PackArgs px{};
+    px.src = a->x; px.ld = a->x_stride; px.rows = a->n; px.cols = a->hidden; px.target = target; px.ignore = a->ignore_index; px.maxpart = f32(p.xmax);
+    px.img = p.pack_x ? ws + p.ximg : nullptr; px.ldi = p.kimg;
+    px.imgt = p.backward && a->dw ? ws + p.xt : nullptr; px.ldt = p.ldt;
+    if (Op::split) {
+        PackArgs pm = px;
+        hipLaunchKernelGGL(absmax_kernel, dim3(kMaxParts), dim3(256), 0, s, pm, f32(p.xmax));
+        pm.src = a->w; pm.ld = a->w_stride; pm.rows = a->classes; pm.target = nullptr;
+        hipLaunchKernelGGL(absmax_kernel, dim3(kMaxParts), dim3(256), 0, s, pm, f32(p.wmax));
+    }
+    if (px.img || px.imgt) OPS_TRY(launch_pack<Op>(px, s));
+    CeArgs c{};
+    c.x = p.pack_x ? Operand{ws + p.ximg, p.kimg, a->n} : Operand{a->x, a->x_stride, a->n};
+    c.kvalid = p.pack_x && p.pack_w ? p.kimg : a->hidden;   // (a direct operand has a multiple of 8 features)
+    c.ktiles = (int)((p.kimg + 63) / 64);
+    c.n = a->n; c.target = target; c.ignore = a->ignore_index; c.ldp = a->probs_stride;
+    c.xmax = f32(p.xmax); c.wmax = f32(p.wmax);
+
+    auto piece = [&](long long i, bool want_t, bool want_img) -> int {
+        const long long v0 = i * p.vp, vn = std::min(p.vp, a->classes - v0);
+        c.v0 = v0; c.classes = vn;
+        c.bias = a->bias ? static_cast<const In *>(a->bias) + v0 : nullptr;
+        c.probs = a->probs ? a->probs + v0 : nullptr;
+        PackArgs pw{};
+        pw.src = W + v0 * a->w_stride; pw.ld = a->w_stride; pw.rows = vn; pw.cols = a->hidden; pw.maxpart = f32(p.wmax);
+        pw.img = p.pack_w && want_img ? ws + p.wimg : nullptr; pw.ldi = p.kimg;
+        pw.imgt = want_t ? ws + p.wt : nullptr; pw.ldt = Op::split ? up_to(vn, 32) * 2 : up_to(vn, 64);
+        if (pw.img || pw.imgt) OPS_TRY(launch_pack<Op>(pw, s));
+        c.w = p.pack_w ? Operand{ws + p.wimg, p.kimg, vn} : Operand{W + v0 * a->w_stride, a->w_stride, vn};
+        return AZG_OK;
+    };
+
+    const ShapeDim dim = kDims[p.lshape];
+    if (p.forward) {
+        const long long full = (p.vp + dim.tm - 1) / dim.tm;
+        long long tiles = 0;
+        for (long long i = 0; i < p.pieces; i++) {
+            OPS_TRY(piece(i, p.backward && a->dx && p.pieces == 1, true));
+            c.part = reinterpret_cast<float2 *>(ws + p.part) + i * full * a->n;
+            c.part_e = a->entropy ? f32(p.part_e) + i * full * a->n : nullptr;
+            c.part_t = a->probs ? reinterpret_cast<float4 *>(ws + p.part_t) + i * full * a->n : nullptr;
+            c.tlogit = f32(p.tlogit);
+            OPS_TRY((launch_logits<Op, false>(p.lshape, c, s)));
+            tiles += (c.classes + dim.tm - 1) / dim.tm;
+        }
+        RowArgs r{};
+        r.n = a->n; r.classes = a->classes; r.tiles = (int)tiles;
+        r.part = reinterpret_cast<float2 *>(ws + p.part); r.part_e = a->entropy ? f32(p.part_e) : nullptr;
+        r.part_t = a->probs ? reinterpret_cast<float4 *>(ws + p.part_t) : nullptr; r.tlogit = f32(p.tlogit);
+        r.target = target; r.ignore = a->ignore_index; r.stats = stats; r.ent = a->entropy ? f32(p.ent) : nullptr;
+        hipLaunchKernelGGL(rows_kernel, dim3((unsigned)((a->n + 3) / 4)), dim3(256), 0, s, r);
+    }
+    TotalArgs t{};
+    t.n = a->n; t.reduction = a->reduction; t.stats = stats; t.ent = p.forward && a->entropy ? f32(p.ent) : nullptr;
+    t.target = target; t.ignore = a->ignore_index; t.loss = p.forward ? a->loss : nullptr; t.ent_out = p.forward ? a->entropy : nullptr;
+    t.dloss = a->dloss; t.grad_scale = (float)a->grad_scale;
+    t.rowg = p.backward ? f32(p.rowg) : nullptr; t.factor = f32(p.factor);
+    hipLaunchKernelGGL(totals_kernel, dim3(1), dim3(1024), 0, s, t);
+    OPS_HIP(hipGetLastError());
+    if (!p.backward) return AZG_OK;
+
+    for (long long i = 0; i < p.pieces; i++) {
+        if (!(p.forward && p.pieces == 1)) OPS_TRY(piece(i, a->dx != nullptr, true));
+        const long long vn = c.classes, ldd = Op::split ? up_to(vn, 32) * 2 : up_to(vn, 64);
+        c.stats = stats; c.rowg = f32(p.rowg);
+        c.d = a->dx ? ws + p.d : nullptr; c.ldd = ldd;
+        c.dt = a->dw ? ws + p.dt : nullptr; c.ldt = p.ldt;
+        c.dbpart = a->db ? f32(p.dbpart) : nullptr;
+        OPS_TRY((launch_logits<Op, true>(p.lshape, c, s)));
+        if (a->dx) {
+            GradArgs g{};
+            g.a = Operand{ws + p.wt, ldd, a->hidden}; g.b = Operand{ws + p.d, ldd, a->n};
+            g.kvalid = ldd; g.ktiles = (int)(ldd / 64); g.m = a->hidden; g.n = a->n;
+            g.amax = f32(p.wmax); g.factor = f32(p.factor);
+            const bool acc = p.gx.splits > 1 || p.pieces > 1;
+            g.acc = acc ? f32(p.dxacc) : nullptr; g.add = i > 0;
+            g.out = a->dx; g.ldo = a->dx_stride; g.vec = true;
+            OPS_TRY(launch_grad<Op>(p.gx, g, s));
+            if (acc && i == p.pieces - 1) {
+                JoinArgs j{};
+                j.acc = f32(p.dxacc); j.splits = p.gx.splits; j.n = a->n; j.m = a->hidden; j.out = a->dx; j.ldo = a->dx_stride;
+                j.amax = f32(p.wmax); j.factor = f32(p.factor); j.extra = kDScale;
+                OPS_TRY(launch_join<Op>(j, s));
+            }
+        }
+        if (a->dw) {
+            GradArgs g{};
+            g.a = Operand{ws + p.xt, p.ldt, a->hidden}; g.b = Operand{ws + p.dt, p.ldt, vn};
+            g.kvalid = p.ldt; g.ktiles = (int)((p.ldt + 63) / 64); g.m = a->hidden; g.n = vn;
+            g.amax = f32(p.xmax); g.factor = f32(p.factor);
+            g.acc = p.gw.splits > 1 ? f32(p.dwacc) : nullptr; g.add = false;
+            g.out = static_cast<In *>(a->dw) + i * p.vp * a->dw_stride; g.ldo = a->dw_stride; g.vec = true;
+            OPS_TRY(launch_grad<Op>(p.gw, g, s));
+            if (g.acc) {
+                JoinArgs j{};
+                j.acc = g.acc; j.splits = p.gw.splits; j.n = vn; j.m = a->hidden; j.out = g.out; j.ldo = a->dw_stride;
+                j.amax = f32(p.xmax); j.factor = f32(p.factor); j.extra = kDScale;
+                OPS_TRY(launch_join<Op>(j, s));
+            }
+        }
+        if (a->db) {
+            JoinArgs j{};
+            j.acc = f32(p.dbpart); j.splits = (int)((a->n + dim.tn - 1) / dim.tn); j.n = 1; j.m = vn;
+            j.out = static_cast<In *>(a->db) + i * p.vp; j.ldo = vn; j.factor = f32(p.factor); j.extra = 1.f;
+            OPS_TRY(launch_join<Op>(j, s));
+        }
+    }
+    return AZG_OK;
+}
+
+template <typename In>
+int empty_batch(const azg_linear_ce_args *a)
+{
+    hipStream_t s = static_cast<hipStream_t>(a->stream);
+    if (a->dw) hipLaunchKernelGGL((zero_rows_kernel<In>), dim3(1024), dim3(256), 0, s, static_cast<In *>(a->dw), (long long)a->classes, (long long)a->hidden, (long long)a->dw_stride);
+    if (a->db) hipLaunchKernelGGL((zero_rows_kernel<In>), dim3(64), dim3(256), 0, s, static_cast<In *>(a->db), 1LL, (long long)a->classes, (long long)a->classes);
+    if (a->reduction != AZG_REDUCE_NONE) {
+        if (a->loss) hipLaunchKernelGGL((zero_rows_kernel<float>), dim3(1), dim3(64), 0, s, a->loss, 1LL, 1LL, 1LL);
+        if (a->entropy) hipLaunchKernelGGL((zero_rows_kernel<float>), dim3(1), dim3(64), 0, s, a->entropy, 1LL, 1LL, 1LL);
+    }
+    OPS_HIP(hipGetLastError());
+    return AZG_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t azg_linear_ce_workspace(const azg_linear_ce_args *a)
+{
+    const int rc = check(a);
+    if (rc) return rc;
+    if (a->n == 0) return 0;
+    Plan p{};
+    const int rc2 = make_plan(a, &p);
+    return rc2 ? rc2 : (int64_t)p.total;
+}
+
+extern "C" int azg_linear_ce(const azg_linear_ce_args *a)
+{
+    OPS_TRY(check(a));
+    const bool backward = a->dx || a->dw || a->db;
+    if (!a->loss && !backward) return fail(AZG_EINVAL, "azg_linear_ce: neither a loss nor a gradient is asked for");
+    if (!a->loss && !a->stats) return fail(AZG_EINVAL, "azg_linear_ce: a backward pass by itself needs the forward pass's stats");
+    if (a->entropy && !a->loss) return fail(AZG_EINVAL, "azg_linear_ce: the entropy comes with the loss");
+    if ((a->dx && bad_matrix(a->n, a->hidden, a->dx_stride)) || (a->dw && bad_matrix(a->classes, a->hidden, a->dw_stride)))
+        return fail(AZG_EINVAL, "azg_linear_ce: a row stride is smaller than a row");
+    if (a->n > 0) {
+        if (!a->x || !a->w) return fail(AZG_EINVAL, "null argument");
+        if ((a->target != nullptr) == (a->probs != nullptr)) return fail(AZG_EINVAL, "azg_linear_ce: either target or probs");
+        if (a->probs && bad_matrix(a->n, a->classes, a->probs_stride)) return fail(AZG_EINVAL, "azg_linear_ce: a row stride is smaller than a row");
+    }
+    DeviceScope scope;
+    OPS_TRY(scope.enter(a->device));
+    if (a->n == 0) return a->dtype == AZG_F32 ? empty_batch<float>(a) : a->dtype == AZG_F16 ? empty_batch<_Float16>(a) : empty_batch<__bf16>(a);
+    Plan p{};
+    OPS_TRY(make_plan(a, &p));
+    if (!a->workspace || (reinterpret_cast<uintptr_t>(a->workspace) & 255) || a->workspace_bytes < (int64_t)p.total)
+        return fail(AZG_EINVAL, "azg_linear_ce: the workspace must be 256-byte aligned and hold %lld bytes", (long long)p.total);
+    if (a->dtype == AZG_F32) return run_ce<OpF32>(a, p);
+    if (a->dtype == AZG_F16) return run_ce<OpF16>(a, p);
+    return run_ce<OpBF16>(a, p);
+}

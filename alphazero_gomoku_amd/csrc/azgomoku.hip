@@ -464,6 +464,9 @@ static int refresh_mirrors(azg_handle *h)
 }
 
 // ---------------------------------------------------------------- create / destroy
+// (for azg_ops.hip, whose entry points have no handle)
+extern "C" __attribute__((visibility("hidden"))) void azg_set_error_text(const char *text) { g_create_error = text; }
+
 extern "C" const char *azg_last_error(const azg_handle *h) { return h ? h->err.c_str() : g_create_error.c_str(); }
 
 extern "C" void azg_destroy(azg_handle *h)

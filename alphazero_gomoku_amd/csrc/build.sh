@@ -20,10 +20,20 @@ log="$(mktemp)"
 tmp="$(mktemp -d)"
 trap 'rm -rf "$tmp"' EXIT
 # (the device assembly is kept as a by-product of the one compilation: -save-temps, in a scratch directory)
-( cd "$tmp" && hipcc --offload-arch=gfx950 -O3 -ffp-contract=off -fno-slp-vectorize -fPIC -shared -std=c++17 -Wall -no-hip-rt \
+# azg_ops.hip (the training heads' operators) is a translation unit of its own, compiled beside it, in which the compiler may
+# not form two-wide float32 instructions at all.
+opsflags="--offload-arch=gfx950 -O3 -fno-slp-vectorize -fPIC -std=c++17 -Wall -Wno-unknown-warning-option -Xclang -target-feature -Xclang -packed-fp32-ops"
+( hipcc $opsflags -c "$here/azg_ops.hip" -o "$tmp/azg_ops.o" > "$tmp/ops.log" 2>&1; echo $? > "$tmp/ops.rc" ) &
+ops=$!
+( cd "$tmp" && hipcc --offload-arch=gfx950 -O3 -ffp-contract=off -fno-slp-vectorize -fPIC -c -std=c++17 -Wall \
     -Rpass-analysis=kernel-resource-usage -save-temps=cwd \
-    "$here/azgomoku.hip" -o "$out" -lpthread "$@" ) 2> "$log" || { cat "$log" >&2; rm -f "$log"; exit 1; }
-asm="$(ls "$tmp"/*gfx950.s 2>/dev/null | head -1)"
+    "$here/azgomoku.hip" -o "$tmp/azgomoku.o" "$@" ) 2> "$log" || { cat "$log" >&2; rm -f "$log"; exit 1; }
+wait $ops
+# (the host pass does not know the device feature and says so: harmless)
+grep -v "packed-fp32-ops" "$tmp/ops.log" >&2 || true
+[ "$(cat "$tmp/ops.rc")" = 0 ] || exit 1
+hipcc --offload-arch=gfx950 -fPIC -shared -no-hip-rt "$tmp/azgomoku.o" "$tmp/azg_ops.o" -o "$out" -lpthread
+asm="$(ls "$tmp"/azgomoku*gfx950.s 2>/dev/null | head -1)"
 if [ -z "$asm" ]; then echo "build.sh: no device assembly to check" >&2; rm -f "$out" "$log"; exit 1; fi
 # (only the kernels that run beside matrix-dense waves: search, evaluation, caller-evaluated playouts;
 #  the training kernels may use two-wide arithmetic)

@@ -281,6 +281,74 @@ int azg_train_epoch(azg_handle *h, int n, const float *states, const float *mcts
                     const float *states_all, float *probs, float *values, const float *old_probs,
                     double *kl);
 
+/* Operators of the training heads on the caller's tensors: no handle, DEVICE pointers, enqueued on `stream` (a
+ * hipStream_t of `device`, NULL = its default stream) and NOT waited for; they allocate nothing, keep nothing and can be
+ * captured into a HIP graph.  `device` is made current for the call.  Calls from several threads may overlap.
+ * azg_last_error(NULL) is the calling thread's last failure.  Matrices are row-major with a row stride in elements;
+ * outputs must not overlap inputs except where said. */
+#define AZG_F32   0
+#define AZG_BF16  1
+#define AZG_F16   2
+
+/* out = residual + (keep ? x * s : 0), rounded once: dropout with a mask that is a function of (seed, offset, element
+ * number) and never stored.  T = round(65536 p); an element is kept when its 16 random bits are >= T; s = 65536 / (65536 - T)
+ * (T = 65536 drops everything).  Element (r, c) has number (first_row + r * row_step) * cols + c modulo 2^64, so ranks that
+ * hold rows of one batch draw one mask.  Bits: Philox4x32-10, counter = (number div 8, offset [+ *offset_dev]), key = seed;
+ * element number mod 8 = q takes half-word q, low halves first.  The gradient at x is the same map of the gradient at out,
+ * without residual.  A dropped element contributes exact zero whatever it holds.  out may be x or residual itself. */
+typedef struct azg_dropout_args {
+    int32_t device, dtype;
+    int64_t rows, cols;
+    const void *x; int64_t x_stride;
+    const void *residual; int64_t residual_stride;   /* NULL: none */
+    void *out; int64_t out_stride;
+    double p;                                        /* 0 .. 1 */
+    uint64_t seed, offset;
+    const int64_t *offset_dev;                       /* NULL, or one device word added to offset when the kernel runs */
+    uint64_t first_row, row_step;
+    void *stream;
+} azg_dropout_args;
+int azg_dropout(const azg_dropout_args *a);
+
+/* Softmax cross entropy of the projection l = x w^T + bias (x [n,hidden], w [classes,hidden], bias [classes] or NULL, one
+ * type), against class numbers or against probabilities (any real weights), and its gradients, in pieces of the classes:
+ * no array of n * classes logits exists, only 16-bit images of the gradient at one piece of them (1 GiB at most with the
+ * other images, or 1024 classes).  For every row
+ *   loss = lse - l[target]                        target int64 [n]; rows whose target is ignore_index count for nothing,
+ *                                                 whatever x holds there (loss 0, gradient 0); any other target outside
+ *                                                 0 .. classes - 1 makes the row's loss, and every gradient it reaches, NaN
+ *   loss = lse sum_v probs - sum_v probs l        probs float32 [n,classes]; a weight of 0 contributes 0
+ *   entropy = lse - sum_v p l                     p = softmax(l)
+ * reduction AZG_REDUCE_NONE: loss, entropy float32 [n]; _SUM, _MEAN (over the rows that count; 0 if none does): [1].
+ * Gradients are those of sum_i dloss_i loss_i (NONE, dloss [n]) or dloss loss ([1]), times grad_scale; dloss NULL = 1.
+ * One call does the forward pass (loss not NULL), the backward pass (any of dx, dw, db not NULL), or both.  A backward pass
+ * by itself takes the stats [n][4] (float32, 16-byte aligned, the caller's) that the forward pass of the same inputs wrote.
+ * Sums, statistics and accumulators are float32 or wider; the gradient at the logits is rounded to x's type (float32: to 22
+ * bits) before the two products that use it.  Results do not depend on anything but the arguments: the same bits every time.
+ * azg_linear_ce_workspace: bytes of workspace (256-byte aligned) the call needs with these very arguments, or AZG_E*. */
+#define AZG_REDUCE_NONE  0
+#define AZG_REDUCE_SUM   1
+#define AZG_REDUCE_MEAN  2
+typedef struct azg_linear_ce_args {
+    int32_t device, dtype, reduction, reserved;
+    int64_t n, hidden, classes;
+    const void *x; int64_t x_stride;
+    const void *w; int64_t w_stride;
+    const void *bias;
+    const int64_t *target; int64_t ignore_index;     /* either target */
+    const float *probs; int64_t probs_stride;        /* or probs */
+    float *loss, *entropy;                           /* entropy may be NULL */
+    void *stats;                                     /* [n][4]; NULL: kept in the workspace */
+    const float *dloss; double grad_scale;
+    void *dx; int64_t dx_stride;
+    void *dw; int64_t dw_stride;
+    void *db;
+    void *workspace; int64_t workspace_bytes;
+    void *stream;
+} azg_linear_ce_args;
+int64_t azg_linear_ce_workspace(const azg_linear_ce_args *a);
+int azg_linear_ce(const azg_linear_ce_args *a);
+
 /* Timing of the search of a move (MCTS.get_move_probs, mcts_alphaZero.py:154-181), measured with HIP
  * events on the handle's stream: number of searches since the last call, summed milliseconds, and
  * summed leaf evaluations (playouts that reached the CNN).  Resets the counters.
