@@ -2,18 +2,19 @@
 // live in the accumulators of a matrix-core tile and leave it as softmax statistics (forward) or as the gradient
 // at the logits, 16 bits an element and one piece of the classes at a time (backward).
 //
-//   lse_i  = log sum_v exp l_iv, from the tiles' running (maximum, sum) pairs
+//   lse_i  = log sum_v exp l_iv, from (maximum, sum) pairs of runs of classes
 //   loss_i = lse_i - l_{i,t}   or   lse_i sum_v pi_iv - sum_v pi_iv l_iv
 //   D_iv   = g_i (p_iv sum_v pi_iv - pi_iv);   dX = D W;   dW = D^T X;   db = sum_i D_i
 //
-// All three products are one kernel core: C[m][n] = sum_k A[m][k] B[n][k] with both operands contiguous along k.
-// Operands that are not laid out so (transposes, float32, odd sizes) are copied once into such an "image".
+// All three products are one kernel core: C[m][n] = sum_k A[m][k] B[n][k], each operand stored with either index
+// contiguous: what runs against the sum is transposed on its way from LDS to the registers.  Operands that the loads
+// cannot take (float32, odd sizes or alignments) and rows that must read as zero are copied once into an "image".
 //
 // float32 runs on the 16-bit matrix cores too: x 2^s = hi + lo with hi, lo in half precision (s a power of two
 // from the tensor's largest magnitude, so that nothing overflows and what underflows is 2^-38 of the largest
 // element), and a product takes three instructions, hi hi + hi lo + lo hi.  hi carries 11 bits and lo 11 more, so
 // an operand is off by at most 2^-22 of itself and the dropped lo lo is at most 2^-22 of the product; sums are
-// float32.  An image row holds blocks of 64: 32 hi, then the 32 lo of the same k.
+// float32.  An image row holds blocks of 64: 32 hi, then the 32 lo of the same columns.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -47,14 +48,19 @@ template <> struct Frag<__bf16> {
 };
 
 // ---------------------------------------------------------------- the tile product
-// TM x TN output tile, 64 image elements of k per stage, WM x WN waves, 16x16x32 matrix instructions.
-// LDS rows are 128 bytes = eight 16-byte chunks; chunk c of row r sits at c ^ (r & 7), so the sixteen rows that a
-// fragment read touches spread over all banks.  Stages are double-buffered and filled by loads that go from global
-// memory straight to LDS.
+// TM x TN output tile, WM x WN waves, 16x16x32 matrix instructions, stages of 64 k (float32: 32).  Stages are
+// double-buffered in LDS and filled by loads that go from global memory straight there, 16 bytes a lane.
+//   k contiguous in memory: LDS rows are 128 bytes of one m, eight 16-byte chunks, chunk c of row r at c ^ (r & 7), so the
+//     sixteen rows of a fragment read (16 bytes a lane) spread over all banks;
+//   k across the rows: LDS rows are one k, TM columns of the image; a fragment is read by the transposing load
+//     (ds_read_b64_tr_b16: a group of sixteen lanes reads four k of sixteen columns, 8 bytes a lane, and lane i gets
+//     column i's four k), 32-byte unit j of row k at j ^ unit_swizzle(k), so that the eight rows that half a wave reads
+//     lie in different banks.
 struct Operand {
     const void *p;       // image, or the caller's 16-bit tensor
-    long long ld;        // elements
-    long long rows;
+    long long ld;        // row stride, elements
+    long long rows;      // rows that exist; past them: k contiguous - any row, the result is not stored; k across - zero
+    long long cols;      // elements of a row that exist (a multiple of 8); past them zero
 };
 
 template <int TM, int TN, int WM, int WN>
@@ -66,69 +72,126 @@ struct TileShape {
 
 typedef __attribute__((address_space(3))) void *lds_ptr;
 typedef const __attribute__((address_space(1))) void *glb_ptr;
+typedef short sx4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) sx4 *lds_sx4;
 
 __device__ inline void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-template <typename Op, int TM, int TN, int WM, int WN>
+// One operand of a tile: T rows of m, k contiguous (TR false) or across the rows (TR true).  `groups` of 1024 LDS bytes, one
+// load instruction of a wave each.
+template <typename Op, int T, bool TR>
+struct Side {
+    using V = typename Frag<typename Op::Img>::V;
+    static constexpr int ks = Op::split ? 32 : 64;                              // k of a stage
+    static constexpr int groups = T / 8;
+    static constexpr int row_bytes = TR ? T * 128 / ks : 128, row_chunks = row_bytes / 16;
+
+    static __device__ inline int unit_swizzle(int k)
+    {
+        return row_bytes >= 256 ? (k & 3) | ((k >> 1) & 4) : ((k >> 1) & 1) | ((k >> 2) & 2);
+    }
+    // this lane's 16 bytes of group g: source address in stage k0, whether its columns exist, its k (TR) or column (not TR)
+    static __device__ inline const char *source(const Operand &O, long long m0, int g, int lane, int k0, int *at, bool *there)
+    {
+        const int c = g * 64 + lane, row = c / row_chunks, pos = c % row_chunks;
+        if constexpr (TR) {
+            const long long col = m0 * (64 / ks) + (pos ^ (unit_swizzle(row) << 1)) * 8;
+            *at = row;
+            *there = col < O.cols;
+            return static_cast<const char *>(O.p) + (((long long)k0 * ks + row) * O.ld + col) * 2;
+        } else {
+            long long r = m0 + row;
+            r = r < O.rows ? r : O.rows - 1;
+            *at = (pos ^ (row & 7)) * 8;
+            *there = true;
+            return static_cast<const char *>(O.p) + (r * O.ld + (long long)k0 * 64 + *at) * 2;
+        }
+    }
+    // in the last stage: is this lane past the end of k?
+    static __device__ inline bool past(const Operand &O, int kt, int at) { return (long long)kt * (TR ? ks : 64) + at >= (TR ? O.rows : O.cols); }
+    static __device__ inline long long step(const Operand &O) { return TR ? O.ld * (ks * 2) : 128; }
+
+    // fragment t (sixteen m), half h of the stage: float32 - h = 0 the hi, 1 the lo of the 32 k;  else k 32 h .. 32 h + 31
+    static __device__ inline V read(const char *base, int lane, int t, int h)
+    {
+        if constexpr (TR) {
+            const int g = lane >> 4, s = lane & 15, k = g * 8 + (s >> 2);
+            const int unit = Op::split ? (t >> 1) * 4 + (t & 1) + 2 * h : t;
+            const char *p = base + ((Op::split ? 0 : 32 * h) + k) * row_bytes + ((unit ^ unit_swizzle(k)) * 32) + (s & 3) * 8;
+            union { sx4 q[2]; V v; } u;
+            u.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_sx4)p);
+            u.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_sx4)(p + 4 * row_bytes));
+            return u.v;
+        } else {
+            return *reinterpret_cast<const V *>(base + (t * 16 + (lane & 15)) * 128 + (((h * 4 + (lane >> 4)) ^ (lane & 7)) * 16));
+        }
+    }
+};
+
+template <typename Op, int TM, int TN, int WM, int WN, bool TA, bool TB>
 struct TileProduct {
     using S = TileShape<TM, TN, WM, WN>;
     using F = Frag<typename Op::Img>;
-    static constexpr int kA = TM / 8, kAll = (TM + TN) / 8;                     // groups of eight rows a stage
+    using A_ = Side<Op, TM, TA>;
+    using B_ = Side<Op, TN, TB>;
+    static constexpr int kAll = A_::groups + B_::groups, kLoads = (kAll + S::waves - 1) / S::waves;
 
     // acc[mt][nt][i]: row wm*(TM/WM) + 16 mt + 4 (lane >> 4) + i of A, row wn*(TN/WN) + 16 nt + (lane & 15) of B.
-    // Stages k0 .. k1 - 1; kvalid (a multiple of 8) image elements of k exist.
+    // Stages k0 .. k1 - 1 of ktotal.
     static __device__ inline void run(fx4 (&acc)[S::MT][S::NT], const Operand &A, long long m0, const Operand &B, long long n0,
-                                      long long kvalid, int k0, int k1, char *lds)
+                                      int k0, int k1, int ktotal, char *lds)
     {
+        if (k0 >= k1) return;
         const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const int wm = wave / WN, wn = wave % WN;
-        constexpr int kLoads = (kAll + S::waves - 1) / S::waves;
         const char *src[kLoads];
-        const int chunk = (lane & 7) ^ (lane >> 3);
+        int at[kLoads];
+        bool there[kLoads];
+        const char *zero = reinterpret_cast<const char *>(g_zero_page);
 #pragma unroll
         for (int i = 0; i < kLoads; i++) {
-            const int g = i * S::waves + wave;                                  // wave-uniform
-            const bool is_a = g < kA;
-            const Operand &O = is_a ? A : B;
-            long long r = (is_a ? m0 + g * 8 : n0 + (g - kA) * 8) + (lane >> 3);
-            r = r < O.rows ? r : O.rows - 1;                                    // rows past the end: any finite place, never stored
-            src[i] = static_cast<const char *>(O.p) + (r * O.ld + (long long)k0 * 64 + chunk * 8) * 2;
+            const int g = i * S::waves + wave;                                  // wave-uniform; a load is all A or all B
+            if (g < A_::groups) src[i] = A_::source(A, m0, g, lane, k0, &at[i], &there[i]);
+            else src[i] = B_::source(B, n0, g - A_::groups, lane, k0, &at[i], &there[i]);
         }
+        const long long step_a = A_::step(A), step_b = B_::step(B);
         auto load = [&](int kt, int buf) {
-            const bool past = (long long)kt * 64 + chunk * 8 >= kvalid;          // only in the last stage of an odd k
+            const bool last = kt + 1 == ktotal;
 #pragma unroll
             for (int i = 0; i < kLoads; i++) {
                 const int g = i * S::waves + wave;
                 if (kAll % S::waves == 0 || g < kAll) {
-                    const char *p = past ? reinterpret_cast<const char *>(g_zero_page) : src[i];
+                    const char *p = src[i];
+                    if ((TA || TB) && !there[i]) p = zero;
+                    if (last && (g < A_::groups ? A_::past(A, kt, at[i]) : B_::past(B, kt, at[i]))) p = zero;
                     __builtin_amdgcn_global_load_lds((glb_ptr)p, (lds_ptr)(lds + buf * S::stage_bytes + g * 1024), 16, 0, 0);
-                    src[i] += 128;
+                    src[i] += g < A_::groups ? step_a : step_b;
                 }
             }
         };
-        const int fr = (lane & 15) * 128, fc = ((lane >> 4) ^ (lane & 7)) * 16;
-        const char *fa = lds + wm * (TM / WM) * 128 + fr, *fb = lds + TM * 128 + wn * (TN / WN) * 128 + fr;
-        if (k0 >= k1) return;
         // (the barrier alone does not wait for loads that write LDS)
         load(k0, 0);
         wait_loads();
         __syncthreads();
+        // a wave's part of a side begins a whole number of rows or 32-byte units into it
+        const int oa = TA ? 0 : wm * (TM / WM) * 128, ob = A_::groups * 1024 + (TB ? 0 : wn * (TN / WN) * 128);
+        const int ta = TA ? wm * S::MT : 0, tb = TB ? wn * S::NT : 0;
         for (int kt = k0; kt < k1; kt++) {
             const int buf = (kt - k0) & 1;
             if (kt + 1 < k1) load(kt + 1, buf ^ 1);
-            const char *pa = fa + buf * S::stage_bytes, *pb = fb + buf * S::stage_bytes;
+            const char *pa = lds + buf * S::stage_bytes + oa, *pb = lds + buf * S::stage_bytes + ob;
             typename F::V a[2][S::MT], b[2][S::NT];
 #pragma unroll
-            for (int ks = 0; ks < 2; ks++) {
+            for (int h = 0; h < 2; h++) {
 #pragma unroll
-                for (int t = 0; t < S::NT; t++) b[ks][t] = *reinterpret_cast<const typename F::V *>(pb + t * 2048 + (fc ^ (ks * 64)));
+                for (int t = 0; t < S::NT; t++) b[h][t] = B_::read(pb, lane, tb + t, h);
 #pragma unroll
-                for (int t = 0; t < S::MT; t++) a[ks][t] = *reinterpret_cast<const typename F::V *>(pa + t * 2048 + (fc ^ (ks * 64)));
+                for (int t = 0; t < S::MT; t++) a[h][t] = A_::read(pa, lane, ta + t, h);
                 if (!Op::split)
 #pragma unroll
                     for (int mt = 0; mt < S::MT; mt++)
 #pragma unroll
-                        for (int nt = 0; nt < S::NT; nt++) acc[mt][nt] = F::mfma(a[ks][mt], b[ks][nt], acc[mt][nt]);
+                        for (int nt = 0; nt < S::NT; nt++) acc[mt][nt] = F::mfma(a[h][mt], b[h][nt], acc[mt][nt]);
             }
             if (Op::split) {
 #pragma unroll
@@ -161,17 +224,16 @@ __device__ inline void tile_of(unsigned wg, int mt, int nt, int *m, int *n)
 }
 
 // ---------------------------------------------------------------- images
+template <typename T, int N> struct __attribute__((packed)) Pack { T v[N]; };      // N elements of any alignment
+
 struct PackArgs {
     const void *src;              // [rows][cols], stride ld
     long long ld, rows, cols;
-    void *img;                    // [rows][ldi] or null
+    void *img;                    // [rows][ldi]
     long long ldi;                // padded columns (image elements)
-    void *imgt;                   // [cols][ldt] or null: the transpose
-    long long ldt;                // padded rows (image elements)
     const long long *target;      // not null: rows whose target is ignore_index are read as zero
     long long ignore;
     const float *maxpart;         // float32: kMaxParts partial maxima of the tensor
-    long long r_first;            // first row of this launch
 };
 constexpr int kMaxParts = 256;
 
@@ -216,52 +278,41 @@ __global__ __launch_bounds__(256) void absmax_kernel(PackArgs a, float *parts)
     if (threadIdx.x == 0) parts[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
 
-template <typename Op>
-__device__ inline void store_image(typename Op::Img *row, long long k, float v)
-{
-    if constexpr (Op::split) {
-        const _Float16 hi = (_Float16)v;
-        const float r = v - (float)hi;
-        const long long at = (k >> 5) * 64 + (k & 31);
-        row[at] = hi;
-        row[at + 32] = fabsf((float)hi) < INFINITY ? (_Float16)r : (_Float16)0.f;
-    } else {
-        row[k] = (typename Op::Img)v;
-    }
-}
-
-// 64 x 64 elements per workgroup: the image of the rows and / or of their transpose, zeros in the padding
+// The image of a matrix, zeros in the padding: a thread eight columns of a row.
 template <typename Op>
 __global__ __launch_bounds__(256) void pack_kernel(PackArgs a)
 {
-    __shared__ float tile[64][65];
-    const long long c0 = (long long)blockIdx.x * 64, r0 = a.r_first + (long long)blockIdx.y * 64;
-    const typename Op::In *src = static_cast<const typename Op::In *>(a.src);
+    constexpr int per = Op::split ? 2 : 1;
     const float scale = Op::split ? split_scale(max_of_parts(a.maxpart)) : 1.f;
-    const int tid = threadIdx.x;
+    const long long row_chunks = a.ldi / (8 * per), total = a.rows * row_chunks;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const long long r = i / row_chunks, c = (i - r * row_chunks) * 8;
+        const typename Op::In *p = static_cast<const typename Op::In *>(a.src) + r * a.ld + c;
+        const bool skip = a.target && a.target[r] == a.ignore;
+        typename Op::In v[8];
+        if (!skip && c + 8 <= a.cols) {
+            *reinterpret_cast<Pack<typename Op::In, 8> *>(v) = *reinterpret_cast<const Pack<typename Op::In, 8> *>(p);
+        } else {
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const int r = i * 4 + (tid >> 6), c = tid & 63;
-        float v = 0.f;
-        if (r0 + r < a.rows && c0 + c < a.cols && !(a.target && a.target[r0 + r] == a.ignore)) v = (float)src[(r0 + r) * a.ld + c0 + c] * scale;
-        tile[r][c] = v;
-    }
-    __syncthreads();
-    const int per = Op::split ? 2 : 1;
-    if (a.img) {
-        typename Op::Img *img = static_cast<typename Op::Img *>(a.img);
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const int r = i * 4 + (tid >> 6), c = tid & 63;
-            if (r0 + r < a.rows && (c0 + c) * per < a.ldi) store_image<Op>(img + (r0 + r) * a.ldi, c0 + c, tile[r][c]);
+            for (int q = 0; q < 8; q++) {
+                v[q] = (typename Op::In)0.f;
+                if (!skip && c + q < a.cols) v[q] = p[q];
+            }
         }
-    }
-    if (a.imgt) {
-        typename Op::Img *img = static_cast<typename Op::Img *>(a.imgt);
+        typename Op::Img *o = static_cast<typename Op::Img *>(a.img) + r * a.ldi;
+        if constexpr (Op::split) {
+            hx8 hi, lo;
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const int c = i * 4 + (tid >> 6), r = tid & 63;
-            if (c0 + c < a.cols && (r0 + r) * per < a.ldt) store_image<Op>(img + (c0 + c) * a.ldt, r0 + r, tile[r][c]);
+            for (int q = 0; q < 8; q++) {
+                const float x = v[q] * scale;
+                hi[q] = (_Float16)x;
+                lo[q] = fabsf((float)hi[q]) < INFINITY ? (_Float16)(x - (float)hi[q]) : (_Float16)0.f;
+            }
+            o += (c >> 5) * 64 + (c & 31);
+            *reinterpret_cast<hx8 *>(o) = hi;
+            *reinterpret_cast<hx8 *>(o + 32) = lo;
+        } else {
+            *reinterpret_cast<Pack<typename Op::In, 8> *>(o + c) = *reinterpret_cast<const Pack<typename Op::In, 8> *>(v);
         }
     }
 }
@@ -269,7 +320,6 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a)
 // ---------------------------------------------------------------- logits: statistics or gradient
 struct CeArgs {
     Operand w, x;                 // classes (of this piece) x k, rows x k
-    long long kvalid;
     int ktiles, mtiles, ntiles;
     long long n, classes, v0;     // classes of this piece; v0 = first class of the piece
     const void *bias;             // this piece's, operand type, or null
@@ -278,20 +328,23 @@ struct CeArgs {
     long long ignore;
     const float *probs;           // [n][ldp], already offset to the piece's first class
     long long ldp;
-    // statistics
-    float2 *part;                 // [tiles of classes][n]: maximum, sum of exp(l - maximum)
-    float *part_e;                // [tiles of classes][n]: sum of exp(l - maximum) l, or null
+    // statistics, one entry a row and a wave's run of TM / WM classes ("span")
+    float2 *part;                 // [spans][n]: maximum, sum of exp(l - maximum)
+    float *part_e;                // [spans][n]: sum of exp(l - maximum) l, or null
     float4 *part_t;               // probabilities: sum pi l, sum pi, sum |pi|, -
     float *tlogit;                // index: [n]
     // gradient
     const float4 *stats;          // [n]: m, sum pi / s, ... (RowArgs)
     const float *rowg;            // [n]
-    void *d, *dt;                 // images of D [n][ldd] and of its transpose [classes][ldt]
-    long long ldd, ldt;
+    void *d;                      // image [n][ldd] of D; statistics: of exp(l - the span's maximum), or null
+    long long ldd;
     float *dbpart;                // [ntiles][classes] or null
 };
 
-template <typename T> __device__ inline float as_float(T v) { return (float)v; }
+// exp(l - the span's maximum) on its way to becoming D in the same place: half precision (11 bits; what lies below 2^-24 of
+// the span's largest probability is off by 2^-25 of that) where D will be 16 bits, float32 where D will be two halves
+template <typename Op> struct Expo { using T = _Float16; };
+template <> struct Expo<OpF32> { using T = float; };
 
 template <typename Op, int TM, int TN, int WM, int WN, bool GRAD>
 __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
@@ -306,7 +359,7 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
     for (int i = 0; i < S::MT; i++)
 #pragma unroll
         for (int j = 0; j < S::NT; j++) acc[i][j] = fx4{0.f, 0.f, 0.f, 0.f};
-    TileProduct<Op, TM, TN, WM, WN>::run(acc, a.w, m0, a.x, n0, a.kvalid, 0, a.ktiles, lds);
+    TileProduct<Op, TM, TN, WM, WN, false, false>::run(acc, a.w, m0, a.x, n0, 0, a.ktiles, a.ktiles, lds);
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
     const float ux = Op::split ? 1.f / split_scale(max_of_parts(a.xmax)) : 1.f, uw = Op::split ? 1.f / split_scale(max_of_parts(a.wmax)) : 1.f;
@@ -322,13 +375,14 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
             for (int nt = 0; nt < S::NT; nt++) acc[mt][nt][i] = v < a.classes ? acc[mt][nt][i] * ux * uw + b : -INFINITY;
         }
     const long long nw = n0 + wn * (TN / WN) + (lane & 15);
+    const long long dpad = Op::split ? a.ldd / 2 : a.ldd;
     if constexpr (!GRAD) {
-        // per row: maximum and sum over this tile's classes; lanes 16 and 32 apart, then the WM waves, share a row
-        constexpr int kCol = TN;
-        float *sm = reinterpret_cast<float *>(lds);                             // [WM][6][TN]; the stages are done with
+        // per row: maximum and sum over the span; lanes 16 and 32 apart share a row
+        using E = typename Expo<Op>::T;
 #pragma unroll
         for (int nt = 0; nt < S::NT; nt++) {
             const long long row = nw + nt * 16;
+            const bool live = row < a.n;
             float mx = -INFINITY;
 #pragma unroll
             for (int mt = 0; mt < S::MT; mt++)
@@ -340,14 +394,18 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
             const float base = mx == -INFINITY ? 0.f : mx;
             float s = 0.f, e = 0.f, tl = 0.f, ts = 0.f, ta = 0.f;
 #pragma unroll
-            for (int mt = 0; mt < S::MT; mt++)
+            for (int mt = 0; mt < S::MT; mt++) {
+                Pack<E, 4> keep;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const float l = acc[mt][nt][i], x = __builtin_amdgcn_exp2f((l - base) * kLog2e);
                     s += x;
                     if (a.part_e) e += x != 0.f ? x * l : 0.f;
+                    keep.v[i] = (E)x;
                 }
-            if (a.probs && row < a.n) {
+                if (a.d && live && vw + mt * 16 < dpad) *reinterpret_cast<Pack<E, 4> *>(static_cast<E *>(a.d) + row * dpad + vw + mt * 16) = keep;
+            }
+            if (a.probs && live) {
                 const float *pr = a.probs + row * a.ldp;
 #pragma unroll
                 for (int mt = 0; mt < S::MT; mt++)
@@ -361,7 +419,7 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
                         }
                     }
             }
-            if (a.target && row < a.n) {
+            if (a.target && live) {
                 const long long t = a.target[row] - a.v0 - vw;
                 if (t >= 0 && t < TM)
 #pragma unroll
@@ -370,39 +428,20 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
                         for (int i = 0; i < 4; i++)
                             if (t == mt * 16 + i && vw + t < a.classes) a.tlogit[row] = acc[mt][nt][i];
             }
-            const int col = wn * (TN / WN) + nt * 16 + (lane & 15);
 #define AZG_PAIR(v) v += __shfl_xor(v, 16, 64); v += __shfl_xor(v, 32, 64)
             AZG_PAIR(s);
             if (a.part_e) { AZG_PAIR(e); }
             if (a.probs) { AZG_PAIR(tl); AZG_PAIR(ts); AZG_PAIR(ta); }
 #undef AZG_PAIR
-            if (lane < 16) {
-                float *q = sm + (wm * 6) * kCol + col;
-                q[0] = mx; q[kCol] = s; q[2 * kCol] = e; q[3 * kCol] = tl; q[4 * kCol] = ts; q[5 * kCol] = ta;
+            if (lane < 16 && live) {
+                const long long at = ((long long)tm * WM + wm) * a.n + row;
+                a.part[at] = make_float2(mx, s);
+                if (a.part_e) a.part_e[at] = e;
+                if (a.probs) a.part_t[at] = make_float4(tl, ts, ta, 0.f);
             }
-        }
-        __syncthreads();
-        for (int col = tid; col < TN; col += S::threads) {
-            const long long row = n0 + col;
-            if (row >= a.n) continue;
-            float mx = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < WM; w++) mx = fmaxf(mx, sm[w * 6 * kCol + col]);
-            float s = 0.f, e = 0.f, tl = 0.f, ts = 0.f, ta = 0.f;
-#pragma unroll
-            for (int w = 0; w < WM; w++) {
-                const float *q = sm + w * 6 * kCol + col;
-                const float f = q[0] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((q[0] - mx) * kLog2e);
-                s += q[kCol] * f; e += q[2 * kCol] * f; tl += q[3 * kCol]; ts += q[4 * kCol]; ta += q[5 * kCol];
-            }
-            const long long at = (long long)tm * a.n + row;
-            a.part[at] = make_float2(mx, s);
-            if (a.part_e) a.part_e[at] = e;
-            if (a.probs) a.part_t[at] = make_float4(tl, ts, ta, 0.f);
         }
     } else {
-        typename Op::Img *d = static_cast<typename Op::Img *>(a.d), *dt = static_cast<typename Op::Img *>(a.dt);
-        const long long dpad = Op::split ? a.ldd / 2 : a.ldd, tpad = Op::split ? a.ldt / 2 : a.ldt;
+        typename Op::Img *d = static_cast<typename Op::Img *>(a.d);
         float db[S::MT][4];
 #pragma unroll
         for (int mt = 0; mt < S::MT; mt++)
@@ -418,57 +457,28 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
             const float *pr = a.probs ? a.probs + row * a.ldp : nullptr;
 #pragma unroll
             for (int mt = 0; mt < S::MT; mt++) {
-                float v[4];
+                Pack<typename Op::Img, 4> h, l;
+                const long long cls = vw + mt * 16;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const long long cls = vw + mt * 16 + i;
                     float q = __builtin_amdgcn_exp2f((acc[mt][nt][i] - st.x) * kLog2e) * st.y;
-                    if (pr) { if (live && cls < a.classes) q -= pr[cls]; }
+                    if (pr) { if (live && cls + i < a.classes) q -= pr[cls + i]; }
                     else if (t == mt * 16 + i) q -= 1.f;
-                    v[i] = g == 0.f || cls >= a.classes ? 0.f : q * g;          // a row that counts for nothing: zero whatever it holds
-                    db[mt][i] += v[i];
-                    v[i] *= kDScale;
+                    q = g == 0.f || cls + i >= a.classes ? 0.f : q * g;         // a row that counts for nothing: zero whatever it holds
+                    db[mt][i] += q;
+                    q *= kDScale;
+                    h.v[i] = (typename Op::Img)q;
+                    if (Op::split) l.v[i] = (typename Op::Img)(q - (float)h.v[i]);
                 }
-                // D: four classes of one row;  D^T: a 4 x 4 transpose among four neighbouring lanes, then four rows of one class
-                const long long cls = vw + mt * 16;
-                if (a.d && live && cls < dpad) {
-                    typename Op::Img h[4], l[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        h[i] = (typename Op::Img)v[i];
-                        if (Op::split) l[i] = (typename Op::Img)(v[i] - (float)h[i]);
-                    }
+                if (d && live && cls < dpad) {
                     typename Op::Img *o = d + row * a.ldd + (Op::split ? (cls >> 5) * 64 + (cls & 31) : cls);
-                    *reinterpret_cast<uint64_t *>(o) = *reinterpret_cast<uint64_t *>(h);
-                    if (Op::split) *reinterpret_cast<uint64_t *>(o + 32) = *reinterpret_cast<uint64_t *>(l);
-                }
-                if (a.dt) {
-                    const bool b0 = lane & 1, b1 = lane & 2;
-                    float w[4];
-                    {
-                        const float r01 = __shfl_xor(b0 ? v[0] : v[1], 1, 64), r23 = __shfl_xor(b0 ? v[2] : v[3], 1, 64);
-                        const float x0 = b0 ? r01 : v[0], x1 = b0 ? v[1] : r01, y0 = b0 ? r23 : v[2], y1 = b0 ? v[3] : r23;
-                        // even lanes: classes 0, 2 of rows (t, t+1); odd lanes: classes 1, 3
-                        const float p0 = __shfl_xor(b1 ? x0 : y0, 2, 64), p1 = __shfl_xor(b1 ? x1 : y1, 2, 64);
-                        w[0] = b1 ? p0 : x0; w[1] = b1 ? p1 : x1; w[2] = b1 ? y0 : p0; w[3] = b1 ? y1 : p1;
-                    }
-                    const long long c = cls + (lane & 3), r4 = row - (lane & 3);
-                    if (c < a.classes && r4 < tpad) {
-                        typename Op::Img h[4], l[4];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            h[i] = (typename Op::Img)w[i];
-                            if (Op::split) l[i] = (typename Op::Img)(w[i] - (float)h[i]);
-                        }
-                        typename Op::Img *o = dt + c * a.ldt + (Op::split ? (r4 >> 5) * 64 + (r4 & 31) : r4);
-                        *reinterpret_cast<uint64_t *>(o) = *reinterpret_cast<uint64_t *>(h);
-                        if (Op::split) *reinterpret_cast<uint64_t *>(o + 32) = *reinterpret_cast<uint64_t *>(l);
-                    }
+                    *reinterpret_cast<Pack<typename Op::Img, 4> *>(o) = h;
+                    if (Op::split) *reinterpret_cast<Pack<typename Op::Img, 4> *>(o + 32) = l;
                 }
             }
         }
         if (a.dbpart) {
-            float *sm = reinterpret_cast<float *>(lds);                         // [WN][TM]
+            float *sm = reinterpret_cast<float *>(lds);                         // [WN][TM]; the stages are done with
 #pragma unroll
             for (int mt = 0; mt < S::MT; mt++)
 #pragma unroll
@@ -489,23 +499,93 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
     }
 }
 
+// ---------------------------------------------------------------- exponentials -> D, in place
+constexpr int kFixRows = 128, kFixCols = 128;
+struct FixArgs {
+    long long n, classes, span;   // classes an entry of part stands for
+    void *d; long long ldd;
+    const float2 *part; const float4 *stats; const float *rowg;
+    const long long *target;
+    const float *probs; long long ldp;
+    float *dbpart;                // [blocks of kFixRows][classes] or null
+};
+// 128 rows x 128 classes per workgroup, sixteen threads a row with eight classes each
+template <typename Op>
+__global__ __launch_bounds__(256) void fix_kernel(FixArgs a)
+{
+    __shared__ float red[16][kFixCols + 1];
+    const int tid = threadIdx.x, rg = tid >> 4, cl = (tid & 15) * 8;
+    const long long c0 = (long long)blockIdx.x * kFixCols, r0 = (long long)blockIdx.y * kFixRows, c = c0 + cl;
+    const long long dpad = Op::split ? a.ldd / 2 : a.ldd;
+    float db[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (c < dpad)
+#pragma unroll 4
+        for (int j = 0; j < kFixRows / 16; j++) {
+            const long long row = r0 + j * 16 + rg;
+            if (row >= a.n) break;
+            const float4 st = a.stats[row];
+            const float g = a.rowg[row], mp = a.part[c / a.span * a.n + row].x;
+            const float f = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mp - st.x) * kLog2e) * st.y;
+            const long long t = a.target ? a.target[row] - c : -1;
+            float v[8];
+            if constexpr (Op::split) {
+                const fx4 *p = reinterpret_cast<const fx4 *>(static_cast<float *>(a.d) + row * dpad + c);
+                const fx4 v0 = p[0], v1 = p[1];
+#pragma unroll
+                for (int i = 0; i < 4; i++) { v[i] = v0[i]; v[4 + i] = v1[i]; }
+            } else {
+                const hx8 p = *reinterpret_cast<const hx8 *>(static_cast<_Float16 *>(a.d) + row * dpad + c);
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = (float)p[i];
+            }
+            typename Frag<typename Op::Img>::V h, l;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const bool out = c + i >= a.classes;
+                float q = v[i] * f;
+                if (a.probs) { if (!out) q -= a.probs[row * a.ldp + c + i]; }
+                else if (t == i) q -= 1.f;
+                q = g == 0.f || out ? 0.f : q * g;
+                db[i] += q;
+                q *= kDScale;
+                h[i] = (typename Op::Img)q;
+                if (Op::split) l[i] = (typename Op::Img)(q - (float)h[i]);
+            }
+            // (float32: the halves land on exponentials of the same row that other lanes of this wave have read: a wave's
+            //  stores follow the loads that every one of its values depends on)
+            typename Op::Img *o = static_cast<typename Op::Img *>(a.d) + row * a.ldd + (Op::split ? (c >> 5) * 64 + (c & 31) : c);
+            *reinterpret_cast<typename Frag<typename Op::Img>::V *>(o) = h;
+            if (Op::split) *reinterpret_cast<typename Frag<typename Op::Img>::V *>(o + 32) = l;
+        }
+    if (!a.dbpart) return;
+#pragma unroll
+    for (int i = 0; i < 8; i++) red[rg][cl + i] = db[i];
+    __syncthreads();
+    if (tid < kFixCols && c0 + tid < a.classes) {
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < 16; w++) s += red[w][tid];
+        a.dbpart[(long long)blockIdx.y * a.classes + c0 + tid] = s;
+    }
+}
+
 // ---------------------------------------------------------------- rows and totals
 struct RowArgs {
     long long n, classes;
-    int tiles;
+    int spans;
     const float2 *part; const float *part_e; const float4 *part_t; const float *tlogit;
     const long long *target; long long ignore;
     float4 *stats;                // [n]: m, sum pi / s, sum |pi|, loss with lse = m + log s (so that p takes no rounding of lse)
     float *ent;                   // [n] or null
 };
-// one wave per row: join the tiles' (maximum, sum) pairs in a fixed order
+// one wave per row: join the spans' (maximum, sum) pairs in a fixed order
 __global__ __launch_bounds__(256) void rows_kernel(RowArgs a)
 {
     const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     if (row >= a.n) return;
     float mx = -INFINITY, s = 0.f, e = 0.f, tl = 0.f, ts = 0.f, ta = 0.f;
-    for (int t = lane; t < a.tiles; t += 64) {
+    for (int t = lane; t < a.spans; t += 64) {
         const float2 p = a.part[(long long)t * a.n + row];
         const float m = fmaxf(mx, p.x), base = m == -INFINITY ? 0.f : m;
         const float f0 = __builtin_amdgcn_exp2f((mx - base) * kLog2e), f1 = __builtin_amdgcn_exp2f((p.x - base) * kLog2e);
@@ -613,20 +693,17 @@ __global__ __launch_bounds__(1024) void totals_kernel(TotalArgs a)
 // ---------------------------------------------------------------- the gradients' products
 struct GradArgs {
     Operand a, b;                 // a: the output's contiguous dimension, b: its rows
-    long long kvalid;
     int ktiles, mtiles, ntiles, kper;   // stages per split
     long long m, n;
     void *out; long long ldo;     // [n][ldo], operand type (one split), or
     float *acc;                   // float32 [splits][n][m]
     bool add;                     // one split: add to acc instead of starting it
-    bool vec;                     // out can be stored four elements at a time
     const float *amax;            // float32: partial maxima of the operand that is not D
     const float *factor;
 };
 
-template <typename T, int N> struct __attribute__((packed)) Pack { T v[N]; };
-
-template <typename Op, int TM, int TN, int WM, int WN>
+// dX: TB false (D as it lies), dW: TB true (D transposed); the other factor, W or X, is transposed in both
+template <typename Op, int TM, int TN, int WM, int WN, bool TB>
 __global__ __launch_bounds__(WM * WN * 64) void grad_kernel(GradArgs a)
 {
     using S = TileShape<TM, TN, WM, WN>;
@@ -640,7 +717,7 @@ __global__ __launch_bounds__(WM * WN * 64) void grad_kernel(GradArgs a)
     for (int i = 0; i < S::MT; i++)
 #pragma unroll
         for (int j = 0; j < S::NT; j++) acc[i][j] = fx4{0.f, 0.f, 0.f, 0.f};
-    TileProduct<Op, TM, TN, WM, WN>::run(acc, a.a, m0, a.b, n0, a.kvalid, k0, k1, lds);
+    TileProduct<Op, TM, TN, WM, WN, true, TB>::run(acc, a.a, m0, a.b, n0, k0, k1, a.ktiles, lds);
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
     float f = *a.factor / kDScale;
@@ -662,7 +739,7 @@ __global__ __launch_bounds__(WM * WN * 64) void grad_kernel(GradArgs a)
                     if (m + i < a.m) o[i] = a.add ? o[i] + v[i] : v[i];
             } else {
                 typename Op::In *o = static_cast<typename Op::In *>(a.out) + n * a.ldo + m;
-                if (a.vec && m + 4 <= a.m) {
+                if (m + 4 <= a.m) {
                     Pack<typename Op::In, 4> q;
 #pragma unroll
                     for (int i = 0; i < 4; i++) q.v[i] = (typename Op::In)(v[i] * f);

@@ -103,8 +103,8 @@ struct Take {                                                 // offsets into th
 };
 
 enum Shape { T256, T128, T64, TROW };
-struct ShapeDim { int tm, tn; };
-constexpr ShapeDim kDims[4] = {{256, 256}, {128, 128}, {64, 64}, {128, 16}};
+struct ShapeDim { int tm, tn, wm; };
+constexpr ShapeDim kDims[4] = {{256, 256, 2}, {128, 128, 2}, {64, 64, 2}, {128, 16, 4}};
 
 long long tiles_of(Shape s, long long m, long long n) { return ((m + kDims[s].tm - 1) / kDims[s].tm) * ((n + kDims[s].tn - 1) / kDims[s].tn); }
 
@@ -131,14 +131,13 @@ GradPick pick_grad(long long m, long long n, long long ktiles)
 }
 
 struct Plan {
-    bool split, forward, backward, pack_w, pack_x;
-    int isz;                                                  // bytes of an image element
+    bool split, forward, backward, pack_w, pack_x, keep;      // keep: the forward pass leaves exponentials for the backward pass
     long long n, H, V, vp, pieces;
-    long long kimg, ldx, ldw;                                 // image elements along the features
-    long long ldd, ldt;                                       // images of D and of its transpose, elements
+    long long kimg, ldd;                                      // image elements along the features, along a piece's classes
+    int per, ks;                                              // image elements an element takes, k of a stage
     Shape lshape;
     GradPick gx, gw;
-    size_t xmax, wmax, ximg, xt, wimg, wt, part, part_e, part_t, tlogit, stats, ent, rowg, factor, d, dt, dbpart, dxacc, dwacc, total;
+    size_t xmax, wmax, ximg, wimg, part, part_e, part_t, tlogit, stats, ent, rowg, factor, d, dbpart, dxacc, dwacc, total;
 };
 
 bool aligned16(const void *p, long long stride, long long cols, long long rows)
@@ -149,18 +148,18 @@ bool aligned16(const void *p, long long stride, long long cols, long long rows)
 int make_plan(const azg_linear_ce_args *a, Plan *p)
 {
     p->split = a->dtype == AZG_F32;
-    p->isz = 2;
+    p->per = p->split ? 2 : 1;
+    p->ks = p->split ? 32 : 64;
     p->forward = a->loss != nullptr;
     p->backward = a->dx || a->dw || a->db;
     p->n = a->n; p->H = a->hidden; p->V = a->classes;
-    p->kimg = p->split ? up_to(p->H, 32) * 2 : up_to(p->H, 64);
-    p->pack_x = p->split || !aligned16(a->x, a->x_stride, a->hidden, a->n);
+    p->kimg = up_to(p->H, p->ks) * p->per;
+    // (dW multiplies the rows that count for nothing by zero: they are copied as zeros, whatever they hold)
+    p->pack_x = p->split || !aligned16(a->x, a->x_stride, a->hidden, a->n) || (a->dw && a->target);
     p->pack_w = p->split || !aligned16(a->w, a->w_stride, a->hidden, a->classes);
-    const long long np = p->split ? up_to(p->n, 32) * 2 : up_to(p->n, 64);
-    const long long per = (p->split ? 2 : 1);
     // bytes a class of a piece costs
     long long cost = p->pack_w ? p->kimg * 2 : 0;
-    if (p->backward) cost += p->n * per * 2 + np * 2 + (a->dx ? p->H * per * 2 : 0);
+    if (p->backward) cost += p->n * p->per * 2;
     p->vp = p->V;
     if (cost) p->vp = std::min<long long>(p->V, std::max<long long>(1024, kPieceBytes / cost / 256 * 256));
     p->pieces = (p->V + p->vp - 1) / p->vp;
@@ -168,36 +167,34 @@ int make_plan(const azg_linear_ce_args *a, Plan *p)
         p->vp = std::min<long long>(p->V, up_to((p->V + p->pieces - 1) / p->pieces, 256));
         p->pieces = (p->V + p->vp - 1) / p->vp;
     }
-    p->ldd = p->split ? up_to(p->vp, 32) * 2 : up_to(p->vp, 64);
-    p->ldt = np;
+    p->keep = p->forward && p->backward && p->pieces == 1;
+    p->ldd = up_to(p->vp, p->ks) * p->per;
     p->lshape = pick_logits(p->vp, p->n, p->backward);
-    if (p->lshape == TROW && p->backward) p->lshape = T64;
-    p->gx = pick_grad(p->H, p->n, (p->ldd + 63) / 64);
-    p->gw = pick_grad(p->H, p->vp, (p->ldt + 63) / 64);
-    const long long ltiles_m = (p->vp + kDims[p->lshape].tm - 1) / kDims[p->lshape].tm, ltiles_n = (p->n + kDims[p->lshape].tn - 1) / kDims[p->lshape].tn;
-    if (ltiles_m * ltiles_n > INT_MAX / 2 || tiles_of(p->gx.shape, p->H, p->n) > INT_MAX / 2 || tiles_of(p->gw.shape, p->H, p->vp) > INT_MAX / 2)
+    p->gx = pick_grad(p->H, p->n, (p->vp + p->ks - 1) / p->ks);
+    p->gw = pick_grad(p->H, p->vp, (p->n + p->ks - 1) / p->ks);
+    const ShapeDim dim = kDims[p->lshape];
+    const long long lm = (p->vp + dim.tm - 1) / dim.tm, ln = (p->n + dim.tn - 1) / dim.tn;
+    if (lm * ln > INT_MAX / 2 || tiles_of(p->gx.shape, p->H, p->n) > INT_MAX / 2 || tiles_of(p->gw.shape, p->H, p->vp) > INT_MAX / 2 ||
+        (p->n + kFixRows - 1) / kFixRows > 65535)
         return fail(AZG_EINVAL, "azg_linear_ce: the problem is too large");
     Take t;
     p->xmax = t(p->split ? kMaxParts * 4 : 0);
     p->wmax = t(p->split ? kMaxParts * 4 : 0);
     p->ximg = t(p->pack_x ? (size_t)p->n * p->kimg * 2 : 0);
-    p->xt = t(p->backward && a->dw ? (size_t)p->H * p->ldt * 2 : 0);
     p->wimg = t(p->pack_w ? (size_t)p->vp * p->kimg * 2 : 0);
-    p->wt = t(p->backward && a->dx ? (size_t)p->H * p->ldd * 2 : 0);
-    const long long ptiles = p->pieces * ltiles_m;
-    p->part = t(p->forward ? (size_t)ptiles * p->n * 8 : 0);
-    p->part_e = t(p->forward && a->entropy ? (size_t)ptiles * p->n * 4 : 0);
-    p->part_t = t(p->forward && a->probs ? (size_t)ptiles * p->n * 16 : 0);
+    const size_t entries = (size_t)p->pieces * lm * dim.wm * p->n;
+    p->part = t(p->forward ? entries * 8 : 0);
+    p->part_e = t(p->forward && a->entropy ? entries * 4 : 0);
+    p->part_t = t(p->forward && a->probs ? entries * 16 : 0);
     p->tlogit = t((size_t)p->n * 4);
     p->stats = t((size_t)p->n * 16);
     p->ent = t((size_t)p->n * 4);
     p->rowg = t((size_t)p->n * 4);
     p->factor = t(4);
-    p->d = t(p->backward && a->dx ? (size_t)p->n * p->ldd * 2 : 0);
-    p->dt = t(p->backward && a->dw ? (size_t)p->vp * p->ldt * 2 : 0);
-    p->dbpart = t(p->backward && a->db ? (size_t)ltiles_n * p->vp * 4 : 0);
-    p->dxacc = t(p->backward && a->dx && (p->gx.splits > 1 || p->pieces > 1) ? (size_t)p->gx.splits * p->n * p->H * 4 : 0);
-    p->dwacc = t(p->backward && a->dw && p->gw.splits > 1 ? (size_t)p->gw.splits * p->vp * p->H * 4 : 0);
+    p->d = t(p->backward ? (size_t)p->n * p->ldd * 2 : 0);
+    p->dbpart = t(a->db ? (size_t)std::max(ln, (p->n + kFixRows - 1) / kFixRows) * p->vp * 4 : 0);
+    p->dxacc = t(a->dx && (p->gx.splits > 1 || p->pieces > 1) ? (size_t)p->gx.splits * p->n * p->H * 4 : 0);
+    p->dwacc = t(a->dw && p->gw.splits > 1 ? (size_t)p->gw.splits * p->vp * p->H * 4 : 0);
     p->total = t.off;
     return AZG_OK;
 }
@@ -226,7 +223,7 @@ int launch_logits_shape(CeArgs c, hipStream_t s)
     using S = TileShape<TM, TN, WM, WN>;
     c.mtiles = (int)((c.classes + TM - 1) / TM);
     c.ntiles = (int)((c.n + TN - 1) / TN);
-    const int lds = std::max(S::lds_bytes, WM * 6 * TN * 4);
+    const int lds = S::lds_bytes;
     OPS_TRY(allow_lds(logits_kernel<Op, TM, TN, WM, WN, GRAD>, lds));
     hipLaunchKernelGGL((logits_kernel<Op, TM, TN, WM, WN, GRAD>), dim3((unsigned)c.mtiles * c.ntiles), dim3(S::threads), lds, s, c);
     OPS_HIP(hipGetLastError());
@@ -245,25 +242,25 @@ int launch_logits(Shape shape, const CeArgs &c, hipStream_t s)
     }
 }
 
-template <typename Op, int TM, int TN, int WM, int WN>
+template <typename Op, int TM, int TN, int WM, int WN, bool TB>
 int launch_grad_shape(GradArgs g, int splits, hipStream_t s)
 {
     using S = TileShape<TM, TN, WM, WN>;
     g.mtiles = (int)((g.m + TM - 1) / TM);
     g.ntiles = (int)((g.n + TN - 1) / TN);
-    OPS_TRY(allow_lds(grad_kernel<Op, TM, TN, WM, WN>, S::lds_bytes));
-    hipLaunchKernelGGL((grad_kernel<Op, TM, TN, WM, WN>), dim3((unsigned)g.mtiles * g.ntiles, splits), dim3(S::threads), S::lds_bytes, s, g);
+    OPS_TRY(allow_lds(grad_kernel<Op, TM, TN, WM, WN, TB>, S::lds_bytes));
+    hipLaunchKernelGGL((grad_kernel<Op, TM, TN, WM, WN, TB>), dim3((unsigned)g.mtiles * g.ntiles, splits), dim3(S::threads), S::lds_bytes, s, g);
     OPS_HIP(hipGetLastError());
     return AZG_OK;
 }
-template <typename Op>
+template <typename Op, bool TB>
 int launch_grad(const GradPick &pick, GradArgs g, hipStream_t s)
 {
     g.kper = pick.kper;
     switch (pick.shape) {
-    case T256: return launch_grad_shape<Op, 256, 256, 2, 4>(g, pick.splits, s);
-    case T128: return launch_grad_shape<Op, 128, 128, 2, 2>(g, pick.splits, s);
-    default: return launch_grad_shape<Op, 64, 64, 2, 2>(g, pick.splits, s);
+    case T256: return launch_grad_shape<Op, 256, 256, 2, 4, TB>(g, pick.splits, s);
+    case T128: return launch_grad_shape<Op, 128, 128, 2, 2, TB>(g, pick.splits, s);
+    default: return launch_grad_shape<Op, 64, 64, 2, 2, TB>(g, pick.splits, s);
     }
 }
 template <typename Op>
@@ -277,15 +274,8 @@ int launch_join(const JoinArgs &j, hipStream_t s)
 template <typename Op>
 int launch_pack(const PackArgs &p, hipStream_t s)
 {
-    // (the padding of an image of the rows may reach into one more block of columns than the tensor has, and likewise)
-    const int per = Op::split ? 2 : 1;
-    const long long cols = std::max(p.cols, p.img ? p.ldi / per : 0), rows = std::max(p.rows, p.imgt ? p.ldt / per : 0);
-    const long long gx = (cols + 63) / 64, gy = (rows + 63) / 64;
-    for (long long y = 0; y < gy; y += 32768) {               // a grid has at most 65535 rows of workgroups
-        PackArgs q = p;
-        q.r_first = y * 64;
-        hipLaunchKernelGGL((pack_kernel<Op>), dim3((unsigned)gx, (unsigned)std::min<long long>(32768, gy - y)), dim3(256), 0, s, q);
-    }
+    const long long chunks = p.rows * (p.ldi / (Op::split ? 16 : 8));
+    hipLaunchKernelGGL((pack_kernel<Op>), dim3((unsigned)std::min<long long>((chunks + 255) / 256, 1 << 16)), dim3(256), 0, s, p);
     OPS_HIP(hipGetLastError());
     return AZG_OK;
 }
@@ -300,55 +290,51 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
     const long long *target = reinterpret_cast<const long long *>(a->target);
     float4 *stats = a->stats ? static_cast<float4 *>(a->stats) : reinterpret_cast<float4 *>(ws + p.stats);
     const In *W = static_cast<const In *>(a->w);
+    const ShapeDim dim = kDims[p.lshape];
 
-    // images of the rows
     PackArgs px{};
-    px.src = a->x; px.ld = a->x_stride; px.rows = a->n; px.cols = a->hidden; px.target = target; px.ignore = a->ignore_index; px.maxpart = f32(p.xmax);
-    px.img = p.pack_x ? ws + p.ximg : nullptr; px.ldi = p.kimg;
-    px.imgt = p.backward && a->dw ? ws + p.xt : nullptr; px.ldt = p.ldt;
+    px.src = a->x; px.ld = a->x_stride; px.rows = a->n; px.cols = a->hidden; px.target = target; px.ignore = a->ignore_index;
+    px.maxpart = f32(p.xmax); px.img = ws + p.ximg; px.ldi = p.kimg;
+    PackArgs pw{};
+    pw.src = W; pw.ld = a->w_stride; pw.rows = a->classes; pw.cols = a->hidden; pw.maxpart = f32(p.wmax); pw.img = ws + p.wimg; pw.ldi = p.kimg;
     if (Op::split) {
-        PackArgs pm = px;
-        hipLaunchKernelGGL(absmax_kernel, dim3(kMaxParts), dim3(256), 0, s, pm, f32(p.xmax));
-        pm.src = a->w; pm.ld = a->w_stride; pm.rows = a->classes; pm.target = nullptr;
-        hipLaunchKernelGGL(absmax_kernel, dim3(kMaxParts), dim3(256), 0, s, pm, f32(p.wmax));
+        hipLaunchKernelGGL(absmax_kernel, dim3(kMaxParts), dim3(256), 0, s, px, f32(p.xmax));
+        hipLaunchKernelGGL(absmax_kernel, dim3(kMaxParts), dim3(256), 0, s, pw, f32(p.wmax));
     }
-    if (px.img || px.imgt) OPS_TRY(launch_pack<Op>(px, s));
+    if (p.pack_x) OPS_TRY(launch_pack<Op>(px, s));
     CeArgs c{};
-    c.x = p.pack_x ? Operand{ws + p.ximg, p.kimg, a->n} : Operand{a->x, a->x_stride, a->n};
-    c.kvalid = p.pack_x && p.pack_w ? p.kimg : a->hidden;   // (a direct operand has a multiple of 8 features)
-    c.ktiles = (int)((p.kimg + 63) / 64);
+    c.x = p.pack_x ? Operand{ws + p.ximg, p.kimg, a->n, p.kimg} : Operand{a->x, a->x_stride, a->n, a->hidden};
+    c.ktiles = (int)((p.H + p.ks - 1) / p.ks);
     c.n = a->n; c.target = target; c.ignore = a->ignore_index; c.ldp = a->probs_stride;
     c.xmax = f32(p.xmax); c.wmax = f32(p.wmax);
 
-    auto piece = [&](long long i, bool want_t, bool want_img) -> int {
+    auto piece = [&](long long i, bool pack) -> int {
         const long long v0 = i * p.vp, vn = std::min(p.vp, a->classes - v0);
         c.v0 = v0; c.classes = vn;
         c.bias = a->bias ? static_cast<const In *>(a->bias) + v0 : nullptr;
         c.probs = a->probs ? a->probs + v0 : nullptr;
-        PackArgs pw{};
-        pw.src = W + v0 * a->w_stride; pw.ld = a->w_stride; pw.rows = vn; pw.cols = a->hidden; pw.maxpart = f32(p.wmax);
-        pw.img = p.pack_w && want_img ? ws + p.wimg : nullptr; pw.ldi = p.kimg;
-        pw.imgt = want_t ? ws + p.wt : nullptr; pw.ldt = Op::split ? up_to(vn, 32) * 2 : up_to(vn, 64);
-        if (pw.img || pw.imgt) OPS_TRY(launch_pack<Op>(pw, s));
-        c.w = p.pack_w ? Operand{ws + p.wimg, p.kimg, vn} : Operand{W + v0 * a->w_stride, a->w_stride, vn};
+        c.ldd = up_to(vn, p.ks) * p.per;
+        pw.src = W + v0 * a->w_stride; pw.rows = vn;
+        if (p.pack_w && pack) OPS_TRY(launch_pack<Op>(pw, s));
+        c.w = p.pack_w ? Operand{ws + p.wimg, p.kimg, vn, p.kimg} : Operand{W + v0 * a->w_stride, a->w_stride, vn, a->hidden};
         return AZG_OK;
     };
 
-    const ShapeDim dim = kDims[p.lshape];
     if (p.forward) {
-        const long long full = (p.vp + dim.tm - 1) / dim.tm;
-        long long tiles = 0;
+        const long long full = (p.vp + dim.tm - 1) / dim.tm * dim.wm;           // spans of a whole piece
+        long long spans = 0;
         for (long long i = 0; i < p.pieces; i++) {
-            OPS_TRY(piece(i, p.backward && a->dx && p.pieces == 1, true));
+            OPS_TRY(piece(i, true));
             c.part = reinterpret_cast<float2 *>(ws + p.part) + i * full * a->n;
             c.part_e = a->entropy ? f32(p.part_e) + i * full * a->n : nullptr;
             c.part_t = a->probs ? reinterpret_cast<float4 *>(ws + p.part_t) + i * full * a->n : nullptr;
             c.tlogit = f32(p.tlogit);
+            c.d = p.keep ? ws + p.d : nullptr;
             OPS_TRY((launch_logits<Op, false>(p.lshape, c, s)));
-            tiles += (c.classes + dim.tm - 1) / dim.tm;
+            spans += (c.classes + dim.tm - 1) / dim.tm * dim.wm;
         }
         RowArgs r{};
-        r.n = a->n; r.classes = a->classes; r.tiles = (int)tiles;
+        r.n = a->n; r.classes = a->classes; r.spans = (int)spans;
         r.part = reinterpret_cast<float2 *>(ws + p.part); r.part_e = a->entropy ? f32(p.part_e) : nullptr;
         r.part_t = a->probs ? reinterpret_cast<float4 *>(ws + p.part_t) : nullptr; r.tlogit = f32(p.tlogit);
         r.target = target; r.ignore = a->ignore_index; r.stats = stats; r.ent = a->entropy ? f32(p.ent) : nullptr;
@@ -364,22 +350,33 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
     if (!p.backward) return AZG_OK;
 
     for (long long i = 0; i < p.pieces; i++) {
-        if (!(p.forward && p.pieces == 1)) OPS_TRY(piece(i, a->dx != nullptr, true));
-        const long long vn = c.classes, ldd = Op::split ? up_to(vn, 32) * 2 : up_to(vn, 64);
-        c.stats = stats; c.rowg = f32(p.rowg);
-        c.d = a->dx ? ws + p.d : nullptr; c.ldd = ldd;
-        c.dt = a->dw ? ws + p.dt : nullptr; c.ldt = p.ldt;
-        c.dbpart = a->db ? f32(p.dbpart) : nullptr;
-        OPS_TRY((launch_logits<Op, true>(p.lshape, c, s)));
+        if (!p.keep) OPS_TRY(piece(i, !(p.forward && p.pieces == 1)));
+        const long long vn = c.classes;
+        int dbparts;
+        if (p.keep) {
+            FixArgs f{};
+            f.n = a->n; f.classes = vn; f.span = dim.tm / dim.wm; f.d = ws + p.d; f.ldd = c.ldd;
+            f.part = reinterpret_cast<float2 *>(ws + p.part); f.stats = stats; f.rowg = f32(p.rowg);
+            f.target = target; f.probs = a->probs; f.ldp = a->probs_stride; f.dbpart = a->db ? f32(p.dbpart) : nullptr;
+            dbparts = (int)((a->n + kFixRows - 1) / kFixRows);
+            hipLaunchKernelGGL((fix_kernel<Op>), dim3((unsigned)((c.ldd / p.per + kFixCols - 1) / kFixCols), dbparts), dim3(256), 0, s, f);
+            OPS_HIP(hipGetLastError());
+        } else {
+            c.stats = stats; c.rowg = f32(p.rowg);
+            c.d = a->dx || a->dw ? ws + p.d : nullptr;
+            c.dbpart = a->db ? f32(p.dbpart) : nullptr;
+            dbparts = (int)((a->n + dim.tn - 1) / dim.tn);
+            OPS_TRY((launch_logits<Op, true>(p.lshape, c, s)));
+        }
         if (a->dx) {
             GradArgs g{};
-            g.a = Operand{ws + p.wt, ldd, a->hidden}; g.b = Operand{ws + p.d, ldd, a->n};
-            g.kvalid = ldd; g.ktiles = (int)(ldd / 64); g.m = a->hidden; g.n = a->n;
+            g.a = Operand{c.w.p, c.w.ld, vn, c.w.cols}; g.b = Operand{ws + p.d, c.ldd, a->n, c.ldd};
+            g.ktiles = (int)((vn + p.ks - 1) / p.ks); g.m = a->hidden; g.n = a->n;
             g.amax = f32(p.wmax); g.factor = f32(p.factor);
             const bool acc = p.gx.splits > 1 || p.pieces > 1;
             g.acc = acc ? f32(p.dxacc) : nullptr; g.add = i > 0;
-            g.out = a->dx; g.ldo = a->dx_stride; g.vec = true;
-            OPS_TRY(launch_grad<Op>(p.gx, g, s));
+            g.out = a->dx; g.ldo = a->dx_stride;
+            OPS_TRY((launch_grad<Op, false>(p.gx, g, s)));
             if (acc && i == p.pieces - 1) {
                 JoinArgs j{};
                 j.acc = f32(p.dxacc); j.splits = p.gx.splits; j.n = a->n; j.m = a->hidden; j.out = a->dx; j.ldo = a->dx_stride;
@@ -389,12 +386,12 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
         }
         if (a->dw) {
             GradArgs g{};
-            g.a = Operand{ws + p.xt, p.ldt, a->hidden}; g.b = Operand{ws + p.dt, p.ldt, vn};
-            g.kvalid = p.ldt; g.ktiles = (int)((p.ldt + 63) / 64); g.m = a->hidden; g.n = vn;
+            g.a = c.x; g.b = Operand{ws + p.d, c.ldd, a->n, c.ldd};
+            g.ktiles = (int)((a->n + p.ks - 1) / p.ks); g.m = a->hidden; g.n = vn;
             g.amax = f32(p.xmax); g.factor = f32(p.factor);
             g.acc = p.gw.splits > 1 ? f32(p.dwacc) : nullptr; g.add = false;
-            g.out = static_cast<In *>(a->dw) + i * p.vp * a->dw_stride; g.ldo = a->dw_stride; g.vec = true;
-            OPS_TRY(launch_grad<Op>(p.gw, g, s));
+            g.out = static_cast<In *>(a->dw) + i * p.vp * a->dw_stride; g.ldo = a->dw_stride;
+            OPS_TRY((launch_grad<Op, true>(p.gw, g, s)));
             if (g.acc) {
                 JoinArgs j{};
                 j.acc = g.acc; j.splits = p.gw.splits; j.n = vn; j.m = a->hidden; j.out = g.out; j.ldo = a->dw_stride;
@@ -404,7 +401,7 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
         }
         if (a->db) {
             JoinArgs j{};
-            j.acc = f32(p.dbpart); j.splits = (int)((a->n + dim.tn - 1) / dim.tn); j.n = 1; j.m = vn;
+            j.acc = f32(p.dbpart); j.splits = dbparts; j.n = 1; j.m = vn;
             j.out = static_cast<In *>(a->db) + i * p.vp; j.ldo = vn; j.factor = f32(p.factor); j.extra = 1.f;
             OPS_TRY(launch_join<Op>(j, s));
         }

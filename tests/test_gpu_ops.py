@@ -7,7 +7,9 @@ Tolerances are bounds, computed element by element from the inputs.  With u = ha
   so a logit is off by dl = ((H + 2) f + 3 * 2**-22 [float32]) sum|x w| + f |l|, a probability by p (2 max dl + 2**-20): the
   exponential, its argument (|l - m| <= 40 here: 40 f log2 e) and the reciprocal of the sum take less than 2**-20;
   the loss by 2 max dl + 8 f (|lse| + |l_t| + 2); the gradient at the logits D by its probability's part, its own rounding
-  u |D| (float32: 2**-22; half precision holds D 2**14, so 2**-39 of D's scale below its smallest normal number), and the
+  u |D| (float32: 2**-22; half precision holds D 2**14, so 2**-39 of D's scale below its smallest normal number); where
+  loss and gradients come from one call, 16-bit types keep exp(l - m') of a run of classes with maximum m' in half precision
+  meanwhile: 2**-11 of itself, or 2**-25 of exp(m' - lse) <= the row's largest probability, more; and the
   gradients by the two operands' errors, the float32 sum and the result's rounding (half precision: 2**-25 at least)."""
 import math
 
@@ -183,13 +185,15 @@ def reference(x, w, b, t, g, ignore=-100):
     qs, qa = q.sum(1), q.abs().sum(1)
     fin = torch.where(torch.isfinite(l), l.abs(), zero)
     big = lse.abs() + (q.abs() * fin).sum(1) / qa.clamp_min(1e-30) + 2
-    tiles = v / 64 + 64                                            # (sums of many classes: the tiles' sums and their joining)
     b_loss = torch.where(used, qa * (2 * dlm + (8 + math.log2(v) + 40) * F * big), zero)
     b_ent = torch.where(used, 2 * dlm * (1 + (p * fin).sum(1)) + 2.0 ** -19 * ((p * fin).sum(1) + lse.abs() + 1), zero)
     rel_p = 2 * dlm[:, None] + 2.0 ** -20
     uD = 2.0 ** -22 if f32 else half_step(dt)
     top = float((gd.abs() * qa).max()) * 2                          # the images' scale
-    bD0 = gd.abs()[:, None] * (p * qs.abs()[:, None] * rel_p + 4 * F * (p * qs.abs()[:, None] + q.abs()))
+    if not f32:
+        rel_p = rel_p + 2.0 ** -11
+    kept = 0.0 if f32 else 2.0 ** -25 * p.max(1, keepdim=True).values
+    bD0 = gd.abs()[:, None] * ((p * rel_p + kept) * qs.abs()[:, None] + 4 * F * (p * qs.abs()[:, None] + q.abs()))
     bD = bD0 + uD * D.abs() + (2.0 ** -39 * top if dt != torch.bfloat16 else 0)
     out_abs = 2.0 ** -25 if dt == torch.float16 else 0.0
     u = half_step(dt)
