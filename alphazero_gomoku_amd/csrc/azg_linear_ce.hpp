@@ -75,8 +75,6 @@ typedef const __attribute__((address_space(1))) void *glb_ptr;
 typedef short sx4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) sx4 *lds_sx4;
 
-__device__ inline void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
 // One operand of a tile: T rows of m, k contiguous (TR false) or across the rows (TR true).  `groups` of 1024 LDS bytes, one
 // load instruction of a wave each.
 template <typename Op, int T, bool TR>
@@ -90,26 +88,29 @@ struct Side {
     {
         return row_bytes >= 256 ? (k & 3) | ((k >> 1) & 4) : ((k >> 1) & 1) | ((k >> 2) & 2);
     }
-    // this lane's 16 bytes of group g: source address in stage k0, whether its columns exist, its k (TR) or column (not TR)
-    static __device__ inline const char *source(const Operand &O, long long m0, int g, int lane, int k0, int *at, bool *there)
+    // where stage k0 begins in memory for a tile that starts at m0, and how far a stage is
+    static __device__ inline const char *base(const Operand &O, long long m0, int k0)
+    {
+        return static_cast<const char *>(O.p) + (TR ? (long long)k0 * ks * O.ld + m0 * (64 / ks) : m0 * O.ld + (long long)k0 * 64) * 2;
+    }
+    static __device__ inline long long step(const Operand &O) { return TR ? O.ld * (ks * 2) : 128; }
+    // this lane's 16 bytes of group g: offset from the base and its k (TR: row of the stage, else image element).  What lies
+    // past the last m repeats the last one: it reaches only results that are not stored.
+    static __device__ inline unsigned offset(const Operand &O, long long m0, int g, int lane, int *at)
     {
         const int c = g * 64 + lane, row = c / row_chunks, pos = c % row_chunks;
         if constexpr (TR) {
             const long long col = m0 * (64 / ks) + (pos ^ (unit_swizzle(row) << 1)) * 8;
             *at = row;
-            *there = col < O.cols;
-            return static_cast<const char *>(O.p) + (((long long)k0 * ks + row) * O.ld + col) * 2;
+            return (unsigned)((row * O.ld + (col < O.cols ? col : O.cols - 8) - m0 * (64 / ks)) * 2);
         } else {
-            long long r = m0 + row;
-            r = r < O.rows ? r : O.rows - 1;
+            const long long last = O.rows - 1 - m0;
             *at = (pos ^ (row & 7)) * 8;
-            *there = true;
-            return static_cast<const char *>(O.p) + (r * O.ld + (long long)k0 * 64 + *at) * 2;
+            return (unsigned)(((row < last ? row : last) * O.ld + *at) * 2);
         }
     }
-    // in the last stage: is this lane past the end of k?
-    static __device__ inline bool past(const Operand &O, int kt, int at) { return (long long)kt * (TR ? ks : 64) + at >= (TR ? O.rows : O.cols); }
-    static __device__ inline long long step(const Operand &O) { return TR ? O.ld * (ks * 2) : 128; }
+    static __device__ inline long long kcount(const Operand &O) { return TR ? O.rows : O.cols; }
+    static constexpr int kstep = TR ? ks : 64;
 
     // fragment t (sixteen m), half h of the stage: float32 - h = 0 the hi, 1 the lo of the 32 k;  else k 32 h .. 32 h + 31
     static __device__ inline V read(const char *base, int lane, int t, int h)
@@ -135,77 +136,138 @@ struct TileProduct {
     using A_ = Side<Op, TM, TA>;
     using B_ = Side<Op, TN, TB>;
     static constexpr int kAll = A_::groups + B_::groups, kLoads = (kAll + S::waves - 1) / S::waves;
+    static constexpr int MH = S::MT / 2, RA = TA ? 2 : 1, RB = TB ? 2 : 1;       // LDS reads a fragment
+    static_assert(kAll % S::waves == 0 && A_::groups % S::waves == 0, "a load instruction is all A or all B");
+
+    // A phase: the reads are spread over the first half of its matrix instructions, so that they have arrived at its end,
+    // where they are waited for in one go.
+    template <int products, int reads>
+    static __device__ inline void phase_end()
+    {
+        constexpr int each = products / reads / 2 > 0 ? products / reads / 2 : 1;
+#pragma unroll
+        for (int i = 0; i < reads; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, each, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(0xC07F);                  // lgkmcnt(0)
+        __builtin_amdgcn_sched_barrier(0);
+    }
 
     // acc[mt][nt][i]: row wm*(TM/WM) + 16 mt + 4 (lane >> 4) + i of A, row wn*(TN/WN) + 16 nt + (lane & 15) of B.
-    // Stages k0 .. k1 - 1 of ktotal.
+    // Stages k0 .. k1 - 1 of ktotal.  A stage has four phases, each with half of A's fragments of one kind (half of k;
+    // float32: hi or lo); a phase reads the next one's fragments from LDS behind its own matrix instructions.  In front of
+    // the fourth phase every wave holds the rest of the stage in registers and the next stage has arrived: the one after it
+    // is loaded into the buffer just left, a whole stage ahead of its use.
     static __device__ inline void run(fx4 (&acc)[S::MT][S::NT], const Operand &A, long long m0, const Operand &B, long long n0,
                                       int k0, int k1, int ktotal, char *lds)
     {
         if (k0 >= k1) return;
         const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const int wm = wave / WN, wn = wave % WN;
-        const char *src[kLoads];
+        unsigned off[kLoads];
         int at[kLoads];
-        bool there[kLoads];
-        const char *zero = reinterpret_cast<const char *>(g_zero_page);
+        constexpr int kLoadsA = A_::groups / S::waves;
 #pragma unroll
         for (int i = 0; i < kLoads; i++) {
-            const int g = i * S::waves + wave;                                  // wave-uniform; a load is all A or all B
-            if (g < A_::groups) src[i] = A_::source(A, m0, g, lane, k0, &at[i], &there[i]);
-            else src[i] = B_::source(B, n0, g - A_::groups, lane, k0, &at[i], &there[i]);
+            const int g = i * S::waves + wave;
+            off[i] = i < kLoadsA ? A_::offset(A, m0, g, lane, &at[i]) : B_::offset(B, n0, g - A_::groups, lane, &at[i]);
         }
+        const char *base_a = A_::base(A, m0, k0), *base_b = B_::base(B, n0, k0);
         const long long step_a = A_::step(A), step_b = B_::step(B);
-        auto load = [&](int kt, int buf) {
-            const bool last = kt + 1 == ktotal;
+        char *lds_wave = lds + wave * 1024;
+        // (buffer addressing: a scalar base that moves and a 32-bit offset that stays; the offsets are in range by construction)
+        auto load = [&](int buf) {
+            const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base_a), 0, -1, 0x00020000);
+            const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base_b), 0, -1, 0x00020000);
+#pragma unroll
+            for (int i = 0; i < kLoads; i++)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(i < kLoadsA ? ra : rb, (lds_ptr)(lds_wave + buf * S::stage_bytes + i * S::waves * 1024),
+                                                         16, (int)off[i], 0, 0, 0);
+            base_a += step_a;
+            base_b += step_b;
+        };
+        // the last stage of k: zeros past its end
+        auto load_last = [&](int kt, int buf) {
+            const char *zero = reinterpret_cast<const char *>(g_zero_page);
+            const long long left_a = A_::kcount(A) - (long long)kt * A_::kstep, left_b = B_::kcount(B) - (long long)kt * B_::kstep;
 #pragma unroll
             for (int i = 0; i < kLoads; i++) {
-                const int g = i * S::waves + wave;
-                if (kAll % S::waves == 0 || g < kAll) {
-                    const char *p = src[i];
-                    if ((TA || TB) && !there[i]) p = zero;
-                    if (last && (g < A_::groups ? A_::past(A, kt, at[i]) : B_::past(B, kt, at[i]))) p = zero;
-                    __builtin_amdgcn_global_load_lds((glb_ptr)p, (lds_ptr)(lds + buf * S::stage_bytes + g * 1024), 16, 0, 0);
-                    src[i] += g < A_::groups ? step_a : step_b;
-                }
+                const char *p = (i < kLoadsA ? base_a : base_b) + off[i];
+                if (at[i] >= (i < kLoadsA ? left_a : left_b)) p = zero;
+                __builtin_amdgcn_global_load_lds((glb_ptr)p, (lds_ptr)(lds_wave + buf * S::stage_bytes + i * S::waves * 1024), 16, 0, 0);
             }
+            base_a += step_a;
+            base_b += step_b;
         };
-        // (the barrier alone does not wait for loads that write LDS)
-        load(k0, 0);
-        wait_loads();
-        __syncthreads();
+        auto load_any = [&](int kt, int buf) { if (kt + 1 == ktotal) load_last(kt, buf); else load(buf); };
         // a wave's part of a side begins a whole number of rows or 32-byte units into it
         const int oa = TA ? 0 : wm * (TM / WM) * 128, ob = A_::groups * 1024 + (TB ? 0 : wn * (TN / WN) * 128);
         const int ta = TA ? wm * S::MT : 0, tb = TB ? wn * S::NT : 0;
-        for (int kt = k0; kt < k1; kt++) {
+        typename F::V a[2][MH], b[2][S::NT];
+        // fragments of phase p of the stage in `buf`
+        auto read_a = [&](int buf, int p) {
+            const char *pa = lds + buf * S::stage_bytes + oa;
+            const int h = Op::split ? p & 1 : p >> 1, half = Op::split ? p >> 1 : p & 1;
+#pragma unroll
+            for (int t = 0; t < MH; t++) a[p & 1][t] = A_::read(pa, lane, ta + half * MH + t, h);
+        };
+        auto read_b = [&](int buf, int h) {
+            const char *pb = lds + buf * S::stage_bytes + ob;
+#pragma unroll
+            for (int t = 0; t < S::NT; t++) b[h][t] = B_::read(pb, lane, tb + t, h);
+        };
+        auto products = [&](int p, int hb) {
+            const int half = Op::split ? p >> 1 : p & 1;
+#pragma unroll
+            for (int mt = 0; mt < MH; mt++)
+#pragma unroll
+                for (int nt = 0; nt < S::NT; nt++) acc[half * MH + mt][nt] = F::mfma(a[p & 1][mt], b[hb][nt], acc[half * MH + mt][nt]);
+        };
+        auto meet = [&]() {                                   // own reads done, own loads arrived; then everyone's
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        load_any(k0, 0);
+        meet();
+        if (k0 + 1 < k1) load_any(k0 + 1, 1);
+        read_b(0, 0);
+        if (Op::split) read_b(0, 1);
+        read_a(0, 0);
+        int kt = k0;
+        constexpr int PP = MH * S::NT;
+        auto stage = [&](auto fast) {
             const int buf = (kt - k0) & 1;
-            if (kt + 1 < k1) load(kt + 1, buf ^ 1);
-            const char *pa = lds + buf * S::stage_bytes + oa, *pb = lds + buf * S::stage_bytes + ob;
-            typename F::V a[2][S::MT], b[2][S::NT];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-#pragma unroll
-                for (int t = 0; t < S::NT; t++) b[h][t] = B_::read(pb, lane, tb + t, h);
-#pragma unroll
-                for (int t = 0; t < S::MT; t++) a[h][t] = A_::read(pa, lane, ta + t, h);
-                if (!Op::split)
-#pragma unroll
-                    for (int mt = 0; mt < S::MT; mt++)
-#pragma unroll
-                        for (int nt = 0; nt < S::NT; nt++) acc[mt][nt] = F::mfma(a[h][mt], b[h][nt], acc[mt][nt]);
+            if constexpr (Op::split) {                        // (hi hi, hi lo), (lo hi) for either half of A
+                read_a(buf, 1); products(0, 0); products(0, 1); phase_end<2 * PP, MH * RA>();
+                read_a(buf, 2); products(1, 0); phase_end<PP, MH * RA>();
+                read_a(buf, 3); products(2, 0); products(2, 1); phase_end<2 * PP, MH * RA>();
+            } else {
+                read_a(buf, 1); products(0, 0); phase_end<PP, MH * RA>();
+                read_a(buf, 2); read_b(buf, 1); products(1, 0); phase_end<PP, MH * RA + S::NT * RB>();
+                read_a(buf, 3); products(2, 1); phase_end<PP, MH * RA>();
             }
-            if (Op::split) {
-#pragma unroll
-                for (int mt = 0; mt < S::MT; mt++)
-#pragma unroll
-                    for (int nt = 0; nt < S::NT; nt++) {
-                        acc[mt][nt] = F::mfma(a[1][mt], b[0][nt], acc[mt][nt]);
-                        acc[mt][nt] = F::mfma(a[0][mt], b[1][nt], acc[mt][nt]);
-                        acc[mt][nt] = F::mfma(a[0][mt], b[0][nt], acc[mt][nt]);
-                    }
+            meet();
+            if constexpr (fast.value) load(buf);
+            else if (kt + 2 < k1) load_any(kt + 2, buf);
+            // (after the last stage the other buffer is stale: read, not used)
+            if constexpr (Op::split) {
+                read_a(buf ^ 1, 0);
+                products(3, 0);
+                read_b(buf ^ 1, 0); read_b(buf ^ 1, 1);
+            } else {
+                read_a(buf ^ 1, 0); read_b(buf ^ 1, 0);
+                products(3, 1);
             }
-            wait_loads();
-            __syncthreads();
-        }
+            phase_end<PP, MH * RA + S::NT * RB * (Op::split ? 2 : 1)>();
+            kt++;
+        };
+        const int fast_end = k1 - 2 - (k1 == ktotal ? 1 : 0);
+        while (kt < fast_end) stage(std::true_type{});
+        while (kt < k1) stage(std::false_type{});
+        __syncthreads();
     }
 };
 

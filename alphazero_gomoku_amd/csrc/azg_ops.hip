@@ -104,13 +104,13 @@ struct Take {                                                 // offsets into th
 
 enum Shape { T256, T128, T64, TROW };
 struct ShapeDim { int tm, tn, wm; };
-constexpr ShapeDim kDims[4] = {{256, 256, 2}, {128, 128, 2}, {64, 64, 2}, {128, 16, 4}};
+constexpr ShapeDim kDims[4] = {{256, 256, 2}, {128, 128, 2}, {64, 64, 2}, {128, 32, 4}};
 
 long long tiles_of(Shape s, long long m, long long n) { return ((m + kDims[s].tm - 1) / kDims[s].tm) * ((n + kDims[s].tn - 1) / kDims[s].tn); }
 
 Shape pick_logits(long long m, long long n, bool grad)
 {
-    if (!grad && n <= 16) return TROW;
+    if (!grad && n <= 32) return TROW;
     if (tiles_of(T256, m, n) >= 200) return T256;
     if (tiles_of(T128, m, n) >= 200) return T128;
     return T64;
@@ -207,7 +207,7 @@ int check(const azg_linear_ce_args *a)
     if (a->n > INT_MAX || a->classes > INT_MAX || a->hidden > (1 << 22)) return fail(AZG_EINVAL, "azg_linear_ce: a size is too large");
     if (a->reduction < AZG_REDUCE_NONE || a->reduction > AZG_REDUCE_MEAN) return fail(AZG_EINVAL, "azg_linear_ce: unknown reduction %d", a->reduction);
     if (bad_matrix(a->n, a->hidden, a->x_stride) || bad_matrix(a->classes, a->hidden, a->w_stride)) return fail(AZG_EINVAL, "azg_linear_ce: a row stride is smaller than a row");
-    if (a->x_stride > (1 << 22) * 64LL || a->w_stride > (1 << 22) * 64LL) return fail(AZG_EINVAL, "azg_linear_ce: a row stride is too large");
+    if (a->x_stride > (1LL << 22) || a->w_stride > (1LL << 22)) return fail(AZG_EINVAL, "azg_linear_ce: a row stride is too large");
     return AZG_OK;
 }
 
@@ -237,7 +237,7 @@ int launch_logits(Shape shape, const CeArgs &c, hipStream_t s)
     case T128: return launch_logits_shape<Op, 128, 128, 2, 2, GRAD>(c, s);
     case T64: return launch_logits_shape<Op, 64, 64, 2, 2, GRAD>(c, s);
     default:
-        if constexpr (!GRAD) return launch_logits_shape<Op, 128, 16, 4, 1, false>(c, s);
+        if constexpr (!GRAD) return launch_logits_shape<Op, 128, 32, 4, 1, false>(c, s);
         return fail(AZG_EINVAL, "azg_linear_ce: internal: no such tile");
     }
 }
