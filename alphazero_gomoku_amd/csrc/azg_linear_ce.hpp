@@ -48,8 +48,8 @@ template <> struct Frag<__bf16> {
 };
 
 // ---------------------------------------------------------------- the tile product
-// TM x TN output tile, WM x WN waves, 16x16x32 matrix instructions, stages of 64 k (float32: 32).  Stages are
-// double-buffered in LDS and filled by loads that go from global memory straight there, 16 bytes a lane.
+// TM x TN output tile, WM x WN waves, 16x16x32 matrix instructions, stages of 64 k (float32: 32).  Each operand has a ring
+// of stages in LDS, filled by loads that go from global memory straight there, 16 bytes a lane.
 //   k contiguous in memory: LDS rows are 128 bytes of one m, eight 16-byte chunks, chunk c of row r at c ^ (r & 7), so the
 //     sixteen rows of a fragment read (16 bytes a lane) spread over all banks;
 //   k across the rows: LDS rows are one k, TM columns of the image; a fragment is read by the transposing load
@@ -67,7 +67,10 @@ template <int TM, int TN, int WM, int WN>
 struct TileShape {
     static constexpr int waves = WM * WN, threads = waves * 64;
     static constexpr int MT = TM / WM / 16, NT = TN / WN / 16;
-    static constexpr int stage_bytes = (TM + TN) * 128, lds_bytes = 2 * stage_bytes;
+    // stages of A and of B in LDS: the 256 x 256 tile takes all of a CU's 160 KB, 128 x 128 leaves room for a second
+    // workgroup; the tile for few rows does little but wait for memory and keeps more in flight
+    static constexpr int ring_a = TN <= 32 ? 5 : 3, ring_b = TN <= 32 ? 5 : 2;
+    static constexpr int bytes_a = TM * 128, bytes_b = TN * 128, lds_bytes = ring_a * bytes_a + ring_b * bytes_b;
 };
 
 typedef __attribute__((address_space(3))) void *lds_ptr;
@@ -135,14 +138,20 @@ struct TileProduct {
     using F = Frag<typename Op::Img>;
     using A_ = Side<Op, TM, TA>;
     using B_ = Side<Op, TN, TB>;
-    static constexpr int kAll = A_::groups + B_::groups, kLoads = (kAll + S::waves - 1) / S::waves;
+    static constexpr int kLoadsA = A_::groups / S::waves, kLoadsB = B_::groups / S::waves, kLoads = kLoadsA + kLoadsB;
     static constexpr int MH = S::MT / 2, RA = TA ? 2 : 1, RB = TB ? 2 : 1;       // LDS reads a fragment
-    static_assert(kAll % S::waves == 0 && A_::groups % S::waves == 0, "a load instruction is all A or all B");
+    static_assert(A_::groups % S::waves == 0 && B_::groups % S::waves == 0, "every wave issues the same loads");
 
-    // A phase: the reads are spread over the first half of its matrix instructions, so that they have arrived at its end,
-    // where they are waited for in one go.
-    template <int products, int reads>
+    // The end of a phase: everything read from LDS during it is there.
     static __device__ inline void phase_end()
+    {
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(0xC07F);                  // lgkmcnt(0)
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    // Spreads `reads` LDS reads over the first half of `products` matrix instructions.
+    template <int products, int reads>
+    static __device__ inline void interleave()
     {
         constexpr int each = products / reads / 2 > 0 ? products / reads / 2 : 1;
 #pragma unroll
@@ -150,123 +159,204 @@ struct TileProduct {
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x008, each, 0);
         }
+    }
+    // 16 bytes a lane from base + off to LDS at `to` + 16 lane.  Written out because the compiler, which cannot tell the
+    // ring's places apart, would wait for all of these loads in front of every transposing read; what is read has arrived is
+    // seen to by meet().  Buffer addressing: a scalar base that moves and a 32-bit offset that stays, in range by construction.
+    static __device__ inline void load_lds(const char *base, unsigned off, unsigned to)
+    {
+        typedef unsigned ux4 __attribute__((ext_vector_type(4)));
+        const uint64_t at = reinterpret_cast<uint64_t>(base);
+        const ux4 rsrc = {(unsigned)at, (unsigned)(at >> 32) & 0xFFFFu, 0xFFFFFFFFu, 0x00020000u};
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(rsrc) : "memory", "m0");
+    }
+    // Own reads done and all but the newest `left` of the own loads arrived; then everyone's.  (A barrier by itself does not
+    // wait for loads that write LDS.)
+    template <int left>
+    static __device__ inline void meet()
+    {
         __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_waitcnt(0xC07F);                  // lgkmcnt(0)
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(left) : "memory");
         __builtin_amdgcn_sched_barrier(0);
     }
 
     // acc[mt][nt][i]: row wm*(TM/WM) + 16 mt + 4 (lane >> 4) + i of A, row wn*(TN/WN) + 16 nt + (lane & 15) of B.
     // Stages k0 .. k1 - 1 of ktotal.  A stage has four phases, each with half of A's fragments of one kind (half of k;
     // float32: hi or lo); a phase reads the next one's fragments from LDS behind its own matrix instructions.  In front of
-    // the fourth phase every wave holds the rest of the stage in registers and the next stage has arrived: the one after it
-    // is loaded into the buffer just left, a whole stage ahead of its use.
+    // the fourth phase the waves meet: all hold the rest of the stage in registers, the next stage has arrived, and the
+    // places of this one are free.  They are refilled a few loads at a time -- B's during the fourth and the next stage's
+    // first phase, A's, whose ring is longer, during the two phases after that -- because a burst of loads holds up the
+    // wave's matrix instructions behind it.
     static __device__ inline void run(fx4 (&acc)[S::MT][S::NT], const Operand &A, long long m0, const Operand &B, long long n0,
                                       int k0, int k1, int ktotal, char *lds)
     {
         if (k0 >= k1) return;
         const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const int wm = wave / WN, wn = wave % WN;
-        unsigned off[kLoads];
-        int at[kLoads];
-        constexpr int kLoadsA = A_::groups / S::waves;
+        unsigned off_a[kLoadsA], off_b[kLoadsB];
+        int at_a[kLoadsA], at_b[kLoadsB];
 #pragma unroll
-        for (int i = 0; i < kLoads; i++) {
-            const int g = i * S::waves + wave;
-            off[i] = i < kLoadsA ? A_::offset(A, m0, g, lane, &at[i]) : B_::offset(B, n0, g - A_::groups, lane, &at[i]);
-        }
+        for (int i = 0; i < kLoadsA; i++) off_a[i] = A_::offset(A, m0, i * S::waves + wave, lane, &at_a[i]);
+#pragma unroll
+        for (int i = 0; i < kLoadsB; i++) off_b[i] = B_::offset(B, n0, i * S::waves + wave, lane, &at_b[i]);
+        // next stage to load of either side: its place in memory and in the ring
         const char *base_a = A_::base(A, m0, k0), *base_b = B_::base(B, n0, k0);
         const long long step_a = A_::step(A), step_b = B_::step(B);
-        char *lds_wave = lds + wave * 1024;
-        // (buffer addressing: a scalar base that moves and a 32-bit offset that stays; the offsets are in range by construction)
-        auto load = [&](int buf) {
-            const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base_a), 0, -1, 0x00020000);
-            const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base_b), 0, -1, 0x00020000);
-#pragma unroll
-            for (int i = 0; i < kLoads; i++)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(i < kLoadsA ? ra : rb, (lds_ptr)(lds_wave + buf * S::stage_bytes + i * S::waves * 1024),
-                                                         16, (int)off[i], 0, 0, 0);
-            base_a += step_a;
-            base_b += step_b;
+        int la = k0, lb = k0, slot_a = 0, slot_b = 0;
+        char *lds_b = lds + S::ring_a * S::bytes_a;
+        const unsigned lds0 = (unsigned)(uintptr_t)(lds_ptr)lds + wave * 1024;
+        // load i of the next stage
+        auto load = [&](auto side_a, int i) {
+            if constexpr (side_a.value) load_lds(base_a, off_a[i], lds0 + slot_a * S::bytes_a + i * S::waves * 1024);
+            else load_lds(base_b, off_b[i], lds0 + S::ring_a * S::bytes_a + slot_b * S::bytes_b + i * S::waves * 1024);
         };
-        // the last stage of k: zeros past its end
-        auto load_last = [&](int kt, int buf) {
-            const char *zero = reinterpret_cast<const char *>(g_zero_page);
-            const long long left_a = A_::kcount(A) - (long long)kt * A_::kstep, left_b = B_::kcount(B) - (long long)kt * B_::kstep;
+        // a whole stage; the last stage of k has zeros past its end
+        auto load_stage = [&](auto side_a, bool last) {
+            constexpr bool a_side = side_a.value;
+            constexpr int loads = a_side ? kLoadsA : kLoadsB;
+            if (!last) {
 #pragma unroll
-            for (int i = 0; i < kLoads; i++) {
-                const char *p = (i < kLoadsA ? base_a : base_b) + off[i];
-                if (at[i] >= (i < kLoadsA ? left_a : left_b)) p = zero;
-                __builtin_amdgcn_global_load_lds((glb_ptr)p, (lds_ptr)(lds_wave + buf * S::stage_bytes + i * S::waves * 1024), 16, 0, 0);
+                for (int i = 0; i < loads; i++) load(side_a, i);
+            } else {
+                const char *base = a_side ? base_a : base_b;
+                char *to = (a_side ? lds + slot_a * S::bytes_a : lds_b + slot_b * S::bytes_b) + wave * 1024;
+                const long long left = a_side ? A_::kcount(A) - (long long)la * A_::kstep : B_::kcount(B) - (long long)lb * B_::kstep;
+#pragma unroll
+                for (int i = 0; i < loads; i++) {
+                    const char *p = base + (a_side ? off_a[i] : off_b[i]);
+                    if ((a_side ? at_a[i] : at_b[i]) >= left) p = reinterpret_cast<const char *>(g_zero_page);
+                    __builtin_amdgcn_global_load_lds((glb_ptr)p, (lds_ptr)(to + i * S::waves * 1024), 16, 0, 0);
+                }
             }
-            base_a += step_a;
-            base_b += step_b;
         };
-        auto load_any = [&](int kt, int buf) { if (kt + 1 == ktotal) load_last(kt, buf); else load(buf); };
+        constexpr std::true_type side_a{};
+        constexpr std::false_type side_b{};
+        auto next_a = [&]() { base_a += step_a; la++; slot_a = slot_a + 1 == S::ring_a ? 0 : slot_a + 1; };
+        auto next_b = [&]() { base_b += step_b; lb++; slot_b = slot_b + 1 == S::ring_b ? 0 : slot_b + 1; };
+        auto whole_a = [&](int before) { if (la < min(k1, before)) { load_stage(side_a, la + 1 == ktotal); next_a(); } };
+        auto whole_b = [&](int before) { if (lb < min(k1, before)) { load_stage(side_b, lb + 1 == ktotal); next_b(); } };
         // a wave's part of a side begins a whole number of rows or 32-byte units into it
-        const int oa = TA ? 0 : wm * (TM / WM) * 128, ob = A_::groups * 1024 + (TB ? 0 : wn * (TN / WN) * 128);
+        const int oa = TA ? 0 : wm * (TM / WM) * 128, ob = TB ? 0 : wn * (TN / WN) * 128;
         const int ta = TA ? wm * S::MT : 0, tb = TB ? wn * S::NT : 0;
         typename F::V a[2][MH], b[2][S::NT];
-        // fragments of phase p of the stage in `buf`
-        auto read_a = [&](int buf, int p) {
-            const char *pa = lds + buf * S::stage_bytes + oa;
+        int ra = 0, rb = 0;                                   // ring places that are being read
+        // fragments of phase p of a stage
+        auto read_a = [&](int slot, int p) {
+            const char *pa = lds + slot * S::bytes_a + oa;
             const int h = Op::split ? p & 1 : p >> 1, half = Op::split ? p >> 1 : p & 1;
 #pragma unroll
             for (int t = 0; t < MH; t++) a[p & 1][t] = A_::read(pa, lane, ta + half * MH + t, h);
         };
-        auto read_b = [&](int buf, int h) {
-            const char *pb = lds + buf * S::stage_bytes + ob;
+        auto read_b = [&](typename F::V (&to)[S::NT], int slot, int h) {
+            const char *pb = lds_b + slot * S::bytes_b + ob;
 #pragma unroll
-            for (int t = 0; t < S::NT; t++) b[h][t] = B_::read(pb, lane, tb + t, h);
+            for (int t = 0; t < S::NT; t++) to[t] = B_::read(pb, lane, tb + t, h);
         };
-        auto products = [&](int p, int hb) {
+        constexpr int PP = MH * S::NT;
+        // matrix instructions i0 .. i1 - 1 of phase p's A fragments and B's fragments h
+        auto products = [&](int p, int h, int i0, int i1) {
             const int half = Op::split ? p >> 1 : p & 1;
 #pragma unroll
             for (int mt = 0; mt < MH; mt++)
 #pragma unroll
-                for (int nt = 0; nt < S::NT; nt++) acc[half * MH + mt][nt] = F::mfma(a[p & 1][mt], b[hb][nt], acc[half * MH + mt][nt]);
+                for (int nt = 0; nt < S::NT; nt++)
+                    if (mt * S::NT + nt >= i0 && mt * S::NT + nt < i1)
+                        acc[half * MH + mt][nt] = F::mfma(a[p & 1][mt], b[h][nt], acc[half * MH + mt][nt]);
         };
-        auto meet = [&]() {                                   // own reads done, own loads arrived; then everyone's
-            __builtin_amdgcn_sched_barrier(0);
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            __builtin_amdgcn_sched_barrier(0);
+        // phase p's matrix instructions (with B's fragments h; float32, even phases: h = 0 and 1) behind its `reads` LDS reads,
+        // with loads l0 .. l1 - 1 of the next stage of a side near their end
+        auto phase = [&](int p, int h, auto reads, auto both, auto side, auto l0, auto l1) {
+            constexpr int loads = l1.value - l0.value, per = loads ? loads : 1, tail = PP - 2 * loads > 0 ? PP - 2 * loads : 0, total = both.value ? PP + tail : tail;
+            if constexpr (both.value) { products(p, 0, 0, PP); products(p, 1, 0, tail); }
+            else products(p, h, 0, tail);
+            interleave<total, reads.value>();
+#pragma unroll
+            for (int i = 0; i < loads; i++) {
+                __builtin_amdgcn_sched_barrier(0);
+                load(side, l0.value + i);
+                __builtin_amdgcn_sched_barrier(0);
+                products(p, both.value ? 1 : h, tail + (PP - tail) * i / per, tail + (PP - tail) * (i + 1) / per);
+            }
+            phase_end();
         };
-        load_any(k0, 0);
-        meet();
-        if (k0 + 1 < k1) load_any(k0 + 1, 1);
-        read_b(0, 0);
-        if (Op::split) read_b(0, 1);
+        // fill the rings in the order of the loop's loads and wait for the first stage
+        whole_a(k1);
+        if (S::ring_b == S::ring_a) whole_b(k1);
+#pragma unroll
+        for (int i = 1; i < S::ring_a; i++) {
+            if (S::ring_b == S::ring_a || i > S::ring_a - 1 - S::ring_b) whole_b(k1);
+            whole_a(k1);
+        }
+        if (k1 - k0 >= S::ring_a) meet<(S::ring_a - 1) * kLoadsA + (S::ring_b - 1) * kLoadsB>();
+        else meet<0>();
+        read_b(b[0], 0, 0);
+        if (Op::split) read_b(b[1], 0, 1);
         read_a(0, 0);
         int kt = k0;
-        constexpr int PP = MH * S::NT;
-        auto stage = [&](auto fast) {
-            const int buf = (kt - k0) & 1;
+        constexpr int B1 = kLoadsB / 2, A1 = kLoadsA / 2;
+        // loads issued after the later of the two that the next stage needs
+        constexpr int newer = S::ring_a > S::ring_b ? kLoadsA + (S::ring_b - 2) * kLoads : (S::ring_a - 2) * kLoads;
+        constexpr std::true_type yes{};
+        constexpr std::false_type no{};
+#define AZG_INT(v) std::integral_constant<int, v>{}
+        auto stage = [&](auto fast_, auto full_) {            // fast: with the loads of a steady state; full: the rings are
+            constexpr bool fast = fast_.value, full = full_.value;
+            const int sa = ra + 1 == S::ring_a ? 0 : ra + 1, sb = rb + 1 == S::ring_b ? 0 : rb + 1;
             if constexpr (Op::split) {                        // (hi hi, hi lo), (lo hi) for either half of A
-                read_a(buf, 1); products(0, 0); products(0, 1); phase_end<2 * PP, MH * RA>();
-                read_a(buf, 2); products(1, 0); phase_end<PP, MH * RA>();
-                read_a(buf, 3); products(2, 0); products(2, 1); phase_end<2 * PP, MH * RA>();
+                read_a(ra, 1);
+                phase(0, 0, AZG_INT(MH * RA), yes, side_b, AZG_INT(B1), AZG_INT(fast ? kLoadsB : B1));
+                if (fast) next_b();
+                read_a(ra, 2);
+                phase(1, 0, AZG_INT(MH * RA), no, side_a, AZG_INT(0), AZG_INT(fast ? A1 : 0));
+                read_a(ra, 3);
+                phase(2, 0, AZG_INT(MH * RA), yes, side_a, AZG_INT(A1), AZG_INT(fast ? kLoadsA : A1));
             } else {
-                read_a(buf, 1); products(0, 0); phase_end<PP, MH * RA>();
-                read_a(buf, 2); read_b(buf, 1); products(1, 0); phase_end<PP, MH * RA + S::NT * RB>();
-                read_a(buf, 3); products(2, 1); phase_end<PP, MH * RA>();
+                read_a(ra, 1);
+                phase(0, 0, AZG_INT(MH * RA), no, side_b, AZG_INT(B1), AZG_INT(fast ? kLoadsB : B1));
+                if (fast) next_b();
+                read_a(ra, 2);
+                read_b(b[1], rb, 1);
+                phase(1, 0, AZG_INT(MH * RA + S::NT * RB), no, side_a, AZG_INT(0), AZG_INT(fast ? A1 : 0));
+                read_a(ra, 3);
+                phase(2, 1, AZG_INT(MH * RA), no, side_a, AZG_INT(A1), AZG_INT(fast ? kLoadsA : A1));
             }
-            meet();
-            if constexpr (fast.value) load(buf);
-            else if (kt + 2 < k1) load_any(kt + 2, buf);
-            // (after the last stage the other buffer is stale: read, not used)
+            if (fast) next_a();
+            meet<full ? newer : 0>();
+            // (after the last stage what is read is stale and not used)
+            read_a(sa, 0);
             if constexpr (Op::split) {
-                read_a(buf ^ 1, 0);
-                products(3, 0);
-                read_b(buf ^ 1, 0); read_b(buf ^ 1, 1);
+                typename F::V bn[2][S::NT];
+                read_b(bn[0], sb, 0);
+                read_b(bn[1], sb, 1);
+                phase(3, 0, AZG_INT(MH * RA + 2 * S::NT * RB), no, side_b, AZG_INT(0), AZG_INT(fast ? B1 : 0));
+#pragma unroll
+                for (int t = 0; t < S::NT; t++) { b[0][t] = bn[0][t]; b[1][t] = bn[1][t]; }
             } else {
-                read_a(buf ^ 1, 0); read_b(buf ^ 1, 0);
-                products(3, 1);
+                read_b(b[0], sb, 0);
+                phase(3, 1, AZG_INT(MH * RA + S::NT * RB), no, side_b, AZG_INT(0), AZG_INT(fast ? B1 : 0));
             }
-            phase_end<PP, MH * RA + S::NT * RB * (Op::split ? 2 : 1)>();
+            ra = sa; rb = sb;
             kt++;
         };
-        const int fast_end = k1 - 2 - (k1 == ktotal ? 1 : 0);
-        while (kt < fast_end) stage(std::true_type{});
-        while (kt < k1) stage(std::false_type{});
+        // The fast loop's stage kt issues the rest of B's stage kt - 1 + ring_b, all of A's kt - 1 + ring_a and the first part of
+        // B's kt + ring_b; around it: the first stage's loads in one go, whole stages, and the rest of a begun one.
+        const bool tail = k1 == ktotal && (A_::kcount(A) % A_::kstep != 0 || B_::kcount(B) % B_::kstep != 0);
+        const int end = k1 - (tail ? 1 : 0), fast_end = min(end - S::ring_a + 1, end - S::ring_b);
+        if (kt + 1 < fast_end) {
+            stage(no, yes);
+#pragma unroll
+            for (int i = 0; i < B1; i++) load(side_b, i);
+            while (kt < fast_end) stage(yes, yes);
+#pragma unroll
+            for (int i = B1; i < kLoadsB; i++) load(side_b, i);
+            next_b();
+        }
+        while (kt < k1) {
+            whole_b(kt + S::ring_b);
+            whole_a(kt + S::ring_a);
+            stage(no, no);
+        }
+#undef AZG_INT
         __syncthreads();
     }
 };
@@ -292,7 +382,7 @@ struct PackArgs {
     const void *src;              // [rows][cols], stride ld
     long long ld, rows, cols;
     void *img;                    // [rows][ldi]
-    long long ldi;                // padded columns (image elements)
+    long long ldi, icols;         // row stride, padded columns (image elements)
     const long long *target;      // not null: rows whose target is ignore_index are read as zero
     long long ignore;
     const float *maxpart;         // float32: kMaxParts partial maxima of the tensor
@@ -346,7 +436,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a)
 {
     constexpr int per = Op::split ? 2 : 1;
     const float scale = Op::split ? split_scale(max_of_parts(a.maxpart)) : 1.f;
-    const long long row_chunks = a.ldi / (8 * per), total = a.rows * row_chunks;
+    const long long row_chunks = a.icols / (8 * per), total = a.rows * row_chunks;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
         const long long r = i / row_chunks, c = (i - r * row_chunks) * 8;
         const typename Op::In *p = static_cast<const typename Op::In *>(a.src) + r * a.ld + c;
@@ -399,7 +489,7 @@ struct CeArgs {
     const float4 *stats;          // [n]: m, sum pi / s, ... (RowArgs)
     const float *rowg;            // [n]
     void *d;                      // image [n][ldd] of D; statistics: of exp(l - the span's maximum), or null
-    long long ldd;
+    long long ldd, dcols;         // row stride in image elements; padded classes
     float *dbpart;                // [ntiles][classes] or null
 };
 
@@ -437,7 +527,7 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
             for (int nt = 0; nt < S::NT; nt++) acc[mt][nt][i] = v < a.classes ? acc[mt][nt][i] * ux * uw + b : -INFINITY;
         }
     const long long nw = n0 + wn * (TN / WN) + (lane & 15);
-    const long long dpad = Op::split ? a.ldd / 2 : a.ldd;
+    const long long dpad = a.dcols;
     if constexpr (!GRAD) {
         // per row: maximum and sum over the span; lanes 16 and 32 apart share a row
         using E = typename Expo<Op>::T;
@@ -465,7 +555,7 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
                     if (a.part_e) e += x != 0.f ? x * l : 0.f;
                     keep.v[i] = (E)x;
                 }
-                if (a.d && live && vw + mt * 16 < dpad) *reinterpret_cast<Pack<E, 4> *>(static_cast<E *>(a.d) + row * dpad + vw + mt * 16) = keep;
+                if (a.d && live && vw + mt * 16 < dpad) *reinterpret_cast<Pack<E, 4> *>(static_cast<E *>(a.d) + row * (a.ldd / (Op::split ? 2 : 1)) + vw + mt * 16) = keep;
             }
             if (a.probs && live) {
                 const float *pr = a.probs + row * a.ldp;
@@ -565,7 +655,7 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
 constexpr int kFixRows = 128, kFixCols = 128;
 struct FixArgs {
     long long n, classes, span;   // classes an entry of part stands for
-    void *d; long long ldd;
+    void *d; long long ldd, dcols;
     const float2 *part; const float4 *stats; const float *rowg;
     const long long *target;
     const float *probs; long long ldp;
@@ -578,7 +668,7 @@ __global__ __launch_bounds__(256) void fix_kernel(FixArgs a)
     __shared__ float red[16][kFixCols + 1];
     const int tid = threadIdx.x, rg = tid >> 4, cl = (tid & 15) * 8;
     const long long c0 = (long long)blockIdx.x * kFixCols, r0 = (long long)blockIdx.y * kFixRows, c = c0 + cl;
-    const long long dpad = Op::split ? a.ldd / 2 : a.ldd;
+    const long long dpad = a.dcols, lde = a.ldd / (Op::split ? 2 : 1);
     float db[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (c < dpad)
 #pragma unroll 4
@@ -591,12 +681,12 @@ __global__ __launch_bounds__(256) void fix_kernel(FixArgs a)
             const long long t = a.target ? a.target[row] - c : -1;
             float v[8];
             if constexpr (Op::split) {
-                const fx4 *p = reinterpret_cast<const fx4 *>(static_cast<float *>(a.d) + row * dpad + c);
+                const fx4 *p = reinterpret_cast<const fx4 *>(static_cast<float *>(a.d) + row * lde + c);
                 const fx4 v0 = p[0], v1 = p[1];
 #pragma unroll
                 for (int i = 0; i < 4; i++) { v[i] = v0[i]; v[4 + i] = v1[i]; }
             } else {
-                const hx8 p = *reinterpret_cast<const hx8 *>(static_cast<_Float16 *>(a.d) + row * dpad + c);
+                const hx8 p = *reinterpret_cast<const hx8 *>(static_cast<_Float16 *>(a.d) + row * lde + c);
 #pragma unroll
                 for (int i = 0; i < 8; i++) v[i] = (float)p[i];
             }

@@ -48,6 +48,9 @@ struct DeviceScope {
 };
 
 long long up_to(long long v, long long m) { return (v + m - 1) / m * m; }
+// Row stride of an image of `cols` elements of 16 bits: an odd number of 128-byte lines, so that the lines that the rows of a
+// tile have in one stage lie in different channels of the L2 and of memory.
+long long image_stride(long long cols) { const long long l = up_to(cols, 64) / 64; return (l | 1) * 64; }
 
 bool bad_matrix(long long rows, long long cols, long long stride) { return rows > 1 && stride < cols; }
 
@@ -133,7 +136,7 @@ GradPick pick_grad(long long m, long long n, long long ktiles)
 struct Plan {
     bool split, forward, backward, pack_w, pack_x, keep;      // keep: the forward pass leaves exponentials for the backward pass
     long long n, H, V, vp, pieces;
-    long long kimg, ldd;                                      // image elements along the features, along a piece's classes
+    long long kimg, ldk, ldd;                                 // image elements along the features; row strides of the images of X, W and D
     int per, ks;                                              // image elements an element takes, k of a stage
     Shape lshape;
     GradPick gx, gw;
@@ -154,11 +157,12 @@ int make_plan(const azg_linear_ce_args *a, Plan *p)
     p->backward = a->dx || a->dw || a->db;
     p->n = a->n; p->H = a->hidden; p->V = a->classes;
     p->kimg = up_to(p->H, p->ks) * p->per;
+    p->ldk = image_stride(p->kimg);
     // (dW multiplies the rows that count for nothing by zero: they are copied as zeros, whatever they hold)
     p->pack_x = p->split || !aligned16(a->x, a->x_stride, a->hidden, a->n) || (a->dw && a->target);
     p->pack_w = p->split || !aligned16(a->w, a->w_stride, a->hidden, a->classes);
     // bytes a class of a piece costs
-    long long cost = p->pack_w ? p->kimg * 2 : 0;
+    long long cost = p->pack_w ? p->ldk * 2 : 0;
     if (p->backward) cost += p->n * p->per * 2;
     p->vp = p->V;
     if (cost) p->vp = std::min<long long>(p->V, std::max<long long>(1024, kPieceBytes / cost / 256 * 256));
@@ -168,7 +172,7 @@ int make_plan(const azg_linear_ce_args *a, Plan *p)
         p->pieces = (p->V + p->vp - 1) / p->vp;
     }
     p->keep = p->forward && p->backward && p->pieces == 1;
-    p->ldd = up_to(p->vp, p->ks) * p->per;
+    p->ldd = image_stride(up_to(p->vp, p->ks) * p->per);
     p->lshape = pick_logits(p->vp, p->n, p->backward);
     p->gx = pick_grad(p->H, p->n, (p->vp + p->ks - 1) / p->ks);
     p->gw = pick_grad(p->H, p->vp, (p->n + p->ks - 1) / p->ks);
@@ -180,8 +184,8 @@ int make_plan(const azg_linear_ce_args *a, Plan *p)
     Take t;
     p->xmax = t(p->split ? kMaxParts * 4 : 0);
     p->wmax = t(p->split ? kMaxParts * 4 : 0);
-    p->ximg = t(p->pack_x ? (size_t)p->n * p->kimg * 2 : 0);
-    p->wimg = t(p->pack_w ? (size_t)p->vp * p->kimg * 2 : 0);
+    p->ximg = t(p->pack_x ? (size_t)p->n * p->ldk * 2 : 0);
+    p->wimg = t(p->pack_w ? (size_t)p->vp * p->ldk * 2 : 0);
     const size_t entries = (size_t)p->pieces * lm * dim.wm * p->n;
     p->part = t(p->forward ? entries * 8 : 0);
     p->part_e = t(p->forward && a->entropy ? entries * 4 : 0);
@@ -274,7 +278,7 @@ int launch_join(const JoinArgs &j, hipStream_t s)
 template <typename Op>
 int launch_pack(const PackArgs &p, hipStream_t s)
 {
-    const long long chunks = p.rows * (p.ldi / (Op::split ? 16 : 8));
+    const long long chunks = p.rows * (p.icols / (Op::split ? 16 : 8));
     hipLaunchKernelGGL((pack_kernel<Op>), dim3((unsigned)std::min<long long>((chunks + 255) / 256, 1 << 16)), dim3(256), 0, s, p);
     OPS_HIP(hipGetLastError());
     return AZG_OK;
@@ -294,16 +298,16 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
 
     PackArgs px{};
     px.src = a->x; px.ld = a->x_stride; px.rows = a->n; px.cols = a->hidden; px.target = target; px.ignore = a->ignore_index;
-    px.maxpart = f32(p.xmax); px.img = ws + p.ximg; px.ldi = p.kimg;
+    px.maxpart = f32(p.xmax); px.img = ws + p.ximg; px.ldi = p.ldk; px.icols = p.kimg;
     PackArgs pw{};
-    pw.src = W; pw.ld = a->w_stride; pw.rows = a->classes; pw.cols = a->hidden; pw.maxpart = f32(p.wmax); pw.img = ws + p.wimg; pw.ldi = p.kimg;
+    pw.src = W; pw.ld = a->w_stride; pw.rows = a->classes; pw.cols = a->hidden; pw.maxpart = f32(p.wmax); pw.img = ws + p.wimg; pw.ldi = p.ldk; pw.icols = p.kimg;
     if (Op::split) {
         hipLaunchKernelGGL(absmax_kernel, dim3(kMaxParts), dim3(256), 0, s, px, f32(p.xmax));
         hipLaunchKernelGGL(absmax_kernel, dim3(kMaxParts), dim3(256), 0, s, pw, f32(p.wmax));
     }
     if (p.pack_x) OPS_TRY(launch_pack<Op>(px, s));
     CeArgs c{};
-    c.x = p.pack_x ? Operand{ws + p.ximg, p.kimg, a->n, p.kimg} : Operand{a->x, a->x_stride, a->n, a->hidden};
+    c.x = p.pack_x ? Operand{ws + p.ximg, p.ldk, a->n, p.kimg} : Operand{a->x, a->x_stride, a->n, a->hidden};
     c.ktiles = (int)((p.H + p.ks - 1) / p.ks);
     c.n = a->n; c.target = target; c.ignore = a->ignore_index; c.ldp = a->probs_stride;
     c.xmax = f32(p.xmax); c.wmax = f32(p.wmax);
@@ -313,10 +317,11 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
         c.v0 = v0; c.classes = vn;
         c.bias = a->bias ? static_cast<const In *>(a->bias) + v0 : nullptr;
         c.probs = a->probs ? a->probs + v0 : nullptr;
-        c.ldd = up_to(vn, p.ks) * p.per;
+        c.ldd = p.ldd;
+        c.dcols = up_to(vn, p.ks);
         pw.src = W + v0 * a->w_stride; pw.rows = vn;
         if (p.pack_w && pack) OPS_TRY(launch_pack<Op>(pw, s));
-        c.w = p.pack_w ? Operand{ws + p.wimg, p.kimg, vn, p.kimg} : Operand{W + v0 * a->w_stride, a->w_stride, vn, a->hidden};
+        c.w = p.pack_w ? Operand{ws + p.wimg, p.ldk, vn, p.kimg} : Operand{W + v0 * a->w_stride, a->w_stride, vn, a->hidden};
         return AZG_OK;
     };
 
@@ -355,11 +360,11 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
         int dbparts;
         if (p.keep) {
             FixArgs f{};
-            f.n = a->n; f.classes = vn; f.span = dim.tm / dim.wm; f.d = ws + p.d; f.ldd = c.ldd;
+            f.n = a->n; f.classes = vn; f.span = dim.tm / dim.wm; f.d = ws + p.d; f.ldd = c.ldd; f.dcols = c.dcols;
             f.part = reinterpret_cast<float2 *>(ws + p.part); f.stats = stats; f.rowg = f32(p.rowg);
             f.target = target; f.probs = a->probs; f.ldp = a->probs_stride; f.dbpart = a->db ? f32(p.dbpart) : nullptr;
             dbparts = (int)((a->n + kFixRows - 1) / kFixRows);
-            hipLaunchKernelGGL((fix_kernel<Op>), dim3((unsigned)((c.ldd / p.per + kFixCols - 1) / kFixCols), dbparts), dim3(256), 0, s, f);
+            hipLaunchKernelGGL((fix_kernel<Op>), dim3((unsigned)((c.dcols + kFixCols - 1) / kFixCols), dbparts), dim3(256), 0, s, f);
             OPS_HIP(hipGetLastError());
         } else {
             c.stats = stats; c.rowg = f32(p.rowg);
@@ -370,7 +375,7 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
         }
         if (a->dx) {
             GradArgs g{};
-            g.a = Operand{c.w.p, c.w.ld, vn, c.w.cols}; g.b = Operand{ws + p.d, c.ldd, a->n, c.ldd};
+            g.a = Operand{c.w.p, c.w.ld, vn, c.w.cols}; g.b = Operand{ws + p.d, c.ldd, a->n, c.dcols * p.per};
             g.ktiles = (int)((vn + p.ks - 1) / p.ks); g.m = a->hidden; g.n = a->n;
             g.amax = f32(p.wmax); g.factor = f32(p.factor);
             const bool acc = p.gx.splits > 1 || p.pieces > 1;
@@ -386,7 +391,7 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
         }
         if (a->dw) {
             GradArgs g{};
-            g.a = c.x; g.b = Operand{ws + p.d, c.ldd, a->n, c.ldd};
+            g.a = c.x; g.b = Operand{ws + p.d, c.ldd, a->n, c.dcols * p.per};
             g.ktiles = (int)((a->n + p.ks - 1) / p.ks); g.m = a->hidden; g.n = vn;
             g.amax = f32(p.xmax); g.factor = f32(p.factor);
             g.acc = p.gw.splits > 1 ? f32(p.dwacc) : nullptr; g.add = false;
