@@ -74,7 +74,6 @@ struct TileShape {
 };
 
 typedef __attribute__((address_space(3))) void *lds_ptr;
-typedef const __attribute__((address_space(1))) void *glb_ptr;
 typedef short sx4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) sx4 *lds_sx4;
 
@@ -162,13 +161,18 @@ struct TileProduct {
     }
     // 16 bytes a lane from base + off to LDS at `to` + 16 lane.  Written out because the compiler, which cannot tell the
     // ring's places apart, would wait for all of these loads in front of every transposing read; what is read has arrived is
-    // seen to by meet().  Buffer addressing: a scalar base that moves and a 32-bit offset that stays, in range by construction.
+    // seen to by meet().  (No other instruction of these kernels uses m0.)  Buffer addressing: a scalar base that moves and a
+    // 32-bit offset that stays, in range by construction.
     static __device__ inline void load_lds(const char *base, unsigned off, unsigned to)
     {
         typedef unsigned ux4 __attribute__((ext_vector_type(4)));
         const uint64_t at = reinterpret_cast<uint64_t>(base);
         const ux4 rsrc = {(unsigned)at, (unsigned)(at >> 32) & 0xFFFFu, 0xFFFFFFFFu, 0x00020000u};
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(rsrc) : "memory", "m0");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(rsrc) : "memory");
+    }
+    static __device__ inline void load_lds(const char *from, unsigned to)        // from an address of the lane's own
+    {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
     }
     // Own reads done and all but the newest `left` of the own loads arrived; then everyone's.  (A barrier by itself does not
     // wait for loads that write LDS.)
@@ -219,13 +223,13 @@ struct TileProduct {
                 for (int i = 0; i < loads; i++) load(side_a, i);
             } else {
                 const char *base = a_side ? base_a : base_b;
-                char *to = (a_side ? lds + slot_a * S::bytes_a : lds_b + slot_b * S::bytes_b) + wave * 1024;
+                const unsigned to = lds0 + (a_side ? slot_a * S::bytes_a : S::ring_a * S::bytes_a + slot_b * S::bytes_b);
                 const long long left = a_side ? A_::kcount(A) - (long long)la * A_::kstep : B_::kcount(B) - (long long)lb * B_::kstep;
 #pragma unroll
                 for (int i = 0; i < loads; i++) {
                     const char *p = base + (a_side ? off_a[i] : off_b[i]);
                     if ((a_side ? at_a[i] : at_b[i]) >= left) p = reinterpret_cast<const char *>(g_zero_page);
-                    __builtin_amdgcn_global_load_lds((glb_ptr)p, (lds_ptr)(to + i * S::waves * 1024), 16, 0, 0);
+                    load_lds(p, to + i * S::waves * 1024);
                 }
             }
         };
@@ -481,12 +485,12 @@ struct CeArgs {
     const float *probs;           // [n][ldp], already offset to the piece's first class
     long long ldp;
     // statistics, one entry a row and a wave's run of TM / WM classes ("span")
-    float2 *part;                 // [spans][n]: maximum, sum of exp(l - maximum)
-    float *part_e;                // [spans][n]: sum of exp(l - maximum) l, or null
+    float2 *part;                 // [spans][n]: M = maximum times log2e, sum of 2^(l log2e - M)
+    float *part_e;                // [spans][n]: sum of 2^(l log2e - M) l, or null
     float4 *part_t;               // probabilities: sum pi l, sum pi, sum |pi|, -
     float *tlogit;                // index: [n]
     // gradient
-    const float4 *stats;          // [n]: m, sum pi / s, ... (RowArgs)
+    const float4 *stats;          // [n]: M, sum pi / s, ... (RowArgs)
     const float *rowg;            // [n]
     void *d;                      // image [n][ldd] of D; statistics: of exp(l - the span's maximum), or null
     long long ldd, dcols;         // row stride in image elements; padded classes
@@ -517,15 +521,17 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
     const float ux = Op::split ? 1.f / split_scale(max_of_parts(a.xmax)) : 1.f, uw = Op::split ? 1.f / split_scale(max_of_parts(a.wmax)) : 1.f;
     const typename Op::In *bias = static_cast<const typename Op::In *>(a.bias);
     const long long vw = m0 + wm * (TM / WM) + 4 * (lane >> 4);                  // this lane's first class of the piece
+    if (Op::split || bias || m0 + TM > a.classes) {
 #pragma unroll
-    for (int mt = 0; mt < S::MT; mt++)
+        for (int mt = 0; mt < S::MT; mt++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const long long v = vw + mt * 16 + i;
-            const float b = bias && v < a.classes ? (float)bias[v] : 0.f;
+            for (int i = 0; i < 4; i++) {
+                const long long v = vw + mt * 16 + i;
+                const float b = bias && v < a.classes ? (float)bias[v] : 0.f;
 #pragma unroll
-            for (int nt = 0; nt < S::NT; nt++) acc[mt][nt][i] = v < a.classes ? acc[mt][nt][i] * ux * uw + b : -INFINITY;
-        }
+                for (int nt = 0; nt < S::NT; nt++) acc[mt][nt][i] = v < a.classes ? acc[mt][nt][i] * ux * uw + b : -INFINITY;
+            }
+    }
     const long long nw = n0 + wn * (TN / WN) + (lane & 15);
     const long long dpad = a.dcols;
     if constexpr (!GRAD) {
@@ -542,7 +548,9 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
                 for (int i = 0; i < 4; i++) mx = fmaxf(mx, acc[mt][nt][i]);
             mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            // (a NaN is passed over by fmaxf: it comes back through the sum; a maximum of -inf leaves every term exp(-inf))
+            // Sums are of 2^(l log2e - M), M = the maximum times log2e as rounded: one operation in front of the exponential.
+            // (A NaN is passed over by fmaxf: it comes back through the sum; a maximum of -inf leaves every term 2^-inf.)
+            mx *= kLog2e;
             const float base = mx == -INFINITY ? 0.f : mx;
             float s = 0.f, e = 0.f, tl = 0.f, ts = 0.f, ta = 0.f;
 #pragma unroll
@@ -550,7 +558,7 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
                 Pack<E, 4> keep;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float l = acc[mt][nt][i], x = __builtin_amdgcn_exp2f((l - base) * kLog2e);
+                    const float l = acc[mt][nt][i], x = __builtin_amdgcn_exp2f(__builtin_fmaf(l, kLog2e, -base));
                     s += x;
                     if (a.part_e) e += x != 0.f ? x * l : 0.f;
                     keep.v[i] = (E)x;
@@ -613,7 +621,7 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
                 const long long cls = vw + mt * 16;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    float q = __builtin_amdgcn_exp2f((acc[mt][nt][i] - st.x) * kLog2e) * st.y;
+                    float q = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mt][nt][i], kLog2e, -st.x)) * st.y;
                     if (pr) { if (live && cls + i < a.classes) q -= pr[cls + i]; }
                     else if (t == mt * 16 + i) q -= 1.f;
                     q = g == 0.f || cls + i >= a.classes ? 0.f : q * g;         // a row that counts for nothing: zero whatever it holds
@@ -652,73 +660,73 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
 }
 
 // ---------------------------------------------------------------- exponentials -> D, in place
-constexpr int kFixRows = 128, kFixCols = 128;
+constexpr int kFixRows = 64, kFixCols = 512;
 struct FixArgs {
-    long long n, classes, span;   // classes an entry of part stands for
+    long long n, classes;
+    int span;                     // classes an entry of part stands for
     void *d; long long ldd, dcols;
     const float2 *part; const float4 *stats; const float *rowg;
     const long long *target;
     const float *probs; long long ldp;
     float *dbpart;                // [blocks of kFixRows][classes] or null
 };
-// 128 rows x 128 classes per workgroup, sixteen threads a row with eight classes each
+// 64 rows x 512 classes per workgroup; a wave takes a row at a time, a lane eight classes of it.  Bound by memory: 2 bytes
+// (float32: 4) read and written an element.
 template <typename Op>
 __global__ __launch_bounds__(256) void fix_kernel(FixArgs a)
 {
-    __shared__ float red[16][kFixCols + 1];
-    const int tid = threadIdx.x, rg = tid >> 4, cl = (tid & 15) * 8;
-    const long long c0 = (long long)blockIdx.x * kFixCols, r0 = (long long)blockIdx.y * kFixRows, c = c0 + cl;
-    const long long dpad = a.dcols, lde = a.ldd / (Op::split ? 2 : 1);
+    using V = typename Frag<typename Op::Img>::V;
+    __shared__ float red[4][kFixCols];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const long long c0 = (long long)blockIdx.x * kFixCols, c = c0 + lane * 8;
+    const long long r0 = (long long)blockIdx.y * kFixRows, lde = a.ldd / (Op::split ? 2 : 1);
+    const float2 *part = a.part + (c < a.classes ? c : 0) / a.span * a.n;
     float db[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (c < dpad)
 #pragma unroll 4
-        for (int j = 0; j < kFixRows / 16; j++) {
-            const long long row = r0 + j * 16 + rg;
-            if (row >= a.n) break;
-            const float4 st = a.stats[row];
-            const float g = a.rowg[row], mp = a.part[c / a.span * a.n + row].x;
-            const float f = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mp - st.x) * kLog2e) * st.y;
-            const long long t = a.target ? a.target[row] - c : -1;
-            float v[8];
-            if constexpr (Op::split) {
-                const fx4 *p = reinterpret_cast<const fx4 *>(static_cast<float *>(a.d) + row * lde + c);
-                const fx4 v0 = p[0], v1 = p[1];
+    for (int j = 0; j < kFixRows / 4; j++) {
+        const long long row = r0 + j * 4 + wave;
+        if (row >= a.n) break;
+        const float4 st = a.stats[row];
+        const float g = a.rowg[row];
+        const long long t = a.target ? a.target[row] - c : -1;
+        if (c >= a.dcols) continue;
+        const float mp = part[row].x, f = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mp - st.x) * st.y;
+        float v[8];
+        if constexpr (Op::split) {
+            const fx4 *p = reinterpret_cast<const fx4 *>(static_cast<float *>(a.d) + row * lde + c);
+            const fx4 v0 = p[0], v1 = p[1];
 #pragma unroll
-                for (int i = 0; i < 4; i++) { v[i] = v0[i]; v[4 + i] = v1[i]; }
-            } else {
-                const hx8 p = *reinterpret_cast<const hx8 *>(static_cast<_Float16 *>(a.d) + row * lde + c);
+            for (int i = 0; i < 4; i++) { v[i] = v0[i]; v[4 + i] = v1[i]; }
+        } else {
+            const hx8 p = *reinterpret_cast<const hx8 *>(static_cast<_Float16 *>(a.d) + row * lde + c);
 #pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = (float)p[i];
-            }
-            typename Frag<typename Op::Img>::V h, l;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const bool out = c + i >= a.classes;
-                float q = v[i] * f;
-                if (a.probs) { if (!out) q -= a.probs[row * a.ldp + c + i]; }
-                else if (t == i) q -= 1.f;
-                q = g == 0.f || out ? 0.f : q * g;
-                db[i] += q;
-                q *= kDScale;
-                h[i] = (typename Op::Img)q;
-                if (Op::split) l[i] = (typename Op::Img)(q - (float)h[i]);
-            }
-            // (float32: the halves land on exponentials of the same row that other lanes of this wave have read: a wave's
-            //  stores follow the loads that every one of its values depends on)
-            typename Op::Img *o = static_cast<typename Op::Img *>(a.d) + row * a.ldd + (Op::split ? (c >> 5) * 64 + (c & 31) : c);
-            *reinterpret_cast<typename Frag<typename Op::Img>::V *>(o) = h;
-            if (Op::split) *reinterpret_cast<typename Frag<typename Op::Img>::V *>(o + 32) = l;
+            for (int i = 0; i < 8; i++) v[i] = (float)p[i];
         }
+        V h, l;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const bool out = c + i >= a.classes;
+            float q = v[i] * f;
+            if (a.probs) { if (!out) q -= a.probs[row * a.ldp + c + i]; }
+            else if (t == i) q -= 1.f;
+            q = g == 0.f || out ? 0.f : q * g;                                  // a row that counts for nothing: zero whatever it holds
+            db[i] += q;
+            q *= kDScale;
+            h[i] = (typename Op::Img)q;
+            if (Op::split) l[i] = (typename Op::Img)(q - (float)h[i]);
+        }
+        // (float32: the halves land on exponentials of the same row that other lanes of this wave have read: a wave's
+        //  stores follow the loads that every one of its values depends on)
+        typename Op::Img *o = static_cast<typename Op::Img *>(a.d) + row * a.ldd + (Op::split ? (c >> 5) * 64 + (c & 31) : c);
+        *reinterpret_cast<V *>(o) = h;
+        if (Op::split) *reinterpret_cast<V *>(o + 32) = l;
+    }
     if (!a.dbpart) return;
 #pragma unroll
-    for (int i = 0; i < 8; i++) red[rg][cl + i] = db[i];
+    for (int i = 0; i < 8; i++) red[wave][lane * 8 + i] = db[i];
     __syncthreads();
-    if (tid < kFixCols && c0 + tid < a.classes) {
-        float s = 0.f;
-#pragma unroll
-        for (int w = 0; w < 16; w++) s += red[w][tid];
-        a.dbpart[(long long)blockIdx.y * a.classes + c0 + tid] = s;
-    }
+    for (int i = tid; i < kFixCols; i += 256)
+        if (c0 + i < a.classes) a.dbpart[(long long)blockIdx.y * a.classes + c0 + i] = (red[0][i] + red[1][i]) + (red[2][i] + red[3][i]);
 }
 
 // ---------------------------------------------------------------- rows and totals
@@ -727,7 +735,7 @@ struct RowArgs {
     int spans;
     const float2 *part; const float *part_e; const float4 *part_t; const float *tlogit;
     const long long *target; long long ignore;
-    float4 *stats;                // [n]: m, sum pi / s, sum |pi|, loss with lse = m + log s (so that p takes no rounding of lse)
+    float4 *stats;                // [n]: M, sum pi / s, sum |pi|, loss with lse = M ln2 + log s (so that p takes no rounding of lse)
     float *ent;                   // [n] or null
 };
 // one wave per row: join the spans' (maximum, sum) pairs in a fixed order
@@ -740,7 +748,7 @@ __global__ __launch_bounds__(256) void rows_kernel(RowArgs a)
     for (int t = lane; t < a.spans; t += 64) {
         const float2 p = a.part[(long long)t * a.n + row];
         const float m = fmaxf(mx, p.x), base = m == -INFINITY ? 0.f : m;
-        const float f0 = __builtin_amdgcn_exp2f((mx - base) * kLog2e), f1 = __builtin_amdgcn_exp2f((p.x - base) * kLog2e);
+        const float f0 = __builtin_amdgcn_exp2f(mx - base), f1 = __builtin_amdgcn_exp2f(p.x - base);
         // (a pair without a class adds nothing; a NaN sum stays NaN)
         s = (mx == -INFINITY ? s : s * f0) + (p.x == -INFINITY ? p.y : p.y * f1);
         if (a.part_e) {
@@ -754,20 +762,20 @@ __global__ __launch_bounds__(256) void rows_kernel(RowArgs a)
     for (int d = 1; d < 64; d <<= 1) {
         const float om = __shfl_xor(mx, d, 64), os = __shfl_xor(s, d, 64), oe = __shfl_xor(e, d, 64);
         const float m = fmaxf(mx, om), base = m == -INFINITY ? 0.f : m;
-        const float f0 = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mx - base) * kLog2e);
-        const float f1 = om == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((om - base) * kLog2e);
+        const float f0 = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - base);
+        const float f1 = om == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(om - base);
         s = s * f0 + os * f1; e = e * f0 + oe * f1; mx = m;
         if (a.part_t) { tl += __shfl_xor(tl, d, 64); ts += __shfl_xor(ts, d, 64); ta += __shfl_xor(ta, d, 64); }
     }
     if (lane) return;
-    const float ls = logf(s), lse = (mx == -INFINITY ? 0.f : mx) + ls;
+    const float ls = logf(s), m = mx == -INFINITY ? 0.f : mx * kLn2, lse = m + ls;
     float loss, ent = lse - e / s;
     if (a.target) {
         const long long t = a.target[row];
         ts = ta = 1.f;
         if (t == a.ignore) { loss = 0.f; ent = 0.f; ts = ta = 0.f; }
         else if (t < 0 || t >= a.classes) { loss = ent = NAN; ts = ta = NAN; }
-        else loss = (mx - a.tlogit[row]) + ls;
+        else loss = (m - a.tlogit[row]) + ls;
     } else {
         loss = lse * ts - tl;
     }
