@@ -9,6 +9,7 @@
 #include "../../include/azgomoku.h"
 #include "azg_dropout.hpp"
 #include "azg_linear_ce.hpp"
+#include "azg_linear_ce_small.hpp"
 
 using namespace azgops;
 
@@ -97,6 +98,9 @@ extern "C" int azg_dropout(const azg_dropout_args *a)
 // ---------------------------------------------------------------- projection + softmax cross entropy
 namespace {
 
+// Problems of at most this many multiplications a product (and classes) take the three-launch float32 path: AAA
+constexpr long long kSmallWork = 1LL << 27, kSmallClasses = 4096;
+
 // Room that the images of D, of W and of its transpose may take together before the classes are cut into pieces.
 constexpr long long kPieceBytes = 1LL << 30;
 
@@ -134,13 +138,13 @@ GradPick pick_grad(long long m, long long n, long long ktiles)
 }
 
 struct Plan {
-    bool split, forward, backward, pack_w, pack_x, keep;      // keep: the forward pass leaves exponentials for the backward pass
+    bool small, split, forward, backward, pack_w, pack_x, keep;      // keep: the forward pass leaves exponentials for the backward pass
     long long n, H, V, vp, pieces;
     long long kimg, ldk, ldd;                                 // image elements along the features; row strides of the images of X, W and D
     int per, ks;                                              // image elements an element takes, k of a stage
     Shape lshape;
     GradPick gx, gw;
-    size_t xmax, wmax, ximg, wimg, part, part_e, part_t, tlogit, stats, ent, rowg, factor, d, dbpart, dxacc, dwacc, total;
+    size_t xmax, wmax, ximg, wimg, part, part_e, part_t, tlogit, stats, ent, rowg, factor, d, dbpart, dxacc, dwacc, logits, count, total;
 };
 
 bool aligned16(const void *p, long long stride, long long cols, long long rows)
@@ -156,6 +160,16 @@ int make_plan(const azg_linear_ce_args *a, Plan *p)
     p->forward = a->loss != nullptr;
     p->backward = a->dx || a->dw || a->db;
     p->n = a->n; p->H = a->hidden; p->V = a->classes;
+    p->small = p->V <= kSmallClasses && (double)p->n * (double)p->H * (double)p->V <= (double)kSmallWork;
+    if (p->small) {
+        Take t;
+        p->logits = t((size_t)p->n * p->V * 4);
+        p->stats = t((size_t)p->n * 16);
+        p->ent = t((size_t)p->n * 4);
+        p->count = t(4);
+        p->total = t.off;
+        return AZG_OK;
+    }
     p->kimg = up_to(p->H, p->ks) * p->per;
     p->ldk = image_stride(p->kimg);
     // (dW multiplies the rows that count for nothing by zero: they are copied as zeros, whatever they hold)
@@ -415,6 +429,39 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
 }
 
 template <typename In>
+int run_small(const azg_linear_ce_args *a, const Plan &p)
+{
+    hipStream_t s = static_cast<hipStream_t>(a->stream);
+    char *ws = static_cast<char *>(a->workspace);
+    SmallArgs g{};
+    g.x = a->x; g.w = a->w; g.bias = a->bias; g.xs = a->x_stride; g.ws = a->w_stride;
+    g.n = (int)a->n; g.H = (int)a->hidden; g.V = (int)a->classes;
+    g.target = reinterpret_cast<const long long *>(a->target); g.ignore = a->ignore_index; g.probs = a->probs; g.ldp = a->probs_stride;
+    g.logits = reinterpret_cast<float *>(ws + p.logits); g.ldl = g.V;
+    // (a backward pass by itself repeats the rows' statistics; the caller's are left alone)
+    g.stats = a->stats && p.forward ? static_cast<float4 *>(a->stats) : reinterpret_cast<float4 *>(ws + p.stats);
+    g.ent = a->entropy ? reinterpret_cast<float *>(ws + p.ent) : nullptr;
+    g.reduction = a->reduction; g.loss = a->loss; g.ent_out = a->entropy;
+    g.dloss = a->dloss; g.grad_scale = (float)a->grad_scale;
+    g.count = reinterpret_cast<int *>(ws + p.count);
+    g.backward = p.backward; g.dx = a->dx; g.dw = a->dw; g.db = a->db; g.dxs = a->dx_stride; g.dws = a->dw_stride;
+    auto tiles = [](int v) { return (v + kSmallTile - 1) / kSmallTile; };
+    hipLaunchKernelGGL((small_logits_kernel<In>), dim3(tiles(g.n) * tiles(g.V) + 1), dim3(256), 0, s, g);
+    hipLaunchKernelGGL(small_rows_kernel, dim3(g.n), dim3(256), 0, s, g);
+    const bool totals = p.forward && g.reduction != AZG_REDUCE_NONE;
+    if (p.backward) {
+        g.tiles_x = g.dx ? tiles(g.n) * tiles(g.H) : 0;
+        g.tiles_w = g.dw ? tiles(g.V) * tiles(g.H) : 0;
+        const int grid = g.tiles_x + g.tiles_w + (g.db ? (g.V + 63) / 64 : 0) + (totals ? 1 : 0);
+        hipLaunchKernelGGL((small_grads_kernel<In>), dim3(grid), dim3(256), 0, s, g);
+    } else if (totals) {
+        hipLaunchKernelGGL(small_totals_kernel, dim3(1), dim3(256), 0, s, g);
+    }
+    OPS_HIP(hipGetLastError());
+    return AZG_OK;
+}
+
+template <typename In>
 int empty_batch(const azg_linear_ce_args *a)
 {
     hipStream_t s = static_cast<hipStream_t>(a->stream);
@@ -461,6 +508,7 @@ extern "C" int azg_linear_ce(const azg_linear_ce_args *a)
     OPS_TRY(make_plan(a, &p));
     if (!a->workspace || (reinterpret_cast<uintptr_t>(a->workspace) & 255) || a->workspace_bytes < (int64_t)p.total)
         return fail(AZG_EINVAL, "azg_linear_ce: the workspace must be 256-byte aligned and hold %lld bytes", (long long)p.total);
+    if (p.small) return a->dtype == AZG_F32 ? run_small<float>(a, p) : a->dtype == AZG_F16 ? run_small<_Float16>(a, p) : run_small<__bf16>(a, p);
     if (a->dtype == AZG_F32) return run_ce<OpF32>(a, p);
     if (a->dtype == AZG_F16) return run_ce<OpF16>(a, p);
     return run_ce<OpBF16>(a, p);
