@@ -267,11 +267,11 @@ struct TileProduct {
                     if (mt * S::NT + nt >= i0 && mt * S::NT + nt < i1)
                         acc[half * MH + mt][nt] = F::mfma(a[p & 1][mt], b[h][nt], acc[half * MH + mt][nt]);
         };
-        // phase p's matrix instructions (with B's fragments h; float32, even phases: h = 0 and 1) behind its `reads` LDS reads,
+        // phase p's matrix instructions (with B's fragments h; float32, even phases: h = 1, then 0) behind its `reads` LDS reads,
         // with loads l0 .. l1 - 1 of the next stage of a side near their end
         auto phase = [&](int p, int h, auto reads, auto both, auto side, auto l0, auto l1) {
             constexpr int loads = l1.value - l0.value, per = loads ? loads : 1, tail = PP - 2 * loads > 0 ? PP - 2 * loads : 0, total = both.value ? PP + tail : tail;
-            if constexpr (both.value) { products(p, 0, 0, PP); products(p, 1, 0, tail); }
+            if constexpr (both.value) { products(p, 1, 0, PP); products(p, 0, 0, tail); }
             else products(p, h, 0, tail);
             interleave<total, reads.value>();
 #pragma unroll
@@ -279,7 +279,7 @@ struct TileProduct {
                 __builtin_amdgcn_sched_barrier(0);
                 load(side, l0.value + i);
                 __builtin_amdgcn_sched_barrier(0);
-                products(p, both.value ? 1 : h, tail + (PP - tail) * i / per, tail + (PP - tail) * (i + 1) / per);
+                products(p, both.value ? 0 : h, tail + (PP - tail) * i / per, tail + (PP - tail) * (i + 1) / per);
             }
             phase_end();
         };
@@ -293,8 +293,7 @@ struct TileProduct {
         }
         if (k1 - k0 >= S::ring_a) meet<(S::ring_a - 1) * kLoadsA + (S::ring_b - 1) * kLoadsB>();
         else meet<0>();
-        read_b(b[0], 0, 0);
-        if (Op::split) read_b(b[1], 0, 1);
+        read_b(b[Op::split], 0, Op::split);
         read_a(0, 0);
         int kt = k0;
         constexpr int B1 = kLoadsB / 2, A1 = kLoadsA / 2;
@@ -306,9 +305,10 @@ struct TileProduct {
         auto stage = [&](auto fast_, auto full_) {            // fast: with the loads of a steady state; full: the rings are
             constexpr bool fast = fast_.value, full = full_.value;
             const int sa = ra + 1 == S::ring_a ? 0 : ra + 1, sb = rb + 1 == S::ring_b ? 0 : rb + 1;
-            if constexpr (Op::split) {                        // (hi hi, hi lo), (lo hi) for either half of A
+            if constexpr (Op::split) {                        // (hi lo, hi hi), (lo hi) for either half of A; B's hi arrives behind the first
+                read_b(b[0], rb, 0);
                 read_a(ra, 1);
-                phase(0, 0, AZG_INT(MH * RA), yes, side_b, AZG_INT(B1), AZG_INT(fast ? kLoadsB : B1));
+                phase(0, 0, AZG_INT(MH * RA + S::NT * RB), yes, side_b, AZG_INT(B1), AZG_INT(fast ? kLoadsB : B1));
                 if (fast) next_b();
                 read_a(ra, 2);
                 phase(1, 0, AZG_INT(MH * RA), no, side_a, AZG_INT(0), AZG_INT(fast ? A1 : 0));
@@ -329,12 +329,8 @@ struct TileProduct {
             // (after the last stage what is read is stale and not used)
             read_a(sa, 0);
             if constexpr (Op::split) {
-                typename F::V bn[2][S::NT];
-                read_b(bn[0], sb, 0);
-                read_b(bn[1], sb, 1);
-                phase(3, 0, AZG_INT(MH * RA + 2 * S::NT * RB), no, side_b, AZG_INT(0), AZG_INT(fast ? B1 : 0));
-#pragma unroll
-                for (int t = 0; t < S::NT; t++) { b[0][t] = bn[0][t]; b[1][t] = bn[1][t]; }
+                read_b(b[1], sb, 1);
+                phase(3, 0, AZG_INT(MH * RA + S::NT * RB), no, side_b, AZG_INT(0), AZG_INT(fast ? B1 : 0));
             } else {
                 read_b(b[0], sb, 0);
                 phase(3, 1, AZG_INT(MH * RA + S::NT * RB), no, side_b, AZG_INT(0), AZG_INT(fast ? B1 : 0));
@@ -389,7 +385,7 @@ struct PackArgs {
     long long ldi, icols;         // row stride, padded columns (image elements)
     const long long *target;      // not null: rows whose target is ignore_index are read as zero
     long long ignore;
-    const float *maxpart;         // float32: kMaxParts partial maxima of the tensor
+    float *maxpart;               // float32: kMaxParts partial maxima of the tensor
 };
 constexpr int kMaxParts = 256;
 
@@ -412,14 +408,17 @@ __device__ inline float max_of_parts(const float *parts)                        
     return m;
 }
 
-// partial maxima of the finite magnitudes of a float32 tensor (rows whose target is ignore_index left out)
-__global__ __launch_bounds__(256) void absmax_kernel(PackArgs a, float *parts)
+// partial maxima of the finite magnitudes of two float32 tensors (rows whose target is ignore_index left out), kMaxParts
+// workgroups each
+__global__ __launch_bounds__(256) void absmax_kernel(PackArgs a0, PackArgs a1)
 {
     __shared__ float red[4];
+    const PackArgs a = blockIdx.x < kMaxParts ? a0 : a1;
+    const unsigned wg = blockIdx.x % kMaxParts;
     const float *src = static_cast<const float *>(a.src);
     float m = 0.f;
     const long long per_row = (a.cols + 1023) / 1024, total = a.rows * per_row;
-    for (long long u = blockIdx.x; u < total; u += gridDim.x) {
+    for (long long u = wg; u < total; u += kMaxParts) {
         const long long row = u / per_row, c0 = (u - row * per_row) * 1024 + threadIdx.x * 4;
         if (a.target && a.target[row] == a.ignore) continue;
         const float *p = src + row * a.ld;
@@ -431,17 +430,20 @@ __global__ __launch_bounds__(256) void absmax_kernel(PackArgs a, float *parts)
     for (int s = 1; s < 64; s <<= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
     __syncthreads();
-    if (threadIdx.x == 0) parts[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    if (threadIdx.x == 0) a.maxpart[wg] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
 
-// The image of a matrix, zeros in the padding: a thread eight columns of a row.
+// The images of two matrices, zeros in the padding: a thread eight columns of a row; the first matrix has wgs0 workgroups.
 template <typename Op>
-__global__ __launch_bounds__(256) void pack_kernel(PackArgs a)
+__global__ __launch_bounds__(256) void pack_kernel(PackArgs a0, PackArgs a1, unsigned wgs0)
 {
     constexpr int per = Op::split ? 2 : 1;
+    const bool first = blockIdx.x < wgs0;
+    const PackArgs a = first ? a0 : a1;
+    const unsigned wg = first ? blockIdx.x : blockIdx.x - wgs0, wgs = first ? wgs0 : gridDim.x - wgs0;
     const float scale = Op::split ? split_scale(max_of_parts(a.maxpart)) : 1.f;
     const long long row_chunks = a.icols / (8 * per), total = a.rows * row_chunks;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    for (long long i = (long long)wg * 256 + threadIdx.x; i < total; i += (long long)wgs * 256) {
         const long long r = i / row_chunks, c = (i - r * row_chunks) * 8;
         const typename Op::In *p = static_cast<const typename Op::In *>(a.src) + r * a.ld + c;
         const bool skip = a.target && a.target[r] == a.ignore;
@@ -659,76 +661,6 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
     }
 }
 
-// ---------------------------------------------------------------- exponentials -> D, in place
-constexpr int kFixRows = 64, kFixCols = 512;
-struct FixArgs {
-    long long n, classes;
-    int span;                     // classes an entry of part stands for
-    void *d; long long ldd, dcols;
-    const float2 *part; const float4 *stats; const float *rowg;
-    const long long *target;
-    const float *probs; long long ldp;
-    float *dbpart;                // [blocks of kFixRows][classes] or null
-};
-// 64 rows x 512 classes per workgroup; a wave takes a row at a time, a lane eight classes of it.  Bound by memory: 2 bytes
-// (float32: 4) read and written an element.
-template <typename Op>
-__global__ __launch_bounds__(256) void fix_kernel(FixArgs a)
-{
-    using V = typename Frag<typename Op::Img>::V;
-    __shared__ float red[4][kFixCols];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const long long c0 = (long long)blockIdx.x * kFixCols, c = c0 + lane * 8;
-    const long long r0 = (long long)blockIdx.y * kFixRows, lde = a.ldd / (Op::split ? 2 : 1);
-    const float2 *part = a.part + (c < a.classes ? c : 0) / a.span * a.n;
-    float db[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int j = 0; j < kFixRows / 4; j++) {
-        const long long row = r0 + j * 4 + wave;
-        if (row >= a.n) break;
-        const float4 st = a.stats[row];
-        const float g = a.rowg[row];
-        const long long t = a.target ? a.target[row] - c : -1;
-        if (c >= a.dcols) continue;
-        const float mp = part[row].x, f = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mp - st.x) * st.y;
-        float v[8];
-        if constexpr (Op::split) {
-            const fx4 *p = reinterpret_cast<const fx4 *>(static_cast<float *>(a.d) + row * lde + c);
-            const fx4 v0 = p[0], v1 = p[1];
-#pragma unroll
-            for (int i = 0; i < 4; i++) { v[i] = v0[i]; v[4 + i] = v1[i]; }
-        } else {
-            const hx8 p = *reinterpret_cast<const hx8 *>(static_cast<_Float16 *>(a.d) + row * lde + c);
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = (float)p[i];
-        }
-        V h, l;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const bool out = c + i >= a.classes;
-            float q = v[i] * f;
-            if (a.probs) { if (!out) q -= a.probs[row * a.ldp + c + i]; }
-            else if (t == i) q -= 1.f;
-            q = g == 0.f || out ? 0.f : q * g;                                  // a row that counts for nothing: zero whatever it holds
-            db[i] += q;
-            q *= kDScale;
-            h[i] = (typename Op::Img)q;
-            if (Op::split) l[i] = (typename Op::Img)(q - (float)h[i]);
-        }
-        // (float32: the halves land on exponentials of the same row that other lanes of this wave have read: a wave's
-        //  stores follow the loads that every one of its values depends on)
-        typename Op::Img *o = static_cast<typename Op::Img *>(a.d) + row * a.ldd + (Op::split ? (c >> 5) * 64 + (c & 31) : c);
-        *reinterpret_cast<V *>(o) = h;
-        if (Op::split) *reinterpret_cast<V *>(o + 32) = l;
-    }
-    if (!a.dbpart) return;
-#pragma unroll
-    for (int i = 0; i < 8; i++) red[wave][lane * 8 + i] = db[i];
-    __syncthreads();
-    for (int i = tid; i < kFixCols; i += 256)
-        if (c0 + i < a.classes) a.dbpart[(long long)blockIdx.y * a.classes + c0 + i] = (red[0][i] + red[1][i]) + (red[2][i] + red[3][i]);
-}
-
 // ---------------------------------------------------------------- rows and totals
 struct RowArgs {
     long long n, classes;
@@ -791,18 +723,20 @@ struct TotalArgs {
     float *loss, *ent_out;        // [n] or [1]; null: not asked for
     const float *dloss;           // [n], [1] or null
     float grad_scale;
-    float *rowg;                  // [n]: g_i / 2^e, or null without a backward pass
-    float *factor;                // [1]: 2^e (times the common g)
+    float *rowg;                  // [n]: g_i / 2^e; null: every row that counts has 1 (class numbers and a common g) or no gradient is asked for
+    float *factor;                // [1]: 2^e (times the common g); null without a backward pass
 };
 // totals of the rows in a fixed order, in double; the rows' gradient factors, scaled so that the largest |D| fits an image
-__global__ __launch_bounds__(1024) void totals_kernel(TotalArgs a)
+template <int THREADS>
+__device__ inline void totals(const TotalArgs &a)
 {
-    __shared__ double red[3][16];
-    __shared__ float redm[16];
+    constexpr int W = THREADS / 64;
+    __shared__ double red[3][W];
+    __shared__ float redm[W];
     const int tid = threadIdx.x;
     double sl = 0.0, se = 0.0, cnt = 0.0;
     float mx = 0.f;
-    for (long long i = tid; i < a.n; i += 1024) {
+    for (long long i = tid; i < a.n; i += THREADS) {
         const float4 st = a.stats[i];
         const bool used = !(a.target && a.target[i] == a.ignore);
         sl += st.w; cnt += used ? 1.0 : 0.0;
@@ -824,54 +758,131 @@ __global__ __launch_bounds__(1024) void totals_kernel(TotalArgs a)
     if ((tid & 63) == 0) { red[0][tid >> 6] = sl; red[1][tid >> 6] = se; red[2][tid >> 6] = cnt; redm[tid >> 6] = mx; }
     __syncthreads();
     sl = se = cnt = 0.0; mx = 0.f;
-    for (int i = 0; i < 16; i++) { sl += red[0][i]; se += red[1][i]; cnt += red[2][i]; mx = fmaxf(mx, redm[i]); }
+    for (int i = 0; i < W; i++) { sl += red[0][i]; se += red[1][i]; cnt += red[2][i]; mx = fmaxf(mx, redm[i]); }
     const double by = a.reduction == 2 ? (cnt > 0.0 ? 1.0 / cnt : 0.0) : 1.0;
     if (a.reduction && tid == 0) {
         if (a.loss) a.loss[0] = (float)(sl * by);
         if (a.ent_out) a.ent_out[0] = (float)(se * by);
     }
-    if (!a.rowg) return;
+    if (!a.factor) return;
     // 2^e >= the largest g_i sum|pi_i| (1 for an index target and a common g)
     float up = 1.f;
-    if (mx > 0.f) {
+    if (a.rowg && mx > 0.f) {
         int E = (int)((__builtin_bit_cast(uint32_t, mx) >> 23) & 255) - 126;     // mx <= 2^E
         if ((__builtin_bit_cast(uint32_t, mx) & 0x7FFFFFu) == 0) E--;
         E = E > 126 ? 126 : (E < -120 ? -120 : E);
         up = __builtin_bit_cast(float, (uint32_t)((E + 127) << 23));
     }
-    for (long long i = tid; i < a.n; i += 1024) {
-        const bool used = !(a.target && a.target[i] == a.ignore);
-        const float g = a.reduction == 0 ? (a.dloss ? a.dloss[i] : 1.f) * a.grad_scale : 1.f;
-        a.rowg[i] = used ? g / up : 0.f;
-    }
+    if (a.rowg)
+        for (long long i = tid; i < a.n; i += THREADS) {
+            const bool used = !(a.target && a.target[i] == a.ignore);
+            const float g = a.reduction == 0 ? (a.dloss ? a.dloss[i] : 1.f) * a.grad_scale : 1.f;
+            a.rowg[i] = used ? g / up : 0.f;
+        }
     if (tid == 0) {
         const float common = a.reduction ? (a.dloss ? a.dloss[0] : 1.f) * a.grad_scale * (float)by : 1.f;
         a.factor[0] = up * common;
     }
 }
+__global__ __launch_bounds__(1024) void totals_kernel(TotalArgs a) { totals<1024>(a); }
+
+// ---------------------------------------------------------------- exponentials -> D, in place
+constexpr int kFixCols = 512;
+struct FixArgs {
+    long long n, classes;
+    int rows;                     // a workgroup's, a multiple of 4
+    TotalArgs totals;             // the last row of workgroups does these instead (rowg null), or has n < 0
+    int span;                     // classes an entry of part stands for
+    void *d; long long ldd, dcols;
+    const float2 *part; const float4 *stats; const float *rowg;
+    const long long *target; long long ignore;
+    const float *probs; long long ldp;
+    float *dbpart;                // [runs of `rows`][classes] or null
+};
+// `rows` rows x 512 classes per workgroup; a wave takes a row at a time, a lane eight classes of it.  Bound by memory: 2 bytes
+// (float32: 4) read and written an element.
+template <typename Op>
+__global__ __launch_bounds__(256) void fix_kernel(FixArgs a)
+{
+    using V = typename Frag<typename Op::Img>::V;
+    __shared__ float red[4][kFixCols];
+    if (a.totals.n >= 0 && blockIdx.y == gridDim.y - 1) {
+        if (blockIdx.x == 0) totals<256>(a.totals);
+        return;
+    }
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const long long c0 = (long long)blockIdx.x * kFixCols, c = c0 + lane * 8;
+    const long long r0 = (long long)blockIdx.y * a.rows, lde = a.ldd / (Op::split ? 2 : 1);
+    const float2 *part = a.part + (c < a.classes ? c : 0) / a.span * a.n;
+    float db[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int j = 0; j < a.rows / 4; j++) {
+        const long long row = r0 + j * 4 + wave;
+        if (row >= a.n) break;
+        const float4 st = a.stats[row];
+        const long long cls = a.target ? a.target[row] : -1, t = a.target ? cls - c : -1;
+        const float g = a.rowg ? a.rowg[row] : (a.target && cls == a.ignore ? 0.f : 1.f);
+        if (c >= a.dcols) continue;
+        const float mp = part[row].x, f = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mp - st.x) * st.y;
+        float v[8];
+        if constexpr (Op::split) {
+            const fx4 *p = reinterpret_cast<const fx4 *>(static_cast<float *>(a.d) + row * lde + c);
+            const fx4 v0 = p[0], v1 = p[1];
+#pragma unroll
+            for (int i = 0; i < 4; i++) { v[i] = v0[i]; v[4 + i] = v1[i]; }
+        } else {
+            const hx8 p = *reinterpret_cast<const hx8 *>(static_cast<_Float16 *>(a.d) + row * lde + c);
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = (float)p[i];
+        }
+        V h, l;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const bool out = c + i >= a.classes;
+            float q = v[i] * f;
+            if (a.probs) { if (!out) q -= a.probs[row * a.ldp + c + i]; }
+            else if (t == i) q -= 1.f;
+            q = g == 0.f || out ? 0.f : q * g;                                  // a row that counts for nothing: zero whatever it holds
+            db[i] += q;
+            q *= kDScale;
+            h[i] = (typename Op::Img)q;
+            if (Op::split) l[i] = (typename Op::Img)(q - (float)h[i]);
+        }
+        // (float32: the halves land on exponentials of the same row that other lanes of this wave have read: a wave's
+        //  stores follow the loads that every one of its values depends on)
+        typename Op::Img *o = static_cast<typename Op::Img *>(a.d) + row * a.ldd + (Op::split ? (c >> 5) * 64 + (c & 31) : c);
+        *reinterpret_cast<V *>(o) = h;
+        if (Op::split) *reinterpret_cast<V *>(o + 32) = l;
+    }
+    if (!a.dbpart) return;
+#pragma unroll
+    for (int i = 0; i < 8; i++) red[wave][lane * 8 + i] = db[i];
+    __syncthreads();
+    for (int i = tid; i < kFixCols; i += 256)
+        if (c0 + i < a.classes) a.dbpart[(long long)blockIdx.y * a.classes + c0 + i] = (red[0][i] + red[1][i]) + (red[2][i] + red[3][i]);
+}
 
 // ---------------------------------------------------------------- the gradients' products
 struct GradArgs {
     Operand a, b;                 // a: the output's contiguous dimension, b: its rows
-    int ktiles, mtiles, ntiles, kper;   // stages per split
+    int ktiles, mtiles, ntiles, kper, splits;   // kper: stages per split
     long long m, n;
     void *out; long long ldo;     // [n][ldo], operand type (one split), or
     float *acc;                   // float32 [splits][n][m]
-    bool add;                     // one split: add to acc instead of starting it
+    bool add;                     // add to acc instead of starting it
     const float *amax;            // float32: partial maxima of the operand that is not D
     const float *factor;
 };
 
-// dX: TB false (D as it lies), dW: TB true (D transposed); the other factor, W or X, is transposed in both
 template <typename Op, int TM, int TN, int WM, int WN, bool TB>
-__global__ __launch_bounds__(WM * WN * 64) void grad_kernel(GradArgs a)
+__device__ inline void grad_tile(const GradArgs &a, unsigned wg, char *lds)
 {
     using S = TileShape<TM, TN, WM, WN>;
-    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const unsigned tiles = (unsigned)a.mtiles * a.ntiles, split = wg / tiles;
     int tm, tn;
-    tile_of(blockIdx.x, a.mtiles, a.ntiles, &tm, &tn);
+    tile_of(wg - split * tiles, a.mtiles, a.ntiles, &tm, &tn);
     const long long m0 = (long long)tm * TM, n0 = (long long)tn * TN;
-    const int k0 = blockIdx.y * a.kper, k1 = min(a.ktiles, k0 + a.kper);
+    const int k0 = (int)split * a.kper, k1 = min(a.ktiles, k0 + a.kper);
     fx4 acc[S::MT][S::NT];
 #pragma unroll
     for (int i = 0; i < S::MT; i++)
@@ -893,7 +904,7 @@ __global__ __launch_bounds__(WM * WN * 64) void grad_kernel(GradArgs a)
             if (m >= a.m) continue;
             fx4 v = acc[mt][nt];
             if (a.acc) {
-                float *o = a.acc + ((long long)blockIdx.y * a.n + n) * a.m + m;
+                float *o = a.acc + ((long long)split * a.n + n) * a.m + m;
 #pragma unroll
                 for (int i = 0; i < 4; i++)
                     if (m + i < a.m) o[i] = a.add ? o[i] + v[i] : v[i];
@@ -914,6 +925,16 @@ __global__ __launch_bounds__(WM * WN * 64) void grad_kernel(GradArgs a)
     }
 }
 
+// dX = D W (D as it lies) by the first wgs_x workgroups, dW = D^T X (D transposed) by the others; the other factor, W or X,
+// is transposed in both
+template <typename Op, int TM, int TN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64) void grads_kernel(GradArgs x, GradArgs w, unsigned wgs_x)
+{
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    if (blockIdx.x < wgs_x) grad_tile<Op, TM, TN, WM, WN, false>(x, blockIdx.x, lds);
+    else grad_tile<Op, TM, TN, WM, WN, true>(w, blockIdx.x - wgs_x, lds);
+}
+
 struct JoinArgs {
     const float *acc;             // [splits][n][m]
     int splits;
@@ -921,16 +942,23 @@ struct JoinArgs {
     void *out; long long ldo;
     const float *amax, *factor;   // amax null: no image scale
     float extra;                  // kDScale for products of D images, 1 for sums of unscaled D
+    unsigned wgs;                 // workgroups of this one
 };
-// out[n][m] = factor * sum over splits, in their order; rows of the batch a thread each four columns apart
+struct JoinList { JoinArgs j[3]; };
+// out[n][m] = factor * sum over splits, in their order
 template <typename Op>
-__global__ __launch_bounds__(256) void join_kernel(JoinArgs a)
+__global__ __launch_bounds__(256) void join_kernel(JoinList l)
 {
+    unsigned wg = blockIdx.x;
+    int q = 0;
+    while (wg >= l.j[q].wgs) wg -= l.j[q++].wgs;
+    const JoinArgs a = l.j[q];
     float f = *a.factor / a.extra;
     if (Op::split && a.amax) f /= split_scale(max_of_parts(a.amax));
     const long long total = a.n * a.m;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    for (long long i = (long long)wg * 256 + threadIdx.x; i < total; i += (long long)a.wgs * 256) {
         float s = 0.f;
+#pragma unroll 4
         for (int z = 0; z < a.splits; z++) s += a.acc[(long long)z * total + i];
         const long long r = i / a.m, c = i - r * a.m;
         static_cast<typename Op::In *>(a.out)[r * a.ldo + c] = (typename Op::In)(s * f);

@@ -5,7 +5,7 @@
 //   small_rows_kernel    a row's statistics, loss, entropy, and D in place of its logits
 //   small_grads_kernel   dX = D W, dW = D^T X, db, and the totals
 //
-// A workgroup makes a 32 x 32 tile of a product; its four waves take a quarter of the sum each (blocks of 16 in turn) and
+// A workgroup makes a 32 x 32 tile of a product; its eight waves take an eighth of the sum each (blocks of 16 in turn) and
 // join through LDS.  Operands come straight from memory (L2) into the fragments of v_mfma_f32_16x16x4_f32: a lane of group
 // g = lane / 16 holds k = 4 g + j for the j-th of four instructions, so that where k is contiguous the four are one load.
 #pragma once
@@ -35,73 +35,80 @@ struct SmallArgs {
     int tiles_x, tiles_w;                     // workgroups of the products, then db's, then one for the totals
 };
 
-__device__ inline float block_sum(float v, float *red)      // 256 threads; every thread gets the sum, in a fixed order
+// sum over a workgroup of W waves in a fixed order, for every thread
+template <int W, typename T>
+__device__ inline T block_sum(T v, T *red)
 {
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) v += __shfl_xor(v, s, 64);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    return (red[0] + red[1]) + (red[2] + red[3]);
-}
-__device__ inline double block_sum(double v, double *red)
-{
+    T r = red[0];
 #pragma unroll
-    for (int s = 1; s < 64; s <<= 1) v += __shfl_xor(v, s, 64);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return (red[0] + red[1]) + (red[2] + red[3]);
+    for (int w = 1; w < W; w++) r += red[w];
+    return r;
 }
 
-// Four k of one m: k contiguous (KC) or across rows.  Outside the matrix: zero.  `skip`: null, or the targets whose rows (k)
-// read as zero where they are `ignore`.
-template <typename T, bool KC>
-__device__ inline fx4 small_frag(const T *p, long long ld, int m, int M, int k, int K, const long long *skip, long long ignore)
+// Four k of one m (the caller keeps m inside): k contiguous (KC) or across rows.  WHOLE: all four exist; else zero past K.
+// `skip`: null, or the targets whose rows (k) read as zero where they are `ignore`.
+template <bool WHOLE, typename T, bool KC>
+__device__ inline fx4 small_frag(const T *p, long long ld, int m, int k, int K, const long long *skip, long long ignore)
 {
     fx4 f = {0.f, 0.f, 0.f, 0.f};
-    if (m >= M) return f;
-    if constexpr (KC) {
-        const T *q = p + (long long)m * ld + k;
-        if (k + 4 <= K) {
-            const Pack<T, 4> v = *reinterpret_cast<const Pack<T, 4> *>(q);
+    if constexpr (KC && WHOLE) {
+        const Pack<T, 4> v = *reinterpret_cast<const Pack<T, 4> *>(p + (long long)m * ld + k);
 #pragma unroll
-            for (int j = 0; j < 4; j++) f[j] = (float)v.v[j];
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (k + j < K) f[j] = (float)q[j];
-        }
+        for (int j = 0; j < 4; j++) f[j] = (float)v.v[j];
     } else {
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            if (k + j < K && !(skip && skip[k + j] == ignore)) f[j] = (float)p[(long long)(k + j) * ld + m];
+            if (WHOLE || k + j < K) {
+                const float v = (float)(KC ? p[(long long)m * ld + k + j] : p[(long long)(k + j) * ld + m]);
+                f[j] = skip && skip[k + j] == ignore ? 0.f : v;
+            }
     }
     return f;
 }
 
-// acc[a][b] of the 32 x 32 tile at (m0, n0): row m0 + 16 a + 4 g + i, column n0 + 16 b + (lane & 15); summed over the four
-// waves through LDS; out: rows 8 wave + lane / 32 + 2 i, column lane & 31 of the sum
+// A 32 x 32 tile at (m0, n0), the eight waves' parts of the sum joined through LDS; out: rows 4 wave + lane / 32 + 2 i, column
+// lane & 31.  The next block's operands are on their way while one is multiplied.
+constexpr int kSmallWaves = 8;
+typedef float SmallLds[kSmallWaves][kSmallTile][kSmallTile + 1];
 template <typename TA, bool KA, typename TB, bool KB>
 __device__ inline void small_product(const TA *A, long long lda, int m0, int M, const TB *B, long long ldb, int n0, int N, int K,
-                                     const long long *skip, long long ignore, float (*lds)[kSmallTile][kSmallTile + 1], float (&out)[4])
+                                     const long long *skip, long long ignore, SmallLds &lds, float (&out)[2])
 {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
     fx4 acc[2][2] = {{{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}};
-#pragma unroll 2
-    for (int k = wave * 16; k < K; k += 64) {
-        fx4 a[2], b[2];
+    fx4 a[2], b[2], an[2], bn[2];
+    // (rows past the end repeat the last one: they reach only results that are not stored)
+    int ma[2], nb[2];
+#pragma unroll
+    for (int t = 0; t < 2; t++) { ma[t] = min(m0 + 16 * t + c, M - 1); nb[t] = min(n0 + 16 * t + c, N - 1); }
+    auto load = [&](fx4 (&x)[2], fx4 (&y)[2], int k) {
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            a[t] = small_frag<TA, KA>(A, lda, m0 + 16 * t + c, M, k + 4 * g, K, nullptr, 0);
-            b[t] = small_frag<TB, KB>(B, ldb, n0 + 16 * t + c, N, k + 4 * g, K, skip, ignore);
+            if (k + 16 <= K) {
+                x[t] = small_frag<true, TA, KA>(A, lda, ma[t], k + 4 * g, K, nullptr, 0);
+                y[t] = small_frag<true, TB, KB>(B, ldb, nb[t], k + 4 * g, K, skip, ignore);
+            } else {
+                x[t] = small_frag<false, TA, KA>(A, lda, ma[t], k + 4 * g, K, nullptr, 0);
+                y[t] = small_frag<false, TB, KB>(B, ldb, nb[t], k + 4 * g, K, skip, ignore);
+            }
         }
+    };
+    load(a, b, wave * 16);
+    for (int k = wave * 16; k < K; k += kSmallWaves * 16) {
+        load(an, bn, k + kSmallWaves * 16);                   // (past the end: zeros)
 #pragma unroll
         for (int j = 0; j < 4; j++)
 #pragma unroll
             for (int s = 0; s < 2; s++)
 #pragma unroll
                 for (int t = 0; t < 2; t++) acc[s][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s][j], b[t][j], acc[s][t], 0, 0, 0);
+#pragma unroll
+        for (int t = 0; t < 2; t++) { a[t] = an[t]; b[t] = bn[t]; }
     }
 #pragma unroll
     for (int s = 0; s < 2; s++)
@@ -111,34 +118,37 @@ __device__ inline void small_product(const TA *A, long long lda, int m0, int M, 
             for (int i = 0; i < 4; i++) lds[wave][16 * s + 4 * g + i][16 * t + c] = acc[s][t][i];
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int r = wave * 8 + (lane >> 5) + 2 * i, q = lane & 31;
-        out[i] = (lds[0][r][q] + lds[1][r][q]) + (lds[2][r][q] + lds[3][r][q]);
+    for (int i = 0; i < 2; i++) {
+        const int r = wave * 4 + (lane >> 5) + 2 * i, q = lane & 31;
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < kSmallWaves; w++) s += lds[w][r][q];
+        out[i] = s;
     }
 }
 
 // l[n][v]: rows of the tile are rows of X, columns are classes
 template <typename T>
-__global__ __launch_bounds__(256) void small_logits_kernel(SmallArgs a)
+__global__ __launch_bounds__(kSmallWaves * 64) void small_logits_kernel(SmallArgs a)
 {
-    __shared__ float lds[4][kSmallTile][kSmallTile + 1];
+    __shared__ SmallLds lds;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int tv = (a.V + kSmallTile - 1) / kSmallTile, tn = (a.n + kSmallTile - 1) / kSmallTile;
     if ((int)blockIdx.x == tv * tn) {                         // the last workgroup: how many rows count
         float s = 0.f;
-        for (int i = tid; i < a.n; i += 256) s += a.target && a.target[i] == a.ignore ? 0.f : 1.f;
-        s = block_sum(s, &lds[0][0][0]);
+        for (int i = tid; i < a.n; i += kSmallWaves * 64) s += a.target && a.target[i] == a.ignore ? 0.f : 1.f;
+        s = block_sum<kSmallWaves>(s, &lds[0][0][0]);
         if (tid == 0) *a.count = (int)s;
         return;
     }
     const int n0 = (int)blockIdx.x / tv * kSmallTile, v0 = (int)blockIdx.x % tv * kSmallTile;
-    float out[4];
+    float out[2];
     small_product<T, true, T, true>(static_cast<const T *>(a.x), a.xs, n0, a.n, static_cast<const T *>(a.w), a.ws, v0, a.V, a.H, nullptr, 0, lds, out);
     const int v = v0 + (lane & 31);
     const float b = a.bias && v < a.V ? (float)static_cast<const T *>(a.bias)[v] : 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int r = n0 + wave * 8 + (lane >> 5) + 2 * i;
+    for (int i = 0; i < 2; i++) {
+        const int r = n0 + wave * 4 + (lane >> 5) + 2 * i;
         if (r < a.n && v < a.V) a.logits[(long long)r * a.ldl + v] = out[i] + b;
     }
 }
@@ -166,9 +176,9 @@ __global__ __launch_bounds__(256) void small_rows_kernel(SmallArgs a)
         e += p != 0.f ? p * x : 0.f;
         if (pr) { const float q = pr[v]; ts += q; ta += fabsf(q); tl += q != 0.f ? q * x : 0.f; }
     }
-    s = block_sum(s, red);
-    if (a.ent) e = block_sum(e, red);
-    if (pr) { tl = block_sum(tl, red); ts = block_sum(ts, red); ta = block_sum(ta, red); }
+    s = block_sum<4>(s, red);
+    if (a.ent) e = block_sum<4>(e, red);
+    if (pr) { tl = block_sum<4>(tl, red); ts = block_sum<4>(ts, red); ta = block_sum<4>(ta, red); }
     const float ls = logf(s);                                 // (everything relative to the maximum: loss and entropy need no large difference)
     const long long t = a.target ? a.target[row] : -1;
     bool used = true;
@@ -203,16 +213,17 @@ __global__ __launch_bounds__(256) void small_rows_kernel(SmallArgs a)
 }
 
 // sum or mean of the rows' losses and entropies, in double and in a fixed order
+template <int W>
 __device__ inline void small_totals(const SmallArgs &a)
 {
-    __shared__ double red[4];
+    __shared__ double red[W];
     double l = 0.0, e = 0.0;
-    for (int i = threadIdx.x; i < a.n; i += 256) {
+    for (int i = threadIdx.x; i < a.n; i += W * 64) {
         l += a.stats[i].w;
         if (a.ent) e += a.ent[i];
     }
-    l = block_sum(l, red);
-    if (a.ent) e = block_sum(e, red);
+    l = block_sum<W>(l, red);
+    if (a.ent) e = block_sum<W>(e, red);
     if (threadIdx.x) return;
     const int c = *a.count;
     const double by = a.reduction == 2 ? (c > 0 ? 1.0 / c : 0.0) : 1.0;
@@ -222,19 +233,19 @@ __device__ inline void small_totals(const SmallArgs &a)
 
 // Workgroups: tiles of dX, tiles of dW, columns of db, totals.  Output tiles have the contiguous dimension (features) as columns.
 template <typename T>
-__global__ __launch_bounds__(256) void small_grads_kernel(SmallArgs a)
+__global__ __launch_bounds__(kSmallWaves * 64) void small_grads_kernel(SmallArgs a)
 {
-    __shared__ float lds[4][kSmallTile][kSmallTile + 1];
+    __shared__ SmallLds lds;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, th = (a.H + kSmallTile - 1) / kSmallTile;
     int b = blockIdx.x;
-    float out[4];
+    float out[2];
     if (b < a.tiles_x) {
         const int n0 = b / th * kSmallTile, h0 = b % th * kSmallTile;
         small_product<float, true, T, false>(a.logits, a.ldl, n0, a.n, static_cast<const T *>(a.w), a.ws, h0, a.H, a.V, nullptr, 0, lds, out);
         const int h = h0 + (lane & 31);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int r = n0 + wave * 8 + (lane >> 5) + 2 * i;
+        for (int i = 0; i < 2; i++) {
+            const int r = n0 + wave * 4 + (lane >> 5) + 2 * i;
             if (r < a.n && h < a.H) static_cast<T *>(a.dx)[(long long)r * a.dxs + h] = (T)out[i];
         }
         return;
@@ -246,30 +257,35 @@ __global__ __launch_bounds__(256) void small_grads_kernel(SmallArgs a)
         small_product<float, false, T, false>(a.logits, a.ldl, v0, a.V, static_cast<const T *>(a.x), a.xs, h0, a.H, a.n, a.target, a.ignore, lds, out);
         const int h = h0 + (lane & 31);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int v = v0 + wave * 8 + (lane >> 5) + 2 * i;
+        for (int i = 0; i < 2; i++) {
+            const int v = v0 + wave * 4 + (lane >> 5) + 2 * i;
             if (v < a.V && h < a.H) static_cast<T *>(a.dw)[(long long)v * a.dws + h] = (T)out[i];
         }
         return;
     }
     b -= a.tiles_w;
     const int tb = a.db ? (a.V + 63) / 64 : 0;
-    if (b < tb) {                                             // 64 classes, a quarter of the rows a wave
+    if (b < tb) {                                             // 64 classes, an eighth of the rows a wave
         const int v = b * 64 + lane;
         float s = 0.f;
         if (v < a.V)
 #pragma unroll 8
-            for (int r = wave; r < a.n; r += 4) s += a.logits[(long long)r * a.ldl + v];
+            for (int r = wave; r < a.n; r += kSmallWaves) s += a.logits[(long long)r * a.ldl + v];
         float *red = &lds[0][0][0];
         red[wave * 64 + lane] = s;
         __syncthreads();
-        if (wave == 0 && v < a.V) static_cast<T *>(a.db)[v] = (T)((red[lane] + red[64 + lane]) + (red[128 + lane] + red[192 + lane]));
+        if (wave == 0 && v < a.V) {
+            s = red[lane];
+#pragma unroll
+            for (int w = 1; w < kSmallWaves; w++) s += red[w * 64 + lane];
+            static_cast<T *>(a.db)[v] = (T)s;
+        }
         return;
     }
-    small_totals(a);
+    small_totals<kSmallWaves>(a);
 }
 
 // forward alone: the totals
-__global__ __launch_bounds__(256) void small_totals_kernel(SmallArgs a) { small_totals(a); }
+__global__ __launch_bounds__(256) void small_totals_kernel(SmallArgs a) { small_totals<4>(a); }
 
 }  // namespace azgops

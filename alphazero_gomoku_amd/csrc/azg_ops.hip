@@ -122,19 +122,40 @@ Shape pick_logits(long long m, long long n, bool grad)
     if (tiles_of(T128, m, n) >= 200) return T128;
     return T64;
 }
-// tile and number of splits of k of a gradient's product
-struct GradPick { Shape shape; int splits, kper; };
-GradPick pick_grad(long long m, long long n, long long ktiles)
+// Tile of the gradients' products, which share a launch, and the splits of their sums, by an estimate in microseconds: the
+// launch takes its stages at the rate of the whole card or as long as its longest workgroup, whichever is more, and splits
+// cost a join.  Per stage and tile (measured at 16 bits; float32 half as much again): 256 x 256 1.0 with a CU to itself,
+// 128 x 128 0.33 a CU's share and 0.7 from start to end, 64 x 64 0.12 and 0.45.
+struct GradPick { Shape shape; int splits_x, kper_x, splits_w, kper_w; };
+GradPick pick_grads(long long n, long long h, long long v, long long kx, long long kw, bool want_x, bool want_w)
 {
-    GradPick g{T64, 1, (int)ktiles};
-    const long long most = std::max<long long>(1, ktiles / 8);
-    if (m > 128 && n > 128 && tiles_of(T256, m, n) * std::min<long long>(most, 32) >= 200) g.shape = T256;
-    else if (m > 64 && n > 64 && tiles_of(T128, m, n) * std::min<long long>(most, 32) >= 200) g.shape = T128;
-    const long long tiles = tiles_of(g.shape, m, n);
-    long long s = std::max<long long>(1, std::min<long long>({256 / std::max<long long>(tiles, 1), most, 32}));
-    g.kper = (int)((ktiles + s - 1) / s);
-    g.splits = (int)((ktiles + g.kper - 1) / g.kper);
-    return g;
+    static constexpr double share[3] = {1.0, 0.33, 0.12}, alone[3] = {1.0, 0.7, 0.45};
+    GradPick best{};
+    double least = 1e30;
+    for (Shape s : {T256, T128, T64}) {
+        const long long tx = want_x ? tiles_of(s, h, n) : 0, tw = want_w ? tiles_of(s, h, v) : 0;
+        if ((double)(tx + tw) * 32 > INT_MAX / 2 && s != T256) continue;
+        for (long long per = 4; per < 2 * std::max(kx, kw); per *= 2) {          // stages of a workgroup at most
+            GradPick g{};
+            auto split = [&](long long k, int *splits, int *kper) {
+                const long long parts = std::min<long long>(32, (k + per - 1) / per);
+                *kper = (int)((k + parts - 1) / parts);
+                *splits = (int)((k + *kper - 1) / *kper);
+            };
+            g.shape = s;
+            split(kx, &g.splits_x, &g.kper_x);
+            split(kw, &g.splits_w, &g.kper_w);
+            double joined = 0;                                                  // bytes of the splits, written and read
+            if (tx && g.splits_x > 1) joined += 8.0 * g.splits_x * n * h;
+            if (tw && g.splits_w > 1) joined += 8.0 * g.splits_w * v * h;
+            const double work = (double)(tx * kx + tw * kw) * share[s] / 256.0;
+            const double longest = std::max(tx ? g.kper_x : 0, tw ? g.kper_w : 0) * alone[s];
+            // (workgroups come in rounds: half a longest one on average is lost at the end)
+            const double t = std::max(work + 0.5 * longest, longest) + joined / 4e6 + (joined > 0 ? 3.0 : 0.0);
+            if (t < least) { least = t; best = g; }
+        }
+    }
+    return best;
 }
 
 struct Plan {
@@ -143,7 +164,8 @@ struct Plan {
     long long kimg, ldk, ldd;                                 // image elements along the features; row strides of the images of X, W and D
     int per, ks;                                              // image elements an element takes, k of a stage
     Shape lshape;
-    GradPick gx, gw;
+    GradPick g;
+    int fix_rows;
     size_t xmax, wmax, ximg, wimg, part, part_e, part_t, tlogit, stats, ent, rowg, factor, d, dbpart, dxacc, dwacc, logits, count, total;
 };
 
@@ -188,12 +210,14 @@ int make_plan(const azg_linear_ce_args *a, Plan *p)
     p->keep = p->forward && p->backward && p->pieces == 1;
     p->ldd = image_stride(up_to(p->vp, p->ks) * p->per);
     p->lshape = pick_logits(p->vp, p->n, p->backward);
-    p->gx = pick_grad(p->H, p->n, (p->vp + p->ks - 1) / p->ks);
-    p->gw = pick_grad(p->H, p->vp, (p->n + p->ks - 1) / p->ks);
+    p->g = pick_grads(p->n, p->H, p->vp, (p->vp + p->ks - 1) / p->ks, (p->n + p->ks - 1) / p->ks, a->dx != nullptr, a->dw != nullptr);
+    // rows a workgroup turns into D: up to 64, fewer while they would not give four workgroups a CU
+    p->fix_rows = 64;
+    while (p->fix_rows > 8 && (p->n + p->fix_rows - 1) / p->fix_rows * ((p->vp + kFixCols - 1) / kFixCols) < 1024) p->fix_rows /= 2;
     const ShapeDim dim = kDims[p->lshape];
     const long long lm = (p->vp + dim.tm - 1) / dim.tm, ln = (p->n + dim.tn - 1) / dim.tn;
-    if (lm * ln > INT_MAX / 2 || tiles_of(p->gx.shape, p->H, p->n) > INT_MAX / 2 || tiles_of(p->gw.shape, p->H, p->vp) > INT_MAX / 2 ||
-        (p->n + kFixRows - 1) / kFixRows > 65535)
+    if (lm * ln > INT_MAX / 2 || (tiles_of(p->g.shape, p->H, p->n) + tiles_of(p->g.shape, p->H, p->vp)) * 32 > INT_MAX / 2 ||
+        (p->n + p->fix_rows - 1) / p->fix_rows > 65534)
         return fail(AZG_EINVAL, "azg_linear_ce: the problem is too large");
     Take t;
     p->xmax = t(p->split ? kMaxParts * 4 : 0);
@@ -210,9 +234,9 @@ int make_plan(const azg_linear_ce_args *a, Plan *p)
     p->rowg = t((size_t)p->n * 4);
     p->factor = t(4);
     p->d = t(p->backward ? (size_t)p->n * p->ldd * 2 : 0);
-    p->dbpart = t(a->db ? (size_t)std::max(ln, (p->n + kFixRows - 1) / kFixRows) * p->vp * 4 : 0);
-    p->dxacc = t(a->dx && (p->gx.splits > 1 || p->pieces > 1) ? (size_t)p->gx.splits * p->n * p->H * 4 : 0);
-    p->dwacc = t(a->dw && p->gw.splits > 1 ? (size_t)p->gw.splits * p->vp * p->H * 4 : 0);
+    p->dbpart = t(a->db ? (size_t)std::max(ln, (p->n + p->fix_rows - 1) / p->fix_rows) * p->vp * 4 : 0);
+    p->dxacc = t(a->dx && (p->g.splits_x > 1 || p->pieces > 1) ? (size_t)p->g.splits_x * p->n * p->H * 4 : 0);
+    p->dwacc = t(a->dw && p->g.splits_w > 1 ? (size_t)p->g.splits_w * p->vp * p->H * 4 : 0);
     p->total = t.off;
     return AZG_OK;
 }
@@ -260,40 +284,53 @@ int launch_logits(Shape shape, const CeArgs &c, hipStream_t s)
     }
 }
 
-template <typename Op, int TM, int TN, int WM, int WN, bool TB>
-int launch_grad_shape(GradArgs g, int splits, hipStream_t s)
+template <typename Op, int TM, int TN, int WM, int WN>
+int launch_grads_shape(GradArgs x, GradArgs w, hipStream_t s)
 {
     using S = TileShape<TM, TN, WM, WN>;
-    g.mtiles = (int)((g.m + TM - 1) / TM);
-    g.ntiles = (int)((g.n + TN - 1) / TN);
-    OPS_TRY(allow_lds(grad_kernel<Op, TM, TN, WM, WN, TB>, S::lds_bytes));
-    hipLaunchKernelGGL((grad_kernel<Op, TM, TN, WM, WN, TB>), dim3((unsigned)g.mtiles * g.ntiles, splits), dim3(S::threads), S::lds_bytes, s, g);
+    unsigned wgs[2];
+    int i = 0;
+    for (GradArgs *g : {&x, &w}) {
+        g->mtiles = (int)((g->m + TM - 1) / TM);
+        g->ntiles = (int)((g->n + TN - 1) / TN);
+        wgs[i++] = g->out ? (unsigned)g->mtiles * g->ntiles * g->splits : 0;
+    }
+    OPS_TRY(allow_lds(grads_kernel<Op, TM, TN, WM, WN>, S::lds_bytes));
+    hipLaunchKernelGGL((grads_kernel<Op, TM, TN, WM, WN>), dim3(wgs[0] + wgs[1]), dim3(S::threads), S::lds_bytes, s, x, w, wgs[0]);
     OPS_HIP(hipGetLastError());
     return AZG_OK;
 }
-template <typename Op, bool TB>
-int launch_grad(const GradPick &pick, GradArgs g, hipStream_t s)
+template <typename Op>
+int launch_grads(Shape shape, const GradArgs &x, const GradArgs &w, hipStream_t s)
 {
-    g.kper = pick.kper;
-    switch (pick.shape) {
-    case T256: return launch_grad_shape<Op, 256, 256, 2, 4, TB>(g, pick.splits, s);
-    case T128: return launch_grad_shape<Op, 128, 128, 2, 2, TB>(g, pick.splits, s);
-    default: return launch_grad_shape<Op, 64, 64, 2, 2, TB>(g, pick.splits, s);
+    switch (shape) {
+    case T256: return launch_grads_shape<Op, 256, 256, 2, 4>(x, w, s);
+    case T128: return launch_grads_shape<Op, 128, 128, 2, 2>(x, w, s);
+    default: return launch_grads_shape<Op, 64, 64, 2, 2>(x, w, s);
     }
 }
+// up to three joins in one launch
 template <typename Op>
-int launch_join(const JoinArgs &j, hipStream_t s)
+int launch_joins(JoinList l, int count, hipStream_t s)
 {
-    const long long grid = std::min<long long>((j.n * j.m + 255) / 256, 1 << 16);
-    hipLaunchKernelGGL((join_kernel<Op>), dim3((unsigned)grid), dim3(256), 0, s, j);
+    unsigned grid = 0;
+    for (int i = 0; i < count; i++) {
+        l.j[i].wgs = (unsigned)std::min<long long>((l.j[i].n * l.j[i].m + 255) / 256, 1 << 16);
+        grid += l.j[i].wgs;
+    }
+    if (!grid) return AZG_OK;
+    hipLaunchKernelGGL((join_kernel<Op>), dim3(grid), dim3(256), 0, s, l);
     OPS_HIP(hipGetLastError());
     return AZG_OK;
 }
+// one image or two (null: none)
 template <typename Op>
-int launch_pack(const PackArgs &p, hipStream_t s)
+int launch_packs(const PackArgs *p, const PackArgs *q, hipStream_t s)
 {
-    const long long chunks = p.rows * (p.icols / (Op::split ? 16 : 8));
-    hipLaunchKernelGGL((pack_kernel<Op>), dim3((unsigned)std::min<long long>((chunks + 255) / 256, 1 << 16)), dim3(256), 0, s, p);
+    if (!p) std::swap(p, q);
+    if (!p) return AZG_OK;
+    auto wgs = [](const PackArgs &a) { return (unsigned)std::min<long long>((a.rows * (a.icols / (Op::split ? 16 : 8)) + 255) / 256, 1 << 16); };
+    hipLaunchKernelGGL((pack_kernel<Op>), dim3(wgs(*p) + (q ? wgs(*q) : 0)), dim3(256), 0, s, *p, q ? *q : *p, wgs(*p));
     OPS_HIP(hipGetLastError());
     return AZG_OK;
 }
@@ -315,11 +352,8 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
     px.maxpart = f32(p.xmax); px.img = ws + p.ximg; px.ldi = p.ldk; px.icols = p.kimg;
     PackArgs pw{};
     pw.src = W; pw.ld = a->w_stride; pw.rows = a->classes; pw.cols = a->hidden; pw.maxpart = f32(p.wmax); pw.img = ws + p.wimg; pw.ldi = p.ldk; pw.icols = p.kimg;
-    if (Op::split) {
-        hipLaunchKernelGGL(absmax_kernel, dim3(kMaxParts), dim3(256), 0, s, px, f32(p.xmax));
-        hipLaunchKernelGGL(absmax_kernel, dim3(kMaxParts), dim3(256), 0, s, pw, f32(p.wmax));
-    }
-    if (p.pack_x) OPS_TRY(launch_pack<Op>(px, s));
+    if (Op::split) hipLaunchKernelGGL(absmax_kernel, dim3(2 * kMaxParts), dim3(256), 0, s, px, pw);
+    bool x_packed = !p.pack_x;
     CeArgs c{};
     c.x = p.pack_x ? Operand{ws + p.ximg, p.ldk, a->n, p.kimg} : Operand{a->x, a->x_stride, a->n, a->hidden};
     c.ktiles = (int)((p.H + p.ks - 1) / p.ks);
@@ -334,7 +368,8 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
         c.ldd = p.ldd;
         c.dcols = up_to(vn, p.ks);
         pw.src = W + v0 * a->w_stride; pw.rows = vn;
-        if (p.pack_w && pack) OPS_TRY(launch_pack<Op>(pw, s));
+        if (pack) OPS_TRY(launch_packs<Op>(x_packed ? nullptr : &px, p.pack_w ? &pw : nullptr, s));
+        x_packed = true;
         c.w = p.pack_w ? Operand{ws + p.wimg, p.ldk, vn, p.kimg} : Operand{W + v0 * a->w_stride, a->w_stride, vn, a->hidden};
         return AZG_OK;
     };
@@ -363,8 +398,11 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
     t.n = a->n; t.reduction = a->reduction; t.stats = stats; t.ent = p.forward && a->entropy ? f32(p.ent) : nullptr;
     t.target = target; t.ignore = a->ignore_index; t.loss = p.forward ? a->loss : nullptr; t.ent_out = p.forward ? a->entropy : nullptr;
     t.dloss = a->dloss; t.grad_scale = (float)a->grad_scale;
-    t.rowg = p.backward ? f32(p.rowg) : nullptr; t.factor = f32(p.factor);
-    hipLaunchKernelGGL(totals_kernel, dim3(1), dim3(1024), 0, s, t);
+    t.rowg = p.backward ? f32(p.rowg) : nullptr; t.factor = p.backward ? f32(p.factor) : nullptr;
+    // class numbers and a common g: the rows' factors are 1 or 0, and the totals can ride on the next launch
+    const bool ride = p.keep && target && a->reduction != AZG_REDUCE_NONE;
+    if (ride) t.rowg = nullptr;
+    else hipLaunchKernelGGL(totals_kernel, dim3(1), dim3(1024), 0, s, t);
     OPS_HIP(hipGetLastError());
     if (!p.backward) return AZG_OK;
 
@@ -374,11 +412,13 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
         int dbparts;
         if (p.keep) {
             FixArgs f{};
-            f.n = a->n; f.classes = vn; f.span = dim.tm / dim.wm; f.d = ws + p.d; f.ldd = c.ldd; f.dcols = c.dcols;
-            f.part = reinterpret_cast<float2 *>(ws + p.part); f.stats = stats; f.rowg = f32(p.rowg);
-            f.target = target; f.probs = a->probs; f.ldp = a->probs_stride; f.dbpart = a->db ? f32(p.dbpart) : nullptr;
-            dbparts = (int)((a->n + kFixRows - 1) / kFixRows);
-            hipLaunchKernelGGL((fix_kernel<Op>), dim3((unsigned)((c.dcols + kFixCols - 1) / kFixCols), dbparts), dim3(256), 0, s, f);
+            f.n = a->n; f.classes = vn; f.rows = p.fix_rows; f.span = dim.tm / dim.wm; f.d = ws + p.d; f.ldd = c.ldd; f.dcols = c.dcols;
+            f.part = reinterpret_cast<float2 *>(ws + p.part); f.stats = stats; f.rowg = t.rowg;
+            f.target = target; f.ignore = a->ignore_index; f.probs = a->probs; f.ldp = a->probs_stride; f.dbpart = a->db ? f32(p.dbpart) : nullptr;
+            f.totals = t;
+            if (!ride) f.totals.n = -1;
+            dbparts = (int)((a->n + p.fix_rows - 1) / p.fix_rows);
+            hipLaunchKernelGGL((fix_kernel<Op>), dim3((unsigned)((c.dcols + kFixCols - 1) / kFixCols), dbparts + (ride ? 1 : 0)), dim3(256), 0, s, f);
             OPS_HIP(hipGetLastError());
         } else {
             c.stats = stats; c.rowg = f32(p.rowg);
@@ -387,43 +427,30 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
             dbparts = (int)((a->n + dim.tn - 1) / dim.tn);
             OPS_TRY((launch_logits<Op, true>(p.lshape, c, s)));
         }
+        GradArgs gx{}, gw{};
+        JoinList joins{};
+        int count = 0;
+        const Operand d{ws + p.d, c.ldd, a->n, c.dcols * p.per};
         if (a->dx) {
-            GradArgs g{};
-            g.a = Operand{c.w.p, c.w.ld, vn, c.w.cols}; g.b = Operand{ws + p.d, c.ldd, a->n, c.dcols * p.per};
-            g.ktiles = (int)((vn + p.ks - 1) / p.ks); g.m = a->hidden; g.n = a->n;
-            g.amax = f32(p.wmax); g.factor = f32(p.factor);
-            const bool acc = p.gx.splits > 1 || p.pieces > 1;
-            g.acc = acc ? f32(p.dxacc) : nullptr; g.add = i > 0;
-            g.out = a->dx; g.ldo = a->dx_stride;
-            OPS_TRY((launch_grad<Op, false>(p.gx, g, s)));
-            if (acc && i == p.pieces - 1) {
-                JoinArgs j{};
-                j.acc = f32(p.dxacc); j.splits = p.gx.splits; j.n = a->n; j.m = a->hidden; j.out = a->dx; j.ldo = a->dx_stride;
-                j.amax = f32(p.wmax); j.factor = f32(p.factor); j.extra = kDScale;
-                OPS_TRY(launch_join<Op>(j, s));
-            }
+            gx.a = Operand{c.w.p, c.w.ld, vn, c.w.cols}; gx.b = d;
+            gx.ktiles = (int)((vn + p.ks - 1) / p.ks); gx.kper = p.g.kper_x; gx.splits = p.g.splits_x; gx.m = a->hidden; gx.n = a->n;
+            gx.amax = f32(p.wmax); gx.factor = f32(p.factor);
+            const bool acc = p.g.splits_x > 1 || p.pieces > 1;
+            gx.acc = acc ? f32(p.dxacc) : nullptr; gx.add = i > 0;
+            gx.out = a->dx; gx.ldo = a->dx_stride;
+            if (acc && i == p.pieces - 1) joins.j[count++] = {gx.acc, gx.splits, gx.n, gx.m, gx.out, gx.ldo, gx.amax, gx.factor, kDScale, 0};
         }
         if (a->dw) {
-            GradArgs g{};
-            g.a = c.x; g.b = Operand{ws + p.d, c.ldd, a->n, c.dcols * p.per};
-            g.ktiles = (int)((a->n + p.ks - 1) / p.ks); g.m = a->hidden; g.n = vn;
-            g.amax = f32(p.xmax); g.factor = f32(p.factor);
-            g.acc = p.gw.splits > 1 ? f32(p.dwacc) : nullptr; g.add = false;
-            g.out = static_cast<In *>(a->dw) + i * p.vp * a->dw_stride; g.ldo = a->dw_stride;
-            OPS_TRY((launch_grad<Op, true>(p.gw, g, s)));
-            if (g.acc) {
-                JoinArgs j{};
-                j.acc = g.acc; j.splits = p.gw.splits; j.n = vn; j.m = a->hidden; j.out = g.out; j.ldo = a->dw_stride;
-                j.amax = f32(p.xmax); j.factor = f32(p.factor); j.extra = kDScale;
-                OPS_TRY(launch_join<Op>(j, s));
-            }
+            gw.a = c.x; gw.b = d;
+            gw.ktiles = (int)((a->n + p.ks - 1) / p.ks); gw.kper = p.g.kper_w; gw.splits = p.g.splits_w; gw.m = a->hidden; gw.n = vn;
+            gw.amax = f32(p.xmax); gw.factor = f32(p.factor);
+            gw.acc = p.g.splits_w > 1 ? f32(p.dwacc) : nullptr; gw.add = false;
+            gw.out = static_cast<In *>(a->dw) + i * p.vp * a->dw_stride; gw.ldo = a->dw_stride;
+            if (gw.acc) joins.j[count++] = {gw.acc, gw.splits, gw.n, gw.m, gw.out, gw.ldo, gw.amax, gw.factor, kDScale, 0};
         }
-        if (a->db) {
-            JoinArgs j{};
-            j.acc = f32(p.dbpart); j.splits = dbparts; j.n = 1; j.m = vn;
-            j.out = static_cast<In *>(a->db) + i * p.vp; j.ldo = vn; j.factor = f32(p.factor); j.extra = 1.f;
-            OPS_TRY(launch_join<Op>(j, s));
-        }
+        if (a->dx || a->dw) OPS_TRY(launch_grads<Op>(p.g.shape, gx, gw, s));
+        if (a->db) joins.j[count++] = {f32(p.dbpart), dbparts, 1, vn, static_cast<In *>(a->db) + i * p.vp, vn, nullptr, f32(p.factor), 1.f, 0};
+        OPS_TRY(launch_joins<Op>(joins, count, s));
     }
     return AZG_OK;
 }
@@ -446,14 +473,14 @@ int run_small(const azg_linear_ce_args *a, const Plan &p)
     g.count = reinterpret_cast<int *>(ws + p.count);
     g.backward = p.backward; g.dx = a->dx; g.dw = a->dw; g.db = a->db; g.dxs = a->dx_stride; g.dws = a->dw_stride;
     auto tiles = [](int v) { return (v + kSmallTile - 1) / kSmallTile; };
-    hipLaunchKernelGGL((small_logits_kernel<In>), dim3(tiles(g.n) * tiles(g.V) + 1), dim3(256), 0, s, g);
+    hipLaunchKernelGGL((small_logits_kernel<In>), dim3(tiles(g.n) * tiles(g.V) + 1), dim3(kSmallWaves * 64), 0, s, g);
     hipLaunchKernelGGL(small_rows_kernel, dim3(g.n), dim3(256), 0, s, g);
     const bool totals = p.forward && g.reduction != AZG_REDUCE_NONE;
     if (p.backward) {
         g.tiles_x = g.dx ? tiles(g.n) * tiles(g.H) : 0;
         g.tiles_w = g.dw ? tiles(g.V) * tiles(g.H) : 0;
         const int grid = g.tiles_x + g.tiles_w + (g.db ? (g.V + 63) / 64 : 0) + (totals ? 1 : 0);
-        hipLaunchKernelGGL((small_grads_kernel<In>), dim3(grid), dim3(256), 0, s, g);
+        hipLaunchKernelGGL((small_grads_kernel<In>), dim3(grid), dim3(kSmallWaves * 64), 0, s, g);
     } else if (totals) {
         hipLaunchKernelGGL(small_totals_kernel, dim3(1), dim3(256), 0, s, g);
     }
