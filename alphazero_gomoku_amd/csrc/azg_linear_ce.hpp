@@ -410,27 +410,35 @@ __device__ inline float max_of_parts(const float *parts)                        
 
 // partial maxima of the finite magnitudes of two float32 tensors (rows whose target is ignore_index left out), kMaxParts
 // workgroups each
-__global__ __launch_bounds__(256) void absmax_kernel(PackArgs a0, PackArgs a1)
+__global__ __launch_bounds__(512) void absmax_kernel(PackArgs a0, PackArgs a1)
 {
-    __shared__ float red[4];
+    __shared__ float red[8];
     const PackArgs a = blockIdx.x < kMaxParts ? a0 : a1;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const unsigned wg = blockIdx.x % kMaxParts;
     const float *src = static_cast<const float *>(a.src);
     float m = 0.f;
-    const long long per_row = (a.cols + 1023) / 1024, total = a.rows * per_row;
-    for (long long u = wg; u < total; u += kMaxParts) {
-        const long long row = u / per_row, c0 = (u - row * per_row) * 1024 + threadIdx.x * 4;
+    auto take = [&](float v) { v = fabsf(v); m = v < INFINITY ? fmaxf(m, v) : m; };
+    for (long long row = wg * 8 + wave; row < a.rows; row += kMaxParts * 8) {
         if (a.target && a.target[row] == a.ignore) continue;
         const float *p = src + row * a.ld;
+        const long long whole = a.cols / 4 * 4;
+#pragma unroll 4
+        for (long long c = lane * 4; c < whole; c += 256) {
+            const Pack<float, 4> v = *reinterpret_cast<const Pack<float, 4> *>(p + c);
 #pragma unroll
-        for (int q = 0; q < 4; q++)
-            if (c0 + q < a.cols) { const float v = fabsf(p[c0 + q]); m = v < INFINITY ? fmaxf(m, v) : m; }
+            for (int q = 0; q < 4; q++) take(v.v[q]);
+        }
+        if (whole + lane < a.cols) take(p[whole + lane]);
     }
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    if (lane == 0) red[wave] = m;
     __syncthreads();
-    if (threadIdx.x == 0) a.maxpart[wg] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 8; w++) m = fmaxf(m, red[w]);
+        a.maxpart[wg] = m;
+    }
 }
 
 // The images of two matrices, zeros in the padding: a thread eight columns of a row; the first matrix has wgs0 workgroups.
@@ -667,6 +675,7 @@ struct RowArgs {
     int spans;
     const float2 *part; const float *part_e; const float4 *part_t; const float *tlogit;
     const long long *target; long long ignore;
+    float *loss_out, *ent_out;    // [n], or null: rows' results that nothing else has to be added to
     float4 *stats;                // [n]: M, sum pi / s, sum |pi|, loss with lse = M ln2 + log s (so that p takes no rounding of lse)
     float *ent;                   // [n] or null
 };
@@ -677,18 +686,30 @@ __global__ __launch_bounds__(256) void rows_kernel(RowArgs a)
     const int lane = threadIdx.x & 63;
     if (row >= a.n) return;
     float mx = -INFINITY, s = 0.f, e = 0.f, tl = 0.f, ts = 0.f, ta = 0.f;
-    for (int t = lane; t < a.spans; t += 64) {
-        const float2 p = a.part[(long long)t * a.n + row];
-        const float m = fmaxf(mx, p.x), base = m == -INFINITY ? 0.f : m;
-        const float f0 = __builtin_amdgcn_exp2f(mx - base), f1 = __builtin_amdgcn_exp2f(p.x - base);
+    // four spans a lane at a time: their maximum first, so that the loads do not wait for the sums
+    for (int t0 = lane; t0 < a.spans; t0 += 256) {
+        float2 p[4];
+        float q[4];
+        float4 u[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const bool in = t0 + 64 * j < a.spans;
+            const long long at = (long long)(in ? t0 + 64 * j : t0) * a.n + row;
+            p[j] = a.part[at];
+            q[j] = a.part_e ? a.part_e[at] : 0.f;
+            u[j] = a.part_t ? a.part_t[at] : make_float4(0.f, 0.f, 0.f, 0.f);
+            if (!in) { p[j] = make_float2(-INFINITY, 0.f); q[j] = 0.f; u[j] = make_float4(0.f, 0.f, 0.f, 0.f); }
+        }
+        const float m = fmaxf(fmaxf(mx, fmaxf(p[0].x, p[1].x)), fmaxf(p[2].x, p[3].x)), base = m == -INFINITY ? 0.f : m;
         // (a pair without a class adds nothing; a NaN sum stays NaN)
-        s = (mx == -INFINITY ? s : s * f0) + (p.x == -INFINITY ? p.y : p.y * f1);
-        if (a.part_e) {
-            const float q = a.part_e[(long long)t * a.n + row];
-            e = (mx == -INFINITY ? e : e * f0) + (p.x == -INFINITY ? q : q * f1);
+        const float f0 = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - base);
+        s *= f0; e *= f0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float f = p[j].x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(p[j].x - base);
+            s += p[j].y * f; e += q[j] * f; tl += u[j].x; ts += u[j].y; ta += u[j].z;
         }
         mx = m;
-        if (a.part_t) { const float4 q = a.part_t[(long long)t * a.n + row]; tl += q.x; ts += q.y; ta += q.z; }
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -713,6 +734,8 @@ __global__ __launch_bounds__(256) void rows_kernel(RowArgs a)
     }
     a.stats[row] = make_float4(mx, ts / s, ta, loss);
     if (a.ent) a.ent[row] = ent;
+    if (a.loss_out) a.loss_out[row] = loss;
+    if (a.ent_out) a.ent_out[row] = ent;
 }
 
 struct TotalArgs {
@@ -720,7 +743,7 @@ struct TotalArgs {
     int reduction;                // 0 none, 1 sum, 2 mean
     const float4 *stats; const float *ent;
     const long long *target; long long ignore;
-    float *loss, *ent_out;        // [n] or [1]; null: not asked for
+    float *loss, *ent_out;        // [1]; null: not asked for
     const float *dloss;           // [n], [1] or null
     float grad_scale;
     float *rowg;                  // [n]: g_i / 2^e; null: every row that counts has 1 (class numbers and a common g) or no gradient is asked for
@@ -742,11 +765,7 @@ __device__ inline void totals(const TotalArgs &a)
         sl += st.w; cnt += used ? 1.0 : 0.0;
         if (a.ent) se += a.ent[i];
         float g = 1.f;
-        if (a.reduction == 0) {
-            if (a.loss) a.loss[i] = st.w;
-            if (a.ent_out) a.ent_out[i] = a.ent[i];
-            if (a.rowg) g = (a.dloss ? a.dloss[i] : 1.f) * a.grad_scale;
-        }
+        if (a.reduction == 0 && a.rowg) g = (a.dloss ? a.dloss[i] : 1.f) * a.grad_scale;
         const float m = fabsf(g) * st.z;
         if (used && m < INFINITY) mx = fmaxf(mx, m);
     }

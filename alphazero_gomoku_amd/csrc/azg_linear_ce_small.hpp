@@ -72,7 +72,7 @@ __device__ inline fx4 small_frag(const T *p, long long ld, int m, int k, int K, 
 }
 
 // A 32 x 32 tile at (m0, n0), the eight waves' parts of the sum joined through LDS; out: rows 4 wave + lane / 32 + 2 i, column
-// lane & 31.  The next block's operands are on their way while one is multiplied.
+// lane & 31.  Four of a wave's blocks are on their way while four are multiplied: the loads' latency is what bounds these tiles.
 constexpr int kSmallWaves = 8;
 typedef float SmallLds[kSmallWaves][kSmallTile][kSmallTile + 1];
 template <typename TA, bool KA, typename TB, bool KB>
@@ -81,7 +81,8 @@ __device__ inline void small_product(const TA *A, long long lda, int m0, int M, 
 {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
     fx4 acc[2][2] = {{{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}};
-    fx4 a[2], b[2], an[2], bn[2];
+    constexpr int kAhead = 4, kStep = kSmallWaves * 16;
+    fx4 a[kAhead][2], b[kAhead][2], an[kAhead][2], bn[kAhead][2];
     // (rows past the end repeat the last one: they reach only results that are not stored)
     int ma[2], nb[2];
 #pragma unroll
@@ -98,17 +99,28 @@ __device__ inline void small_product(const TA *A, long long lda, int m0, int M, 
             }
         }
     };
-    load(a, b, wave * 16);
-    for (int k = wave * 16; k < K; k += kSmallWaves * 16) {
-        load(an, bn, k + kSmallWaves * 16);                   // (past the end: zeros)
+    auto load4 = [&](fx4 (&x)[kAhead][2], fx4 (&y)[kAhead][2], int k) {
 #pragma unroll
-        for (int j = 0; j < 4; j++)
+        for (int u = 0; u < kAhead; u++)
+            if (k + u * kStep < K) load(x[u], y[u], k + u * kStep);
+    };
+    load4(a, b, wave * 16);
+    for (int k = wave * 16; k < K; k += kAhead * kStep) {
+        load4(an, bn, k + kAhead * kStep);
 #pragma unroll
-            for (int s = 0; s < 2; s++)
+        for (int u = 0; u < kAhead; u++)
+            if (k + u * kStep < K) {
 #pragma unroll
-                for (int t = 0; t < 2; t++) acc[s][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s][j], b[t][j], acc[s][t], 0, 0, 0);
+                for (int j = 0; j < 4; j++)
 #pragma unroll
-        for (int t = 0; t < 2; t++) { a[t] = an[t]; b[t] = bn[t]; }
+                    for (int s = 0; s < 2; s++)
+#pragma unroll
+                        for (int t = 0; t < 2; t++) acc[s][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][s][j], b[u][t][j], acc[s][t], 0, 0, 0);
+            }
+#pragma unroll
+        for (int u = 0; u < kAhead; u++)
+#pragma unroll
+            for (int t = 0; t < 2; t++) { a[u][t] = an[u][t]; b[u][t] = bn[u][t]; }
     }
 #pragma unroll
     for (int s = 0; s < 2; s++)

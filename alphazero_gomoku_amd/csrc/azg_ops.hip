@@ -125,11 +125,11 @@ Shape pick_logits(long long m, long long n, bool grad)
 // Tile of the gradients' products, which share a launch, and the splits of their sums, by an estimate in microseconds: the
 // launch takes its stages at the rate of the whole card or as long as its longest workgroup, whichever is more, and splits
 // cost a join.  Per stage and tile (measured at 16 bits; float32 half as much again): 256 x 256 1.0 with a CU to itself,
-// 128 x 128 0.33 a CU's share and 0.7 from start to end, 64 x 64 0.12 and 0.45.
+// 128 x 128 0.30 a CU's share and 0.6 from start to end, 64 x 64 0.16 and 0.45.
 struct GradPick { Shape shape; int splits_x, kper_x, splits_w, kper_w; };
 GradPick pick_grads(long long n, long long h, long long v, long long kx, long long kw, bool want_x, bool want_w)
 {
-    static constexpr double share[3] = {1.0, 0.33, 0.12}, alone[3] = {1.0, 0.7, 0.45};
+    static constexpr double share[3] = {1.0, 0.30, 0.16}, alone[3] = {1.0, 0.6, 0.45};
     GradPick best{};
     double least = 1e30;
     for (Shape s : {T256, T128, T64}) {
@@ -150,8 +150,9 @@ GradPick pick_grads(long long n, long long h, long long v, long long kx, long lo
             if (tw && g.splits_w > 1) joined += 8.0 * g.splits_w * v * h;
             const double work = (double)(tx * kx + tw * kw) * share[s] / 256.0;
             const double longest = std::max(tx ? g.kper_x : 0, tw ? g.kper_w : 0) * alone[s];
-            // (workgroups come in rounds: half a longest one on average is lost at the end)
-            const double t = std::max(work + 0.5 * longest, longest) + joined / 4e6 + (joined > 0 ? 3.0 : 0.0);
+            // (dX's workgroups start first; of the others half a one on average is lost at the end)
+            const double last = (tw ? g.kper_w : g.kper_x) * alone[s];
+            const double t = std::max(work + 0.5 * last, longest) + joined / 4e6 + (joined > 0 ? 3.0 : 0.0);
             if (t < least) { least = t; best = g; }
         }
     }
@@ -352,7 +353,7 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
     px.maxpart = f32(p.xmax); px.img = ws + p.ximg; px.ldi = p.ldk; px.icols = p.kimg;
     PackArgs pw{};
     pw.src = W; pw.ld = a->w_stride; pw.rows = a->classes; pw.cols = a->hidden; pw.maxpart = f32(p.wmax); pw.img = ws + p.wimg; pw.ldi = p.ldk; pw.icols = p.kimg;
-    if (Op::split) hipLaunchKernelGGL(absmax_kernel, dim3(2 * kMaxParts), dim3(256), 0, s, px, pw);
+    if (Op::split) hipLaunchKernelGGL(absmax_kernel, dim3(2 * kMaxParts), dim3(512), 0, s, px, pw);
     bool x_packed = !p.pack_x;
     CeArgs c{};
     c.x = p.pack_x ? Operand{ws + p.ximg, p.ldk, a->n, p.kimg} : Operand{a->x, a->x_stride, a->n, a->hidden};
@@ -392,17 +393,19 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
         r.part = reinterpret_cast<float2 *>(ws + p.part); r.part_e = a->entropy ? f32(p.part_e) : nullptr;
         r.part_t = a->probs ? reinterpret_cast<float4 *>(ws + p.part_t) : nullptr; r.tlogit = f32(p.tlogit);
         r.target = target; r.ignore = a->ignore_index; r.stats = stats; r.ent = a->entropy ? f32(p.ent) : nullptr;
+        if (a->reduction == AZG_REDUCE_NONE) { r.loss_out = a->loss; r.ent_out = a->entropy; }
         hipLaunchKernelGGL(rows_kernel, dim3((unsigned)((a->n + 3) / 4)), dim3(256), 0, s, r);
     }
     TotalArgs t{};
     t.n = a->n; t.reduction = a->reduction; t.stats = stats; t.ent = p.forward && a->entropy ? f32(p.ent) : nullptr;
-    t.target = target; t.ignore = a->ignore_index; t.loss = p.forward ? a->loss : nullptr; t.ent_out = p.forward ? a->entropy : nullptr;
+    t.target = target; t.ignore = a->ignore_index;
+    if (p.forward && a->reduction != AZG_REDUCE_NONE) { t.loss = a->loss; t.ent_out = a->entropy; }
     t.dloss = a->dloss; t.grad_scale = (float)a->grad_scale;
     t.rowg = p.backward ? f32(p.rowg) : nullptr; t.factor = p.backward ? f32(p.factor) : nullptr;
     // class numbers and a common g: the rows' factors are 1 or 0, and the totals can ride on the next launch
     const bool ride = p.keep && target && a->reduction != AZG_REDUCE_NONE;
     if (ride) t.rowg = nullptr;
-    else hipLaunchKernelGGL(totals_kernel, dim3(1), dim3(1024), 0, s, t);
+    else if (p.backward || a->reduction != AZG_REDUCE_NONE) hipLaunchKernelGGL(totals_kernel, dim3(1), dim3(1024), 0, s, t);
     OPS_HIP(hipGetLastError());
     if (!p.backward) return AZG_OK;
 

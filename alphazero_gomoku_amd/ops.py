@@ -53,7 +53,7 @@ def _refuse_capture(*tensors):
 
 
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)     # torch.cuda.current_stream(device).cuda_stream, without its object
 
 
 # ---------------------------------------------------------------- dropout
