@@ -563,6 +563,14 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
             mx *= kLog2e;
             const float base = mx == -INFINITY ? 0.f : mx;
             float s = 0.f, e = 0.f, tl = 0.f, ts = 0.f, ta = 0.f;
+            if (a.part_e)
+#pragma unroll
+                for (int mt = 0; mt < S::MT; mt++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float l = acc[mt][nt][i], x = __builtin_amdgcn_exp2f(__builtin_fmaf(l, kLog2e, -base));
+                        e += x != 0.f ? x * l : 0.f;
+                    }
 #pragma unroll
             for (int mt = 0; mt < S::MT; mt++) {
                 Pack<E, 4> keep;
@@ -570,7 +578,6 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
                 for (int i = 0; i < 4; i++) {
                     const float l = acc[mt][nt][i], x = __builtin_amdgcn_exp2f(__builtin_fmaf(l, kLog2e, -base));
                     s += x;
-                    if (a.part_e) e += x != 0.f ? x * l : 0.f;
                     keep.v[i] = (E)x;
                 }
                 if (a.d && live && vw + mt * 16 < dpad) *reinterpret_cast<Pack<E, 4> *>(static_cast<E *>(a.d) + row * (a.ldd / (Op::split ? 2 : 1)) + vw + mt * 16) = keep;

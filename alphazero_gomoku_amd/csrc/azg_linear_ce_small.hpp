@@ -82,45 +82,40 @@ __device__ inline void small_product(const TA *A, long long lda, int m0, int M, 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
     fx4 acc[2][2] = {{{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}};
     constexpr int kAhead = 4, kStep = kSmallWaves * 16;
-    fx4 a[kAhead][2], b[kAhead][2], an[kAhead][2], bn[kAhead][2];
+    fx4 a[kAhead][2], b[kAhead][2];
     // (rows past the end repeat the last one: they reach only results that are not stored)
     int ma[2], nb[2];
 #pragma unroll
     for (int t = 0; t < 2; t++) { ma[t] = min(m0 + 16 * t + c, M - 1); nb[t] = min(n0 + 16 * t + c, N - 1); }
-    auto load = [&](fx4 (&x)[2], fx4 (&y)[2], int k) {
+    auto load = [&](auto whole, int u, int k) {
+        constexpr bool W = whole.value;
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            if (k + 16 <= K) {
-                x[t] = small_frag<true, TA, KA>(A, lda, ma[t], k + 4 * g, K, nullptr, 0);
-                y[t] = small_frag<true, TB, KB>(B, ldb, nb[t], k + 4 * g, K, skip, ignore);
-            } else {
-                x[t] = small_frag<false, TA, KA>(A, lda, ma[t], k + 4 * g, K, nullptr, 0);
-                y[t] = small_frag<false, TB, KB>(B, ldb, nb[t], k + 4 * g, K, skip, ignore);
-            }
+            a[u][t] = small_frag<W, TA, KA>(A, lda, ma[t], k + 4 * g, K, nullptr, 0);
+            b[u][t] = small_frag<W, TB, KB>(B, ldb, nb[t], k + 4 * g, K, skip, ignore);
         }
     };
-    auto load4 = [&](fx4 (&x)[kAhead][2], fx4 (&y)[kAhead][2], int k) {
+    auto multiply = [&](int u) {
 #pragma unroll
-        for (int u = 0; u < kAhead; u++)
-            if (k + u * kStep < K) load(x[u], y[u], k + u * kStep);
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+#pragma unroll
+                for (int t = 0; t < 2; t++) acc[s][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][s][j], b[u][t][j], acc[s][t], 0, 0, 0);
     };
-    load4(a, b, wave * 16);
     for (int k = wave * 16; k < K; k += kAhead * kStep) {
-        load4(an, bn, k + kAhead * kStep);
+        // whole blocks of this round; a block cut short by the end of K can only be its wave's last one
+        const int whole = max(0, min(kAhead, (K - 16 - k) / kStep + (K - 16 >= k)));
 #pragma unroll
         for (int u = 0; u < kAhead; u++)
-            if (k + u * kStep < K) {
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-#pragma unroll
-                    for (int s = 0; s < 2; s++)
-#pragma unroll
-                        for (int t = 0; t < 2; t++) acc[s][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][s][j], b[u][t][j], acc[s][t], 0, 0, 0);
-            }
+            if (u < whole) load(std::true_type{}, u, k + u * kStep);
 #pragma unroll
         for (int u = 0; u < kAhead; u++)
-#pragma unroll
-            for (int t = 0; t < 2; t++) { a[u][t] = an[u][t]; b[u][t] = bn[u][t]; }
+            if (u < whole) multiply(u);
+        if (whole < kAhead && k + whole * kStep < K) {
+            load(std::false_type{}, 0, k + whole * kStep);
+            multiply(0);
+        }
     }
 #pragma unroll
     for (int s = 0; s < 2; s++)
