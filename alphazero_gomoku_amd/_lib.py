@@ -23,7 +23,7 @@ SYMBOLS = ["azg_create", "azg_destroy", "azg_last_error", "azg_set_weights", "az
            "azg_selfplay_end", "azg_equi_data", "azg_pure_search", "azg_host_timing", "azg_arena_stats", "azg_reroot_stats", "azg_selfplay_fetch_packed", "azg_unpack_states", "azg_playout_begin", "azg_playout_end",
            "azg_board_step_batch_static", "azg_gate_stats", "azg_gate_poke",
            "azg_train_param_count", "azg_train_forward", "azg_train_backward", "azg_train_adam", "azg_train_step", "azg_train_epoch",
-           "azg_dropout", "azg_linear_ce", "azg_linear_ce_workspace"]
+           "azg_train_set_dropout", "azg_dropout", "azg_linear_ce", "azg_linear_ce_workspace"]
 
 
 class AzgError(RuntimeError):
@@ -148,6 +148,7 @@ def load():
     L.azg_set_search_parts.argtypes = [vp, C.c_int]
     L.azg_stream.argtypes = [vp]
     L.azg_stream.restype = vp
+    L.azg_train_set_dropout.argtypes = [vp, C.c_double, C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint64]
     L.azg_dropout.argtypes = [C.POINTER(DropoutArgs)]
     L.azg_linear_ce.argtypes = [C.POINTER(LinearCeArgs)]
     L.azg_linear_ce_workspace.argtypes = [C.POINTER(LinearCeArgs)]

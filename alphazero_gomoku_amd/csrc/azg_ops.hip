@@ -522,7 +522,8 @@ extern "C" int azg_linear_ce(const azg_linear_ce_args *a)
     OPS_TRY(check(a));
     const bool backward = a->dx || a->dw || a->db;
     if (!a->loss && !backward) return fail(AZG_EINVAL, "azg_linear_ce: neither a loss nor a gradient is asked for");
-    if (!a->loss && !a->stats) return fail(AZG_EINVAL, "azg_linear_ce: a backward pass by itself needs the forward pass's stats");
+    if (a->n > 0 && !a->loss && !a->stats) return fail(AZG_EINVAL, "azg_linear_ce: a backward pass by itself needs the forward pass's stats");
+    if (reinterpret_cast<uintptr_t>(a->stats) & 15) return fail(AZG_EINVAL, "azg_linear_ce: stats must be 16-byte aligned");
     if (a->entropy && !a->loss) return fail(AZG_EINVAL, "azg_linear_ce: the entropy comes with the loss");
     if ((a->dx && bad_matrix(a->n, a->hidden, a->dx_stride)) || (a->dw && bad_matrix(a->classes, a->hidden, a->dw_stride)))
         return fail(AZG_EINVAL, "azg_linear_ce: a row stride is smaller than a row");

@@ -463,7 +463,9 @@ struct FcArgs {
     float *dh8;                      // [n*S][8]: gradient at the six head pre-activations, channels-last
     float *lossparts;                // [n][3]: value loss, policy loss, entropy of the sample
     int n, S, ldhv;                  // ldhv: row stride of hv (2S rounded up to 4)
+    float hscale;                    // factor of the value features' gradient (1; with dropout the kept elements' scale)
 };
+// With wp null the policy head is somebody else's: only the value head's results are made.
 
 __device__ inline float block_reduce(float v, float *red, int tid, bool is_max)
 {
@@ -485,11 +487,13 @@ __global__ __launch_bounds__(256) void fc_sample_kernel(FcArgs a)
     __shared__ __attribute__((aligned(16))) float hp[4 * MAXS], hv[2 * MAXS];
     __shared__ float lg[MAXS], dl[MAXS], h1s[64], dh1s[64], red[256];
     const int tid = threadIdx.x, b = blockIdx.x, S = a.S;
-    for (int k = tid; k < 4 * S; k += 256) hp[k] = a.hp[(size_t)b * 4 * S + k];
+    if (a.wp)
+        for (int k = tid; k < 4 * S; k += 256) hp[k] = a.hp[(size_t)b * 4 * S + k];
     for (int k = tid; k < 2 * S; k += 256) hv[k] = a.hv[(size_t)b * a.ldhv + k];
     __syncthreads();
     for (int item = tid; item < S + 64; item += 256) {
         if (item < S) {
+            if (!a.wp) continue;
             const float *w = a.wp + (size_t)item * 4 * S;
             float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
             for (int k = 0; k < 4 * S; k += 4) {
@@ -509,13 +513,15 @@ __global__ __launch_bounds__(256) void fc_sample_kernel(FcArgs a)
     }
     __syncthreads();
     // log_softmax over the S logits
-    float mx = -3.0e38f;
-    for (int o = tid; o < S; o += 256) mx = fmaxf(mx, lg[o]);
-    mx = block_reduce(mx, red, tid, true);
-    float se = 0.f;
-    for (int o = tid; o < S; o += 256) se += expf(lg[o] - mx);
-    se = block_reduce(se, red, tid, false);
-    const float lse = logf(se);
+    float mx = -3.0e38f, lse = 0.f;
+    if (a.wp) {
+        for (int o = tid; o < S; o += 256) mx = fmaxf(mx, lg[o]);
+        mx = block_reduce(mx, red, tid, true);
+        float se = 0.f;
+        for (int o = tid; o < S; o += 256) se += expf(lg[o] - mx);
+        se = block_reduce(se, red, tid, false);
+        lse = logf(se);
+    }
     // value
     float pv = tid < 64 ? h1s[tid] * a.wv2[tid] : 0.f;
     pv = block_reduce(pv, red, tid, false);
@@ -538,27 +544,29 @@ __global__ __launch_bounds__(256) void fc_sample_kernel(FcArgs a)
         }
         if (tid == 0) a.klparts[b] = dred[0];
     }
-    if (!a.pi) return;
+    if (!a.z) return;
 
     // losses of the sample and the gradient at the logits: d(-mean_b sum_o pi log p)/dlogit = (p * sum(pi) - pi) / n
     float spi = 0.f, pl = 0.f, en = 0.f;
-    for (int o = tid; o < S; o += 256) {
-        const float logp = (lg[o] - mx) - lse, pr = expf(logp), t = a.pi[(size_t)b * S + o];
-        spi += t; pl -= t * logp; en -= pr * logp;
-    }
-    spi = block_reduce(spi, red, tid, false);
-    pl = block_reduce(pl, red, tid, false);
-    en = block_reduce(en, red, tid, false);
     const float inv_n = 1.0f / (float)a.n;
-    const int Sp = (S + 3) & ~3;
-    for (int o = tid; o < Sp; o += 256) {
-        float g = 0.f;
-        if (o < S) {
-            const float pr = expf((lg[o] - mx) - lse);
-            g = (pr * spi - a.pi[(size_t)b * S + o]) * inv_n;
-            dl[o] = g;
+    if (a.wp) {
+        for (int o = tid; o < S; o += 256) {
+            const float logp = (lg[o] - mx) - lse, pr = expf(logp), t = a.pi[(size_t)b * S + o];
+            spi += t; pl -= t * logp; en -= pr * logp;
         }
-        a.dlogit[(size_t)b * Sp + o] = g;
+        spi = block_reduce(spi, red, tid, false);
+        pl = block_reduce(pl, red, tid, false);
+        en = block_reduce(en, red, tid, false);
+        const int Sp = (S + 3) & ~3;
+        for (int o = tid; o < Sp; o += 256) {
+            float g = 0.f;
+            if (o < S) {
+                const float pr = expf((lg[o] - mx) - lse);
+                g = (pr * spi - a.pi[(size_t)b * S + o]) * inv_n;
+                dl[o] = g;
+            }
+            a.dlogit[(size_t)b * Sp + o] = g;
+        }
     }
     const float err = value - a.z[b];
     const float dpre2 = 2.0f * err * inv_n * (1.0f - value * value);      // through mse_loss's mean and tanh
@@ -575,7 +583,7 @@ __global__ __launch_bounds__(256) void fc_sample_kernel(FcArgs a)
     }
     __syncthreads();
     // down to the head convolutions: dh[k] = sum_o W[o][k] dlogit[o], masked by the head's ReLU
-    for (int k = tid; k < 6 * S; k += 256) {
+    for (int k = (a.wp ? 0 : 4 * S) + tid; k < 6 * S; k += 256) {
         float s = 0.f;
         int c, p;
         float hval;
@@ -586,10 +594,20 @@ __global__ __launch_bounds__(256) void fc_sample_kernel(FcArgs a)
             const int kv = k - 4 * S;
             for (int j = 0; j < 64; j++) s = __builtin_fmaf(a.wv1[(size_t)j * 2 * S + kv], dh1s[j], s);
             c = 4 + kv / S; p = kv - (c - 4) * S; hval = hv[kv];
+            s *= a.hscale;
         }
         a.dh8[((size_t)b * S + p) * 8 + c] = hval > 0.f ? s : 0.f;
     }
     for (int p = tid; p < S; p += 256) { a.dh8[((size_t)b * S + p) * 8 + 6] = 0.f; a.dh8[((size_t)b * S + p) * 8 + 7] = 0.f; }
+}
+
+// The policy features' gradient [n][4S], zero where the (dropped-out) feature is not positive, into dh8's first four channels.
+__global__ void policy_dh8_kernel(const float *dhp, const float *hp, int n, int S, float *dh8)
+{
+    const int idx = blockIdx.x * blockDim.x + threadIdx.x;       // (sample, channel, cell)
+    if (idx >= n * 4 * S) return;
+    const int b = idx / (4 * S), k = idx - b * 4 * S, c = k / S, p = k - c * S;
+    dh8[((size_t)b * S + p) * 8 + c] = hp[idx] > 0.f ? dhp[idx] : 0.f;
 }
 
 // gradient at conv3's pre-activation from the six head channels: dz3[m][ch] = a3 > 0 ? sum_c wh[c][ch] dh8[m][c] : 0
@@ -676,7 +694,8 @@ __global__ __launch_bounds__(256) void grad_assemble_kernel(GradSegs g, int S, f
 }
 
 // loss = mean value loss + mean policy loss, entropy = mean entropy (policy_value_net_pytorch.py:128-147)
-__global__ __launch_bounds__(256) void loss_kernel(const float *parts, int n, float *out)
+// `policy`: null, or the policy head's mean loss and entropy where parts holds the value head's alone
+__global__ __launch_bounds__(256) void loss_kernel(const float *parts, int n, const float *policy, float *out)
 {
     __shared__ double red[3][256];
     const int tid = threadIdx.x;
@@ -691,8 +710,8 @@ __global__ __launch_bounds__(256) void loss_kernel(const float *parts, int n, fl
         __syncthreads();
     }
     if (tid == 0) {
-        out[0] = (float)(red[0][0] / n + red[1][0] / n);
-        out[1] = (float)(red[2][0] / n);
+        out[0] = (float)(red[0][0] / n + (policy ? (double)policy[0] : red[1][0] / n));
+        out[1] = policy ? policy[1] : (float)(red[2][0] / n);
     }
 }
 

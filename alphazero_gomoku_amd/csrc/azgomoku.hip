@@ -215,6 +215,11 @@ struct azg_handle {
         const float *checked[16] = {nullptr};    // parameter pointers already seen to be device memory
         float *h_loss = nullptr;                 // pinned: loss, entropy, and a double (KL) at +8
         double *klparts = nullptr;               // [n] per-sample sums of the KL test
+        // dropout of the head features (azg_train_set_dropout)
+        double drop_p = 0.0;
+        uint64_t drop_seed = 0, drop_offset = 0, drop_first = 0, drop_step = 1;
+        char *drop_block = nullptr;              // gradient at the policy features, policy loss and entropy, operator workspace
+        size_t drop_cap = 0;
     } tw;
     // profiling
     std::vector<std::pair<hipEvent_t, hipEvent_t>> ev_pool;
@@ -483,6 +488,7 @@ extern "C" void azg_destroy(azg_handle *h)
     if (h->h_mirror) (void)hipHostFree(h->h_mirror);
     if (h->h_static_bad) (void)hipHostFree(h->h_static_bad);
     if (h->tw.block) (void)hipFree(h->tw.block);
+    if (h->tw.drop_block) (void)hipFree(h->tw.drop_block);
     if (h->tw.h_loss) (void)hipHostFree(h->tw.h_loss);
     if (h->tw.stream) (void)hipStreamDestroy(h->tw.stream);
     if (h->sp.h_map) (void)hipHostFree(h->sp.h_map);
@@ -1782,6 +1788,7 @@ static FcArgs train_fc_args(azg_handle *h, int n, const TrainParams &P)
     f.hp = w.hp; f.hv = w.hv; f.wp = P.p[8]; f.bp = P.p[9]; f.wv1 = P.p[12]; f.bv1 = P.p[13]; f.wv2 = P.p[14]; f.bv2 = P.p[15];
     f.dlogit = w.dlogit; f.dh1 = w.dh1; f.g2 = w.g2; f.dh8 = w.dh8; f.lossparts = w.lossparts;
     f.n = n; f.S = h->st.S; f.ldhv = (2 * h->st.S + 3) & ~3;
+    f.hscale = 1.0f;
     return f;
 }
 
@@ -1826,6 +1833,64 @@ extern "C" int azg_train_forward(azg_handle *h, int n, const float *states, cons
     return AZG_OK;
 }
 
+// The heads of a training pass with dropout: features hp and hv are dropped out in place, the policy head's loss, entropy and
+// gradients come from the projection's softmax cross entropy (weight and bias gradients straight into the flat vector), the
+// gradient at the policy features goes through the mask again into dh8.  The value head is fc_sample_kernel's.
+static int train_dropout_heads(azg_handle *h, int n, const float *mcts_probs, const TrainParams &P, float *grads, const float **policy)
+{
+    auto &w = h->tw;
+    const int S = h->st.S;
+    const ParamLayout L = param_layout(S);
+    auto ops = [&](int rc) { return rc ? fail(h, rc, "%s", azg_last_error(nullptr)) : AZG_OK; };
+    const size_t dhp_bytes = ((size_t)n * 4 * S * 4 + 255) / 256 * 256;
+    azg_linear_ce_args c{};
+    c.device = h->cfg.device; c.dtype = AZG_F32; c.reduction = AZG_REDUCE_MEAN;
+    c.n = n; c.hidden = 4 * S; c.classes = S;
+    c.x = w.hp; c.x_stride = 4 * S; c.w = P.p[8]; c.w_stride = 4 * S; c.bias = P.p[9];
+    c.probs = mcts_probs; c.probs_stride = S; c.grad_scale = 1.0;
+    // (sizes first: the pointers that decide what is asked for have to be there)
+    c.loss = grads; c.entropy = grads; c.dx = w.hp; c.dx_stride = 4 * S;
+    c.dw = grads + L.off[8]; c.dw_stride = 4 * S; c.db = grads + L.off[9];
+    const int64_t ws = azg_linear_ce_workspace(&c);
+    if (ws < 0) return ops((int)ws);
+    const size_t need = dhp_bytes + 256 + (size_t)ws;
+    if (need > w.drop_cap) {
+        HIPCHK(h, hipStreamSynchronize(w.stream));
+        if (w.drop_block) HIPCHK(h, hipFree(w.drop_block));
+        w.drop_block = nullptr;
+        w.drop_cap = 0;
+        HIPCHK(h, hipMalloc((void **)&w.drop_block, need));
+        w.drop_cap = need;
+    }
+    float *dhp = reinterpret_cast<float *>(w.drop_block), *out = reinterpret_cast<float *>(w.drop_block + dhp_bytes);
+    azg_dropout_args d{};
+    d.device = h->cfg.device; d.dtype = AZG_F32; d.rows = n; d.p = w.drop_p; d.seed = w.drop_seed;
+    d.first_row = w.drop_first; d.row_step = w.drop_step; d.stream = w.stream;
+    d.cols = 4 * S; d.x = d.out = w.hp; d.x_stride = d.out_stride = 4 * S; d.offset = 2 * w.drop_offset;
+    int rc = ops(azg_dropout(&d));
+    if (rc) return rc;
+    d.cols = 2 * S; d.x = d.out = w.hv; d.x_stride = d.out_stride = (2 * S + 3) & ~3; d.offset = 2 * w.drop_offset + 1;
+    if ((rc = ops(azg_dropout(&d)))) return rc;
+    c.loss = out; c.entropy = out + 1; c.dx = dhp; c.stream = w.stream;
+    c.workspace = w.drop_block + dhp_bytes + 256; c.workspace_bytes = ws;
+    if ((rc = ops(azg_linear_ce(&c)))) return rc;
+    d.cols = 4 * S; d.x = d.out = dhp; d.x_stride = d.out_stride = 4 * S; d.offset = 2 * w.drop_offset;
+    if ((rc = ops(azg_dropout(&d)))) return rc;
+    hipLaunchKernelGGL(policy_dh8_kernel, dim3((n * 4 * S + 255) / 256), dim3(256), 0, w.stream, (const float *)dhp, (const float *)w.hp, n, S, w.dh8);
+    HIPCHK(h, hipGetLastError());
+    *policy = out;
+    return AZG_OK;
+}
+
+extern "C" int azg_train_set_dropout(azg_handle *h, double p, uint64_t seed, uint64_t offset, uint64_t first_row, uint64_t row_step)
+{
+    if (!h) return AZG_EINVAL;
+    if (!(p >= 0.0 && p < 1.0)) return fail(h, AZG_EINVAL, "azg_train_set_dropout: p must lie in [0, 1)");
+    auto &w = h->tw;
+    w.drop_p = p; w.drop_seed = seed; w.drop_offset = offset; w.drop_first = first_row; w.drop_step = row_step;
+    return AZG_OK;
+}
+
 // forward + backward of one mini-batch, enqueued on the training stream (no synchronisation)
 static int train_backward_enqueue(azg_handle *h, int n, const float *states, const float *mcts_probs, const float *winners,
                                   const TrainParams &P, float *grads)
@@ -1837,14 +1902,23 @@ static int train_backward_enqueue(azg_handle *h, int n, const float *states, con
     train_forward_convs(h, n, P);
     FcArgs f = train_fc_args(h, n, P);
     f.pi = mcts_probs; f.z = winners;
+    const bool drop = w.drop_p > 0.0;
+    const float *policy = nullptr;                                              // mean policy loss and entropy, with dropout
+    if (drop) {
+        const int rc = train_dropout_heads(h, n, mcts_probs, P, grads, &policy);
+        if (rc) return rc;
+        f.wp = nullptr;
+        const long T = std::lround(w.drop_p * 65536.0);
+        f.hscale = T < 65536 ? (float)(65536.0 / (double)(65536 - T)) : 0.f;
+    }
     hipLaunchKernelGGL(fc_sample_kernel, dim3(n), dim3(256), 0, s, f);
-    hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(256), 0, s, (const float *)w.lossparts, n, w.lossout);
+    hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(256), 0, s, (const float *)w.lossparts, n, policy, w.lossout);
     // fully connected layers: weight gradients as [input][output] partial sums, bias gradients with them
     {
         WgradArgs g{};
         g.taps = 1; g.M = n; g.S = 1; g.Nb = 1; g.rows_per_split = w.frows;
         g.src = w.hp; g.Cs = 4 * S; g.I = 4 * S; g.dz = w.dlogit; g.ldz = (S + 3) & ~3; g.J = S; g.part = w.ppart; g.bpart = w.pbpart;
-        hipLaunchKernelGGL((wgrad_gemm_kernel<64>), dim3((g.I + TBM - 1) / TBM, (g.J + 63) / 64, w.fsplits), dim3(256), 0, s, g);
+        if (!drop) hipLaunchKernelGGL((wgrad_gemm_kernel<64>), dim3((g.I + TBM - 1) / TBM, (g.J + 63) / 64, w.fsplits), dim3(256), 0, s, g);
         g.src = w.hv; g.Cs = (2 * S + 3) & ~3; g.I = 2 * S; g.dz = w.dh1; g.ldz = 64; g.J = 64; g.part = w.vpart; g.bpart = w.vbpart;
         hipLaunchKernelGGL((wgrad_gemm_kernel<64>), dim3((g.I + TBM - 1) / TBM, 1, w.fsplits), dim3(256), 0, s, g);
         hipLaunchKernelGGL(colsum_kernel, dim3(w.gsplits), dim3(256), 0, s, (const float *)w.g2, n, 128, 128, w.grows, w.g2part);
@@ -1889,8 +1963,10 @@ static int train_backward_enqueue(azg_handle *h, int n, const float *states, con
     }
     seg(w.hpart, 128 * 8, w.hsplits, GS_HEAD_W, 0, 0);
     seg(w.hbpart, 8, w.hsplits, GS_HEAD_B, 0, 0);
-    seg(w.ppart, 4 * S * S, w.fsplits, GS_FC_W, 8, S);
-    seg(w.pbpart, S, w.fsplits, GS_PLAIN, 9, 0);
+    if (!drop) {                                              // (with dropout they are in place already)
+        seg(w.ppart, 4 * S * S, w.fsplits, GS_FC_W, 8, S);
+        seg(w.pbpart, S, w.fsplits, GS_PLAIN, 9, 0);
+    }
     seg(w.vpart, 2 * S * 64, w.fsplits, GS_FC_W, 12, 64);
     seg(w.vbpart, 64, w.fsplits, GS_PLAIN, 13, 0);
     seg(w.g2part, 128, w.gsplits, GS_G2, 0, 0);

@@ -57,38 +57,56 @@ class Net(nn.Module):
         self.val_fc1 = nn.Linear(2 * s, 64)
         self.val_fc2 = nn.Linear(64, 1)
 
-    def forward(self, x):
+    def features(self, x):
+        """What the two heads' fully connected layers read: [n, 4S], [n, 2S]."""
         s = self.board_width * self.board_height
         x = F.relu(self.conv3(F.relu(self.conv2(F.relu(self.conv1(x))))))
-        a = F.relu(self.act_conv1(x)).reshape(-1, 4 * s)
-        a = F.log_softmax(self.act_fc1(a), dim=1)
-        v = F.relu(self.val_conv1(x)).reshape(-1, 2 * s)
-        v = torch.tanh(self.val_fc2(F.relu(self.val_fc1(v))))
-        return a, v
+        return F.relu(self.act_conv1(x)).reshape(-1, 4 * s), F.relu(self.val_conv1(x)).reshape(-1, 2 * s)
+
+    def value(self, v):
+        return torch.tanh(self.val_fc2(F.relu(self.val_fc1(v))))
+
+    def forward(self, x):
+        a, v = self.features(x)
+        return F.log_softmax(self.act_fc1(a), dim=1), self.value(v)
 
 
-def train_step_tensors(module, optimizer, s, p, z, lr, reduce_fn=None):
+def train_step_tensors(module, optimizer, s, p, z, lr, reduce_fn=None, dropout=None):
     """policy_value_net_pytorch.py:117-148 on torch tensors of any device: loss = MSE(v, z) -
     mean(sum(pi * log p)), one optimiser step at learning rate lr; reduce_fn(module), if given, runs
-    between backward and the step (gradient averaging over ranks).  Returns (loss, entropy) as
-    0-dim tensors."""
+    between backward and the step (gradient averaging over ranks).  dropout: (p, seed, offset,
+    first_row, row_step) of azg_train_set_dropout, on CUDA tensors: the heads' features are dropped
+    out and the policy head is ops.linear_cross_entropy.  Returns (loss, entropy) as 0-dim tensors."""
     optimizer.zero_grad()
     for group in optimizer.param_groups:
         group['lr'] = lr
-    logp, v = module(s)
-    value_loss = F.mse_loss(v.view(-1), z)
-    policy_loss = -torch.mean(torch.sum(p * logp, 1))
-    loss = value_loss + policy_loss
+    if dropout is None:
+        logp, v = module(s)
+        policy_loss = -torch.mean(torch.sum(p * logp, 1))
+    else:
+        from . import ops
+        rate, seed, offset, first_row, row_step = dropout
+        a, v = module.features(s)
+        a = ops.dropout(a, rate, seed, 2 * offset, first_row=first_row, row_step=row_step)
+        v = module.value(ops.dropout(v, rate, seed, 2 * offset + 1, first_row=first_row, row_step=row_step))
+        policy_loss, entropy = ops.linear_cross_entropy(a, module.act_fc1.weight, p, module.act_fc1.bias, return_entropy=True)
+    loss = F.mse_loss(v.view(-1), z) + policy_loss
     loss.backward()
     if reduce_fn is not None:
         reduce_fn(module)
     optimizer.step()
-    entropy = -torch.mean(torch.sum(torch.exp(logp) * logp, 1))
+    if dropout is None:
+        entropy = -torch.mean(torch.sum(torch.exp(logp) * logp, 1))
     return loss.detach(), entropy.detach()
 
 
 class PolicyValueNet(object):
-    def __init__(self, board_width, board_height, model_file=None, use_gpu=True, device=0, native_train=True):
+    def __init__(self, board_width, board_height, model_file=None, use_gpu=True, device=0, native_train=True,
+                 dropout=0.0, dropout_seed=0):
+        if not 0.0 <= float(dropout) < 1.0:
+            raise ValueError("dropout must lie in [0, 1)")
+        if not 0 <= int(dropout_seed) < 1 << 64:
+            raise ValueError("dropout_seed must be an integer from 0 to 2**64 - 1")
         if board_width != board_height:
             raise ValueError("only square boards are supported by the HIP engine")
         if not torch.cuda.is_available():
@@ -106,6 +124,9 @@ class PolicyValueNet(object):
         # native_train: train_step runs in the HIP library; False: PyTorch autograd + torch.optim.Adam
         # (the two keep separate optimiser states: use one or the other on a net)
         self.native_train = bool(native_train)
+        # dropout: probability with which train_step drops the features that the heads' fully connected layers read (0: the
+        # reference's step); the mask is a function of dropout_seed, the step's number and the position in the mini-batch
+        self.dropout, self.dropout_seed = float(dropout), int(dropout_seed)
         self._adam = None            # (grad, m, v) flat float32 vectors in state_dict order, step count
         self._ptr_cache = None
         self._adam_step = 0
@@ -220,6 +241,16 @@ class PolicyValueNet(object):
             self._ptr_cache = ((C.c_void_p * 16)(*[t.data_ptr() for t in ts]), ts)
         return self._ptr_cache
 
+    def _dropout_args(self, step):
+        """(p, seed, offset, first_row, row_step) of a training step; ranks hold every world-th row of the mini-batch."""
+        rank, world = 0, 1
+        if self.data_parallel and torch.distributed.is_available() and torch.distributed.is_initialized():
+            rank, world = torch.distributed.get_rank(), torch.distributed.get_world_size()
+        return self.dropout, self.dropout_seed, step, rank, world
+
+    def _set_dropout(self, eng, step):
+        eng._chk(eng.L.azg_train_set_dropout(eng.h, *self._dropout_args(step)))
+
     def policy_value_in_training(self, state_batch, old_probs=None):
         """(probs [B,S], value [B,1]) of a CUDA batch for the KL monitor inside policy_update, from the
         parameters as they are NOW (between two train steps of one update the search engine's packed
@@ -260,7 +291,8 @@ class PolicyValueNet(object):
 
     def native_gradients(self, state_batch, mcts_probs, winner_batch):
         """(flat gradient in state_dict order as a new CUDA tensor, loss, entropy) of the library's
-        backward pass on a batch, without touching the parameters (tests; gradient inspection)."""
+        backward pass on a batch, without touching the parameters (tests; gradient inspection); with
+        dropout, under the mask of the next train_step."""
         dev = self.device
         s = torch.as_tensor(np.asarray(state_batch), dtype=torch.float32, device=dev).contiguous() if not torch.is_tensor(state_batch) \
             else state_batch.to(device=dev, dtype=torch.float32).contiguous()
@@ -271,6 +303,7 @@ class PolicyValueNet(object):
         eng = self._engine_handle()
         grad = torch.zeros(int(eng.L.azg_train_param_count(eng.h)), dtype=torch.float32, device=dev)
         arr, keep = self._param_ptrs()
+        self._set_dropout(eng, self._adam_step + 1)
         loss, entropy = C.c_float(0.0), C.c_float(0.0)
         torch.cuda.current_stream(dev).synchronize()
         eng._chk(eng.L.azg_train_backward(eng.h, int(s.shape[0]), C.c_void_p(s.data_ptr()), C.c_void_p(p.data_ptr()),
@@ -294,8 +327,10 @@ class PolicyValueNet(object):
             if dp:
                 from .dist import allreduce_gradients
                 reduce_fn = allreduce_gradients                  # every rank holds an equal share of the batch
+            self._adam_step += 1
             loss, entropy = train_step_tensors(self.policy_value_net, self.optimizer, tensor(state_batch), tensor(mcts_probs),
-                                               tensor(winner_batch), lr, reduce_fn)
+                                               tensor(winner_batch), lr, reduce_fn,
+                                               self._dropout_args(self._adam_step) if self.dropout else None)
             self.version += 1
             return float(loss.item()), float(entropy.item())
         s, p, z = tensor(state_batch).contiguous(), tensor(mcts_probs).contiguous(), tensor(winner_batch).contiguous().reshape(-1)
@@ -309,6 +344,7 @@ class PolicyValueNet(object):
         loss, entropy = C.c_float(0.0), C.c_float(0.0)
         torch.cuda.current_stream(dev).synchronize()           # the batch exists before the library's stream reads it
         self._adam_step += 1
+        self._set_dropout(eng, self._adam_step)
         if dp:
             from .dist import allreduce_flat
             eng._chk(eng.L.azg_train_backward(eng.h, n, C.c_void_p(s.data_ptr()), C.c_void_p(p.data_ptr()), C.c_void_p(z.data_ptr()),
@@ -350,6 +386,7 @@ class PolicyValueNet(object):
         loss, entropy, kl = C.c_float(0.0), C.c_float(0.0), C.c_double(0.0)
         torch.cuda.current_stream(dev).synchronize()           # the batch exists before the library's stream reads it
         self._adam_step += 1
+        self._set_dropout(eng, self._adam_step)
         eng._chk(eng.L.azg_train_epoch(eng.h, n, C.c_void_p(s.data_ptr()), C.c_void_p(p.data_ptr()), C.c_void_p(z.data_ptr()), arr,
                                        C.c_void_p(grad.data_ptr()), C.c_void_p(m.data_ptr()), C.c_void_p(v.data_ptr()),
                                        self._adam_step, float(lr), 0.9, 0.999, 1e-8, self.l2_const, C.byref(loss), C.byref(entropy),

@@ -56,7 +56,9 @@ class TrainPipeline:
                       1x1 head convolutions zeroed (PolicyValueNet.zero_head_biases says why).  Default
                       (None): only when games are played in batches, where dozens of updates at the full
                       learning rate follow each other on a net that has not moved yet; with this and the
-                      ceiling of 1, twenty of twenty differently seeded runs learned."""
+                      ceiling of 1, twenty of twenty differently seeded runs learned.
+    dropout           probability with which a training step drops the features of the two heads (PolicyValueNet's
+                      dropout, seeded with seed0), for a net created here; 0 is the reference's step."""
 
     @staticmethod
     def controller_defaults(play_batch_size, max_lr_multiplier=None, zero_head_biases=None):
@@ -73,7 +75,8 @@ class TrainPipeline:
                  lr_multiplier=1.0, temp=1.0, n_playout=400, c_puct=5, buffer_size=10000, batch_size=512,
                  play_batch_size=1, epochs=5, kl_targ=0.02, check_freq=50, game_batch_num=1500,
                  n_parallel=1024, device=0, seed0=0, policy_value_net=None, pure_mcts_playout_num=1000,
-                 updates_per_batch=1, continuous=False, rng=None, max_lr_multiplier=None, zero_head_biases=None):
+                 updates_per_batch=1, continuous=False, rng=None, max_lr_multiplier=None, zero_head_biases=None,
+                 dropout=0.0):
         import torch
         from .net import PolicyValueNet
         self.board_width, self.board_height, self.n_in_row = board_width, board_height, n_in_row
@@ -91,8 +94,10 @@ class TrainPipeline:
         self.best_win_ratio = 0.2                                            # train.py:88
         self.pure_mcts_playout_num = pure_mcts_playout_num
         fresh = policy_value_net is None and not init_model
+        if policy_value_net is not None and dropout:
+            raise ValueError("dropout is for a net created here: give the net passed in its own")
         self.policy_value_net = policy_value_net or PolicyValueNet(board_width, board_height, model_file=init_model,
-                                                                   device=device)
+                                                                   device=device, dropout=dropout, dropout_seed=seed0 % (1 << 64))
         self.zeroed_head_biases = bool(fresh and want_zero)      # reported by the training program
         if self.zeroed_head_biases:
             self.policy_value_net.zero_head_biases()
@@ -426,6 +431,8 @@ def main(argv=None):
                     help="the KL controller raises the multiplier only below this (the reference's rule is 10, which "
                          "lets the learning rate reach 0.023: too much for mini-batches of fresh tuples from 1024 games; "
                          "default 1, or 10 with --play-batch 1)")
+    ap.add_argument("--dropout", type=float, default=0.0,
+                    help="probability with which a training step drops the features of the policy and value heads (0 = off)")
     ap.add_argument("--rehearse-on-one-gpu", action="store_true",
                     help="every rank uses GPU 0 and the collectives go over gloo: runs the multi-rank code path on a "
                          "one-GPU machine (RCCL refuses two ranks on one device); not a measurement")
@@ -453,7 +460,7 @@ def main(argv=None):
                        game_batch_num=(args.games + args.play_batch - 1) // args.play_batch, n_parallel=per_rank,
                        device=local, pure_mcts_playout_num=args.pure_playouts, updates_per_batch=upb,
                        continuous=args.continuous, lr_multiplier=args.lr_multiplier,
-                       max_lr_multiplier=args.max_lr_multiplier)
+                       max_lr_multiplier=args.max_lr_multiplier, dropout=args.dropout)
     if world > 1:
         from . import dist as azdist
         azdist.broadcast_weights(tp.policy_value_net)
@@ -505,7 +512,7 @@ def main(argv=None):
                           "entropy_first_last": [tp.loss_history[0][1], tp.loss_history[-1][1]] if tp.loss_history else None,
                           "win_ratio_vs_rollout_player": final, "rollout_playouts": tp.pure_mcts_playout_num,
                           "lr_multiplier": tp.lr_multiplier, "max_lr_multiplier": tp.max_lr_multiplier,
-                          "zero_head_biases": tp.zeroed_head_biases,
+                          "zero_head_biases": tp.zeroed_head_biases, "dropout": args.dropout,
                           "reference_controller": tp.max_lr_multiplier == 10.0 and not tp.zeroed_head_biases,
                           "best_win_ratio": tp.best_win_ratio,
                           "evaluations_batch_playouts_win_ratio": tp.eval_history,

@@ -271,6 +271,13 @@ int azg_train_step(azg_handle *h, int n, const float *states, const float *mcts_
                    const float *winners, float *const params[16], float *grads, float *adam_m,
                    float *adam_v, int64_t step, double lr, double beta1, double beta2, double eps,
                    double weight_decay, float *loss, float *entropy);
+/* Dropout of the two heads' features (what act_fc1 and val_fc1 read) in the training passes that follow on this handle
+ * (azg_train_backward, azg_train_step, azg_train_epoch's step; forward-only passes never drop): probability p in [0, 1),
+ * 0 = off (the default; results are then those of a handle without this call).  The mask is azg_dropout's: policy features
+ * [n,4S] with call number 2 * offset, value features [n,2S] with 2 * offset + 1; set offset to the step's number before every
+ * step.  Row i of the mini-batch is row first_row + i * row_step of the batch that all ranks share.  With dropout on the
+ * policy head's loss, entropy and gradients come from azg_linear_ce. */
+int azg_train_set_dropout(azg_handle *h, double p, uint64_t seed, uint64_t offset, uint64_t first_row, uint64_t row_step);
 /* One epoch of TrainPipeline.policy_update's loop (train.py:176-201) in one call, one wait: azg_train_step on
  * the n training positions, then azg_train_forward of the n_all positions of the KL test with the updated
  * parameters (probs [n_all,S], values [n_all], *kl against old_probs). */

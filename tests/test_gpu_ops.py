@@ -277,3 +277,345 @@ def test_cross_entropy_probabilities(ops, dtype, n, h, v):
 def test_cross_entropy_larger(ops, dtype, n, h, v):
     x, w, b, t = make(n, h, v, dtype, "index", ignored=0.1 if n > 8 else 0.0, seed=5)
     check_all(ops, x, w, b, t, scale=1024.0 if dtype == "f16" else 1.0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("kind,n,h,v", [("index", 7, 40, 4100), ("index", 33, 100, 5003), ("index", 130, 520, 4097), ("index", 300, 33, 9001),
+                                        ("index", 2100, 1030, 7001), ("index", 65, 64, 70001), ("probs", 64, 72, 4100), ("probs", 257, 33, 6001),
+                                        ("probs", 1, 1, 5000), ("probs", 700, 256, 4352)])
+def test_cross_entropy_many_classes(ops, dtype, kind, n, h, v):
+    x, w, b, t = make(n, h, v, dtype, kind, ignored=0.3 if n > 8 and kind == "index" else 0.0, seed=n + h + v)
+    check_all(ops, x, w, b, t, scale=1024.0 if dtype == "f16" else 1.0)
+
+
+# two lists of sizes for what does not depend on a size: one that the path for small problems takes, one that it does not
+PATHS = [(37, 100, 65), (37, 100, 4501)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,h,v", PATHS)
+@pytest.mark.parametrize("kind", ["index", "probs"])
+def test_cross_entropy_rows_with_their_own_gradient(ops, dtype, n, h, v, kind):
+    x, w, b, t = make(n, h, v, dtype, kind, ignored=0.2 if kind == "index" else 0.0)
+    if kind == "probs":
+        t = t * torch.linspace(0.0, 3.0, n, device="cuda")[:, None]             # any real weights, a row of zeros among them
+        t[1, ::7] *= -1.0
+    g = torch.linspace(-1.0, 2.0, n, device="cuda") * (256.0 if dtype == "f16" else 1.0)
+    g[3] = 0.0
+    ref = reference(x, w, b, t, g)
+    r = ops.linear_cross_entropy_grad(x, w, t, b, reduction="none", grad_loss=g, return_entropy=True)
+    close("loss", r.loss, *ref["loss"])
+    close("entropy", r.entropy, *ref["ent"])
+    close("d_hidden", r.d_hidden, *ref["dx"])
+    close("d_weight", r.d_weight, *ref["dw"])
+    close("d_bias", r.d_bias, *ref["db"])
+    s = ops.linear_cross_entropy(x, w, t, b, reduction="sum")
+    close("sum", s, ref["loss"][0].sum(), ref["loss"][1].sum() + F * ref["loss"][0].sum().abs())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,h,v", PATHS + [(1500, 300, 6000)])
+def test_cross_entropy_autograd(ops, dtype, n, h, v):
+    x, w, b, t = make(n, h, v, dtype, "index", ignored=0.2)
+    leaves = [q.clone().requires_grad_() for q in (x, w, b)]
+    scale = 3.0
+    loss, ent = ops.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], return_entropy=True)
+    assert not ent.requires_grad
+    (loss * scale).backward()
+    count = int((t != -100).sum())
+    ref = reference(x, w, b, t, torch.full((n,), scale / count, device="cuda"))
+    for name, leaf, key in (("d_hidden", leaves[0], "dx"), ("d_weight", leaves[1], "dw"), ("d_bias", leaves[2], "db")):
+        close(name, leaf.grad, *ref[key])
+    only = w.clone().requires_grad_()                              # one gradient alone, no bias
+    ops.linear_cross_entropy(x, only, t, reduction="sum").backward()
+    close("d_weight alone", only.grad, *reference(x, w, None, t, torch.ones(n, device="cuda"))["dw"])
+
+
+@pytest.mark.parametrize("n,h,v", PATHS)
+def test_cross_entropy_gradient_against_differences(ops, n, h, v):
+    """Central differences: off by e^2 / 6 times the third derivative along the direction -- at most R^3 a row, R the range of
+    the logits' change -- and by the losses' own bounds over e."""
+    x, w, b, t = make(n, h, v, "f32", "index", ignored=0.2, spread=1.0)
+    r = ops.linear_cross_entropy_grad(x, w, t, b, reduction="sum")
+    ref = reference(x, w, b, t, torch.ones(n, device="cuda"))
+    used = t != -100
+    e = 2.0 ** -6
+    dx, dw, db = torch.randn_like(x) / math.sqrt(h), torch.randn_like(w) / math.sqrt(h), torch.randn_like(b)
+    for d in ((dx, 0 * dw, 0 * db), (0 * dx, dw, 0 * db), (0 * dx, 0 * dw, db)):
+        f = [ops.linear_cross_entropy(x + s * e * d[0], w + s * e * d[1], t, b + s * e * d[2], reduction="sum").double() for s in (1, -1)]
+        want = sum(float((g.double() * q.double()).sum()) for g, q in zip((r.d_hidden, r.d_weight, r.d_bias), d))
+        u = d[0].double() @ w.double().t() + x.double() @ d[1].double().t() + d[2].double()
+        big = (u.max(1).values - u.min(1).values)[used]
+        # (x + e d is itself rounded: 2^-24 of every operand, on both sides)
+        slack = e * e / 6 * float((big ** 3).sum()) * 1.1 + (float(ref["loss"][1].sum()) * 2 + 4 * F * float(ref["loss"][0].sum())) / e
+        slack += 4 * F * float(((x.double().abs() @ w.double().abs().t()) + b.double().abs()).max(1).values.sum()) / e
+        slack += sum(float((bd * q.double().abs()).sum()) for bd, q in zip((ref["dx"][1], ref["dw"][1], ref["db"][1]), d))
+        assert abs(float((f[0] - f[1]) / (2 * e)) - want) <= slack
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,h,v", PATHS)
+def test_cross_entropy_ignored_rows_may_hold_anything(ops, dtype, n, h, v):
+    x, w, b, t = make(n, h, v, dtype, "index", ignored=0.3)
+    t[2], t[9] = -100, -100
+    clean = x.clone()
+    clean[t == -100] = 0
+    dirty = x.clone()
+    dirty[2], dirty[9] = float("nan"), float("inf")
+    dirty[t == -100, ::3] = torch.finfo(DT[dtype]).max
+    a = ops.linear_cross_entropy_grad(clean, w, t, b, return_entropy=True)
+    c = ops.linear_cross_entropy_grad(dirty, w, t, b, return_entropy=True)
+    for p, q in zip(a, c):
+        assert torch.equal(p, q)
+    leaf = dirty.clone().requires_grad_()
+    wl = w.clone().requires_grad_()
+    ops.linear_cross_entropy(leaf, wl, t, b).backward()
+    assert bool(torch.isfinite(wl.grad).all()) and not bool(leaf.grad[t == -100].any())
+    # every row ignored; an ignore_index that is a class
+    t[:] = -100
+    r = ops.linear_cross_entropy_grad(dirty, w, t, b, return_entropy=True)
+    assert float(r.loss) == 0 and float(r.entropy) == 0 and not any(bool(q.any()) for q in r[2:])
+    t = torch.randint(0, 3, (n,), device="cuda")
+    check_all(ops, x, w, b, t, ignore=1)
+
+
+@pytest.mark.parametrize("n,h,v", PATHS)
+def test_cross_entropy_blocked_classes_and_bad_targets(ops, n, h, v):
+    x, w, b, t = make(n, h, v, "f32", "index")
+    b[::3] = float("-inf")                                          # classes nobody may take
+    t = t // 3 * 3 + 1
+    t.clamp_(max=v - 1 - (v - 1) % 3 - 1)
+    check_all(ops, x, w, b, t)
+    b[::3] = torch.finfo(torch.float32).min
+    check_all(ops, x, w, b, t)
+    t[4] = 0                                                        # a blocked target: no finite loss
+    b[::3] = float("-inf")
+    assert float(ops.linear_cross_entropy(x, w, t, b, reduction="none")[4]) == float("inf")
+    every = ops.linear_cross_entropy(x, w, t, torch.full_like(b, float("-inf")), reduction="none")
+    assert not bool(torch.isfinite(every).any())
+    good = ops.linear_cross_entropy(x, w, t, reduction="none")
+    for bad in (v, -1, 1 << 40, -(1 << 62)):
+        u = t.clone()
+        u[5] = bad
+        r = ops.linear_cross_entropy(x, w, u, reduction="none")
+        assert math.isnan(float(r[5]))
+        r[5] = good[5]
+        assert torch.equal(r, good)
+        g = ops.linear_cross_entropy_grad(x, w, u, reduction="none")
+        assert bool(torch.isnan(g.d_hidden[5]).all()) and bool(torch.isfinite(g.d_hidden[:5]).all())
+        assert bool(torch.isnan(g.d_weight).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,h,v", PATHS + [(40, 128, 4608)])
+def test_cross_entropy_strides_and_alignments(ops, dtype, n, h, v):
+    x, w, b, t = make(n, h, v, dtype, "index", ignored=0.2)
+    want = ops.linear_cross_entropy_grad(x, w, t, b)
+
+    def inside(q, pad, at):                                         # q as a view of a larger tensor
+        big = torch.full((q.shape[0] + 2, q.shape[1] + pad), float("nan"), dtype=q.dtype, device="cuda")
+        big[1:-1, at:at + q.shape[1]] = q
+        return big[1:-1, at:at + q.shape[1]]
+    for pad, at in ((1, 1), (3, 0), (8, 8), (64, 24)):
+        for xv, wv in ((inside(x, pad, at), w), (x, inside(w, pad, at)), (inside(x, pad, at), inside(w, pad, at)),
+                       (x.t().contiguous().t(), w.t().contiguous().t())):
+            got = ops.linear_cross_entropy_grad(xv, wv, t, b)
+            for p, q in zip(want, got):
+                assert p is None and q is None or torch.equal(p, q)
+    both = torch.stack([t, t], 1)
+    assert torch.equal(ops.linear_cross_entropy(x, w, both[:, 1], torch.stack([b, b], 1)[:, 0]), ops.linear_cross_entropy(x, w, t, b))
+    p = torch.rand(n, v + 3, device="cuda")
+    assert torch.equal(ops.linear_cross_entropy(x, w, p[:, 2:v + 2], b), ops.linear_cross_entropy(x, w, p[:, 2:v + 2].contiguous(), b))
+    cube = ops.linear_cross_entropy(x[:36].view(4, 9, h), w, t[:36].view(4, 9), b, reduction="none")
+    assert cube.shape == (4, 9) and torch.equal(cube.view(-1), ops.linear_cross_entropy(x[:36], w, t[:36], b, reduction="none"))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_cross_entropy_empty_batch(ops, dtype):
+    w, b = torch.randn(70, 24, device="cuda").to(DT[dtype]), torch.randn(70, device="cuda").to(DT[dtype])
+    x, t = torch.empty(0, 24, dtype=DT[dtype], device="cuda"), torch.empty(0, dtype=torch.int64, device="cuda")
+    r = ops.linear_cross_entropy_grad(x, w, t, b, return_entropy=True)
+    assert float(r.loss) == 0 and float(r.entropy) == 0 and r.d_hidden.shape == (0, 24)
+    assert not bool(r.d_weight.any()) and not bool(r.d_bias.any())
+    assert ops.linear_cross_entropy(x, w, t, reduction="none").shape == (0,)
+    wl, xl = w.clone().requires_grad_(), x.clone().requires_grad_()
+    ops.linear_cross_entropy(xl, wl, t).backward()
+    assert not bool(wl.grad.any()) and xl.grad.shape == (0, 24)
+
+
+@pytest.mark.parametrize("dtype,n,h,v", [("bf16", 70000, 24, 8200), ("f32", 36000, 17, 8200)])
+def test_cross_entropy_in_pieces_of_the_classes(ops, dtype, n, h, v):
+    """More than a gigabyte of images: the classes are cut and their products made twice."""
+    x, w, b, t = make(n, h, v, dtype, "index", ignored=0.1)
+    check_all(ops, x, w, b, t)
+
+
+def test_cross_entropy_weights_beyond_32_bits(ops):
+    n, h, v = 5, 16384, 140001                                      # 4.6 GB of weights
+    w = torch.empty(v, h, dtype=torch.bfloat16, device="cuda")
+    for q in w.split(8192):
+        q.copy_(torch.randn(q.shape, device="cuda") / 128)
+    x = torch.randn(n, h, device="cuda").bfloat16()
+    t = torch.tensor([v - 1, 0, 131072, v - 2, 7], device="cuda")
+    l = torch.cat([x.double() @ q.double().t() for q in w.split(8192)], 1)
+    mag = torch.cat([x.double().abs() @ q.double().abs().t() for q in w.split(8192)], 1)
+    dl = ((h + 2) * F * mag + F * l.abs()).max(1).values
+    want = torch.logsumexp(l, 1) - l.gather(1, t[:, None])[:, 0]
+    r = ops.linear_cross_entropy_grad(x, w, t, reduction="sum")
+    err = (ops.linear_cross_entropy(x, w, t, reduction="none").double() - want).abs()
+    assert bool((err <= 2 * dl + 80 * F * (want.abs() + l.abs().max(1).values + 2)).all())
+    p = torch.softmax(l, 1)
+    d = p.clone()
+    d[torch.arange(n), t] -= 1
+    for c in (0, 7, 131071, 131072, 131073, v - 2, v - 1):
+        got, ref = r.d_weight[c].double(), d[:, c] @ x.double()
+        rel = 2 * dl[:, None] + 2.0 ** -20 + 2.0 ** -11 + 2.0 ** -8
+        bound = ((p * rel).max() + d[:, c].abs() @ (torch.full((n, 1), 2.0 ** -8, device="cuda", dtype=torch.float64) * x.double().abs())
+                 + (p[:, c, None] * rel).t() @ x.double().abs())
+        assert bool(((got - ref).abs() <= bound + 2.0 ** -8 * ref.abs() + 50 * F * (d[:, c].abs() @ x.double().abs())).all()), c
+
+
+def test_dropout_beyond_32_bits_of_elements(ops):
+    n = (1 << 32) + 12345
+    x = torch.ones(1, n, dtype=torch.bfloat16, device="cuda")
+    y = ops.dropout(x, 0.25, 77, 5, residual=x)
+    for at in (0, (1 << 31) - 50, (1 << 32) - 50, n - 100):
+        keep = torch.from_numpy(philox(at, 100, 77, 5) >= 16384).cuda()
+        assert torch.equal(y[0, at:at + 100], torch.where(keep, 1 + 65536 / 49152, 1.0).bfloat16()), at
+    del y
+    assert 0.7499 < float(ops.dropout(x, 0.25, 77, 6).gt(0).sum(dtype=torch.int64)) / n < 0.7501
+
+
+# ---------------------------------------------------------------- streams, graphs, threads, a whole step
+@pytest.mark.parametrize("n,h,v", PATHS + [(600, 256, 5000)])
+def test_cross_entropy_repeats_its_bits_on_any_stream_and_in_threads(ops, n, h, v):
+    import threading
+    x, w, b, t = make(n, h, v, "bf16", "index", ignored=0.2)
+    want = ops.linear_cross_entropy_grad(x, w, t, b, return_entropy=True)
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(5):
+                got = ops.linear_cross_entropy_grad(x, w, t, b, return_entropy=True)
+                s.synchronize()
+                bad.extend(1 for p, q in zip(want, got) if not torch.equal(p, q))
+    work()
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    for q in threads:
+        q.start()
+    for q in threads:
+        q.join()
+    assert not bad
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,h,v", PATHS + [(2100, 200, 6000)])
+def test_training_head_in_replayed_graphs(ops, dtype, n, h, v):
+    """features -> dropout -> projection's loss and gradients -> dropout's gradient, captured twice, replayed in turn with
+    other inputs and eager work between: every replay gives the eager results' bits."""
+    x, w, b, t = make(n, h, v, dtype, "index", ignored=0.2)
+    off = torch.zeros(1, dtype=torch.int64, device="cuda")
+
+    def step(offset):
+        y = ops.dropout(x, 0.3, 9, offset)
+        r = ops.linear_cross_entropy_grad(y, w, t, b, return_entropy=True)
+        return [r.loss, r.entropy, ops.dropout_grad(r.d_hidden, 0.3, 9, offset), r.d_weight, r.d_bias]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step(off)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(off)
+        graphs.append((g, out))
+    for i in range(6):
+        x.copy_(torch.randn(n, h, device="cuda"))
+        t.copy_(torch.where(torch.rand(n, device="cuda") < 0.3, -100, torch.randint(0, v, (n,), device="cuda")))
+        off.fill_(i)
+        want = step(i)
+        torch.cuda.synchronize()
+        g, out = graphs[i % 2]
+        for o in out:
+            o.fill_(float("nan"))
+        g.replay()
+        torch.cuda.synchronize()
+        for p, q in zip(want, out):
+            assert torch.equal(p, q), i
+
+
+def test_autograd_forms_refuse_to_be_captured(ops):
+    x, w, b, t = make(8, 16, 9, "f32")
+    xl = x.clone().requires_grad_()
+    eager = ops.linear_cross_entropy(ops.dropout(xl, 0.2, 1), w, t, b)           # (a live eager graph of the same leaf)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    refused = []
+    with torch.cuda.graph(g):
+        for call in (lambda: ops.linear_cross_entropy(xl, w, t, b), lambda: ops.dropout(xl, 0.2, 1), lambda: ops.dropout(x, 0.2, 1, residual=xl)):
+            try:
+                call()
+            except RuntimeError as err:
+                refused.append(str(err))
+        with torch.no_grad():
+            out = ops.linear_cross_entropy(xl, w, t, b)
+    assert len(refused) == 3 and all("captured" in r for r in refused)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, ops.linear_cross_entropy(x, w, t, b))
+    eager.backward()
+    assert bool(torch.isfinite(xl.grad).all())
+
+
+@pytest.mark.parametrize("n,h,v", PATHS)
+def test_head_step_against_autograd_of_its_definition(ops, n, h, v):
+    """The run of the operators against float64 autograd of the formulas under the same mask."""
+    x, w, b, t = make(n, h, v, "f32", "probs")
+    res = torch.randn_like(x)
+    leaves = [q.clone().requires_grad_() for q in (x, res, w, b)]
+    y = ops.dropout(leaves[0], 0.4, 123, 7, residual=leaves[1], first_row=11)
+    loss = ops.linear_cross_entropy(y, leaves[2], t, leaves[3])
+    loss.backward()
+    keep, thr = keep_mask(n, h, 0.4, 123, 7, 11)
+    d = [q.double().requires_grad_() for q in (x, res, w, b)]
+    yd = d[1] + torch.where(keep, d[0] * (65536.0 / (65536 - thr)), 0.0)
+    logits = yd @ d[2].t() + d[3]
+    ld = -(t.double() * torch.log_softmax(logits, 1)).sum(1).mean()
+    ld.backward()
+    ref = reference(yd.detach().float(), w, b, t, torch.full((n,), 1.0 / n, device="cuda"))
+    scale = 65536.0 / (65536 - thr)
+    # (y is rounded once in float32: 2 * 2^-24 of it, another input error of that size in every bound)
+    near = 4 * F * float((yd.detach().abs() @ w.double().abs().t()).max())
+    for name, leaf, exact, key, k in (("x", leaves[0], d[0], "dx", scale), ("residual", leaves[1], d[1], "dx", 1.0), ("w", leaves[2], d[2], "dw", 1.0),
+                                      ("b", leaves[3], d[3], "db", 1.0)):
+        bound = ref[key][1] * k + 2 * near * float(exact.grad.abs().max()) + 4 * F * exact.grad.abs()
+        assert bool(((leaf.grad.double() - exact.grad).abs() <= bound).all()), name
+    assert abs(float(loss.detach()) - float(ld.detach())) <= float(ref["loss"][1].mean()) + 2 * near + 4 * F * float(ld.detach())
+
+
+def test_refusals(ops):
+    x, w, b, t = make(8, 16, 9, "f32")
+    p = torch.rand(8, 9, device="cuda")
+    ce, grad, drop = ops.linear_cross_entropy, ops.linear_cross_entropy_grad, ops.dropout
+    for call, what in ((lambda: ce(x.cpu(), w, t), "CUDA"), (lambda: ce(x, w.cpu(), t), "CUDA"), (lambda: ce(x, w, t.cpu()), "CUDA"),
+                       (lambda: ce(x.double(), w, t), "float32"), (lambda: ce(x, w.half(), t), "float32"), (lambda: ce(x, w, t, b.bfloat16()), "float32"),
+                       (lambda: ce(x, w[:, :5], t), "features"), (lambda: ce(x, w, t[:5]), "shape"), (lambda: ce(x, w, t.int()), "int64"),
+                       (lambda: ce(x, w, p.half()), "float32"), (lambda: ce(x, w, p[:, :5]), "classes"), (lambda: ce(x, w, t, b[:5]), "classes"),
+                       (lambda: ce(x, w, t, reduction="max"), "reduction"), (lambda: ce(x, w, t, ignore_index=1.5), "ignore_index"),
+                       (lambda: ce(x, w, t, ignore_index=1 << 63), "ignore_index"), (lambda: ce(x, w[:0], t), "class"),
+                       (lambda: ce(x, w, p.clone().requires_grad_()), "gradient"), (lambda: grad(x, w, t, grad_loss=torch.ones(8, device="cuda")), "shape"),
+                       (lambda: grad(x, w, t, grad_loss=torch.ones((), device="cuda").half()), "float32"), (lambda: ce(x[0, 0], w, t), "features"),
+                       (lambda: drop(x.cpu(), 0.1, 1), "CUDA"), (lambda: drop(x.double(), 0.1, 1), "float32"), (lambda: drop(x, 1.1, 1), "p must"),
+                       (lambda: drop(x, -0.1, 1), "p must"), (lambda: drop(x, float("nan"), 1), "p must"), (lambda: drop(x, 0.1, -1), "seed"),
+                       (lambda: drop(x, 0.1, 1 << 64), "seed"), (lambda: drop(x, 0.1, 1, -1), "offset"), (lambda: drop(x, 0.1, 1, residual=x[:4]), "shape"),
+                       (lambda: drop(x, 0.1, 1, residual=x.half()), "residual"), (lambda: drop(x, 0.1, 1, torch.zeros(2, dtype=torch.int64, device="cuda")), "offset"),
+                       (lambda: drop(x, 0.1, 1, torch.zeros(1, device="cuda")), "offset"), (lambda: drop(x[0, 0], 0.1, 1), "dimension"),
+                       (lambda: drop(x, 0.1, 1, first_row=-1), "first_row")):
+        with pytest.raises((ValueError, TypeError), match=what):
+            call()
+    with pytest.raises(TypeError):
+        ce([1.0], w, t)
