@@ -745,8 +745,29 @@ __global__ __launch_bounds__(256) void rows_kernel(RowArgs a)
     if (a.ent_out) a.ent_out[row] = ent;
 }
 
+struct RowSums { double loss, ent, count; float top; };
+constexpr int kMaxSums = 256;                 // a multiple of 64, at most 1024
+constexpr long long kOneTotal = 4096;         // rows that one workgroup adds up in no more time than another launch takes
+
+// sum over a workgroup of W waves in a fixed order, for every thread
+template <int W>
+__device__ inline RowSums join_sums(RowSums v, RowSums *red)
+{
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+        v.loss += __shfl_xor(v.loss, s, 64); v.ent += __shfl_xor(v.ent, s, 64); v.count += __shfl_xor(v.count, s, 64);
+        v.top = fmaxf(v.top, __shfl_xor(v.top, s, 64));
+    }
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[0];
+    for (int w = 1; w < W; w++) { v.loss += red[w].loss; v.ent += red[w].ent; v.count += red[w].count; v.top = fmaxf(v.top, red[w].top); }
+    return v;
+}
+
 struct TotalArgs {
     long long n;
+    RowSums *sums;                // null, or kMaxSums sums over the rows to take instead of the rows
     int reduction;                // 0 none, 1 sum, 2 mean
     const float4 *stats; const float *ent;
     const long long *target; long long ignore;
@@ -756,39 +777,51 @@ struct TotalArgs {
     float *rowg;                  // [n]: g_i / 2^e; null: every row that counts has 1 (class numbers and a common g) or no gradient is asked for
     float *factor;                // [1]: 2^e (times the common g); null without a backward pass
 };
-// totals of the rows in a fixed order, in double; the rows' gradient factors, scaled so that the largest |D| fits an image
-template <int THREADS>
-__device__ inline void totals(const TotalArgs &a)
+// What the rows add up to, W waves: losses, entropies, rows that count; and their largest factor.  A fixed order, in double.
+template <int W>
+__device__ inline RowSums row_sums(const TotalArgs &a, long long first, long long step)
 {
-    constexpr int W = THREADS / 64;
-    __shared__ double red[3][W];
-    __shared__ float redm[W];
-    const int tid = threadIdx.x;
-    double sl = 0.0, se = 0.0, cnt = 0.0;
-    float mx = 0.f;
-    for (long long i = tid; i < a.n; i += THREADS) {
+    __shared__ RowSums red[W];
+    RowSums s{0.0, 0.0, 0.0, 0.f};
+#pragma unroll 4
+    for (long long i = first; i < a.n; i += step) {
         const float4 st = a.stats[i];
         const bool used = !(a.target && a.target[i] == a.ignore);
-        sl += st.w; cnt += used ? 1.0 : 0.0;
-        if (a.ent) se += a.ent[i];
+        s.loss += st.w; s.count += used ? 1.0 : 0.0;
+        if (a.ent) s.ent += a.ent[i];
         float g = 1.f;
         if (a.reduction == 0 && a.rowg) g = (a.dloss ? a.dloss[i] : 1.f) * a.grad_scale;
         const float m = fabsf(g) * st.z;
-        if (used && m < INFINITY) mx = fmaxf(mx, m);
+        if (used && m < INFINITY) s.top = fmaxf(s.top, m);
     }
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-        sl += __shfl_xor(sl, s, 64); se += __shfl_xor(se, s, 64); cnt += __shfl_xor(cnt, s, 64);
-        mx = fmaxf(mx, __shfl_xor(mx, s, 64));
+    return join_sums<W>(s, red);
+}
+// for many rows (more than kOneTotal): the sums of a workgroup's share of them
+__global__ __launch_bounds__(256) void sums_kernel(TotalArgs a)
+{
+    const RowSums s = row_sums<4>(a, (long long)blockIdx.x * 256 + threadIdx.x, (long long)kMaxSums * 256);
+    if (threadIdx.x == 0) a.sums[blockIdx.x] = s;
+}
+// The totals, and the rows' gradient factors, scaled so that the largest |D| fits an image; the first of `wgs` workgroups
+// writes the totals.
+template <int THREADS>
+__device__ inline void totals(const TotalArgs &a, unsigned wg, unsigned wgs)
+{
+    constexpr int W = THREADS / 64;
+    const int tid = threadIdx.x;
+    RowSums s;
+    if (a.sums) {
+        __shared__ RowSums red[W];
+        s = tid < kMaxSums ? a.sums[tid] : RowSums{0.0, 0.0, 0.0, 0.f};
+        s = join_sums<W>(s, red);
+    } else {
+        s = row_sums<W>(a, tid, THREADS);
     }
-    if ((tid & 63) == 0) { red[0][tid >> 6] = sl; red[1][tid >> 6] = se; red[2][tid >> 6] = cnt; redm[tid >> 6] = mx; }
-    __syncthreads();
-    sl = se = cnt = 0.0; mx = 0.f;
-    for (int i = 0; i < W; i++) { sl += red[0][i]; se += red[1][i]; cnt += red[2][i]; mx = fmaxf(mx, redm[i]); }
-    const double by = a.reduction == 2 ? (cnt > 0.0 ? 1.0 / cnt : 0.0) : 1.0;
-    if (a.reduction && tid == 0) {
-        if (a.loss) a.loss[0] = (float)(sl * by);
-        if (a.ent_out) a.ent_out[0] = (float)(se * by);
+    const float mx = s.top;
+    const double by = a.reduction == 2 ? (s.count > 0.0 ? 1.0 / s.count : 0.0) : 1.0;
+    if (a.reduction && wg == 0 && tid == 0) {
+        if (a.loss) a.loss[0] = (float)(s.loss * by);
+        if (a.ent_out) a.ent_out[0] = (float)(s.ent * by);
     }
     if (!a.factor) return;
     // 2^e >= the largest g_i sum|pi_i| (1 for an index target and a common g)
@@ -800,17 +833,17 @@ __device__ inline void totals(const TotalArgs &a)
         up = __builtin_bit_cast(float, (uint32_t)((E + 127) << 23));
     }
     if (a.rowg)
-        for (long long i = tid; i < a.n; i += THREADS) {
+        for (long long i = (long long)wg * THREADS + tid; i < a.n; i += (long long)wgs * THREADS) {
             const bool used = !(a.target && a.target[i] == a.ignore);
             const float g = a.reduction == 0 ? (a.dloss ? a.dloss[i] : 1.f) * a.grad_scale : 1.f;
             a.rowg[i] = used ? g / up : 0.f;
         }
-    if (tid == 0) {
+    if (wg == 0 && tid == 0) {
         const float common = a.reduction ? (a.dloss ? a.dloss[0] : 1.f) * a.grad_scale * (float)by : 1.f;
         a.factor[0] = up * common;
     }
 }
-__global__ __launch_bounds__(1024) void totals_kernel(TotalArgs a) { totals<1024>(a); }
+__global__ __launch_bounds__(1024) void totals_kernel(TotalArgs a) { totals<1024>(a, blockIdx.x, gridDim.x); }
 
 // ---------------------------------------------------------------- exponentials -> D, in place
 constexpr int kFixCols = 512;
@@ -833,7 +866,7 @@ __global__ __launch_bounds__(256) void fix_kernel(FixArgs a)
     using V = typename Frag<typename Op::Img>::V;
     __shared__ float red[4][kFixCols];
     if (a.totals.n >= 0 && blockIdx.y == gridDim.y - 1) {
-        if (blockIdx.x == 0) totals<256>(a.totals);
+        if (blockIdx.x == 0) totals<256>(a.totals, 0, 1);
         return;
     }
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -856,6 +889,8 @@ __global__ __launch_bounds__(256) void fix_kernel(FixArgs a)
             const fx4 v0 = p[0], v1 = p[1];
 #pragma unroll
             for (int i = 0; i < 4; i++) { v[i] = v0[i]; v[4 + i] = v1[i]; }
+            // (the halves land on exponentials of the row that other lanes of this wave read: no store moves in front of the loads)
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         } else {
             const hx8 p = *reinterpret_cast<const hx8 *>(static_cast<_Float16 *>(a.d) + row * lde + c);
 #pragma unroll
@@ -874,8 +909,6 @@ __global__ __launch_bounds__(256) void fix_kernel(FixArgs a)
             h[i] = (typename Op::Img)q;
             if (Op::split) l[i] = (typename Op::Img)(q - (float)h[i]);
         }
-        // (float32: the halves land on exponentials of the same row that other lanes of this wave have read: a wave's
-        //  stores follow the loads that every one of its values depends on)
         typename Op::Img *o = static_cast<typename Op::Img *>(a.d) + row * a.ldd + (Op::split ? (c >> 5) * 64 + (c & 31) : c);
         *reinterpret_cast<V *>(o) = h;
         if (Op::split) *reinterpret_cast<V *>(o + 32) = l;
@@ -984,7 +1017,7 @@ __global__ __launch_bounds__(256) void join_kernel(JoinList l)
     const long long total = a.n * a.m;
     for (long long i = (long long)wg * 256 + threadIdx.x; i < total; i += (long long)a.wgs * 256) {
         float s = 0.f;
-#pragma unroll 4
+#pragma unroll 8
         for (int z = 0; z < a.splits; z++) s += a.acc[(long long)z * total + i];
         const long long r = i / a.m, c = i - r * a.m;
         static_cast<typename Op::In *>(a.out)[r * a.ldo + c] = (typename Op::In)(s * f);

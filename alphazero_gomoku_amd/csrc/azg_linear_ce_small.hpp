@@ -1,7 +1,7 @@
 // Projection + softmax cross entropy for small problems (a policy head on a mini-batch: 512 positions, hundreds of classes),
 // where launches and not arithmetic take the time: three launches, everything in float32 on the f32 matrix cores.
 //
-//   small_logits_kernel  l = X W^T + b to the workspace (a few MB at most), and the number of rows that count
+//   small_logits_kernel  l = X W^T + b to the workspace (16 MB at most), and the number of rows that count
 //   small_rows_kernel    a row's statistics, loss, entropy, and D in place of its logits
 //   small_grads_kernel   dX = D W, dW = D^T X, db, and the totals
 //
@@ -142,10 +142,10 @@ __global__ __launch_bounds__(kSmallWaves * 64) void small_logits_kernel(SmallArg
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int tv = (a.V + kSmallTile - 1) / kSmallTile, tn = (a.n + kSmallTile - 1) / kSmallTile;
     if ((int)blockIdx.x == tv * tn) {                         // the last workgroup: how many rows count
-        float s = 0.f;
-        for (int i = tid; i < a.n; i += kSmallWaves * 64) s += a.target && a.target[i] == a.ignore ? 0.f : 1.f;
-        s = block_sum<kSmallWaves>(s, &lds[0][0][0]);
-        if (tid == 0) *a.count = (int)s;
+        int s = 0;
+        for (int i = tid; i < a.n; i += kSmallWaves * 64) s += a.target && a.target[i] == a.ignore ? 0 : 1;
+        s = block_sum<kSmallWaves>(s, reinterpret_cast<int *>(lds));
+        if (tid == 0) *a.count = s;
         return;
     }
     const int n0 = (int)blockIdx.x / tv * kSmallTile, v0 = (int)blockIdx.x % tv * kSmallTile;

@@ -98,8 +98,22 @@ extern "C" int azg_dropout(const azg_dropout_args *a)
 // ---------------------------------------------------------------- projection + softmax cross entropy
 namespace {
 
-// Problems of at most this many multiplications a product (and classes) take the three-launch float32 path: AAA
-constexpr long long kSmallWork = 1LL << 27, kSmallClasses = 4096;
+// Which problems the three-launch float32 path takes.  Measured, the tiled path against it, microseconds of GPU time:
+//   float32, loss and gradients: 512 x 256 x 64 (rows, features, classes) 32 / 17, 512 x 900 x 225 44 / 32, 256 x 1024 x 1024
+//     53 / 51, then 2048 x 1024 x 256 62 / 94; with long sums or few tiles it falls behind: 32 x 1024 x 4096 56 / 71,
+//     4096 x 64 x 64 35 / 79;
+//   float32, the loss alone: 512 x 1024 x 256 33 / 18, 512 x 2048 x 512 51 / 29, 4096 x 64 x 64 22 / 16, then 16384 x 64 x 64
+//     35 / 47, 8 x 64 x 32768 29 / 58;
+//   16 bits, whose matrix instructions are sixteen times as fast as float32's: 128 x 256 x 1024 25 / 21, 512 x 256 x 64 22 / 17,
+//     then 512 x 1024 x 256 27 / 33, 16 x 512 x 4096 24 / 48 (the loss alone 13 / 11, 13 / 10, 16 / 17, 13 / 17).
+constexpr long long kSmallLogits = 1LL << 22;                 // 16 MB of float32
+bool takes_small(bool f32, bool backward, long long n, long long h, long long v)
+{
+    const long long side = f32 && !backward ? 4096 : 1024;
+    const double work = (double)n * (double)h * (double)v;
+    return n <= side && v <= side && n * v <= kSmallLogits && work <= (f32 ? backward ? 1LL << 28 : 1LL << 29 : 1LL << 25);
+}
+constexpr double kMaxThreads = 4294967295.0;                  // of a launch
 
 // Room that the images of D, of W and of its transpose may take together before the classes are cut into pieces.
 constexpr long long kPieceBytes = 1LL << 30;
@@ -110,16 +124,16 @@ struct Take {                                                 // offsets into th
 };
 
 enum Shape { T256, T128, T64, TROW };
-struct ShapeDim { int tm, tn, wm; };
-constexpr ShapeDim kDims[4] = {{256, 256, 2}, {128, 128, 2}, {64, 64, 2}, {128, 32, 4}};
+struct ShapeDim { int tm, tn, wm, threads; };
+constexpr ShapeDim kDims[4] = {{256, 256, 2, 512}, {128, 128, 2, 256}, {64, 64, 2, 256}, {128, 32, 4, 256}};
 
 long long tiles_of(Shape s, long long m, long long n) { return ((m + kDims[s].tm - 1) / kDims[s].tm) * ((n + kDims[s].tn - 1) / kDims[s].tn); }
 
 Shape pick_logits(long long m, long long n, bool grad)
 {
     if (!grad && n <= 32) return TROW;
-    if (tiles_of(T256, m, n) >= 200) return T256;
-    if (tiles_of(T128, m, n) >= 200) return T128;
+    if (m > 128 && tiles_of(T256, m, n) >= 200) return T256;
+    if (m > 64 && tiles_of(T128, m, n) >= 200) return T128;
     return T64;
 }
 // Tile of the gradients' products, which share a launch, and the splits of their sums, by an estimate in microseconds: the
@@ -134,8 +148,8 @@ GradPick pick_grads(long long n, long long h, long long v, long long kx, long lo
     double least = 1e30;
     for (Shape s : {T256, T128, T64}) {
         const long long tx = want_x ? tiles_of(s, h, n) : 0, tw = want_w ? tiles_of(s, h, v) : 0;
-        if ((double)(tx + tw) * 32 > INT_MAX / 2 && s != T256) continue;
-        for (long long per = 4; per < 2 * std::max(kx, kw); per *= 2) {          // stages of a workgroup at most
+        if ((double)(tx + tw) * 32 * kDims[s].threads > kMaxThreads && s != T256) continue;
+        for (long long per = 4; per == 4 || per < 2 * std::max(kx, kw); per *= 2) {          // stages of a workgroup at most
             GradPick g{};
             auto split = [&](long long k, int *splits, int *kper) {
                 const long long parts = std::min<long long>(32, (k + per - 1) / per);
@@ -167,7 +181,7 @@ struct Plan {
     Shape lshape;
     GradPick g;
     int fix_rows;
-    size_t xmax, wmax, ximg, wimg, part, part_e, part_t, tlogit, stats, ent, rowg, factor, d, dbpart, dxacc, dwacc, logits, count, total;
+    size_t xmax, wmax, ximg, wimg, part, part_e, part_t, tlogit, stats, ent, rowg, sums, factor, d, dbpart, dxacc, dwacc, logits, count, total;
 };
 
 bool aligned16(const void *p, long long stride, long long cols, long long rows)
@@ -183,7 +197,7 @@ int make_plan(const azg_linear_ce_args *a, Plan *p)
     p->forward = a->loss != nullptr;
     p->backward = a->dx || a->dw || a->db;
     p->n = a->n; p->H = a->hidden; p->V = a->classes;
-    p->small = p->V <= kSmallClasses && (double)p->n * (double)p->H * (double)p->V <= (double)kSmallWork;
+    p->small = takes_small(p->split, p->backward, p->n, p->H, p->V);
     if (p->small) {
         Take t;
         p->logits = t((size_t)p->n * p->V * 4);
@@ -213,12 +227,14 @@ int make_plan(const azg_linear_ce_args *a, Plan *p)
     p->lshape = pick_logits(p->vp, p->n, p->backward);
     p->g = pick_grads(p->n, p->H, p->vp, (p->vp + p->ks - 1) / p->ks, (p->n + p->ks - 1) / p->ks, a->dx != nullptr, a->dw != nullptr);
     // rows a workgroup turns into D: up to 64, fewer while they would not give four workgroups a CU
+    // (more for very many rows: db is joined from one sum a run of rows, one after the other)
     p->fix_rows = 64;
+    while ((p->n + p->fix_rows - 1) / p->fix_rows > 1024) p->fix_rows *= 2;
     while (p->fix_rows > 8 && (p->n + p->fix_rows - 1) / p->fix_rows * ((p->vp + kFixCols - 1) / kFixCols) < 1024) p->fix_rows /= 2;
     const ShapeDim dim = kDims[p->lshape];
     const long long lm = (p->vp + dim.tm - 1) / dim.tm, ln = (p->n + dim.tn - 1) / dim.tn;
-    if (lm * ln > INT_MAX / 2 || (tiles_of(p->g.shape, p->H, p->n) + tiles_of(p->g.shape, p->H, p->vp)) * 32 > INT_MAX / 2 ||
-        (p->n + p->fix_rows - 1) / p->fix_rows > 65534)
+    const double grad_tiles = (a->dx ? (double)tiles_of(p->g.shape, p->H, p->n) * p->g.splits_x : 0.0) + (a->dw ? (double)tiles_of(p->g.shape, p->H, p->vp) * p->g.splits_w : 0.0);
+    if ((double)lm * ln * dim.threads > kMaxThreads || grad_tiles * kDims[p->g.shape].threads > kMaxThreads)
         return fail(AZG_EINVAL, "azg_linear_ce: the problem is too large");
     Take t;
     p->xmax = t(p->split ? kMaxParts * 4 : 0);
@@ -233,6 +249,7 @@ int make_plan(const azg_linear_ce_args *a, Plan *p)
     p->stats = t((size_t)p->n * 16);
     p->ent = t((size_t)p->n * 4);
     p->rowg = t((size_t)p->n * 4);
+    p->sums = t(p->n > kOneTotal ? kMaxSums * sizeof(RowSums) : 0);
     p->factor = t(4);
     p->d = t(p->backward ? (size_t)p->n * p->ldd * 2 : 0);
     p->dbpart = t(a->db ? (size_t)std::max(ln, (p->n + p->fix_rows - 1) / p->fix_rows) * p->vp * 4 : 0);
@@ -247,10 +264,10 @@ int check(const azg_linear_ce_args *a)
     if (!a) return fail(AZG_EINVAL, "null argument");
     if (a->dtype != AZG_F32 && a->dtype != AZG_BF16 && a->dtype != AZG_F16) return fail(AZG_EINVAL, "azg_linear_ce: unknown dtype %d", a->dtype);
     if (a->n < 0 || a->hidden < 1 || a->classes < 1) return fail(AZG_EINVAL, "azg_linear_ce: sizes must be n >= 0, hidden >= 1, classes >= 1");
-    if (a->n > INT_MAX || a->classes > INT_MAX || a->hidden > (1 << 22)) return fail(AZG_EINVAL, "azg_linear_ce: a size is too large");
+    if (a->n >= 1 << 26 || a->classes > INT_MAX || a->hidden > (1 << 22)) return fail(AZG_EINVAL, "azg_linear_ce: a size is too large");
     if (a->reduction < AZG_REDUCE_NONE || a->reduction > AZG_REDUCE_MEAN) return fail(AZG_EINVAL, "azg_linear_ce: unknown reduction %d", a->reduction);
     if (bad_matrix(a->n, a->hidden, a->x_stride) || bad_matrix(a->classes, a->hidden, a->w_stride)) return fail(AZG_EINVAL, "azg_linear_ce: a row stride is smaller than a row");
-    if (a->x_stride > (1LL << 22) || a->w_stride > (1LL << 22)) return fail(AZG_EINVAL, "azg_linear_ce: a row stride is too large");
+    if ((a->n > 1 && a->x_stride > (1LL << 22)) || (a->classes > 1 && a->w_stride > (1LL << 22))) return fail(AZG_EINVAL, "azg_linear_ce: a row stride is too large");
     return AZG_OK;
 }
 
@@ -402,10 +419,19 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
     if (p.forward && a->reduction != AZG_REDUCE_NONE) { t.loss = a->loss; t.ent_out = a->entropy; }
     t.dloss = a->dloss; t.grad_scale = (float)a->grad_scale;
     t.rowg = p.backward ? f32(p.rowg) : nullptr; t.factor = p.backward ? f32(p.factor) : nullptr;
-    // class numbers and a common g: the rows' factors are 1 or 0, and the totals can ride on the next launch
-    const bool ride = p.keep && target && a->reduction != AZG_REDUCE_NONE;
+    // class numbers and a common g: the rows' factors are 1 or 0, and the totals can ride on the next launch (with many classes
+    // its other workgroups take longer than the one that does the totals, however many rows there are)
+    const bool ride = p.keep && target && a->reduction != AZG_REDUCE_NONE && (a->n <= kOneTotal || p.V >= 4096);
     if (ride) t.rowg = nullptr;
-    else if (p.backward || a->reduction != AZG_REDUCE_NONE) hipLaunchKernelGGL(totals_kernel, dim3(1), dim3(1024), 0, s, t);
+    else if (p.backward || a->reduction != AZG_REDUCE_NONE) {
+        unsigned grid = 1;
+        if (a->n > kOneTotal) {
+            t.sums = reinterpret_cast<RowSums *>(ws + p.sums);
+            hipLaunchKernelGGL(sums_kernel, dim3(kMaxSums), dim3(256), 0, s, t);
+            grid = 64;
+        }
+        hipLaunchKernelGGL(totals_kernel, dim3(grid), dim3(1024), 0, s, t);
+    }
     OPS_HIP(hipGetLastError());
     if (!p.backward) return AZG_OK;
 

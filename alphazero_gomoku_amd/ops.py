@@ -14,6 +14,7 @@ import torch
 from . import _lib
 
 _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_MAX_STRIDE = 1 << 22                         # of a projection's operands
 _REDUCTIONS = {"none": _lib.REDUCE_NONE, "sum": _lib.REDUCE_SUM, "mean": _lib.REDUCE_MEAN}
 
 LinearCrossEntropyGrad = namedtuple("LinearCrossEntropyGrad", "loss entropy d_hidden d_weight d_bias")
@@ -33,14 +34,14 @@ def _check_tensor(name, t, dtype=None, device=None):
         raise ValueError("%s is on %s, not on %s" % (name, t.device, device))
 
 
-def _rows(name, t):
+def _rows(name, t, max_stride=None):
     """t as (rows, columns, row stride in elements) without a copy, or a copy whose rows are contiguous: (t, rows, cols, stride)."""
     if t.dim() == 0:
         raise ValueError("%s must have at least one dimension" % name)
     cols = t.shape[-1]
     rows = t.numel() // cols if cols else 0
-    if t.dim() == 2 and (cols <= 1 or t.stride(1) == 1) and (rows <= 1 or t.stride(0) >= cols):
-        return t, rows, cols, max(t.stride(0), cols)
+    if t.dim() == 2 and (cols <= 1 or t.stride(1) == 1) and (rows <= 1 or cols <= t.stride(0) <= (max_stride or t.stride(0))):
+        return t, rows, cols, t.stride(0) if rows > 1 else cols
     if not t.is_contiguous():
         t = t.contiguous()
     return t, rows, cols, cols
@@ -185,8 +186,8 @@ class _CeCall:
         self.keep = [hidden, weight, target, bias]
         self.device, self.dtype = hidden.device, hidden.dtype
         self.hidden_shape, self.rows_shape = hidden.shape, hidden.shape[:-1]
-        x, n, h, xs = _rows("hidden", hidden)
-        w, v, _, wst = _rows("weight", weight)
+        x, n, h, xs = _rows("hidden", hidden, _MAX_STRIDE)
+        w, v, _, wst = _rows("weight", weight, _MAX_STRIDE)
         a = self.a = _lib.LinearCeArgs()
         a.device, a.dtype, a.reduction = self.device.index, _DTYPES[hidden.dtype], _REDUCTIONS[reduction]
         a.n, a.hidden, a.classes = (n if h else 0), h, v

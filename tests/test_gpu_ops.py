@@ -293,7 +293,7 @@ PATHS = [(37, 100, 65), (37, 100, 4501)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("n,h,v", PATHS)
+@pytest.mark.parametrize("n,h,v", PATHS + [(5000, 24, 150)])
 @pytest.mark.parametrize("kind", ["index", "probs"])
 def test_cross_entropy_rows_with_their_own_gradient(ops, dtype, n, h, v, kind):
     x, w, b, t = make(n, h, v, dtype, kind, ignored=0.2 if kind == "index" else 0.0)
@@ -314,7 +314,7 @@ def test_cross_entropy_rows_with_their_own_gradient(ops, dtype, n, h, v, kind):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("n,h,v", PATHS + [(1500, 300, 6000)])
+@pytest.mark.parametrize("n,h,v", PATHS + [(1500, 300, 6000), (1100, 64, 300), (40, 33, 1500)])
 def test_cross_entropy_autograd(ops, dtype, n, h, v):
     x, w, b, t = make(n, h, v, dtype, "index", ignored=0.2)
     leaves = [q.clone().requires_grad_() for q in (x, w, b)]
@@ -448,6 +448,47 @@ def test_cross_entropy_in_pieces_of_the_classes(ops, dtype, n, h, v):
     """More than a gigabyte of images: the classes are cut and their products made twice."""
     x, w, b, t = make(n, h, v, dtype, "index", ignored=0.1)
     check_all(ops, x, w, b, t)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,h,v", [(40, 64, 4096), (40, 64, 4097), (1024, 24, 4096), (1025, 24, 4096), (512, 256, 1024), (513, 256, 1024), (40000, 3, 100),
+                                   (1024, 40, 300), (1025, 40, 300), (256, 128, 1024), (257, 128, 1024), (256, 128, 1025), (20000, 48, 60)])
+def test_cross_entropy_around_the_ends_of_the_small_path(ops, dtype, n, h, v):
+    x, w, b, t = make(n, h, v, dtype, "index", ignored=0.2, seed=n + h + v)
+    check_all(ops, x, w, b, t)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,h,v", [(128, 16392, 128), (60, 40001, 64), (1, 1 << 20, 129)])
+def test_cross_entropy_of_very_many_features(ops, dtype, n, h, v):
+    x, w, b, t = make(n, h, v, dtype, "index", seed=n + h + v)
+    check_all(ops, x, w, b, t)
+
+
+@pytest.mark.parametrize("dtype,n", [("bf16", 4300000), ("f32", 300001)])
+def test_cross_entropy_of_very_many_rows(ops, dtype, n):
+    x, w, b, t = make(n, 8, 5, dtype, "index", ignored=0.2)
+    check_all(ops, x, w, b, t)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,h,v", PATHS)
+def test_cross_entropy_of_single_rows_with_any_stride(ops, dtype, n, h, v):
+    """One row (or one class) of a matrix whose row stride says nothing; rows further apart than the kernels take."""
+    x, w, b, t = make(n, h, v, dtype, "index")
+    far = torch.empty(2, 5 << 20, dtype=x.dtype, device="cuda")
+    far[:, :h] = x[:2]
+    want = ops.linear_cross_entropy_grad(x[:2], w, t[:2], b)
+    got = ops.linear_cross_entropy_grad(far[:, :h], w, t[:2], b)
+    assert all(torch.equal(p, q) for p, q in zip(want, got) if p is not None)
+    want = ops.linear_cross_entropy_grad(x[:1], w, t[:1], b)
+    got = ops.linear_cross_entropy_grad(far[:1, :h], w, t[:1], b)
+    assert all(torch.equal(p, q) for p, q in zip(want, got) if p is not None)
+    far[0, :h] = w[0]
+    t1 = torch.zeros_like(t)
+    want, got = ops.linear_cross_entropy_grad(x, w[:1], t1), ops.linear_cross_entropy_grad(x, far[:1, :h], t1)
+    assert torch.equal(want.loss, got.loss) and torch.equal(want.d_weight, got.d_weight)
+    assert torch.equal(ops.dropout(far[:1, :h], 0.5, 1), ops.dropout(w[:1], 0.5, 1))
 
 
 def test_cross_entropy_weights_beyond_32_bits(ops):

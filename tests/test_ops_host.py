@@ -43,7 +43,7 @@ def test_dropout_refuses(lib, kw, what):
 
 
 @pytest.mark.parametrize("kw,what", [(dict(dtype=3), "dtype"), (dict(n=-1), "sizes"), (dict(hidden=0), "sizes"), (dict(classes=0), "sizes"),
-                                     (dict(n=1 << 40), "too large"), (dict(hidden=1 << 23), "too large"), (dict(reduction=3), "reduction"),
+                                     (dict(n=1 << 40), "too large"), (dict(n=1 << 26), "too large"), (dict(hidden=1 << 23), "too large"), (dict(reduction=3), "reduction"),
                                      (dict(reduction=-1), "reduction"), (dict(x_stride=7), "stride"), (dict(w_stride=7), "stride"),
                                      (dict(x_stride=1 << 23), "too large"), (dict(w_stride=1 << 23), "too large")])
 def test_linear_ce_refuses_sizes(lib, kw, what):
@@ -84,6 +84,16 @@ def test_workspace_is_bounded(lib):
     rows = 32768 * 4096 * (2 + 4)                                   # X's image and the float32 sum of the pieces' dX
     stats = 8 * (131072 // 128 + 8) * 32768                         # (maximum, sum) pairs
     assert size < whole / 4 + rows + stats + (1 << 24), size
+
+
+def test_workspace_of_few_features_and_of_single_rows(lib):
+    """The logits that small problems keep are bounded whatever the features; the stride of a single row does not matter."""
+    a = ce_args(lib, dtype=lib.BF16, n=1 << 22, hidden=1, classes=32, x_stride=1, w_stride=1)
+    assert 0 < int(lib.load().azg_linear_ce_workspace(C.byref(a))) < (1 << 22) * (16 + 4 + 4 + 4 + 2 * 8 + 4 * 128)
+    a = ce_args(lib, n=1, classes=1, x_stride=1 << 40, w_stride=1 << 40)
+    assert int(lib.load().azg_linear_ce_workspace(C.byref(a))) > 0
+    a = ce_args(lib, n=(1 << 26) - 1, classes=2)
+    assert int(lib.load().azg_linear_ce_workspace(C.byref(a))) > 0
 
 
 def test_python_forms_need_a_gpu():
