@@ -8,6 +8,8 @@
 // A workgroup makes a 32 x 32 tile of a product; its eight waves take an eighth of the sum each (blocks of 16 in turn) and
 // join through LDS.  Operands come straight from memory (L2) into the fragments of v_mfma_f32_16x16x4_f32: a lane of group
 // g = lane / 16 holds k = 4 g + j for the j-th of four instructions, so that where k is contiguous the four are one load.
+// Bound by latency, of launches and of loads from the L2: 512 positions on 8 x 8 (256 features, 64 classes) take 5 + 4 + 8 us, on
+// 15 x 15 (900, 225) 11 + 5 + 17 us; the tiled path takes 32 us and 44 us for them.
 #pragma once
 #include "azg_linear_ce.hpp"
 

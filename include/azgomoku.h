@@ -318,9 +318,10 @@ typedef struct azg_dropout_args {
 int azg_dropout(const azg_dropout_args *a);
 
 /* Softmax cross entropy of the projection l = x w^T + bias (x [n,hidden], w [classes,hidden], bias [classes] or NULL, one
- * type), against class numbers or against probabilities (any real weights), and its gradients, in pieces of the classes:
- * no array of n * classes logits exists, only 16-bit images of the gradient at one piece of them (1 GiB at most with the
- * other images, or 1024 classes).  For every row
+ * type), against class numbers or against probabilities (any real weights), and its gradients.  The logits of a large problem
+ * are not stored: a backward pass keeps one array of 2 bytes (AZG_F32: 4) an element, of at most 1 GiB together with the
+ * copies of x and w that it needs or of 1024 classes, and takes more classes than fit piece by piece.  Small problems keep at
+ * most 16 MB of float32 logits.  n < 2^26, hidden and the row strides of x and w at most 2^22.  For every row
  *   loss = lse - l[target]                        target int64 [n]; rows whose target is ignore_index count for nothing,
  *                                                 whatever x holds there (loss 0, gradient 0); any other target outside
  *                                                 0 .. classes - 1 makes the row's loss, and every gradient it reaches, NaN
@@ -331,8 +332,10 @@ int azg_dropout(const azg_dropout_args *a);
  * One call does the forward pass (loss not NULL), the backward pass (any of dx, dw, db not NULL), or both.  A backward pass
  * by itself takes the stats [n][4] (float32, 16-byte aligned, the caller's) that the forward pass of the same inputs wrote.
  * Sums, statistics and accumulators are float32 or wider; the gradient at the logits is rounded to x's type (float32: to 22
- * bits) before the two products that use it.  Results do not depend on anything but the arguments: the same bits every time.
- * azg_linear_ce_workspace: bytes of workspace (256-byte aligned) the call needs with these very arguments, or AZG_E*. */
+ * bits) before the two products that use it, and where one call makes loss and gradients its softmax to 11 bits before that
+ * (float32: not).  Results do not depend on anything but the arguments and the alignment of x and w: the same bits every time.
+ * azg_linear_ce_workspace: bytes of workspace (256-byte aligned) the call needs with these very arguments, pointers included
+ * (workspace, workspace_bytes and stream are not looked at), or AZG_E*. */
 #define AZG_REDUCE_NONE  0
 #define AZG_REDUCE_SUM   1
 #define AZG_REDUCE_MEAN  2
