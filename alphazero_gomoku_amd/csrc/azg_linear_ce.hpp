@@ -499,7 +499,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a0, PackArgs a1, uns
 // ---------------------------------------------------------------- logits: statistics or gradient
 struct CeArgs {
     Operand w, x;                 // classes (of this piece) x k, rows x k
-    int ktiles, mtiles, ntiles;
+    int ktiles, mtiles, ntiles, mtiles_behind;
     long long n, classes, v0;     // classes of this piece; v0 = first class of the piece
     const void *bias;             // this piece's, operand type, or null
     const float *xmax, *wmax;     // float32: partial maxima
@@ -527,16 +527,15 @@ template <> struct Expo<OpF32> { using T = float; };
 
 // A tile of logits; a lane holds four classes of a row next to each other (classes are the tile's m), sixteen rows a fragment.
 // Forward (GRAD false): span statistics and, where asked for, the exponentials; GRAD: D from the rows' statistics.  A 256 x 256
-// tile spends 2.6 us in filling its rings and 7.7 us in this epilogue (an exponential an element, on top of the maximum, the
-// sum and the stores), 1.3 us a stage: at 1024 features a third of the time.
+// tile takes 9.7 us around one stage of 64 features (49152 classes of 64 features: 58 us, six rounds; with a bias 11): filling the
+// rings and this epilogue, an exponential an element on top of the maximum, the sum and the stores; and 1.4 us a stage more.
 template <typename Op, int TM, int TN, int WM, int WN, bool GRAD>
-__global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
+__device__ inline void logits_tile(const CeArgs &a, long long m_first, int span_first, int mtiles, int ntiles, unsigned wg, char *lds)
 {
     using S = TileShape<TM, TN, WM, WN>;
-    extern __shared__ __attribute__((aligned(1024))) char lds[];
     int tm, tn;
-    tile_of(blockIdx.x, a.mtiles, a.ntiles, &tm, &tn);
-    const long long m0 = (long long)tm * TM, n0 = (long long)tn * TN;
+    tile_of(wg, mtiles, ntiles, &tm, &tn);
+    const long long m0 = m_first + (long long)tm * TM, n0 = (long long)tn * TN;
     fx4 acc[S::MT][S::NT];
 #pragma unroll
     for (int i = 0; i < S::MT; i++)
@@ -548,19 +547,49 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
     const float ux = Op::split ? 1.f / split_scale(max_of_parts(a.xmax)) : 1.f, uw = Op::split ? 1.f / split_scale(max_of_parts(a.wmax)) : 1.f;
     const typename Op::In *bias = static_cast<const typename Op::In *>(a.bias);
     const long long vw = m0 + wm * (TM / WM) + 4 * (lane >> 4);                  // this lane's first class of the piece
-    if (Op::split || bias || m0 + TM > a.classes) {
+    // (what the rows and classes bring along is loaded in one go: each load by itself would cost its latency)
+    const bool whole = m0 + TM <= a.classes;
+    if (Op::split || bias || !whole) {
+        typename Op::In bv[S::MT][4];
+        if (bias && whole) {
+#pragma unroll
+            for (int mt = 0; mt < S::MT; mt++) *reinterpret_cast<Pack<typename Op::In, 4> *>(bv[mt]) = *reinterpret_cast<const Pack<typename Op::In, 4> *>(bias + vw + mt * 16);
+        } else if (bias) {
+#pragma unroll
+            for (int mt = 0; mt < S::MT; mt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) bv[mt][i] = bias[min(vw + mt * 16 + i, a.classes - 1)];
+        }
 #pragma unroll
         for (int mt = 0; mt < S::MT; mt++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const long long v = vw + mt * 16 + i;
-                const float b = bias && v < a.classes ? (float)bias[v] : 0.f;
+                const float b = bias ? (float)bv[mt][i] : 0.f;
 #pragma unroll
-                for (int nt = 0; nt < S::NT; nt++) acc[mt][nt][i] = v < a.classes ? acc[mt][nt][i] * ux * uw + b : -INFINITY;
+                for (int nt = 0; nt < S::NT; nt++) acc[mt][nt][i] = Op::split ? acc[mt][nt][i] * ux * uw + b : acc[mt][nt][i] + b;
             }
+        if (!whole)
+#pragma unroll
+            for (int mt = 0; mt < S::MT; mt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (vw + mt * 16 + i >= a.classes)
+#pragma unroll
+                        for (int nt = 0; nt < S::NT; nt++) acc[mt][nt][i] = -INFINITY;
     }
     const long long nw = n0 + wn * (TN / WN) + (lane & 15);
     const long long dpad = a.dcols;
+    int tt[S::NT];                                            // the rows' targets, counted from vw; -1: none of this span's classes
+#pragma unroll
+    for (int nt = 0; nt < S::NT; nt++) tt[nt] = -1;
+    if (a.target) {
+        const long long left = min(a.classes - vw, (long long)(TM / WM));
+#pragma unroll
+        for (int nt = 0; nt < S::NT; nt++) {
+            const long long t = a.target[min(nw + nt * 16, a.n - 1)] - a.v0 - vw;
+            tt[nt] = t >= 0 && t < left ? (int)t : -1;
+        }
+    }
     if constexpr (!GRAD) {
         // per row: maximum and sum over the span; lanes 16 and 32 apart share a row
         using E = typename Expo<Op>::T;
@@ -613,14 +642,14 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
                         }
                     }
             }
-            if (a.target && live) {
-                const long long t = a.target[row] - a.v0 - vw;
-                if (t >= 0 && t < TM)
+            if (tt[nt] >= 0 && live) {
+                float l = 0.f;
 #pragma unroll
-                    for (int mt = 0; mt < S::MT; mt++)
+                for (int mt = 0; mt < S::MT; mt++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            if (t == mt * 16 + i && vw + t < a.classes) a.tlogit[row] = acc[mt][nt][i];
+                    for (int i = 0; i < 4; i++) l = tt[nt] == mt * 16 + i ? acc[mt][nt][i] : l;
+                // (a lane has four classes of every sixteen)
+                if ((tt[nt] & 15) < 4) a.tlogit[row] = l;
             }
 #define AZG_PAIR(v) v += __shfl_xor(v, 16, 64); v += __shfl_xor(v, 32, 64)
             AZG_PAIR(s);
@@ -628,7 +657,7 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
             if (a.probs) { AZG_PAIR(tl); AZG_PAIR(ts); AZG_PAIR(ta); }
 #undef AZG_PAIR
             if (lane < 16 && live) {
-                const long long at = ((long long)tm * WM + wm) * a.n + row;
+                const long long at = (span_first + (long long)tm * WM + wm) * a.n + row;
                 a.part[at] = make_float2(mx, s);
                 if (a.part_e) a.part_e[at] = e;
                 if (a.probs) a.part_t[at] = make_float4(tl, ts, ta, 0.f);
@@ -636,18 +665,25 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
         }
     } else {
         typename Op::Img *d = static_cast<typename Op::Img *>(a.d);
-        float db[S::MT][4];
+        float db[S::MT][4], gs[S::NT];
+        float2 sts[S::NT];
 #pragma unroll
         for (int mt = 0; mt < S::MT; mt++)
 #pragma unroll
             for (int i = 0; i < 4; i++) db[mt][i] = 0.f;
 #pragma unroll
         for (int nt = 0; nt < S::NT; nt++) {
+            const long long row = min(nw + nt * 16, a.n - 1);
+            sts[nt] = *reinterpret_cast<const float2 *>(a.stats + row);
+            gs[nt] = a.rowg[row];
+        }
+#pragma unroll
+        for (int nt = 0; nt < S::NT; nt++) {
             const long long row = nw + nt * 16;
             const bool live = row < a.n;
-            const float4 st = live ? a.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
-            const float g = live ? a.rowg[row] : 0.f;
-            const long long t = live && a.target ? a.target[row] - a.v0 - vw : -1;
+            const float2 st = sts[nt];
+            const float g = live ? gs[nt] : 0.f;
+            const int t = tt[nt];
             const float *pr = a.probs ? a.probs + row * a.ldp : nullptr;
 #pragma unroll
             for (int mt = 0; mt < S::MT; mt++) {
@@ -691,6 +727,23 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
                 }
         }
     }
+}
+
+template <typename Op, int TM, int TN, int WM, int WN, bool GRAD>
+__global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
+{
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    logits_tile<Op, TM, TN, WM, WN, GRAD>(a, 0, 0, a.mtiles, a.ntiles, blockIdx.x, lds);
+}
+// The loss alone, where 256 x 256 tiles of all classes would leave the last round of the CUs mostly empty: whole rounds of them,
+// and 128 x 128 tiles of the classes behind.  2048 x 1024 x 50001: 1536 and 112 tiles, 199 us instead of 210.
+template <typename Op>
+__global__ __launch_bounds__(512) void logits_mixed_kernel(CeArgs a)
+{
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const unsigned large = (unsigned)a.mtiles * a.ntiles;
+    if (blockIdx.x < large) logits_tile<Op, 256, 256, 2, 4, false>(a, 0, 0, a.mtiles, a.ntiles, blockIdx.x, lds);
+    else logits_tile<Op, 128, 128, 2, 4, false>(a, a.mtiles * 256LL, a.mtiles * 2, a.mtiles_behind, (int)((a.n + 127) / 128), blockIdx.x - large, lds);
 }
 
 // ---------------------------------------------------------------- rows and totals

@@ -179,6 +179,8 @@ struct Plan {
     long long kimg, ldk, ldd;                                 // image elements along the features; row strides of the images of X, W and D
     int per, ks;                                              // image elements an element takes, k of a stage
     Shape lshape;
+    int large_m, behind_m;                                    // the loss alone: tiles of 256 and, behind them, of 128 classes (0: none)
+    long long spans;                                          // of a piece
     GradPick g;
     int fix_rows;
     size_t xmax, wmax, ximg, wimg, part, part_e, part_t, tlogit, stats, ent, rowg, sums, factor, d, dbpart, dxacc, dwacc, logits, count, total;
@@ -232,16 +234,27 @@ int make_plan(const azg_linear_ce_args *a, Plan *p)
     while ((p->n + p->fix_rows - 1) / p->fix_rows > 1024) p->fix_rows *= 2;
     while (p->fix_rows > 8 && (p->n + p->fix_rows - 1) / p->fix_rows * ((p->vp + kFixCols - 1) / kFixCols) < 1024) p->fix_rows /= 2;
     const ShapeDim dim = kDims[p->lshape];
+    p->large_m = p->behind_m = 0;
     const long long lm = (p->vp + dim.tm - 1) / dim.tm, ln = (p->n + dim.tn - 1) / dim.tn;
     const double grad_tiles = (a->dx ? (double)tiles_of(p->g.shape, p->H, p->n) * p->g.splits_x : 0.0) + (a->dw ? (double)tiles_of(p->g.shape, p->H, p->vp) * p->g.splits_w : 0.0);
     if ((double)lm * ln * dim.threads > kMaxThreads || grad_tiles * kDims[p->g.shape].threads > kMaxThreads)
         return fail(AZG_EINVAL, "azg_linear_ce: the problem is too large");
+    p->spans = lm * dim.wm;
+    if (!p->backward && p->pieces == 1 && p->lshape == T256) {
+        // the tiles that do not fill a round of the 256 CUs, cut into quarters, if one round takes those
+        const long long whole = lm * ln / 256 * 256 / ln, behind = (p->V - whole * 256 + 127) / 128;
+        if (whole > 0 && whole < lm && behind * ((p->n + 127) / 128) <= 256) {
+            p->large_m = (int)whole;
+            p->behind_m = (int)behind;
+            p->spans = (whole + behind) * 2;
+        }
+    }
     Take t;
     p->xmax = t(p->split ? kMaxParts * 4 : 0);
     p->wmax = t(p->split ? kMaxParts * 4 : 0);
     p->ximg = t(p->pack_x ? (size_t)p->n * p->ldk * 2 : 0);
     p->wimg = t(p->pack_w ? (size_t)p->vp * p->ldk * 2 : 0);
-    const size_t entries = (size_t)p->pieces * lm * dim.wm * p->n;
+    const size_t entries = (size_t)p->pieces * p->spans * p->n;
     p->part = t(p->forward ? entries * 8 : 0);
     p->part_e = t(p->forward && a->entropy ? entries * 4 : 0);
     p->part_t = t(p->forward && a->probs ? entries * 16 : 0);
@@ -300,6 +313,16 @@ int launch_logits(Shape shape, const CeArgs &c, hipStream_t s)
         if constexpr (!GRAD) return launch_logits_shape<Op, 128, 32, 4, 1, false>(c, s);
         return fail(AZG_EINVAL, "azg_linear_ce: internal: no such tile");
     }
+}
+
+template <typename Op>
+int launch_logits_mixed(const CeArgs &c, hipStream_t s)
+{
+    using S = TileShape<256, 256, 2, 4>;
+    OPS_TRY(allow_lds(logits_mixed_kernel<Op>, S::lds_bytes));
+    hipLaunchKernelGGL((logits_mixed_kernel<Op>), dim3((unsigned)(c.mtiles * c.ntiles + c.mtiles_behind * ((c.n + 127) / 128))), dim3(S::threads), S::lds_bytes, s, c);
+    OPS_HIP(hipGetLastError());
+    return AZG_OK;
 }
 
 template <typename Op, int TM, int TN, int WM, int WN>
@@ -393,7 +416,7 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
     };
 
     if (p.forward) {
-        const long long full = (p.vp + dim.tm - 1) / dim.tm * dim.wm;           // spans of a whole piece
+        const long long full = p.spans;                       // of a whole piece
         long long spans = 0;
         for (long long i = 0; i < p.pieces; i++) {
             OPS_TRY(piece(i, true));
@@ -402,8 +425,14 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
             c.part_t = a->probs ? reinterpret_cast<float4 *>(ws + p.part_t) + i * full * a->n : nullptr;
             c.tlogit = f32(p.tlogit);
             c.d = p.keep ? ws + p.d : nullptr;
-            OPS_TRY((launch_logits<Op, false>(p.lshape, c, s)));
-            spans += (c.classes + dim.tm - 1) / dim.tm * dim.wm;
+            if (p.behind_m) {
+                c.mtiles = p.large_m; c.mtiles_behind = p.behind_m; c.ntiles = (int)((a->n + 255) / 256);
+                OPS_TRY(launch_logits_mixed<Op>(c, s));
+                spans = full;
+            } else {
+                OPS_TRY((launch_logits<Op, false>(p.lshape, c, s)));
+                spans += (c.classes + dim.tm - 1) / dim.tm * dim.wm;
+            }
         }
         RowArgs r{};
         r.n = a->n; r.classes = a->classes; r.spans = (int)spans;

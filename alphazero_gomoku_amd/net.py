@@ -130,6 +130,7 @@ class PolicyValueNet(object):
         self._adam = None            # (grad, m, v) flat float32 vectors in state_dict order, step count
         self._ptr_cache = None
         self._adam_step = 0
+        self._dropout_step = 0       # training steps done either way: what the masks are numbered by
         self._eval_engine = None
         self._eval_version = -1
 
@@ -303,7 +304,7 @@ class PolicyValueNet(object):
         eng = self._engine_handle()
         grad = torch.zeros(int(eng.L.azg_train_param_count(eng.h)), dtype=torch.float32, device=dev)
         arr, keep = self._param_ptrs()
-        self._set_dropout(eng, self._adam_step + 1)
+        self._set_dropout(eng, self._dropout_step + 1)
         loss, entropy = C.c_float(0.0), C.c_float(0.0)
         torch.cuda.current_stream(dev).synchronize()
         eng._chk(eng.L.azg_train_backward(eng.h, int(s.shape[0]), C.c_void_p(s.data_ptr()), C.c_void_p(p.data_ptr()),
@@ -327,10 +328,10 @@ class PolicyValueNet(object):
             if dp:
                 from .dist import allreduce_gradients
                 reduce_fn = allreduce_gradients                  # every rank holds an equal share of the batch
-            self._adam_step += 1
+            self._dropout_step += 1
             loss, entropy = train_step_tensors(self.policy_value_net, self.optimizer, tensor(state_batch), tensor(mcts_probs),
                                                tensor(winner_batch), lr, reduce_fn,
-                                               self._dropout_args(self._adam_step) if self.dropout else None)
+                                               self._dropout_args(self._dropout_step) if self.dropout else None)
             self.version += 1
             return float(loss.item()), float(entropy.item())
         s, p, z = tensor(state_batch).contiguous(), tensor(mcts_probs).contiguous(), tensor(winner_batch).contiguous().reshape(-1)
@@ -344,7 +345,8 @@ class PolicyValueNet(object):
         loss, entropy = C.c_float(0.0), C.c_float(0.0)
         torch.cuda.current_stream(dev).synchronize()           # the batch exists before the library's stream reads it
         self._adam_step += 1
-        self._set_dropout(eng, self._adam_step)
+        self._dropout_step += 1
+        self._set_dropout(eng, self._dropout_step)
         if dp:
             from .dist import allreduce_flat
             eng._chk(eng.L.azg_train_backward(eng.h, n, C.c_void_p(s.data_ptr()), C.c_void_p(p.data_ptr()), C.c_void_p(z.data_ptr()),
@@ -386,7 +388,8 @@ class PolicyValueNet(object):
         loss, entropy, kl = C.c_float(0.0), C.c_float(0.0), C.c_double(0.0)
         torch.cuda.current_stream(dev).synchronize()           # the batch exists before the library's stream reads it
         self._adam_step += 1
-        self._set_dropout(eng, self._adam_step)
+        self._dropout_step += 1
+        self._set_dropout(eng, self._dropout_step)
         eng._chk(eng.L.azg_train_epoch(eng.h, n, C.c_void_p(s.data_ptr()), C.c_void_p(p.data_ptr()), C.c_void_p(z.data_ptr()), arr,
                                        C.c_void_p(grad.data_ptr()), C.c_void_p(m.data_ptr()), C.c_void_p(v.data_ptr()),
                                        self._adam_step, float(lr), 0.9, 0.999, 1e-8, self.l2_const, C.byref(loss), C.byref(entropy),

@@ -458,6 +458,21 @@ def test_cross_entropy_around_the_ends_of_the_small_path(ops, dtype, n, h, v):
     check_all(ops, x, w, b, t)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("kind,n,h,v", [("index", 1000, 40, 16717), ("probs", 300, 33, 33029), ("index", 256, 64, 65537), ("index", 2048, 72, 8300), ("probs", 1030, 8, 14000)])
+def test_cross_entropy_scores_of_mixed_tiles(ops, dtype, kind, n, h, v):
+    """More tiles than one round of the compute units, and a few: large and small ones in one launch.  Then a backward pass by itself."""
+    x, w, b, t = make(n, h, v, dtype, kind, ignored=0.2 if kind == "index" else 0.0, seed=n + h + v)
+    ref = reference(x, w, b, t, torch.full((n,), 0.5, device="cuda"))
+    loss, ent = ops.linear_cross_entropy(x, w, t, b, reduction="none", return_entropy=True)
+    close("loss", loss, *ref["loss"])
+    close("entropy", ent, *ref["ent"])
+    leaves = [q.clone().requires_grad_() for q in (x, w, b)]
+    (0.5 * ops.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], reduction="sum")).backward()
+    for leaf, key in zip(leaves, ("dx", "dw", "db")):
+        close(key, leaf.grad, *ref[key])
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("n,h,v", [(128, 16392, 128), (60, 40001, 64), (1, 1 << 20, 129)])
 def test_cross_entropy_of_very_many_features(ops, dtype, n, h, v):

@@ -64,6 +64,38 @@ def test_gradients_against_definition(size, n, rate):
     assert at == grad.numel()
 
 
+@pytest.mark.parametrize("world", [2, 4])
+def test_ranks_average_to_the_whole_batch(world):
+    """Every rank's gradient of its rows, under the masks of its rows, averaged: the gradient of the whole batch (bounds as above)."""
+    s, p, z = batch(64, 8)
+    q = net(8, dropout=0.4, dropout_seed=9)
+    total, losses = None, []
+    for rank in range(world):
+        q._dropout_args = lambda step: (0.4, 9, step, rank, world)
+        g, loss, _ = q.native_gradients(s[rank::world], p[rank::world], z[rank::world])
+        total = g.double() if total is None else total + g.double()
+        losses.append(loss)
+    del q._dropout_args
+    l64, _, g64 = definition(q.policy_value_net, s, p, z, 0.4, 9, 1, torch.float64)
+    _, _, g32 = definition(q.policy_value_net, s, p, z, 0.4, 9, 1, torch.float32)
+    assert abs(sum(losses) / world - l64) <= 2.0 ** -18 * abs(l64)
+    at = 0
+    for name, want, other in zip(order(), g64, g32):
+        got = total[at:at + want.numel()] / world
+        at += want.numel()
+        assert float((got - want).norm()) <= 3 * float((other - want).norm()) + 2.0 ** -20 * float(want.norm()), name
+
+
+def test_autograd_steps_leave_the_native_optimiser_alone():
+    """A step through autograd counts for the masks and not for the library's Adam."""
+    s, p, z = batch(64, 8)
+    q = net(8, dropout=0.3, dropout_seed=5)
+    q.train_step(s, p, z, 1e-3)
+    q.native_train = False
+    q.train_step(s, p, z, 1e-3)
+    assert (q._adam_step, q._dropout_step) == (1, 2)
+
+
 def test_step_takes_the_mask_of_its_number_and_repeats():
     s, p, z = batch(128, 8)
     a, b = net(8, dropout=0.3, dropout_seed=5), net(8, dropout=0.3, dropout_seed=5)
