@@ -373,16 +373,21 @@ struct TileProduct {
     }
 };
 
-// Workgroup number -> tile.  Consecutive workgroups go to the eight XCDs in turn, each with an L2 of its own: an XCD
-// gets a contiguous run of tiles, walked in strips of kStrip tiles of m so that the tiles in flight on it share rows
-// of both operands.
-constexpr int kStrip = 8;
-__device__ inline void tile_of(unsigned wg, int mt, int nt, int *m, int *n)
+// Workgroup number -> place in a list of `total`.  Consecutive workgroups go to the eight XCDs in turn, each with an L2 of its
+// own: an XCD gets a contiguous run of the list.
+__device__ inline unsigned xcd_run(unsigned wg, unsigned total)
 {
-    const unsigned total = (unsigned)mt * (unsigned)nt, per = total / 8, rest = total % 8, x = wg % 8, j = wg / 8;
-    const unsigned t = x * per + (x < rest ? x : rest) + j;
-    const unsigned strip = t / (unsigned)(kStrip * nt), first = strip * kStrip;
-    const unsigned h = min((unsigned)kStrip, (unsigned)mt - first), in = t - strip * kStrip * nt;
+    const unsigned per = total / 8, rest = total % 8, x = wg % 8;
+    return x * per + (x < rest ? x : rest) + wg / 8;
+}
+// The list of a product's tiles walks in strips of STRIP tiles of m, so that the tiles in flight on an XCD (32, or 16 where two
+// products share a launch) share rows of both operands: 8 for the logits (4: 2 % slower at 2048 x 1024 x 50001), 4 for the
+// gradients (8: 1 % slower at 8192 x 4096 x 65536).
+template <int STRIP>
+__device__ inline void tile_at(unsigned t, int mt, int nt, int *m, int *n)
+{
+    const unsigned strip = t / (unsigned)(STRIP * nt), first = strip * STRIP;
+    const unsigned h = min((unsigned)STRIP, (unsigned)mt - first), in = t - strip * STRIP * nt;
     *m = (int)(first + in % h);
     *n = (int)(in / h);
 }
@@ -534,7 +539,7 @@ __device__ inline void logits_tile(const CeArgs &a, long long m_first, int span_
 {
     using S = TileShape<TM, TN, WM, WN>;
     int tm, tn;
-    tile_of(wg, mtiles, ntiles, &tm, &tn);
+    tile_at<8>(xcd_run(wg, (unsigned)mtiles * ntiles), mtiles, ntiles, &tm, &tn);
     const long long m0 = m_first + (long long)tm * TM, n0 = (long long)tn * TN;
     fx4 acc[S::MT][S::NT];
 #pragma unroll
@@ -1008,9 +1013,9 @@ template <typename Op, int TM, int TN, int WM, int WN, bool TB>
 __device__ inline void grad_tile(const GradArgs &a, unsigned wg, char *lds)
 {
     using S = TileShape<TM, TN, WM, WN>;
-    const unsigned tiles = (unsigned)a.mtiles * a.ntiles, split = wg / tiles;
+    const unsigned tiles = (unsigned)a.mtiles * a.ntiles, t = xcd_run(wg, tiles * a.splits), split = t / tiles;
     int tm, tn;
-    tile_of(wg - split * tiles, a.mtiles, a.ntiles, &tm, &tn);
+    tile_at<4>(t - split * tiles, a.mtiles, a.ntiles, &tm, &tn);
     const long long m0 = (long long)tm * TM, n0 = (long long)tn * TN;
     const int k0 = (int)split * a.kper, k1 = min(a.ktiles, k0 + a.kper);
     fx4 acc[S::MT][S::NT];
