@@ -356,7 +356,8 @@ int launch_joins(JoinList l, int count, hipStream_t s)
 {
     unsigned grid = 0;
     for (int i = 0; i < count; i++) {
-        l.j[i].wgs = (unsigned)std::min<long long>((l.j[i].n * l.j[i].m + 255) / 256, 1 << 16);
+        const int outputs = l.j[i].splits > kFewSplits ? kJoinCols : 256;           // of a workgroup
+        l.j[i].wgs = (unsigned)std::min<long long>((l.j[i].n * l.j[i].m + outputs - 1) / outputs, 1 << 16);
         grid += l.j[i].wgs;
     }
     if (!grid) return AZG_OK;
