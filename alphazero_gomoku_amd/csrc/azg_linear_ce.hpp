@@ -80,8 +80,10 @@ struct TileShape {
     static constexpr int waves = WM * WN, threads = waves * 64;
     static constexpr int MT = TM / WM / 16, NT = TN / WN / 16;
     // stages of A and of B in LDS: the 256 x 256 tile takes all of a CU's 160 KB, 128 x 128 leaves room for a second
-    // workgroup; the tile for few rows does little but wait for memory and keeps more in flight
-    static constexpr int ring_a = TN <= 32 ? 5 : 3, ring_b = TN <= 32 ? 5 : 2;
+    // workgroup; the tile for few rows, and 64 x 64 where there are few of them (one wave across m), do little but wait for
+    // memory and keep more in flight (550 x 3717 x 488 float32 with gradients 101 -> 78 us; where three workgroups fit a CU
+    // they hide each other's waits, and longer rings cost 8 %: 974 x 2924 x 2167)
+    static constexpr int ring_a = TN <= 32 ? 5 : TN == 64 && WM == 1 ? 4 : 3, ring_b = TN <= 32 ? 5 : TN == 64 && WM == 1 ? 4 : 2;
     static constexpr int bytes_a = TM * 128, bytes_b = TN * 128, lds_bytes = ring_a * bytes_a + ring_b * bytes_b;
 };
 

@@ -123,9 +123,10 @@ struct Take {                                                 // offsets into th
     size_t operator()(size_t bytes) { const size_t at = off; off += (bytes + 255) / 256 * 256; return at; }
 };
 
-enum Shape { T256, T128, T64, TROW };
+enum Shape { T256, T128, T64, T64FEW, TROW };
 struct ShapeDim { int tm, tn, wm, threads; };
-constexpr ShapeDim kDims[4] = {{256, 256, 2, 512}, {128, 128, 2, 256}, {64, 64, 2, 256}, {128, 32, 4, 256}};
+constexpr ShapeDim kDims[5] = {{256, 256, 2, 512}, {128, 128, 2, 256}, {64, 64, 2, 256}, {64, 64, 1, 256}, {128, 32, 4, 256}};
+constexpr long long kFewTiles = 512;                          // T64FEW: two workgroups a CU, longer rings
 
 long long tiles_of(Shape s, long long m, long long n) { return ((m + kDims[s].tm - 1) / kDims[s].tm) * ((n + kDims[s].tn - 1) / kDims[s].tn); }
 
@@ -134,19 +135,19 @@ Shape pick_logits(long long m, long long n, bool grad)
     if (!grad && n <= 32) return TROW;
     if (m > 128 && tiles_of(T256, m, n) >= 200) return T256;
     if (m > 64 && tiles_of(T128, m, n) >= 200) return T128;
-    return T64;
+    return tiles_of(T64, m, n) <= kFewTiles ? T64FEW : T64;
 }
 // Tile of the gradients' products, which share a launch, and the splits of their sums, by an estimate in microseconds: the
 // launch takes its stages at the rate of the whole card or as long as its longest workgroup, whichever is more, and splits
 // cost a join.  Per stage and tile (measured at 16 bits; float32 half as much again): 256 x 256 1.0 with a CU to itself,
-// 128 x 128 0.30 a CU's share and 0.6 from start to end, 64 x 64 0.16 and 0.45.
+// 128 x 128 0.30 a CU's share and 0.6 from start to end, 64 x 64 0.16 and 0.45, with longer rings 0.35.
 struct GradPick { Shape shape; int splits_x, kper_x, splits_w, kper_w; };
 GradPick pick_grads(long long n, long long h, long long v, long long kx, long long kw, bool want_x, bool want_w)
 {
-    static constexpr double share[3] = {1.0, 0.30, 0.16}, alone[3] = {1.0, 0.6, 0.45};
+    static constexpr double share[4] = {1.0, 0.30, 0.16, 0.16}, alone[4] = {1.0, 0.6, 0.45, 0.35};
     GradPick best{};
     double least = 1e30;
-    for (Shape s : {T256, T128, T64}) {
+    for (Shape s : {T256, T128, T64, T64FEW}) {
         const long long tx = want_x ? tiles_of(s, h, n) : 0, tw = want_w ? tiles_of(s, h, v) : 0;
         if ((double)(tx + tw) * 32 * kDims[s].threads > kMaxThreads && s != T256) continue;
         for (long long per = 4; per == 4 || per < 2 * std::max(kx, kw); per *= 2) {          // stages of a workgroup at most
@@ -159,6 +160,7 @@ GradPick pick_grads(long long n, long long h, long long v, long long kx, long lo
             g.shape = s;
             split(kx, &g.splits_x, &g.kper_x);
             split(kw, &g.splits_w, &g.kper_w);
+            if (s == T64FEW && tx * g.splits_x + tw * g.splits_w > kFewTiles) continue;
             double joined = 0;                                                  // bytes of the splits, written and read
             if (tx && g.splits_x > 1) joined += 8.0 * g.splits_x * n * h;
             if (tw && g.splits_w > 1) joined += 8.0 * g.splits_w * v * h;
@@ -309,6 +311,7 @@ int launch_logits(Shape shape, const CeArgs &c, hipStream_t s)
     case T256: return launch_logits_shape<Op, 256, 256, 2, 4, GRAD>(c, s);
     case T128: return launch_logits_shape<Op, 128, 128, 2, 2, GRAD>(c, s);
     case T64: return launch_logits_shape<Op, 64, 64, 2, 2, GRAD>(c, s);
+    case T64FEW: return launch_logits_shape<Op, 64, 64, 1, 4, GRAD>(c, s);
     default:
         if constexpr (!GRAD) return launch_logits_shape<Op, 128, 32, 4, 1, false>(c, s);
         return fail(AZG_EINVAL, "azg_linear_ce: internal: no such tile");
@@ -347,7 +350,8 @@ int launch_grads(Shape shape, const GradArgs &x, const GradArgs &w, hipStream_t 
     switch (shape) {
     case T256: return launch_grads_shape<Op, 256, 256, 2, 4>(x, w, s);
     case T128: return launch_grads_shape<Op, 128, 128, 2, 2>(x, w, s);
-    default: return launch_grads_shape<Op, 64, 64, 2, 2>(x, w, s);
+    case T64: return launch_grads_shape<Op, 64, 64, 2, 2>(x, w, s);
+    default: return launch_grads_shape<Op, 64, 64, 1, 4>(x, w, s);
     }
 }
 // up to three joins in one launch
