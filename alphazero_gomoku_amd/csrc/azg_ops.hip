@@ -176,7 +176,7 @@ GradPick pick_grads(long long n, long long h, long long v, long long kx, long lo
 }
 
 struct Plan {
-    bool small, split, forward, backward, pack_w, pack_x, keep;      // keep: the forward pass leaves exponentials for the backward pass
+    bool small, few, split, forward, backward, pack_w, pack_x, keep;      // keep: the forward pass leaves exponentials for the backward pass
     long long n, H, V, vp, pieces;
     long long kimg, ldk, ldd;                                 // image elements along the features; row strides of the images of X, W and D
     int per, ks;                                              // image elements an element takes, k of a stage
@@ -216,6 +216,8 @@ int make_plan(const azg_linear_ce_args *a, Plan *p)
     // (dW multiplies the rows that count for nothing by zero: they are copied as zeros, whatever they hold)
     p->pack_x = p->split || !aligned16(a->x, a->x_stride, a->hidden, a->n) || (a->dw && a->target);
     p->pack_w = p->split || !aligned16(a->w, a->w_stride, a->hidden, a->classes);
+    p->few = !p->backward && p->n <= 32 && p->pack_w && p->V < 1 << 27;
+    if (p->few) p->pack_x = p->pack_w = false;
     // bytes a class of a piece costs
     long long cost = p->pack_w ? p->ldk * 2 : 0;
     if (p->backward) cost += p->n * p->per * 2;
@@ -242,7 +244,7 @@ int make_plan(const azg_linear_ce_args *a, Plan *p)
     if ((double)lm * ln * dim.threads > kMaxThreads || grad_tiles * kDims[p->g.shape].threads > kMaxThreads)
         return fail(AZG_EINVAL, "azg_linear_ce: the problem is too large");
     p->spans = lm * dim.wm;
-    if (!p->backward && p->pieces == 1 && p->lshape == T256) {
+    if (!p->backward && p->pieces == 1 && p->lshape == T256) {           // (never with few rows)
         // the tiles that do not fill a round of the 256 CUs, cut into quarters, if one round takes those
         const long long whole = lm * ln / 256 * 256 / ln, behind = (p->V - whole * 256 + 127) / 128;
         if (whole > 0 && whole < lm && behind * ((p->n + 127) / 128) <= 256) {
@@ -251,6 +253,7 @@ int make_plan(const azg_linear_ce_args *a, Plan *p)
             p->spans = (whole + behind) * 2;
         }
     }
+    if (p->few) p->spans = (p->V + kSmallTile - 1) / kSmallTile;
     Take t;
     p->xmax = t(p->split ? kMaxParts * 4 : 0);
     p->wmax = t(p->split ? kMaxParts * 4 : 0);
@@ -398,7 +401,7 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
     px.maxpart = f32(p.xmax); px.img = ws + p.ximg; px.ldi = p.ldk; px.icols = p.kimg;
     PackArgs pw{};
     pw.src = W; pw.ld = a->w_stride; pw.rows = a->classes; pw.cols = a->hidden; pw.maxpart = f32(p.wmax); pw.img = ws + p.wimg; pw.ldi = p.ldk; pw.icols = p.kimg;
-    if (Op::split) hipLaunchKernelGGL(absmax_kernel, dim3(2 * kMaxParts), dim3(512), 0, s, px, pw);
+    if (Op::split && !p.few) hipLaunchKernelGGL(absmax_kernel, dim3(2 * kMaxParts), dim3(512), 0, s, px, pw);
     bool x_packed = !p.pack_x;
     CeArgs c{};
     c.x = p.pack_x ? Operand{ws + p.ximg, p.ldk, a->n, p.kimg} : Operand{a->x, a->x_stride, a->n, a->hidden};
@@ -423,7 +426,15 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
     if (p.forward) {
         const long long full = p.spans;                       // of a whole piece
         long long spans = 0;
-        for (long long i = 0; i < p.pieces; i++) {
+        if (p.few) {
+            FewArgs f{};
+            f.x = a->x; f.w = a->w; f.bias = a->bias; f.xs = a->x_stride; f.ws = a->w_stride;
+            f.n = (int)a->n; f.H = (int)a->hidden; f.V = (int)a->classes; f.target = target; f.probs = a->probs; f.ldp = a->probs_stride;
+            f.part = reinterpret_cast<float2 *>(ws + p.part); f.part_e = a->entropy ? f32(p.part_e) : nullptr;
+            f.part_t = a->probs ? reinterpret_cast<float4 *>(ws + p.part_t) : nullptr; f.tlogit = f32(p.tlogit);
+            hipLaunchKernelGGL((few_rows_kernel<In>), dim3((unsigned)full), dim3(kSmallWaves * 64), 0, s, f);
+            spans = full;
+        } else for (long long i = 0; i < p.pieces; i++) {
             OPS_TRY(piece(i, true));
             c.part = reinterpret_cast<float2 *>(ws + p.part) + i * full * a->n;
             c.part_e = a->entropy ? f32(p.part_e) + i * full * a->n : nullptr;

@@ -459,6 +459,32 @@ def test_cross_entropy_around_the_ends_of_the_small_path(ops, dtype, n, h, v):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("kind,n,h,v", [("index", 1, 77, 5000), ("index", 32, 900, 4097), ("probs", 17, 33, 6001), ("probs", 1, 1, 5001), ("index", 4, 1892, 50047),
+                                        ("index", 31, 2049, 20000)])
+def test_cross_entropy_scores_of_few_rows(ops, dtype, kind, n, h, v):
+    """Few rows of odd lengths against many classes, alone and before a backward pass by itself."""
+    x, w, b, t = make(n, h, v, dtype, kind, ignored=0.2 if kind == "index" and n > 8 else 0.0, seed=n + h + v)
+    if kind == "index":
+        t[0] = v - 1
+    ref = reference(x, w, b, t, torch.ones(n, device="cuda"))
+    for bias in (b, None):
+        if bias is None:
+            ref = reference(x, w, None, t, torch.ones(n, device="cuda"))
+        loss, ent = ops.linear_cross_entropy(x, w, t, bias, reduction="none", return_entropy=True)
+        close("loss", loss, *ref["loss"])
+        close("entropy", ent, *ref["ent"])
+    leaves = [q.clone().requires_grad_() for q in (x, w)]
+    ops.linear_cross_entropy(leaves[0], leaves[1], t, reduction="sum").backward()
+    for leaf, key in zip(leaves, ("dx", "dw")):
+        close(key, leaf.grad, *ref[key])
+    with torch.no_grad():
+        blocked = torch.zeros(v, device="cuda").to(x.dtype)
+        blocked[1:v - 1] = float("-inf")                            # spans of which nothing is left
+        tb = torch.zeros(n, dtype=torch.int64, device="cuda")
+        close("blocked", ops.linear_cross_entropy(x, w, tb, blocked, reduction="none"), *reference(x, w, blocked, tb, torch.ones(n, device="cuda"))["loss"])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("kind,n,h,v", [("index", 1000, 40, 16717), ("probs", 300, 33, 33029), ("index", 256, 64, 65537), ("index", 2048, 72, 8300), ("probs", 1030, 8, 14000)])
 def test_cross_entropy_scores_of_mixed_tiles(ops, dtype, kind, n, h, v):
     """More tiles than one round of the compute units, and a few: large and small ones in one launch.  Then a backward pass by itself."""
