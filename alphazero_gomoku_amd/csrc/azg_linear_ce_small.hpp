@@ -106,7 +106,7 @@ __device__ inline void small_product(const TA *A, long long lda, int m0, int M, 
                 for (int t = 0; t < 2; t++) acc[s][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][s][j], b[u][t][j], acc[s][t], 0, 0, 0);
     };
     for (int k = wave * 16; k < K; k += kAhead * kStep) {
-        // whole blocks of this round; a block cut short by the end of K can only be its wave's last one
+        // whole blocks of this turn; a block cut short by the end of K can only be its wave's last one
         const int whole = max(0, min(kAhead, (K - 16 - k) / kStep + (K - 16 >= k)));
 #pragma unroll
         for (int u = 0; u < kAhead; u++)
