@@ -220,7 +220,7 @@ int make_plan(const azg_linear_ce_args *a, Plan *p)
     // (dW multiplies the rows that count for nothing by zero: they are copied as zeros, whatever they hold)
     p->pack_x = p->split || !aligned16(a->x, a->x_stride, a->hidden, a->n) || (a->dw && a->target);
     p->pack_w = p->split || !aligned16(a->w, a->w_stride, a->hidden, a->classes);
-    p->few = !p->backward && p->n <= 32 && p->pack_w && p->V < 1 << 27;
+    p->few = !p->backward && p->n <= 32 && p->pack_w;
     if (p->few) p->pack_x = p->pack_w = false;
     // bytes a class of a piece costs
     long long cost = p->pack_w ? p->ldk * 2 : 0;
@@ -286,7 +286,7 @@ int check(const azg_linear_ce_args *a)
     if (!a) return fail(AZG_EINVAL, "null argument");
     if (a->dtype != AZG_F32 && a->dtype != AZG_BF16 && a->dtype != AZG_F16) return fail(AZG_EINVAL, "azg_linear_ce: unknown dtype %d", a->dtype);
     if (a->n < 0 || a->hidden < 1 || a->classes < 1) return fail(AZG_EINVAL, "azg_linear_ce: sizes must be n >= 0, hidden >= 1, classes >= 1");
-    if (a->n >= 1 << 26 || a->classes > INT_MAX || a->hidden > (1 << 22)) return fail(AZG_EINVAL, "azg_linear_ce: a size is too large");
+    if (a->n >= 1 << 26 || a->classes >= 1 << 27 || a->hidden > (1 << 22)) return fail(AZG_EINVAL, "azg_linear_ce: a size is too large");
     if (a->reduction < AZG_REDUCE_NONE || a->reduction > AZG_REDUCE_MEAN) return fail(AZG_EINVAL, "azg_linear_ce: unknown reduction %d", a->reduction);
     if (bad_matrix(a->n, a->hidden, a->x_stride) || bad_matrix(a->classes, a->hidden, a->w_stride)) return fail(AZG_EINVAL, "azg_linear_ce: a row stride is smaller than a row");
     if ((a->n > 1 && a->x_stride > (1LL << 22)) || (a->classes > 1 && a->w_stride > (1LL << 22))) return fail(AZG_EINVAL, "azg_linear_ce: a row stride is too large");
@@ -320,7 +320,7 @@ int launch_logits(Shape shape, const CeArgs &c, hipStream_t s)
     case T64: return launch_logits_shape<Op, 64, 64, 2, 2, GRAD>(c, s);
     case T64FEW: return launch_logits_shape<Op, 64, 64, 1, 4, GRAD>(c, s);
     default:
-        if constexpr (!GRAD) return launch_logits_shape<Op, 128, 32, 4, 1, false>(c, s);
+        if constexpr (!GRAD && !Op::split) return launch_logits_shape<Op, 128, 32, 4, 1, false>(c, s);
         return fail(AZG_EINVAL, "azg_linear_ce: internal: no such tile");
     }
 }

@@ -321,7 +321,8 @@ int azg_dropout(const azg_dropout_args *a);
  * type), against class numbers or against probabilities (any real weights), and its gradients.  The logits of a large problem
  * are not stored: a backward pass keeps one array of 2 bytes (AZG_F32: 4) an element, of at most 1 GiB together with the
  * copies of x and w that it needs or of 1024 classes, and takes more classes than fit piece by piece.  Small problems keep at
- * most 16 MB of float32 logits.  n < 2^26, hidden and the row strides of x and w at most 2^22.  For every row
+ * most 16 MB of float32 logits.  n < 2^26, classes < 2^27, hidden and the row
+ * strides of x and w at most 2^22.  For every row
  *   loss = lse - l[target]                        target int64 [n]; rows whose target is ignore_index count for nothing,
  *                                                 whatever x holds there (loss 0, gradient 0); any other target outside
  *                                                 0 .. classes - 1 makes the row's loss, and every gradient it reaches, NaN

@@ -43,7 +43,7 @@ def test_dropout_refuses(lib, kw, what):
 
 
 @pytest.mark.parametrize("kw,what", [(dict(dtype=3), "dtype"), (dict(n=-1), "sizes"), (dict(hidden=0), "sizes"), (dict(classes=0), "sizes"),
-                                     (dict(n=1 << 40), "too large"), (dict(n=1 << 26), "too large"), (dict(hidden=1 << 23), "too large"), (dict(reduction=3), "reduction"),
+                                     (dict(n=1 << 40), "too large"), (dict(n=1 << 26), "too large"), (dict(classes=1 << 27), "too large"), (dict(hidden=1 << 23), "too large"), (dict(reduction=3), "reduction"),
                                      (dict(reduction=-1), "reduction"), (dict(x_stride=7), "stride"), (dict(w_stride=7), "stride"),
                                      (dict(x_stride=1 << 23), "too large"), (dict(w_stride=1 << 23), "too large")])
 def test_linear_ce_refuses_sizes(lib, kw, what):
