@@ -510,3 +510,14 @@ def test_bench_reads_the_trained_fixture_net_in_the_reference_layout():
     assert np.array_equal(got[8].numpy(), raw[8].T)
     assert np.array_equal(got[0].numpy(), raw[0][:, :, ::-1, ::-1])
     assert np.array_equal(got[1].numpy(), raw[1])
+
+
+def test_gloo_collectives_always_stage_through_the_host(monkeypatch):
+    """Under gloo the buffers of every collective lie in host memory, whatever the environment says."""
+    import torch
+    from alphazero_gomoku_amd import dist as azdist
+    monkeypatch.setattr(azdist.dist, "get_backend", lambda group=None: "gloo")
+    monkeypatch.setenv("AZG_GLOO_DEVICE_TENSORS", "1")
+    assert azdist._comm_device(torch.device("cuda", 0)) == torch.device("cpu")
+    monkeypatch.setattr(azdist.dist, "get_backend", lambda group=None: "nccl")
+    assert azdist._comm_device(torch.device("cuda", 0)) == torch.device("cuda", 0)
