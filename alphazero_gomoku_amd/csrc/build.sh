@@ -6,9 +6,9 @@
 #   adjacent multiply-adds into v_pk_fma_f32; in the kernel whose tree waves share their SIMDs with
 #   matrix-dense waves such an operation, fed its x from the high dword of a register pair
 #   (op_sel:[0,1,0]), came out one term short in lanes 48-55 (50-70 of 256 identical searches wrong;
-#   the note at AZG_EXP_PKFC in azg_dual.hpp has the measurements).  The build FAILS when a kernel of azgomoku.hip
-#   holds any two-wide float32 instruction (v_pk_fma_f32 / v_pk_mul_f32 / v_pk_add_f32), whatever
-#   flag or compiler version produced it.
+#   the note at AZG_EXP_PKFC in azg_dual.hpp has the measurements).  The build FAILS when a kernel of either
+#   translation unit holds any two-wide float32 instruction (check_asm.sh), whatever flag or compiler
+#   version produced it.
 #  -no-hip-rt leaves the HIP runtime symbols undefined: the process must hold exactly ONE HIP
 #   runtime, and PyTorch ships its own libamdhip64.so.  The loader (alphazero_gomoku_amd/_lib.py)
 #   loads the runtime PyTorch will use (or /opt/rocm's when PyTorch is absent) with RTLD_GLOBAL
@@ -23,7 +23,7 @@ trap 'rm -rf "$tmp"' EXIT
 # No translation unit may form two-wide float32 instructions at all (-packed-fp32-ops).  azg_ops.hip (the training heads'
 # operators) is one of its own, compiled beside the other.
 nopk="-Xclang -target-feature -Xclang -packed-fp32-ops"
-( hipcc --offload-arch=gfx950 -O3 -fno-slp-vectorize -fPIC -std=c++17 -Wall $nopk -c "$here/azg_ops.hip" -o "$tmp/azg_ops.o" > "$tmp/ops.log" 2>&1; echo $? > "$tmp/ops.rc" ) &
+( cd "$tmp" && hipcc --offload-arch=gfx950 -O3 -fno-slp-vectorize -fPIC -std=c++17 -Wall $nopk -save-temps=cwd -c "$here/azg_ops.hip" -o "$tmp/azg_ops.o" > "$tmp/ops.log" 2>&1; echo $? > "$tmp/ops.rc" ) &
 ops=$!
 ( cd "$tmp" && hipcc --offload-arch=gfx950 -O3 -ffp-contract=off -fno-slp-vectorize -fPIC -c -std=c++17 -Wall $nopk \
     -Rpass-analysis=kernel-resource-usage -save-temps=cwd \
@@ -34,15 +34,8 @@ grep -v "packed-fp32-ops" "$tmp/ops.log" >&2 || true
 [ "$(cat "$tmp/ops.rc")" = 0 ] || { rm -f "$out" "$log"; exit 1; }
 grep -v "packed-fp32-ops" "$log" > "$tmp/log" || true
 cp "$tmp/log" "$log"
+sh "$here/check_asm.sh" "$tmp"/azgomoku*gfx950.s "$tmp"/azg_ops*gfx950.s || { rm -f "$out" "$log"; exit 1; }
 hipcc --offload-arch=gfx950 -fPIC -shared -no-hip-rt "$tmp/azgomoku.o" "$tmp/azg_ops.o" -o "$out" -lpthread
-asm="$(ls "$tmp"/azgomoku*gfx950.s 2>/dev/null | head -1)"
-if [ -z "$asm" ]; then echo "build.sh: no device assembly to check" >&2; rm -f "$out" "$log"; exit 1; fi
-bad="$(awk '/^_ZN3azg[^ ]*:/ { fn = $1 } /v_pk_(fma|mul|add)_f32/ { print fn " " $0 }' "$asm" | head -5)"
-if [ -n "$bad" ]; then
-    echo "$bad" >&2
-    echo "build.sh: two-wide float32 instructions (see above): refusing to ship this library" >&2
-    rm -f "$out" "$log"; exit 1
-fi
 # compiler warnings, without the resource-usage remarks and their source excerpts
 if grep -q "warning:" "$log"; then
     awk '/kernel-resource-usage/ { skip = 2; next } skip > 0 { skip--; next } { print }' "$log" >&2
