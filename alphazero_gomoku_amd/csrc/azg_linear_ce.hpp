@@ -974,7 +974,8 @@ __global__ __launch_bounds__(256) void fix_kernel(FixArgs a)
         const long long cls = a.target ? a.target[row] : -1, t = a.target ? cls - c : -1;
         const float g = a.rowg ? a.rowg[row] : (a.target && cls == a.ignore ? 0.f : 1.f);
         if (c >= a.dcols) continue;
-        const float mp = part[row].x, f = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mp - st.x) * st.y;
+        // (a span with every class blocked: zeros, but NaN where the row has no other span or no finite loss)
+        const float mp = part[row].x, f = (mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mp - st.x)) * st.y;
         float v[8];
         if constexpr (Op::split) {
             const fx4 *p = reinterpret_cast<const fx4 *>(static_cast<float *>(a.d) + row * lde + c);

@@ -328,6 +328,7 @@ int azg_dropout(const azg_dropout_args *a);
  *                                                 0 .. classes - 1 makes the row's loss, and every gradient it reaches, NaN
  *   loss = lse sum_v probs - sum_v probs l        probs float32 [n,classes]; a weight of 0 contributes 0
  *   entropy = lse - sum_v p l                     p = softmax(l)
+ * A row whose logits are all -inf has no softmax: its loss, its entropy and every gradient it reaches are NaN.
  * reduction AZG_REDUCE_NONE: loss, entropy float32 [n]; _SUM, _MEAN (over the rows that count; 0 if none does): [1].
  * Gradients are those of sum_i dloss_i loss_i (NONE, dloss [n]) or dloss loss ([1]), times grad_scale; dloss NULL = 1.
  * One call does the forward pass (loss not NULL), the backward pass (any of dx, dw, db not NULL), or both.  A backward pass
