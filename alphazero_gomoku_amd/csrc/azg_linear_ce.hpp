@@ -32,7 +32,7 @@ typedef float fx4 __attribute__((ext_vector_type(4)));
 typedef _Float16 hx8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bx8 __attribute__((ext_vector_type(8)));
 
-constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
+constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kDScale = 16384.0f;      // images of D hold D 2^14: |D| <= 2 then ends below half precision's 65504 and
                                          // probabilities down to 2^-28 keep all their bits
 
@@ -515,12 +515,12 @@ struct CeArgs {
     const float *probs;           // [n][ldp], already offset to the piece's first class
     long long ldp;
     // statistics, one entry a row and a wave's run of TM / WM classes ("span")
-    float2 *part;                 // [spans][n]: M = maximum times log2e, sum of 2^(l log2e - M)
-    float *part_e;                // [spans][n]: sum of 2^(l log2e - M) l, or null
-    float4 *part_t;               // probabilities: sum pi l, sum pi, sum |pi|, -
+    float2 *part;                 // [spans][n]: maximum m, sum of exp(l - m)
+    float *part_e;                // [spans][n]: sum of exp(l - m) (l - m), or null
+    float4 *part_t;               // probabilities: sum pi (l - m), sum pi, sum |pi|, -
     float *tlogit;                // index: [n]
     // gradient
-    const float4 *stats;          // [n]: M, sum pi / s, ... (RowArgs)
+    const float4 *stats;          // [n]: m, sum pi / s, ... (RowArgs)
     const float *rowg;            // [n]
     void *d;                      // image [n][ldd] of D; statistics: of exp(l - the span's maximum), or null
     long long ldd, dcols;         // row stride in image elements; padded classes
@@ -623,9 +623,9 @@ __device__ inline void logits_tile(const CeArgs &a, long long m_first, int span_
                 for (int i = 0; i < 4; i++) mx = fmaxf(mx, acc[mt][nt][i]);
             mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            // Sums are of 2^(l log2e - M), M = the maximum times log2e as rounded: one operation in front of the exponential.
+            // Everything is summed relative to the maximum, which enters unrounded: exp(l - m) is 1 at the maximum, so a sum is at
+            // least 1, a loss and an entropy at least 0, and neither loses bits to an offset that all logits share.
             // (A NaN is passed over by fmaxf: it comes back through the sum; a maximum of -inf leaves every term 2^-inf.)
-            mx *= kLog2e;
             const float base = mx == -INFINITY ? 0.f : mx;
             float s = 0.f, e = 0.f, tl = 0.f, ts = 0.f, ta = 0.f;
             if (a.part_e)
@@ -633,15 +633,15 @@ __device__ inline void logits_tile(const CeArgs &a, long long m_first, int span_
                 for (int mt = 0; mt < S::MT; mt++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const float l = acc[mt][nt][i], x = __builtin_amdgcn_exp2f(__builtin_fmaf(l, kLog2e, -base));
-                        e += x != 0.f ? x * l : 0.f;
+                        const float d = acc[mt][nt][i] - base, x = __builtin_amdgcn_exp2f(d * kLog2e);
+                        e += x != 0.f ? x * d : 0.f;
                     }
 #pragma unroll
             for (int mt = 0; mt < S::MT; mt++) {
                 Pack<E, 4> keep;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float l = acc[mt][nt][i], x = __builtin_amdgcn_exp2f(__builtin_fmaf(l, kLog2e, -base));
+                    const float x = __builtin_amdgcn_exp2f((acc[mt][nt][i] - base) * kLog2e);
                     s += x;
                     keep.v[i] = (E)x;
                 }
@@ -658,7 +658,7 @@ __device__ inline void logits_tile(const CeArgs &a, long long m_first, int span_
                     for (int i = 0; i < 4; i++) {
                         const float p = pv[mt].v[i];
                         ts += p; ta += fabsf(p);
-                        tl += p != 0.f ? p * acc[mt][nt][i] : 0.f;
+                        tl += p != 0.f ? p * (acc[mt][nt][i] - base) : 0.f;
                     }
             }
             if (tt[nt] >= 0 && live) {
@@ -712,7 +712,7 @@ __device__ inline void logits_tile(const CeArgs &a, long long m_first, int span_
                 if (pr) pv = four_of(pr, cls, a.classes, whole);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    float q = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mt][nt][i], kLog2e, -st.x)) * st.y;
+                    float q = __builtin_amdgcn_exp2f((acc[mt][nt][i] - st.x) * kLog2e) * st.y;
                     if (pr) q -= pv.v[i];
                     else if (t == mt * 16 + i) q -= 1.f;
                     q = g == 0.f || cls + i >= a.classes ? 0.f : q * g;         // a row that counts for nothing: zero whatever it holds
@@ -774,11 +774,19 @@ struct RowArgs {
     const float2 *part; const float *part_e; const float4 *part_t; const float *tlogit;
     const long long *target; long long ignore;
     float *loss_out, *ent_out;    // [n], or null: rows' results that nothing else has to be added to
-    float4 *stats;                // [n]: M, sum pi / s, sum |pi|, loss with lse = M ln2 + log s (so that p takes no rounding of lse)
+    float4 *stats;                // [n]: m, sum pi / s, sum |pi|, loss with lse = m + log s (so that p takes no rounding of lse)
     float *ent;                   // [n] or null
 };
-// One wave per row: join the spans' (maximum, sum) pairs in a fixed order.  Latency: 8 us for 2048 rows of 392 spans, 7 us for
+// One wave per row: join the spans' sums, each relative to its span's maximum m_j, in a fixed order; relative to m they are
+// s_j f, (e_j + (m_j - m) s_j) f and t_j + (m_j - m) sum pi, f = exp(m_j - m).  Latency: 8 us for 2048 rows of 392 spans, 7 us for
 // one row of 2048.
+__device__ inline void shift(float m, float base, float &s, float &e, float &tl, float ts)
+{
+    const float from = m == -INFINITY ? 0.f : m, d = from - base, f = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(d * kLog2e);
+    e = f != 0.f ? (e + d * s) * f : 0.f;                     // (d may be as low as the type's lowest value)
+    s *= f;
+    tl += ts != 0.f ? d * ts : 0.f;
+}
 __global__ __launch_bounds__(256) void rows_kernel(RowArgs a)
 {
     const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -800,28 +808,28 @@ __global__ __launch_bounds__(256) void rows_kernel(RowArgs a)
             if (!in) { p[j] = make_float2(-INFINITY, 0.f); q[j] = 0.f; u[j] = make_float4(0.f, 0.f, 0.f, 0.f); }
         }
         const float m = fmaxf(fmaxf(mx, fmaxf(p[0].x, p[1].x)), fmaxf(p[2].x, p[3].x)), base = m == -INFINITY ? 0.f : m;
-        // (a pair without a class adds nothing; a NaN sum stays NaN)
-        const float f0 = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - base);
-        s *= f0; e *= f0;
+        // (a span without a class counts from 0 and adds nothing; a NaN sum stays NaN)
+        shift(mx, base, s, e, tl, ts);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const float f = p[j].x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(p[j].x - base);
-            s += p[j].y * f; e += q[j] * f; tl += u[j].x; ts += u[j].y; ta += u[j].z;
+            shift(p[j].x, base, p[j].y, q[j], u[j].x, u[j].y);
+            s += p[j].y; e += q[j]; tl += u[j].x; ts += u[j].y; ta += u[j].z;
         }
         mx = m;
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const float om = __shfl_xor(mx, d, 64), os = __shfl_xor(s, d, 64), oe = __shfl_xor(e, d, 64);
+        const float om = __shfl_xor(mx, d, 64);
+        float os = __shfl_xor(s, d, 64), oe = __shfl_xor(e, d, 64), ot = 0.f, op = 0.f;
+        if (a.part_t) { ot = __shfl_xor(tl, d, 64); op = __shfl_xor(ts, d, 64); ta += __shfl_xor(ta, d, 64); }
         const float m = fmaxf(mx, om), base = m == -INFINITY ? 0.f : m;
-        const float f0 = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - base);
-        const float f1 = om == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(om - base);
-        s = s * f0 + os * f1; e = e * f0 + oe * f1; mx = m;
-        if (a.part_t) { tl += __shfl_xor(tl, d, 64); ts += __shfl_xor(ts, d, 64); ta += __shfl_xor(ta, d, 64); }
+        shift(mx, base, s, e, tl, ts);
+        shift(om, base, os, oe, ot, op);
+        s += os; e += oe; tl += ot; ts += op; mx = m;
     }
     if (lane) return;
-    const float ls = logf(s), m = mx == -INFINITY ? 0.f : mx * kLn2, lse = m + ls;
-    float loss, ent = lse - e / s;
+    const float ls = logf(s), m = mx == -INFINITY ? 0.f : mx;
+    float loss, ent = ls - e / s;
     if (a.target) {
         const long long t = a.target[row];
         ts = ta = 1.f;
@@ -829,7 +837,7 @@ __global__ __launch_bounds__(256) void rows_kernel(RowArgs a)
         else if (t < 0 || t >= a.classes) { loss = ent = NAN; ts = ta = NAN; }
         else loss = (m - a.tlogit[row]) + ls;
     } else {
-        loss = lse * ts - tl;
+        loss = ls * ts - tl;
     }
     a.stats[row] = make_float4(mx, ts / s, ta, loss);
     if (a.ent) a.ent[row] = ent;
@@ -975,7 +983,7 @@ __global__ __launch_bounds__(256) void fix_kernel(FixArgs a)
         const float g = a.rowg ? a.rowg[row] : (a.target && cls == a.ignore ? 0.f : 1.f);
         if (c >= a.dcols) continue;
         // (a span with every class blocked: zeros, but NaN where the row has no other span or no finite loss)
-        const float mp = part[row].x, f = (mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mp - st.x)) * st.y;
+        const float mp = part[row].x, f = (mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mp - st.x) * kLog2e)) * st.y;
         float v[8];
         if constexpr (Op::split) {
             const fx4 *p = reinterpret_cast<const fx4 *>(static_cast<float *>(a.d) + row * lde + c);

@@ -265,11 +265,10 @@ __global__ __launch_bounds__(kSmallWaves * 64) void few_rows_kernel(FewArgs a)
         float mx = l;
 #pragma unroll
         for (int s = 1; s < 32; s <<= 1) mx = fmaxf(mx, __shfl_xor(mx, s, 64));
-        mx *= kLog2e;
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(l, kLog2e, mx == -INFINITY ? 0.f : -mx));
-        const float s = sum32(x), e = a.part_e ? sum32(x != 0.f ? x * l : 0.f) : 0.f;
+        const float d = l - (mx == -INFINITY ? 0.f : mx), x = __builtin_amdgcn_exp2f(d * kLog2e);
+        const float s = sum32(x), e = a.part_e ? sum32(x != 0.f ? x * d : 0.f) : 0.f;
         const float p = a.probs && live && v < a.V ? a.probs[row * a.ldp + v] : 0.f;
-        const float tl = a.probs ? sum32(p != 0.f ? p * l : 0.f) : 0.f, ts = a.probs ? sum32(p) : 0.f, ta = a.probs ? sum32(fabsf(p)) : 0.f;
+        const float tl = a.probs ? sum32(p != 0.f ? p * d : 0.f) : 0.f, ts = a.probs ? sum32(p) : 0.f, ta = a.probs ? sum32(fabsf(p)) : 0.f;
         if (!live) continue;
         if (a.target && v < a.V && a.target[row] == v) a.tlogit[row] = l;
         if ((lane & 31) == 0) {
@@ -321,7 +320,7 @@ __global__ __launch_bounds__(256) void small_rows_kernel(SmallArgs a)
     }
     __syncthreads();                                          // (l[t] is read before it becomes D)
     if (tid == 0) {
-        a.stats[row] = make_float4(mx * kLog2e, ts / s, ta, loss);
+        a.stats[row] = make_float4(mx, ts / s, ta, loss);
         if (a.ent) a.ent[row] = ent;
         if (a.reduction == 0) {
             if (a.loss) a.loss[row] = loss;

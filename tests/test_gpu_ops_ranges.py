@@ -53,3 +53,61 @@ def test_a_bad_target_reaches_blocked_classes_too(ops, dtype, n, h, v):
     for dx, dw, db in (one[2:], autograd(ops, x, w, t, b, reduction="none")[1:]):
         assert bool(torch.isnan(dx[5]).all()) and bool(torch.isfinite(dx[:5]).all()) and bool(torch.isfinite(dx[6:]).all())
         assert bool(torch.isnan(dw).all()) and bool(torch.isnan(db).all())
+
+
+# ---------------------------------------------------------------- rows that are certain, logits with a common offset
+def exact_logits(n, h, v, dtype, offset, peak, seed=3):
+    """Rows of one 1 each, so that logits are weights and a bias: multiples of 1/8, at most 8 in magnitude, the same in every type
+    and product.  Every bias is `offset`, and `peak` more at one class, which is the target of four rows of five."""
+    gen = torch.Generator("cuda").manual_seed(seed)
+    x = torch.zeros(n, h, device="cuda")
+    at = torch.arange(n, device="cuda") % h
+    x[torch.arange(n, device="cuda"), at] = 1.0
+    w = torch.randint(-64, 65, (v, h), generator=gen, device="cuda").float() / 8
+    b = torch.full((v,), float(offset), device="cuda")
+    best = v // 3
+    b[best] += peak
+    t = torch.full((n,), best, dtype=torch.int64, device="cuda")
+    t[::5] = torch.randint(0, v, (len(t[::5]),), generator=gen, device="cuda")
+    dt = DT[dtype]
+    l = w.double().t()[at] + b.to(dt).double()
+    return x.to(dt), w.to(dt), b.to(dt), t, l
+
+
+CERTAIN = PATHS + [(7, 104, 5003), (7, 100, 5003), (300, 64, 20000), (1000, 40, 16717), (1500, 96, 4300)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,h,v", CERTAIN)
+@pytest.mark.parametrize("offset,peak", [(0, 0), (0, 16), (0, 32), (0, 96), (1024, 16), (-1024, 32)])
+def test_loss_and_entropy_of_exact_logits(ops, dtype, n, h, v, offset, peak):
+    """With d = l - max exact, an exponential is off by (|d| + 2) 2 f of itself (its argument, log2 e, the instruction) and a sum of
+    positive numbers by 80 f (additions one after the other: at most 32 in a lane, 2 across lanes, 32 over spans, 6 across lanes),
+    and by no more than the terms beside the maximum, twice, where these are less.  Nothing depends on an offset of all logits; a certain row's loss and entropy are at least 0."""
+    x, w, b, t, l = exact_logits(n, h, v, dtype, offset, peak)
+    d = l - l.max(1, keepdim=True).values
+    e = torch.exp(d)
+    s = e.sum(1)
+    p = e / s[:, None]
+    rel = (d.abs() + 2) * 2 * F
+    rs = (p * rel).sum(1) + torch.clamp(2 * (1 - 1 / s), max=80 * F)
+    for kind in ("index", "probs"):
+        if kind == "index":
+            target = t
+            want = torch.log(s) - d.gather(1, t[:, None])[:, 0]
+            bound = rs + 4 * F * want.abs()
+        else:
+            target = torch.zeros(n, v, device="cuda")
+            target[torch.arange(n), t] = 0.75
+            target[torch.arange(n), (t + 7) % v] += 0.25
+            want = torch.log(s) - (target.double() * d).sum(1)
+            bound = rs + 4 * F * torch.log(s) + 90 * F * (target.double() * d.abs()).sum(1)
+        ent = torch.log(s) - (p * d).sum(1)
+        b_ent = rs + (p * d.abs() * (rel + rs[:, None] + 90 * F)).sum(1) + 4 * F * ent
+        outs = [ops.linear_cross_entropy(x, w, target, b, reduction="none", return_entropy=True)]
+        one = ops.linear_cross_entropy_grad(x, w, target, b, reduction="none", return_entropy=True)
+        outs.append(one[:2])
+        for loss, entropy in outs:
+            assert float(loss.min()) >= 0 and float(entropy.min()) >= 0
+            assert bool(((loss.double() - want).abs() <= bound).all()), float(((loss.double() - want).abs() / bound.clamp_min(1e-300)).max())
+            assert bool(((entropy.double() - ent).abs() <= b_ent).all()), float(((entropy.double() - ent).abs() / b_ent.clamp_min(1e-300)).max())
