@@ -205,7 +205,10 @@ int make_plan(const azg_linear_ce_args *a, Plan *p)
     p->forward = a->loss != nullptr;
     p->backward = a->dx || a->dw || a->db;
     p->n = a->n; p->H = a->hidden; p->V = a->classes;
-    p->small = takes_small(p->split, p->backward, p->n, p->H, p->V);
+    // A forward pass whose stats are kept takes the path of the backward pass to come: the logits that are made again there have to
+    // be the same bits (every tile adds up k in one order), or a large logit's exponential leaves [0, 1].
+    const bool differentiable = p->backward || a->stats;
+    p->small = takes_small(p->split, differentiable, p->n, p->H, p->V);
     if (p->small) {
         Take t;
         p->logits = t((size_t)p->n * p->V * 4);
@@ -220,7 +223,7 @@ int make_plan(const azg_linear_ce_args *a, Plan *p)
     // (dW multiplies the rows that count for nothing by zero: they are copied as zeros, whatever they hold)
     p->pack_x = p->split || !aligned16(a->x, a->x_stride, a->hidden, a->n) || (a->dw && a->target);
     p->pack_w = p->split || !aligned16(a->w, a->w_stride, a->hidden, a->classes);
-    p->few = !p->backward && p->n <= 32 && p->pack_w;
+    p->few = !differentiable && p->n <= 32 && p->pack_w;
     if (p->few) p->pack_x = p->pack_w = false;
     // bytes a class of a piece costs
     long long cost = p->pack_w ? p->ldk * 2 : 0;
@@ -234,7 +237,7 @@ int make_plan(const azg_linear_ce_args *a, Plan *p)
     }
     p->keep = p->forward && p->backward && p->pieces == 1;
     p->ldd = image_stride(up_to(p->vp, p->ks) * p->per);
-    p->lshape = pick_logits(p->vp, p->n, p->backward);
+    p->lshape = pick_logits(p->vp, p->n, p->backward || p->split);   // (float32 has no tile for few rows)
     p->g = pick_grads(p->n, p->H, p->vp, (p->vp + p->ks - 1) / p->ks, (p->n + p->ks - 1) / p->ks, a->dx != nullptr, a->dw != nullptr);
     // rows a workgroup turns into D: up to 64, fewer while they would not give four workgroups a CU
     // (more for very many rows: db is joined from one sum a run of rows, one after the other)

@@ -55,6 +55,29 @@ def test_a_bad_target_reaches_blocked_classes_too(ops, dtype, n, h, v):
         assert bool(torch.isnan(dw).all()) and bool(torch.isnan(db).all())
 
 
+# ---------------------------------------------------------------- the two halves of the autograd form
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,h,v", PATHS + [(7, 100, 5003), (31, 257, 9001), (300, 130, 2050), (2000, 64, 100), (700, 300, 3000)])
+def test_a_backward_pass_by_itself_makes_the_same_logits(ops, dtype, n, h, v):
+    """Logits of some 1e4 (half precision) to 1e7 with gaps of many times their rounding: a row has one class, so d_hidden is
+    the difference of two classes' weights, off by two roundings of the type -- if the backward pass sees the logits that the
+    forward pass took its maximum from."""
+    x, w, b, t = make(n, h, v, dtype, "index", bias=False, seed=n + h + v)
+    x *= 2.0 ** (12 if dtype == "f16" else 20)
+    l = x.double() @ w.double().t()
+    two = l.topk(2, 1)
+    slack = 4 * ((h + 2) * F + 3 * 2.0 ** -22) * (x.double().abs() @ w.double().abs().t()).max(1).values
+    clear = two.values[:, 0] - two.values[:, 1] > slack + 200       # (the other rows may fall on either side)
+    assert int(clear.sum()) > n // 2
+    want = w.double()[two.indices[:, 0]] - w.double()[t]
+    bound = 2 * half_step(DT[dtype]) * want.abs() + 4 * F * (w.double()[two.indices[:, 0]].abs() + w.double()[t].abs())
+    xl = x.clone().requires_grad_()
+    ops.linear_cross_entropy(xl, w, t, reduction="sum").backward()
+    one = ops.linear_cross_entropy_grad(x, w, t, reduction="sum")
+    for got in (xl.grad, one.d_hidden):
+        assert bool(((got.double() - want).abs() <= bound)[clear].all())
+
+
 # ---------------------------------------------------------------- rows that are certain, logits with a common offset
 def exact_logits(n, h, v, dtype, offset, peak, seed=3):
     """Rows of one 1 each, so that logits are weights and a bias: multiples of 1/8, at most 8 in magnitude, the same in every type
