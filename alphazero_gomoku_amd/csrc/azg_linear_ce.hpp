@@ -16,11 +16,14 @@
 // contiguous: what runs against the sum is transposed on its way from LDS to the registers.  Operands that the loads
 // cannot take (float32, odd sizes or alignments) and rows that must read as zero are copied once into an "image".
 //
-// float32 runs on the 16-bit matrix cores too: x 2^s = hi + lo with hi, lo in half precision (s a power of two
-// from the tensor's largest magnitude, so that nothing overflows and what underflows is 2^-38 of the largest
-// element), and a product takes three instructions, hi hi + hi lo + lo hi.  hi carries 11 bits and lo 11 more, so
-// an operand is off by at most 2^-22 of itself and the dropped lo lo is at most 2^-22 of the product; sums are
-// float32.  An image row holds blocks of 64: 32 hi, then the 32 lo of the same columns.
+// float32 runs on the 16-bit matrix cores too: an element is the sum of three bfloat16 numbers, x = x0 + x1 + x2, each the
+// rounding of what the ones before it leave.  Eight bits a part and its sign hold all 24 bits of x, and every part has
+// float32's range of exponents, so nothing is scaled and what the other elements are does not matter.  A product of two
+// elements is the six products of parts i, j with i + j < 3; what is left out is at most 2^-24 of it (|x1| <= 2^-8 |x|,
+// |x2| <= 2^-17 |x|).  Gradients of half precision take two parts -- all of an operand's 11 bits; the gradient at the logits is
+// off by 2^-17 of itself -- and three products, which leave out 2^-16: half precision itself has not the range for
+// probabilities.  bfloat16 is one part.  An image row holds blocks of 64 columns, 64 elements of part 0, then of part 1, ...; a
+// product walks over the pairs of parts of one block of k and then over the blocks, every pair a stage of its own.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -33,13 +36,19 @@ typedef _Float16 hx8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bx8 __attribute__((ext_vector_type(8)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kDScale = 16384.0f;      // images of D hold D 2^14: |D| <= 2 then ends below half precision's 65504 and
-                                         // probabilities down to 2^-28 keep all their bits
 
-// Operand element types: what an image holds and how many products a pair of image elements takes.
-struct OpF32 { using In = float; using Img = _Float16; static constexpr bool split = true; };
-struct OpF16 { using In = _Float16; using Img = _Float16; static constexpr bool split = false; };
-struct OpBF16 { using In = __bf16; using Img = __bf16; static constexpr bool split = false; };
+// What a product runs on: parts of an element and their type.
+template <typename T, int N> struct Parts {
+    using Img = T;
+    static constexpr int parts = N, pairs = N * (N + 1) / 2, block = 64 * N;
+    // part of either side in the q-th pair, largest products first: (0,0) (0,1) (1,0) (0,2) (1,1) (2,0)
+    static __device__ inline int of_a(int q) { return N == 1 ? 0 : 0x910 >> (2 * q) & 3; }
+    static __device__ inline int of_b(int q) { return N == 1 ? 0 : 0x184 >> (2 * q) & 3; }
+};
+// Operand element types, and what the logits' and the gradients' products run on.
+struct OpF32 { using In = float; using Logits = Parts<__bf16, 3>; using Grad = Parts<__bf16, 3>; };
+struct OpF16 { using In = _Float16; using Logits = Parts<_Float16, 1>; using Grad = Parts<__bf16, 2>; };
+struct OpBF16 { using In = __bf16; using Logits = Parts<__bf16, 1>; using Grad = Parts<__bf16, 1>; };
 
 __device__ __align__(256) unsigned char g_zero_page[256];
 
@@ -60,7 +69,7 @@ template <> struct Frag<__bf16> {
 // tiles for the logits, two workgroups a CU (the whole call 5 % slower there, scores of 2048 x 1024 x 50001 14 %), four waves with 128 x 128 each (the accumulators
 // spill into copies), stages of 32 k with longer rings, workgroups that keep their CU and walk over tiles (no overlap gained:
 // all waves reach their epilogue together).
-// TM x TN output tile, WM x WN waves, 16x16x32 matrix instructions, stages of 64 k (float32: 32).  Each operand has a ring
+// TM x TN output tile, WM x WN waves, 16x16x32 matrix instructions, stages of 64 k of a pair of parts.  Each operand has a ring
 // of stages in LDS, filled by loads that go from global memory straight there, 16 bytes a lane.
 //   k contiguous in memory: LDS rows are 128 bytes of one m, eight 16-byte chunks, chunk c of row r at c ^ (r & 7), so the
 //     sixteen rows of a fragment read (16 bytes a lane) spread over all banks;
@@ -72,7 +81,8 @@ struct Operand {
     const void *p;       // image, or the caller's 16-bit tensor
     long long ld;        // row stride, elements
     long long rows;      // rows that exist; past them: k contiguous - any row, the result is not stored; k across - zero
-    long long cols;      // elements of a row that exist (a multiple of 8); past them zero
+    long long cols;      // columns that exist (a multiple of 8); past them zero
+    int block;           // elements that 64 columns of all parts take
 };
 
 template <int TM, int TN, int WM, int WN>
@@ -93,32 +103,34 @@ typedef __attribute__((address_space(3))) sx4 *lds_sx4;
 
 // One operand of a tile: T rows of m, k contiguous (TR false) or across the rows (TR true).  `groups` of 1024 LDS bytes, one
 // load instruction of a wave each.
-template <typename Op, int T, bool TR>
+template <typename P, int T, bool TR>
 struct Side {
-    using V = typename Frag<typename Op::Img>::V;
-    static constexpr int ks = Op::split ? 32 : 64;                              // k of a stage
+    using V = typename Frag<typename P::Img>::V;
     static constexpr int groups = T / 8;
-    static constexpr int row_bytes = TR ? T * 128 / ks : 128, row_chunks = row_bytes / 16;
+    static constexpr int row_bytes = TR ? T * 2 : 128, row_chunks = row_bytes / 16;
+    static_assert(!TR || T % 64 == 0, "columns of an image come in blocks of 64");
 
     static __device__ inline int unit_swizzle(int k)
     {
         return row_bytes >= 256 ? (k & 3) | ((k >> 1) & 4) : ((k >> 1) & 1) | ((k >> 2) & 2);
     }
-    // where stage k0 begins in memory for a tile that starts at m0, and how far a stage is
-    static __device__ inline const char *base(const Operand &O, long long m0, int k0)
+    // where block kb of k begins in memory, part 0, for a tile that starts at m0, how far a block is, and a part
+    static __device__ inline const char *base(const Operand &O, long long m0, int kb)
     {
-        return static_cast<const char *>(O.p) + (TR ? (long long)k0 * ks * O.ld + m0 * (64 / ks) : m0 * O.ld + (long long)k0 * 64) * 2;
+        return static_cast<const char *>(O.p) + (TR ? (long long)kb * 64 * O.ld + (m0 >> 6) * O.block : m0 * O.ld + (long long)kb * O.block) * 2;
     }
-    static __device__ inline long long step(const Operand &O) { return TR ? O.ld * (ks * 2) : 128; }
-    // this lane's 16 bytes of group g: offset from the base and its k (TR: row of the stage, else image element).  What lies
-    // past the last m repeats the last one: it reaches only results that are not stored.
+    static __device__ inline long long step(const Operand &O) { return TR ? O.ld * 128 : O.block * 2; }
+    static constexpr int part_bytes = 128;
+    // this lane's 16 bytes of group g: offset from the base and its k.  What lies past the last m repeats the last one: it
+    // reaches only results that are not stored.
     static __device__ inline unsigned offset(const Operand &O, long long m0, int g, int lane, int *at)
     {
         const int c = g * 64 + lane, row = c / row_chunks, pos = c % row_chunks;
         if constexpr (TR) {
-            const long long col = m0 * (64 / ks) + (pos ^ (unit_swizzle(row) << 1)) * 8;
+            long long col = m0 + (pos ^ (unit_swizzle(row) << 1)) * 8;
+            if (col >= O.cols) col = O.cols - 8;
             *at = row;
-            return (unsigned)((row * O.ld + (col < O.cols ? col : O.cols - 8) - m0 * (64 / ks)) * 2);
+            return (unsigned)((row * O.ld + ((col >> 6) - (m0 >> 6)) * O.block + (col & 63)) * 2);
         } else {
             const long long last = O.rows - 1 - m0;
             *at = (pos ^ (row & 7)) * 8;
@@ -126,15 +138,13 @@ struct Side {
         }
     }
     static __device__ inline long long kcount(const Operand &O) { return TR ? O.rows : O.cols; }
-    static constexpr int kstep = TR ? ks : 64;
 
-    // fragment t (sixteen m), half h of the stage: float32 - h = 0 the hi, 1 the lo of the 32 k;  else k 32 h .. 32 h + 31
+    // fragment t (sixteen m), half h of the stage: k 32 h .. 32 h + 31
     static __device__ inline V read(const char *base, int lane, int t, int h)
     {
         if constexpr (TR) {
             const int g = lane >> 4, s = lane & 15, k = g * 8 + (s >> 2);
-            const int unit = Op::split ? (t >> 1) * 4 + (t & 1) + 2 * h : t;
-            const char *p = base + ((Op::split ? 0 : 32 * h) + k) * row_bytes + ((unit ^ unit_swizzle(k)) * 32) + (s & 3) * 8;
+            const char *p = base + (32 * h + k) * row_bytes + ((t ^ unit_swizzle(k)) * 32) + (s & 3) * 8;
             union { sx4 q[2]; V v; } u;
             u.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_sx4)p);
             u.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_sx4)(p + 4 * row_bytes));
@@ -145,12 +155,12 @@ struct Side {
     }
 };
 
-template <typename Op, int TM, int TN, int WM, int WN, bool TA, bool TB>
+template <typename P, int TM, int TN, int WM, int WN, bool TA, bool TB>
 struct TileProduct {
     using S = TileShape<TM, TN, WM, WN>;
-    using F = Frag<typename Op::Img>;
-    using A_ = Side<Op, TM, TA>;
-    using B_ = Side<Op, TN, TB>;
+    using F = Frag<typename P::Img>;
+    using A_ = Side<P, TM, TA>;
+    using B_ = Side<P, TN, TB>;
     static constexpr int kLoadsA = A_::groups / S::waves, kLoadsB = B_::groups / S::waves, kLoads = kLoadsA + kLoadsB;
     static constexpr int MH = S::MT / 2, RA = TA ? 2 : 1, RB = TB ? 2 : 1;       // LDS reads a fragment
     static_assert(A_::groups % S::waves == 0 && B_::groups % S::waves == 0, "every wave issues the same loads");
@@ -199,8 +209,8 @@ struct TileProduct {
     }
 
     // acc[mt][nt][i]: row wm*(TM/WM) + 16 mt + 4 (lane >> 4) + i of A, row wn*(TN/WN) + 16 nt + (lane & 15) of B.
-    // Stages k0 .. k1 - 1 of ktotal.  A stage has four phases, each with half of A's fragments of one kind (half of k;
-    // float32: hi or lo); a phase reads the next one's fragments from LDS behind its own matrix instructions.  In front of
+    // Stages k0 .. k1 - 1 of ktotal, P::pairs of them a block of 64 k.  A stage has four phases, each with half of A's fragments
+    // of half of its k; a phase reads the next one's fragments from LDS behind its own matrix instructions.  In front of
     // the fourth phase the waves meet: all hold the rest of the stage in registers, the next stage has arrived, and the
     // places of this one are free.  They are refilled a few loads at a time -- B's during the fourth and the next stage's
     // first phase, A's, whose ring is longer, during the two phases after that -- because a burst of loads holds up the
@@ -217,10 +227,11 @@ struct TileProduct {
         for (int i = 0; i < kLoadsA; i++) off_a[i] = A_::offset(A, m0, i * S::waves + wave, lane, &at_a[i]);
 #pragma unroll
         for (int i = 0; i < kLoadsB; i++) off_b[i] = B_::offset(B, n0, i * S::waves + wave, lane, &at_b[i]);
-        // next stage to load of either side: its place in memory and in the ring
-        const char *base_a = A_::base(A, m0, k0), *base_b = B_::base(B, n0, k0);
+        // next stage to load of either side: its block, its pair of parts, its place in memory and in the ring
+        const char *block_a = A_::base(A, m0, k0 / P::pairs), *block_b = B_::base(B, n0, k0 / P::pairs);
         const long long step_a = A_::step(A), step_b = B_::step(B);
-        int la = k0, lb = k0, slot_a = 0, slot_b = 0;
+        int la = k0, lb = k0, qa = k0 % P::pairs, qb = qa, slot_a = 0, slot_b = 0;
+        const char *base_a = block_a + P::of_a(qa) * A_::part_bytes, *base_b = block_b + P::of_b(qb) * B_::part_bytes;
         char *lds_b = lds + S::ring_a * S::bytes_a;
         const unsigned lds0 = (unsigned)(uintptr_t)(lds_ptr)lds + wave * 1024;
         // load i of the next stage
@@ -228,7 +239,8 @@ struct TileProduct {
             if constexpr (side_a.value) load_lds(base_a, off_a[i], lds0 + slot_a * S::bytes_a + i * S::waves * 1024);
             else load_lds(base_b, off_b[i], lds0 + S::ring_a * S::bytes_a + slot_b * S::bytes_b + i * S::waves * 1024);
         };
-        // a whole stage; the last stage of k has zeros past its end
+        // a whole stage; the stages of the last block have zeros past the end of k
+        const int last_block = (ktotal / P::pairs - 1) * 64;
         auto load_stage = [&](auto side_a, bool last) {
             constexpr bool a_side = side_a.value;
             constexpr int loads = a_side ? kLoadsA : kLoadsB;
@@ -238,7 +250,7 @@ struct TileProduct {
             } else {
                 const char *base = a_side ? base_a : base_b;
                 const unsigned to = lds0 + (a_side ? slot_a * S::bytes_a : S::ring_a * S::bytes_a + slot_b * S::bytes_b);
-                const long long left = a_side ? A_::kcount(A) - (long long)la * A_::kstep : B_::kcount(B) - (long long)lb * B_::kstep;
+                const long long left = (a_side ? A_::kcount(A) : B_::kcount(B)) - last_block;
 #pragma unroll
                 for (int i = 0; i < loads; i++) {
                     const char *p = base + (a_side ? off_a[i] : off_b[i]);
@@ -249,10 +261,20 @@ struct TileProduct {
         };
         constexpr std::true_type side_a{};
         constexpr std::false_type side_b{};
-        auto next_a = [&]() { base_a += step_a; la++; slot_a = slot_a + 1 == S::ring_a ? 0 : slot_a + 1; };
-        auto next_b = [&]() { base_b += step_b; lb++; slot_b = slot_b + 1 == S::ring_b ? 0 : slot_b + 1; };
-        auto whole_a = [&](int before) { if (la < min(k1, before)) { load_stage(side_a, la + 1 == ktotal); next_a(); } };
-        auto whole_b = [&](int before) { if (lb < min(k1, before)) { load_stage(side_b, lb + 1 == ktotal); next_b(); } };
+        auto next_a = [&]() {
+            la++;
+            if (++qa == P::pairs) { qa = 0; block_a += step_a; }
+            base_a = block_a + P::of_a(qa) * A_::part_bytes;
+            slot_a = slot_a + 1 == S::ring_a ? 0 : slot_a + 1;
+        };
+        auto next_b = [&]() {
+            lb++;
+            if (++qb == P::pairs) { qb = 0; block_b += step_b; }
+            base_b = block_b + P::of_b(qb) * B_::part_bytes;
+            slot_b = slot_b + 1 == S::ring_b ? 0 : slot_b + 1;
+        };
+        auto whole_a = [&](int before) { if (la < min(k1, before)) { load_stage(side_a, la + P::pairs >= ktotal); next_a(); } };
+        auto whole_b = [&](int before) { if (lb < min(k1, before)) { load_stage(side_b, lb + P::pairs >= ktotal); next_b(); } };
         // a wave's part of a side begins a whole number of rows or 32-byte units into it
         const int oa = TA ? 0 : wm * (TM / WM) * 128, ob = TB ? 0 : wn * (TN / WN) * 128;
         const int ta = TA ? wm * S::MT : 0, tb = TB ? wn * S::NT : 0;
@@ -261,9 +283,8 @@ struct TileProduct {
         // fragments of phase p of a stage
         auto read_a = [&](int slot, int p) {
             const char *pa = lds + slot * S::bytes_a + oa;
-            const int h = Op::split ? p & 1 : p >> 1, half = Op::split ? p >> 1 : p & 1;
 #pragma unroll
-            for (int t = 0; t < MH; t++) a[p & 1][t] = A_::read(pa, lane, ta + half * MH + t, h);
+            for (int t = 0; t < MH; t++) a[p & 1][t] = A_::read(pa, lane, ta + (p & 1) * MH + t, p >> 1);
         };
         auto read_b = [&](typename F::V (&to)[S::NT], int slot, int h) {
             const char *pb = lds_b + slot * S::bytes_b + ob;
@@ -271,9 +292,9 @@ struct TileProduct {
             for (int t = 0; t < S::NT; t++) to[t] = B_::read(pb, lane, tb + t, h);
         };
         constexpr int PP = MH * S::NT;
-        // matrix instructions i0 .. i1 - 1 of phase p's A fragments and B's fragments h
-        auto products = [&](int p, int h, int i0, int i1) {
-            const int half = Op::split ? p >> 1 : p & 1;
+        // matrix instructions i0 .. i1 - 1 of phase p
+        auto products = [&](int p, int i0, int i1) {
+            const int half = p & 1, h = p >> 1;
 #pragma unroll
             for (int mt = 0; mt < MH; mt++)
 #pragma unroll
@@ -281,19 +302,17 @@ struct TileProduct {
                     if (mt * S::NT + nt >= i0 && mt * S::NT + nt < i1)
                         acc[half * MH + mt][nt] = F::mfma(a[p & 1][mt], b[h][nt], acc[half * MH + mt][nt]);
         };
-        // phase p's matrix instructions (with B's fragments h; float32, even phases: h = 1, then 0) behind its `reads` LDS reads,
-        // with loads l0 .. l1 - 1 of the next stage of a side near their end
-        auto phase = [&](int p, int h, auto reads, auto both, auto side, auto l0, auto l1) {
-            constexpr int loads = l1.value - l0.value, per = loads ? loads : 1, tail = PP - 2 * loads > 0 ? PP - 2 * loads : 0, total = both.value ? PP + tail : tail;
-            if constexpr (both.value) { products(p, 1, 0, PP); products(p, 0, 0, tail); }
-            else products(p, h, 0, tail);
-            interleave<total, reads.value>();
+        // phase p's matrix instructions behind its `reads` LDS reads, with loads l0 .. l1 - 1 of the next stage of a side near their end
+        auto phase = [&](int p, auto reads, auto side, auto l0, auto l1) {
+            constexpr int loads = l1.value - l0.value, per = loads ? loads : 1, tail = PP - 2 * loads > 0 ? PP - 2 * loads : 0;
+            products(p, 0, tail);
+            interleave<tail, reads.value>();
 #pragma unroll
             for (int i = 0; i < loads; i++) {
                 __builtin_amdgcn_sched_barrier(0);
                 load(side, l0.value + i);
                 __builtin_amdgcn_sched_barrier(0);
-                products(p, both.value ? 0 : h, tail + (PP - tail) * i / per, tail + (PP - tail) * (i + 1) / per);
+                products(p, tail + (PP - tail) * i / per, tail + (PP - tail) * (i + 1) / per);
             }
             phase_end();
         };
@@ -307,7 +326,7 @@ struct TileProduct {
         }
         if (k1 - k0 >= S::ring_a) meet<(S::ring_a - 1) * kLoadsA + (S::ring_b - 1) * kLoadsB>();
         else meet<0>();
-        read_b(b[Op::split], 0, Op::split);
+        read_b(b[0], 0, 0);
         read_a(0, 0);
         int kt = k0;
         constexpr int B1 = kLoadsB / 2, A1 = kLoadsA / 2;
@@ -319,43 +338,27 @@ struct TileProduct {
         auto stage = [&](auto fast_, auto full_) {            // fast: with the loads of a steady state; full: the rings are
             constexpr bool fast = fast_.value, full = full_.value;
             const int sa = ra + 1 == S::ring_a ? 0 : ra + 1, sb = rb + 1 == S::ring_b ? 0 : rb + 1;
-            if constexpr (Op::split) {                        // (hi lo, hi hi), (lo hi) for either half of A; B's hi arrives behind the first
-                read_b(b[0], rb, 0);
-                read_a(ra, 1);
-                phase(0, 0, AZG_INT(MH * RA + S::NT * RB), yes, side_b, AZG_INT(B1), AZG_INT(fast ? kLoadsB : B1));
-                if (fast) next_b();
-                read_a(ra, 2);
-                phase(1, 0, AZG_INT(MH * RA), no, side_a, AZG_INT(0), AZG_INT(fast ? A1 : 0));
-                read_a(ra, 3);
-                phase(2, 0, AZG_INT(MH * RA), yes, side_a, AZG_INT(A1), AZG_INT(fast ? kLoadsA : A1));
-            } else {
-                read_a(ra, 1);
-                phase(0, 0, AZG_INT(MH * RA), no, side_b, AZG_INT(B1), AZG_INT(fast ? kLoadsB : B1));
-                if (fast) next_b();
-                read_a(ra, 2);
-                read_b(b[1], rb, 1);
-                phase(1, 0, AZG_INT(MH * RA + S::NT * RB), no, side_a, AZG_INT(0), AZG_INT(fast ? A1 : 0));
-                read_a(ra, 3);
-                phase(2, 1, AZG_INT(MH * RA), no, side_a, AZG_INT(A1), AZG_INT(fast ? kLoadsA : A1));
-            }
+            read_a(ra, 1);
+            phase(0, AZG_INT(MH * RA), side_b, AZG_INT(B1), AZG_INT(fast ? kLoadsB : B1));
+            if (fast) next_b();
+            read_a(ra, 2);
+            read_b(b[1], rb, 1);
+            phase(1, AZG_INT(MH * RA + S::NT * RB), side_a, AZG_INT(0), AZG_INT(fast ? A1 : 0));
+            read_a(ra, 3);
+            phase(2, AZG_INT(MH * RA), side_a, AZG_INT(A1), AZG_INT(fast ? kLoadsA : A1));
             if (fast) next_a();
             meet<full ? newer : 0>();
             // (after the last stage what is read is stale and not used)
             read_a(sa, 0);
-            if constexpr (Op::split) {
-                read_b(b[1], sb, 1);
-                phase(3, 0, AZG_INT(MH * RA + S::NT * RB), no, side_b, AZG_INT(0), AZG_INT(fast ? B1 : 0));
-            } else {
-                read_b(b[0], sb, 0);
-                phase(3, 1, AZG_INT(MH * RA + S::NT * RB), no, side_b, AZG_INT(0), AZG_INT(fast ? B1 : 0));
-            }
+            read_b(b[0], sb, 0);
+            phase(3, AZG_INT(MH * RA + S::NT * RB), side_b, AZG_INT(0), AZG_INT(fast ? B1 : 0));
             ra = sa; rb = sb;
             kt++;
         };
         // The fast loop's stage kt issues the rest of B's stage kt - 1 + ring_b, all of A's kt - 1 + ring_a and the first part of
         // B's kt + ring_b; around it: the first stage's loads in one go, whole stages, and the rest of a begun one.
-        const bool tail = k1 == ktotal && (A_::kcount(A) % A_::kstep != 0 || B_::kcount(B) % B_::kstep != 0);
-        const int end = k1 - (tail ? 1 : 0), fast_end = min(end - S::ring_a + 1, end - S::ring_b);
+        const bool tail = A_::kcount(A) % 64 != 0 || B_::kcount(B) % 64 != 0;
+        const int end = tail ? min(k1, ktotal - P::pairs) : k1, fast_end = min(end - S::ring_a + 1, end - S::ring_b);
         if (kt + 1 < fast_end) {
             stage(no, yes);
 #pragma unroll
@@ -401,105 +404,69 @@ struct PackArgs {
     const void *src;              // [rows][cols], stride ld
     long long ld, rows, cols;
     void *img;                    // [rows][ldi]
-    long long ldi, icols;         // row stride, padded columns (image elements)
+    long long ldi, icols;         // row stride (image elements), padded columns
+    int parts;                    // 1: elements as they are; else bfloat16 parts
     const long long *target;      // not null: rows whose target is ignore_index are read as zero
     long long ignore;
-    float *maxpart;               // float32: kMaxParts partial maxima of the tensor
+    unsigned wgs;                 // workgroups of this one
 };
-constexpr int kMaxParts = 256;
+struct PackList { PackArgs p[4]; };
 
-// power of two that brings the largest magnitude into [2^13, 2^14); 1 for an all-zero tensor
-__device__ inline float split_scale(float mx)
+// N bfloat16 parts of x: part[i] is the rounding of x - part[0] - ... - part[i - 1], exact in float32.  What would round to
+// infinity takes the largest finite number; infinities and NaN are part 0.
+template <int N>
+__device__ inline void split_parts(float x, __bf16 (&part)[N])
 {
-    if (!(mx > 0.f)) return 1.f;
-    int e = 14 - (int)((__builtin_bit_cast(uint32_t, mx) >> 23) & 255) + 126;    // mx = f 2^(E-126), f in [1/2, 1)
-    e = e > 126 ? 126 : (e < -126 ? -126 : e);
-    return __builtin_bit_cast(float, (uint32_t)((e + 127) << 23));
-}
-__device__ inline float max_of_parts(const float *parts)                        // every thread of a wave calls it
-{
-    const int lane = threadIdx.x & 63;
-    float m = 0.f;
+    constexpr float top = 3.3895313892515355e38f;             // (2 - 2^-7) 2^127
 #pragma unroll
-    for (int i = 0; i < kMaxParts / 64; i++) m = fmaxf(m, parts[i * 64 + lane]);
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
-    return m;
-}
-
-// Partial maxima of the finite magnitudes of two float32 tensors (rows whose target is ignore_index left out), kMaxParts
-// workgroups each.  Bound by memory: 139 MB in 30 us, 4.7 TB/s.
-__global__ __launch_bounds__(512) void absmax_kernel(PackArgs a0, PackArgs a1)
-{
-    __shared__ float red[8];
-    const PackArgs a = blockIdx.x < kMaxParts ? a0 : a1;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const unsigned wg = blockIdx.x % kMaxParts;
-    const float *src = static_cast<const float *>(a.src);
-    float m = 0.f;
-    auto take = [&](float v) { v = fabsf(v); m = v < INFINITY ? fmaxf(m, v) : m; };
-    for (long long row = wg * 8 + wave; row < a.rows; row += kMaxParts * 8) {
-        if (a.target && a.target[row] == a.ignore) continue;
-        const float *p = src + row * a.ld;
-        const long long whole = a.cols / 4 * 4;
-#pragma unroll 4
-        for (long long c = lane * 4; c < whole; c += 256) {
-            const Pack<float, 4> v = *reinterpret_cast<const Pack<float, 4> *>(p + c);
-#pragma unroll
-            for (int q = 0; q < 4; q++) take(v.v[q]);
-        }
-        if (whole + lane < a.cols) take(p[whole + lane]);
-    }
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
-    if (lane == 0) red[wave] = m;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < 8; w++) m = fmaxf(m, red[w]);
-        a.maxpart[wg] = m;
+    for (int i = 0; i < N; i++) {
+        __bf16 h = (__bf16)x;
+        if (i == 0 && fabsf(x) < INFINITY && fabsf((float)h) == INFINITY) h = (__bf16)copysignf(top, x);
+        part[i] = h;
+        x = fabsf(x) < INFINITY ? x - (float)h : 0.f;
     }
 }
 
-// The images of two matrices, zeros in the padding: a thread eight columns of a row; the first matrix has wgs0 workgroups.
-// Bound by memory: 139 MB of float32 read and written in 48 us, 5.8 TB/s.
-template <typename Op>
-__global__ __launch_bounds__(256) void pack_kernel(PackArgs a0, PackArgs a1, unsigned wgs0)
+// Images of up to four matrices, zeros in the padding: a thread eight columns of a row.
+template <typename In>
+__global__ __launch_bounds__(256) void pack_kernel(PackList list)
 {
-    constexpr int per = Op::split ? 2 : 1;
-    const bool first = blockIdx.x < wgs0;
-    const PackArgs a = first ? a0 : a1;
-    const unsigned wg = first ? blockIdx.x : blockIdx.x - wgs0, wgs = first ? wgs0 : gridDim.x - wgs0;
-    const float scale = Op::split ? split_scale(max_of_parts(a.maxpart)) : 1.f;
-    const long long row_chunks = a.icols / (8 * per), total = a.rows * row_chunks;
-    for (long long i = (long long)wg * 256 + threadIdx.x; i < total; i += (long long)wgs * 256) {
+    unsigned wg = blockIdx.x;
+    int which = 0;
+    while (wg >= list.p[which].wgs) wg -= list.p[which++].wgs;
+    const PackArgs a = list.p[which];
+    const long long row_chunks = a.icols / 8, total = a.rows * row_chunks;
+    for (long long i = (long long)wg * 256 + threadIdx.x; i < total; i += (long long)a.wgs * 256) {
         const long long r = i / row_chunks, c = (i - r * row_chunks) * 8;
-        const typename Op::In *p = static_cast<const typename Op::In *>(a.src) + r * a.ld + c;
+        const In *p = static_cast<const In *>(a.src) + r * a.ld + c;
         const bool skip = a.target && a.target[r] == a.ignore;
-        typename Op::In v[8];
+        In v[8];
         if (!skip && c + 8 <= a.cols) {
-            *reinterpret_cast<Pack<typename Op::In, 8> *>(v) = *reinterpret_cast<const Pack<typename Op::In, 8> *>(p);
+            *reinterpret_cast<Pack<In, 8> *>(v) = *reinterpret_cast<const Pack<In, 8> *>(p);
         } else {
 #pragma unroll
             for (int q = 0; q < 8; q++) {
-                v[q] = (typename Op::In)0.f;
+                v[q] = (In)0.f;
                 if (!skip && c + q < a.cols) v[q] = p[q];
             }
         }
-        typename Op::Img *o = static_cast<typename Op::Img *>(a.img) + r * a.ldi;
-        if constexpr (Op::split) {
-            hx8 hi, lo;
+        auto in_parts = [&](auto n) {
+            constexpr int N = decltype(n)::value;
+            __bf16 *o = static_cast<__bf16 *>(a.img) + r * a.ldi + (c >> 6) * (64 * N) + (c & 63);
+            bx8 h[N];
 #pragma unroll
             for (int q = 0; q < 8; q++) {
-                const float x = v[q] * scale;
-                hi[q] = (_Float16)x;
-                lo[q] = fabsf((float)hi[q]) < INFINITY ? (_Float16)(x - (float)hi[q]) : (_Float16)0.f;
+                __bf16 part[N];
+                split_parts<N>((float)v[q], part);
+#pragma unroll
+                for (int k = 0; k < N; k++) h[k][q] = part[k];
             }
-            o += (c >> 5) * 64 + (c & 31);
-            *reinterpret_cast<hx8 *>(o) = hi;
-            *reinterpret_cast<hx8 *>(o + 32) = lo;
-        } else {
-            *reinterpret_cast<Pack<typename Op::In, 8> *>(o + c) = *reinterpret_cast<const Pack<typename Op::In, 8> *>(v);
-        }
+#pragma unroll
+            for (int k = 0; k < N; k++) *reinterpret_cast<bx8 *>(o + k * 64) = h[k];
+        };
+        if constexpr (sizeof(In) == 4) in_parts(std::integral_constant<int, 3>{});
+        else if (a.parts == 2) in_parts(std::integral_constant<int, 2>{});
+        else *reinterpret_cast<Pack<In, 8> *>(static_cast<In *>(a.img) + r * a.ldi + c) = *reinterpret_cast<const Pack<In, 8> *>(v);
     }
 }
 
@@ -509,7 +476,6 @@ struct CeArgs {
     int ktiles, mtiles, ntiles, mtiles_behind;
     long long n, classes, v0;     // classes of this piece; v0 = first class of the piece
     const void *bias;             // this piece's, operand type, or null
-    const float *xmax, *wmax;     // float32: partial maxima
     const long long *target;
     long long ignore;
     const float *probs;           // [n][ldp], already offset to the piece's first class
@@ -517,7 +483,7 @@ struct CeArgs {
     // statistics, one entry a row and a wave's run of TM / WM classes ("span")
     float2 *part;                 // [spans][n]: maximum m, sum of exp(l - m)
     float *part_e;                // [spans][n]: sum of exp(l - m) (l - m), or null
-    float4 *part_t;               // probabilities: sum pi (l - m), sum pi, sum |pi|, -
+    float2 *part_t;               // probabilities: sum pi (l - m), sum pi
     float *tlogit;                // index: [n]
     // gradient
     const float4 *stats;          // [n]: m, sum pi / s, ... (RowArgs)
@@ -540,9 +506,14 @@ __device__ inline Pack<float, 4> four_of(const float *row, long long v, long lon
 }
 
 // exp(l - the span's maximum) on its way to becoming D in the same place: half precision (11 bits; what lies below 2^-24 of
-// the span's largest probability is off by 2^-25 of that) where D will be 16 bits, float32 where D will be two halves
-template <typename Op> struct Expo { using T = _Float16; };
-template <> struct Expo<OpF32> { using T = float; };
+// the span's largest probability is off by 2^-25 of that) where D will be 16 bits, float32 where D will be parts
+template <typename Op> using Expo = std::conditional_t<Op::Grad::parts == 1, _Float16, float>;
+// where the image of D (the exponentials on their way there: counted in their own size) holds column c
+template <typename Op, typename T>
+__device__ inline T *place(void *d, long long row, long long ldd, long long c)
+{
+    return reinterpret_cast<T *>(static_cast<uint16_t *>(d) + row * ldd + (c >> 6) * Op::Grad::block) + (c & 63);
+}
 
 // A tile of logits; a lane holds four classes of a row next to each other (classes are the tile's m), sixteen rows a fragment.
 // Forward (GRAD false): span statistics and, where asked for, the exponentials; GRAD: D from the rows' statistics.  A 256 x 256
@@ -560,15 +531,14 @@ __device__ inline void logits_tile(const CeArgs &a, long long m_first, int span_
     for (int i = 0; i < S::MT; i++)
 #pragma unroll
         for (int j = 0; j < S::NT; j++) acc[i][j] = fx4{0.f, 0.f, 0.f, 0.f};
-    TileProduct<Op, TM, TN, WM, WN, false, false>::run(acc, a.w, m0, a.x, n0, 0, a.ktiles, a.ktiles, lds);
+    TileProduct<typename Op::Logits, TM, TN, WM, WN, false, false>::run(acc, a.w, m0, a.x, n0, 0, a.ktiles, a.ktiles, lds);
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
-    const float ux = Op::split ? 1.f / split_scale(max_of_parts(a.xmax)) : 1.f, uw = Op::split ? 1.f / split_scale(max_of_parts(a.wmax)) : 1.f;
     const typename Op::In *bias = static_cast<const typename Op::In *>(a.bias);
     const long long vw = m0 + wm * (TM / WM) + 4 * (lane >> 4);                  // this lane's first class of the piece
     // (what the rows and classes bring along is loaded in one go: each load by itself would cost its latency)
     const bool whole = m0 + TM <= a.classes;
-    if (Op::split || bias || !whole) {
+    if (bias || !whole) {
         typename Op::In bv[S::MT][4];
         if (bias && whole) {
 #pragma unroll
@@ -585,7 +555,7 @@ __device__ inline void logits_tile(const CeArgs &a, long long m_first, int span_
             for (int i = 0; i < 4; i++) {
                 const float b = bias ? (float)bv[mt][i] : 0.f;
 #pragma unroll
-                for (int nt = 0; nt < S::NT; nt++) acc[mt][nt][i] = Op::split ? acc[mt][nt][i] * ux * uw + b : acc[mt][nt][i] + b;
+                for (int nt = 0; nt < S::NT; nt++) acc[mt][nt][i] += b;
             }
         if (!whole)
 #pragma unroll
@@ -611,7 +581,7 @@ __device__ inline void logits_tile(const CeArgs &a, long long m_first, int span_
     }
     if constexpr (!GRAD) {
         // per row: maximum and sum over the span; lanes 16 and 32 apart share a row
-        using E = typename Expo<Op>::T;
+        using E = Expo<Op>;
 #pragma unroll
         for (int nt = 0; nt < S::NT; nt++) {
             const long long row = nw + nt * 16;
@@ -627,7 +597,7 @@ __device__ inline void logits_tile(const CeArgs &a, long long m_first, int span_
             // least 1, a loss and an entropy at least 0, and neither loses bits to an offset that all logits share.
             // (A NaN is passed over by fmaxf: it comes back through the sum; a maximum of -inf leaves every term 2^-inf.)
             const float base = mx == -INFINITY ? 0.f : mx;
-            float s = 0.f, e = 0.f, tl = 0.f, ts = 0.f, ta = 0.f;
+            float s = 0.f, e = 0.f, tl = 0.f, ts = 0.f;
             if (a.part_e)
 #pragma unroll
                 for (int mt = 0; mt < S::MT; mt++)
@@ -645,7 +615,7 @@ __device__ inline void logits_tile(const CeArgs &a, long long m_first, int span_
                     s += x;
                     keep.v[i] = (E)x;
                 }
-                if (a.d && live && vw + mt * 16 < dpad) *reinterpret_cast<Pack<E, 4> *>(static_cast<E *>(a.d) + row * (a.ldd / (Op::split ? 2 : 1)) + vw + mt * 16) = keep;
+                if (a.d && live && vw + mt * 16 < dpad) *reinterpret_cast<Pack<E, 4> *>(place<Op, E>(a.d, row, a.ldd, vw + mt * 16)) = keep;
             }
             if (a.probs) {
                 const float *pr = a.probs + min(row, a.n - 1) * a.ldp;
@@ -657,7 +627,7 @@ __device__ inline void logits_tile(const CeArgs &a, long long m_first, int span_
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const float p = pv[mt].v[i];
-                        ts += p; ta += fabsf(p);
+                        ts += p;
                         tl += p != 0.f ? p * (acc[mt][nt][i] - base) : 0.f;
                     }
             }
@@ -673,17 +643,17 @@ __device__ inline void logits_tile(const CeArgs &a, long long m_first, int span_
 #define AZG_PAIR(v) v += __shfl_xor(v, 16, 64); v += __shfl_xor(v, 32, 64)
             AZG_PAIR(s);
             if (a.part_e) { AZG_PAIR(e); }
-            if (a.probs) { AZG_PAIR(tl); AZG_PAIR(ts); AZG_PAIR(ta); }
+            if (a.probs) { AZG_PAIR(tl); AZG_PAIR(ts); }
 #undef AZG_PAIR
             if (lane < 16 && live) {
                 const long long at = (span_first + (long long)tm * WM + wm) * a.n + row;
                 a.part[at] = make_float2(mx, s);
                 if (a.part_e) a.part_e[at] = e;
-                if (a.probs) a.part_t[at] = make_float4(tl, ts, ta, 0.f);
+                if (a.probs) a.part_t[at] = make_float2(tl, ts);
             }
         }
     } else {
-        typename Op::Img *d = static_cast<typename Op::Img *>(a.d);
+        using Img = typename Op::Grad::Img;
         float db[S::MT][4], gs[S::NT];
         float2 sts[S::NT];
 #pragma unroll
@@ -706,7 +676,8 @@ __device__ inline void logits_tile(const CeArgs &a, long long m_first, int span_
             const float *pr = a.probs ? a.probs + min(row, a.n - 1) * a.ldp : nullptr;
 #pragma unroll
             for (int mt = 0; mt < S::MT; mt++) {
-                Pack<typename Op::Img, 4> h, l;
+                constexpr int N = Op::Grad::parts;
+                Pack<Img, 4> h[N];
                 const long long cls = vw + mt * 16;
                 Pack<float, 4> pv;
                 if (pr) pv = four_of(pr, cls, a.classes, whole);
@@ -717,14 +688,13 @@ __device__ inline void logits_tile(const CeArgs &a, long long m_first, int span_
                     else if (t == mt * 16 + i) q -= 1.f;
                     q = g == 0.f || cls + i >= a.classes ? 0.f : q * g;         // a row that counts for nothing: zero whatever it holds
                     db[mt][i] += q;
-                    q *= kDScale;
-                    h.v[i] = (typename Op::Img)q;
-                    if (Op::split) l.v[i] = (typename Op::Img)(q - (float)h.v[i]);
+#pragma unroll
+                    for (int k = 0; k < N; k++) { h[k].v[i] = (Img)q; q -= (float)h[k].v[i]; }
                 }
-                if (d && live && cls < dpad) {
-                    typename Op::Img *o = d + row * a.ldd + (Op::split ? (cls >> 5) * 64 + (cls & 31) : cls);
-                    *reinterpret_cast<Pack<typename Op::Img, 4> *>(o) = h;
-                    if (Op::split) *reinterpret_cast<Pack<typename Op::Img, 4> *>(o + 32) = l;
+                if (a.d && live && cls < dpad) {
+                    Img *o = place<Op, Img>(a.d, row, a.ldd, cls);
+#pragma unroll
+                    for (int k = 0; k < N; k++) *reinterpret_cast<Pack<Img, 4> *>(o + k * 64) = h[k];
                 }
             }
         }
@@ -771,10 +741,10 @@ __global__ __launch_bounds__(512) void logits_mixed_kernel(CeArgs a)
 struct RowArgs {
     long long n, classes;
     int spans;
-    const float2 *part; const float *part_e; const float4 *part_t; const float *tlogit;
+    const float2 *part; const float *part_e; const float2 *part_t; const float *tlogit;
     const long long *target; long long ignore;
     float *loss_out, *ent_out;    // [n], or null: rows' results that nothing else has to be added to
-    float4 *stats;                // [n]: m, sum pi / s, sum |pi|, loss with lse = m + log s (so that p takes no rounding of lse)
+    float4 *stats;                // [n]: m, sum pi / s, 0, loss with lse = m + log s (so that p takes no rounding of lse)
     float *ent;                   // [n] or null
 };
 // One wave per row: join the spans' sums, each relative to its span's maximum m_j, in a fixed order; relative to m they are
@@ -792,20 +762,20 @@ __global__ __launch_bounds__(256) void rows_kernel(RowArgs a)
     const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     if (row >= a.n) return;
-    float mx = -INFINITY, s = 0.f, e = 0.f, tl = 0.f, ts = 0.f, ta = 0.f;
+    float mx = -INFINITY, s = 0.f, e = 0.f, tl = 0.f, ts = 0.f;
     // four spans a lane at a time: their maximum first, so that the loads do not wait for the sums
     for (int t0 = lane; t0 < a.spans; t0 += 256) {
         float2 p[4];
         float q[4];
-        float4 u[4];
+        float2 u[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const bool in = t0 + 64 * j < a.spans;
             const long long at = (long long)(in ? t0 + 64 * j : t0) * a.n + row;
             p[j] = a.part[at];
             q[j] = a.part_e ? a.part_e[at] : 0.f;
-            u[j] = a.part_t ? a.part_t[at] : make_float4(0.f, 0.f, 0.f, 0.f);
-            if (!in) { p[j] = make_float2(-INFINITY, 0.f); q[j] = 0.f; u[j] = make_float4(0.f, 0.f, 0.f, 0.f); }
+            u[j] = a.part_t ? a.part_t[at] : make_float2(0.f, 0.f);
+            if (!in) { p[j] = make_float2(-INFINITY, 0.f); q[j] = 0.f; u[j] = make_float2(0.f, 0.f); }
         }
         const float m = fmaxf(fmaxf(mx, fmaxf(p[0].x, p[1].x)), fmaxf(p[2].x, p[3].x)), base = m == -INFINITY ? 0.f : m;
         // (a span without a class counts from 0 and adds nothing; a NaN sum stays NaN)
@@ -813,7 +783,7 @@ __global__ __launch_bounds__(256) void rows_kernel(RowArgs a)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             shift(p[j].x, base, p[j].y, q[j], u[j].x, u[j].y);
-            s += p[j].y; e += q[j]; tl += u[j].x; ts += u[j].y; ta += u[j].z;
+            s += p[j].y; e += q[j]; tl += u[j].x; ts += u[j].y;
         }
         mx = m;
     }
@@ -821,7 +791,7 @@ __global__ __launch_bounds__(256) void rows_kernel(RowArgs a)
     for (int d = 1; d < 64; d <<= 1) {
         const float om = __shfl_xor(mx, d, 64);
         float os = __shfl_xor(s, d, 64), oe = __shfl_xor(e, d, 64), ot = 0.f, op = 0.f;
-        if (a.part_t) { ot = __shfl_xor(tl, d, 64); op = __shfl_xor(ts, d, 64); ta += __shfl_xor(ta, d, 64); }
+        if (a.part_t) { ot = __shfl_xor(tl, d, 64); op = __shfl_xor(ts, d, 64); }
         const float m = fmaxf(mx, om), base = m == -INFINITY ? 0.f : m;
         shift(mx, base, s, e, tl, ts);
         shift(om, base, os, oe, ot, op);
@@ -832,20 +802,20 @@ __global__ __launch_bounds__(256) void rows_kernel(RowArgs a)
     float loss, ent = ls - e / s;
     if (a.target) {
         const long long t = a.target[row];
-        ts = ta = 1.f;
-        if (t == a.ignore) { loss = 0.f; ent = 0.f; ts = ta = 0.f; }
-        else if (t < 0 || t >= a.classes) { loss = ent = NAN; ts = ta = NAN; }
+        ts = 1.f;
+        if (t == a.ignore) loss = ent = ts = 0.f;
+        else if (t < 0 || t >= a.classes) loss = ent = ts = NAN;
         else loss = (m - a.tlogit[row]) + ls;
     } else {
         loss = ls * ts - tl;
     }
-    a.stats[row] = make_float4(mx, ts / s, ta, loss);
+    a.stats[row] = make_float4(mx, ts / s, 0.f, loss);
     if (a.ent) a.ent[row] = ent;
     if (a.loss_out) a.loss_out[row] = loss;
     if (a.ent_out) a.ent_out[row] = ent;
 }
 
-struct RowSums { double loss, ent, count; float top; };
+struct RowSums { double loss, ent, count; };
 constexpr int kMaxSums = 256;                 // a multiple of 64, at most 1024
 constexpr long long kOneTotal = 8192;         // rows that one workgroup adds up in no more time than another launch takes
 
@@ -856,12 +826,11 @@ __device__ inline RowSums join_sums(RowSums v, RowSums *red)
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) {
         v.loss += __shfl_xor(v.loss, s, 64); v.ent += __shfl_xor(v.ent, s, 64); v.count += __shfl_xor(v.count, s, 64);
-        v.top = fmaxf(v.top, __shfl_xor(v.top, s, 64));
     }
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     v = red[0];
-    for (int w = 1; w < W; w++) { v.loss += red[w].loss; v.ent += red[w].ent; v.count += red[w].count; v.top = fmaxf(v.top, red[w].top); }
+    for (int w = 1; w < W; w++) { v.loss += red[w].loss; v.ent += red[w].ent; v.count += red[w].count; }
     return v;
 }
 
@@ -874,25 +843,22 @@ struct TotalArgs {
     float *loss, *ent_out;        // [1]; null: not asked for
     const float *dloss;           // [n], [1] or null
     float grad_scale;
-    float *rowg;                  // [n]: g_i / 2^e; null: every row that counts has 1 (class numbers and a common g) or no gradient is asked for
-    float *factor;                // [1]: 2^e (times the common g); null without a backward pass
+    float *rowg;                  // [n]: g_i, 0 for rows that count for nothing; null: they are 1 and 0 (class numbers and a common
+                                  // g, which is `factor`) or no gradient is asked for
+    float *factor;                // [1]: the common g, or 1; null without a backward pass
 };
-// What the rows add up to, W waves: losses, entropies, rows that count; and their largest factor.  A fixed order, in double.
+// What the rows add up to, W waves: losses, entropies, rows that count.  A fixed order, in double.
 template <int W>
 __device__ inline RowSums row_sums(const TotalArgs &a, long long first, long long step)
 {
     __shared__ RowSums red[W];
-    RowSums s{0.0, 0.0, 0.0, 0.f};
+    RowSums s{0.0, 0.0, 0.0};
 #pragma unroll 4
     for (long long i = first; i < a.n; i += step) {
         const float4 st = a.stats[i];
         const bool used = !(a.target && a.target[i] == a.ignore);
         s.loss += st.w; s.count += used ? 1.0 : 0.0;
         if (a.ent) s.ent += a.ent[i];
-        float g = 1.f;
-        if (a.reduction == 0 && a.rowg) g = (a.dloss ? a.dloss[i] : 1.f) * a.grad_scale;
-        const float m = fabsf(g) * st.z;
-        if (used && m < INFINITY) s.top = fmaxf(s.top, m);
     }
     return join_sums<W>(s, red);
 }
@@ -902,46 +868,37 @@ __global__ __launch_bounds__(256) void sums_kernel(TotalArgs a)
     const RowSums s = row_sums<4>(a, (long long)blockIdx.x * 256 + threadIdx.x, (long long)kMaxSums * 256);
     if (threadIdx.x == 0) a.sums[blockIdx.x] = s;
 }
-// The totals, and the rows' gradient factors, scaled so that the largest |D| fits an image; the first of `wgs` workgroups
-// writes the totals.
+// The totals, and the rows' gradient factors; the first of `wgs` workgroups writes the totals.
 template <int THREADS>
 __device__ inline void totals(const TotalArgs &a, unsigned wg, unsigned wgs)
 {
     constexpr int W = THREADS / 64;
     const int tid = threadIdx.x;
-    RowSums s;
-    if (a.sums) {
-        __shared__ RowSums red[W];
-        s = tid < kMaxSums ? a.sums[tid] : RowSums{0.0, 0.0, 0.0, 0.f};
-        s = join_sums<W>(s, red);
-    } else {
-        s = row_sums<W>(a, tid, THREADS);
-    }
-    const float mx = s.top;
-    const double by = a.reduction == 2 ? (s.count > 0.0 ? 1.0 / s.count : 0.0) : 1.0;
-    if (a.reduction && wg == 0 && tid == 0) {
-        if (a.loss) a.loss[0] = (float)(s.loss * by);
-        if (a.ent_out) a.ent_out[0] = (float)(s.ent * by);
+    float common = 1.f;
+    if (a.reduction) {
+        RowSums s;
+        if (a.sums) {
+            __shared__ RowSums red[W];
+            s = tid < kMaxSums ? a.sums[tid] : RowSums{0.0, 0.0, 0.0};
+            s = join_sums<W>(s, red);
+        } else {
+            s = row_sums<W>(a, tid, THREADS);
+        }
+        const double by = a.reduction == 2 ? (s.count > 0.0 ? 1.0 / s.count : 0.0) : 1.0;
+        if (wg == 0 && tid == 0) {
+            if (a.loss) a.loss[0] = (float)(s.loss * by);
+            if (a.ent_out) a.ent_out[0] = (float)(s.ent * by);
+        }
+        common = (a.dloss ? a.dloss[0] : 1.f) * a.grad_scale * (float)by;
     }
     if (!a.factor) return;
-    // 2^e >= the largest g_i sum|pi_i| (1 for an index target and a common g)
-    float up = 1.f;
-    if (a.rowg && mx > 0.f) {
-        int E = (int)((__builtin_bit_cast(uint32_t, mx) >> 23) & 255) - 126;     // mx <= 2^E
-        if ((__builtin_bit_cast(uint32_t, mx) & 0x7FFFFFu) == 0) E--;
-        E = E > 126 ? 126 : (E < -120 ? -120 : E);
-        up = __builtin_bit_cast(float, (uint32_t)((E + 127) << 23));
-    }
     if (a.rowg)
         for (long long i = (long long)wg * THREADS + tid; i < a.n; i += (long long)wgs * THREADS) {
             const bool used = !(a.target && a.target[i] == a.ignore);
-            const float g = a.reduction == 0 ? (a.dloss ? a.dloss[i] : 1.f) * a.grad_scale : 1.f;
-            a.rowg[i] = used ? g / up : 0.f;
+            const float g = a.reduction ? 1.f : (a.dloss ? a.dloss[i] : 1.f) * a.grad_scale;
+            a.rowg[i] = used ? g : 0.f;
         }
-    if (wg == 0 && tid == 0) {
-        const float common = a.reduction ? (a.dloss ? a.dloss[0] : 1.f) * a.grad_scale * (float)by : 1.f;
-        a.factor[0] = up * common;
-    }
+    if (wg == 0 && tid == 0) a.factor[0] = common;
 }
 __global__ __launch_bounds__(1024) void totals_kernel(TotalArgs a) { totals<1024>(a, blockIdx.x, gridDim.x); }
 
@@ -963,7 +920,10 @@ struct FixArgs {
 template <typename Op>
 __global__ __launch_bounds__(256) void fix_kernel(FixArgs a)
 {
-    using V = typename Frag<typename Op::Img>::V;
+    using Img = typename Op::Grad::Img;
+    using E = Expo<Op>;
+    constexpr int N = Op::Grad::parts;
+    typedef E ex8 __attribute__((ext_vector_type(8)));
     __shared__ float red[4][kFixCols];
     if (a.totals.n >= 0 && blockIdx.y == gridDim.y - 1) {
         if (blockIdx.x == 0) totals<256>(a.totals, 0, 1);
@@ -971,7 +931,7 @@ __global__ __launch_bounds__(256) void fix_kernel(FixArgs a)
     }
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const long long c0 = (long long)blockIdx.x * kFixCols, c = c0 + lane * 8;
-    const long long r0 = (long long)blockIdx.y * a.rows, lde = a.ldd / (Op::split ? 2 : 1);
+    const long long r0 = (long long)blockIdx.y * a.rows;
     const float2 *part = a.part + (c < a.classes ? c : 0) / a.span * a.n;
     float db[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
@@ -984,19 +944,9 @@ __global__ __launch_bounds__(256) void fix_kernel(FixArgs a)
         if (c >= a.dcols) continue;
         // (a span with every class blocked: zeros, but NaN where the row has no other span or no finite loss)
         const float mp = part[row].x, f = (mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mp - st.x) * kLog2e)) * st.y;
-        float v[8];
-        if constexpr (Op::split) {
-            const fx4 *p = reinterpret_cast<const fx4 *>(static_cast<float *>(a.d) + row * lde + c);
-            const fx4 v0 = p[0], v1 = p[1];
-#pragma unroll
-            for (int i = 0; i < 4; i++) { v[i] = v0[i]; v[4 + i] = v1[i]; }
-            // (the halves land on exponentials of the row that other lanes of this wave read: no store moves in front of the loads)
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        } else {
-            const hx8 p = *reinterpret_cast<const hx8 *>(static_cast<_Float16 *>(a.d) + row * lde + c);
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = (float)p[i];
-        }
+        const ex8 v = *reinterpret_cast<const ex8 *>(place<Op, E>(a.d, row, a.ldd, c));
+        // (parts land on exponentials of the same 64 columns that other lanes of this wave read: no store moves in front of the loads)
+        if constexpr (N > 1) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         Pack<float, 8> pv;
         if (a.probs) {
             const float *pr = a.probs + row * a.ldp + c;
@@ -1005,22 +955,21 @@ __global__ __launch_bounds__(256) void fix_kernel(FixArgs a)
 #pragma unroll
                 for (int i = 0; i < 8; i++) pv.v[i] = c + i < a.classes ? pr[i] : 0.f;
         }
-        V h, l;
+        typename Frag<Img>::V h[N];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const bool out = c + i >= a.classes;
-            float q = v[i] * f;
+            float q = (float)v[i] * f;
             if (a.probs) q -= pv.v[i];
             else if (t == i) q -= 1.f;
             q = g == 0.f || out ? 0.f : q * g;                                  // a row that counts for nothing: zero whatever it holds
             db[i] += q;
-            q *= kDScale;
-            h[i] = (typename Op::Img)q;
-            if (Op::split) l[i] = (typename Op::Img)(q - (float)h[i]);
+#pragma unroll
+            for (int k = 0; k < N; k++) { h[k][i] = (Img)q; q -= (float)h[k][i]; }
         }
-        typename Op::Img *o = static_cast<typename Op::Img *>(a.d) + row * a.ldd + (Op::split ? (c >> 5) * 64 + (c & 31) : c);
-        *reinterpret_cast<V *>(o) = h;
-        if (Op::split) *reinterpret_cast<V *>(o + 32) = l;
+        Img *o = place<Op, Img>(a.d, row, a.ldd, c);
+#pragma unroll
+        for (int k = 0; k < N; k++) *reinterpret_cast<typename Frag<Img>::V *>(o + k * 64) = h[k];
     }
     if (!a.dbpart) return;
 #pragma unroll
@@ -1038,7 +987,6 @@ struct GradArgs {
     void *out; long long ldo;     // [n][ldo], operand type (one split), or
     float *acc;                   // float32 [splits][n][m]
     bool add;                     // add to acc instead of starting it
-    const float *amax;            // float32: partial maxima of the operand that is not D
     const float *factor;
 };
 
@@ -1056,11 +1004,10 @@ __device__ inline void grad_tile(const GradArgs &a, unsigned wg, char *lds)
     for (int i = 0; i < S::MT; i++)
 #pragma unroll
         for (int j = 0; j < S::NT; j++) acc[i][j] = fx4{0.f, 0.f, 0.f, 0.f};
-    TileProduct<Op, TM, TN, WM, WN, true, TB>::run(acc, a.a, m0, a.b, n0, k0, k1, a.ktiles, lds);
+    TileProduct<typename Op::Grad, TM, TN, WM, WN, true, TB>::run(acc, a.a, m0, a.b, n0, k0, k1, a.ktiles, lds);
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
-    float f = *a.factor / kDScale;
-    if (Op::split) f /= split_scale(max_of_parts(a.amax));
+    const float f = *a.factor;
     const long long mw = m0 + wm * (TM / WM) + 4 * (lane >> 4), nw = n0 + wn * (TN / WN) + (lane & 15);
 #pragma unroll
     for (int nt = 0; nt < S::NT; nt++) {
@@ -1109,8 +1056,7 @@ struct JoinArgs {
     int splits;
     long long n, m;
     void *out; long long ldo;
-    const float *amax, *factor;   // amax null: no image scale
-    float extra;                  // kDScale for products of D images, 1 for sums of unscaled D
+    const float *factor;
     unsigned wgs;                 // workgroups of this one
 };
 struct JoinList { JoinArgs j[3]; };
@@ -1126,8 +1072,7 @@ __global__ __launch_bounds__(256) void join_kernel(JoinList l)
     int q = 0;
     while (wg >= l.j[q].wgs) wg -= l.j[q++].wgs;
     const JoinArgs a = l.j[q];
-    float f = *a.factor / a.extra;
-    if (Op::split && a.amax) f /= split_scale(max_of_parts(a.amax));
+    const float f = *a.factor;
     const long long total = a.n * a.m;
     auto store = [&](long long i, float s) {
         const long long r = i / a.m, c = i - r * a.m;

@@ -239,7 +239,7 @@ struct FewArgs {
     int n, H, V;
     const long long *target;
     const float *probs; long long ldp;
-    float2 *part; float *part_e; float4 *part_t; float *tlogit;                  // as the tiled path's
+    float2 *part; float *part_e; float2 *part_t; float *tlogit;                  // as the tiled path's
 };
 template <typename T>
 __global__ __launch_bounds__(kSmallWaves * 64) void few_rows_kernel(FewArgs a)
@@ -268,14 +268,14 @@ __global__ __launch_bounds__(kSmallWaves * 64) void few_rows_kernel(FewArgs a)
         const float d = l - (mx == -INFINITY ? 0.f : mx), x = __builtin_amdgcn_exp2f(d * kLog2e);
         const float s = sum32(x), e = a.part_e ? sum32(x != 0.f ? x * d : 0.f) : 0.f;
         const float p = a.probs && live && v < a.V ? a.probs[row * a.ldp + v] : 0.f;
-        const float tl = a.probs ? sum32(p != 0.f ? p * d : 0.f) : 0.f, ts = a.probs ? sum32(p) : 0.f, ta = a.probs ? sum32(fabsf(p)) : 0.f;
+        const float tl = a.probs ? sum32(p != 0.f ? p * d : 0.f) : 0.f, ts = a.probs ? sum32(p) : 0.f;
         if (!live) continue;
         if (a.target && v < a.V && a.target[row] == v) a.tlogit[row] = l;
         if ((lane & 31) == 0) {
             const long long at = (long long)blockIdx.x * a.n + row;
             a.part[at] = make_float2(mx, s);
             if (a.part_e) a.part_e[at] = e;
-            if (a.probs) a.part_t[at] = make_float4(tl, ts, ta, 0.f);
+            if (a.probs) a.part_t[at] = make_float2(tl, ts);
         }
     }
 }
@@ -296,31 +296,31 @@ __global__ __launch_bounds__(256) void small_rows_kernel(SmallArgs a)
     mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     __syncthreads();
     const float base = mx == -INFINITY ? 0.f : mx;
-    float s = 0.f, e = 0.f, tl = 0.f, ts = 0.f, ta = 0.f;
+    float s = 0.f, e = 0.f, tl = 0.f, ts = 0.f;
     for (int v = tid; v < a.V; v += 256) {
         const float x = l[v] - base, p = __builtin_amdgcn_exp2f(x * kLog2e);
         s += p;
         e += p != 0.f ? p * x : 0.f;
-        if (pr) { const float q = pr[v]; ts += q; ta += fabsf(q); tl += q != 0.f ? q * x : 0.f; }
+        if (pr) { const float q = pr[v]; ts += q; tl += q != 0.f ? q * x : 0.f; }
     }
     s = block_sum<4>(s, red);
     if (a.ent) e = block_sum<4>(e, red);
-    if (pr) { tl = block_sum<4>(tl, red); ts = block_sum<4>(ts, red); ta = block_sum<4>(ta, red); }
+    if (pr) { tl = block_sum<4>(tl, red); ts = block_sum<4>(ts, red); }
     const float ls = logf(s);                                 // (everything relative to the maximum: loss and entropy need no large difference)
     const long long t = a.target ? a.target[row] : -1;
     bool used = true;
     float loss, ent = ls - e / s;
     if (a.target) {
-        ts = ta = 1.f;
-        if (t == a.ignore) { used = false; loss = ent = ts = ta = 0.f; }
-        else if (t < 0 || t >= a.V) loss = ent = ts = ta = NAN;
+        ts = 1.f;
+        if (t == a.ignore) { used = false; loss = ent = ts = 0.f; }
+        else if (t < 0 || t >= a.V) loss = ent = ts = NAN;
         else loss = ls - (l[t] - base);
     } else {
         loss = ls * ts - tl;
     }
     __syncthreads();                                          // (l[t] is read before it becomes D)
     if (tid == 0) {
-        a.stats[row] = make_float4(mx, ts / s, ta, loss);
+        a.stats[row] = make_float4(mx, ts / s, 0.f, loss);
         if (a.ent) a.ent[row] = ent;
         if (a.reduction == 0) {
             if (a.loss) a.loss[row] = loss;

@@ -49,9 +49,9 @@ struct DeviceScope {
 };
 
 long long up_to(long long v, long long m) { return (v + m - 1) / m * m; }
-// Row stride of an image of `cols` elements of 16 bits: an odd number of 128-byte lines, so that the lines that the rows of a
+// Row stride of an image of `cols` columns in `parts`: an odd number of 128-byte lines, so that the lines that the rows of a
 // tile have in one stage lie in different channels of the L2 and of memory.
-long long image_stride(long long cols) { const long long l = up_to(cols, 64) / 64; return (l | 1) * 64; }
+long long image_stride(long long cols, int parts) { const long long l = up_to(cols, 64) / 64 * parts; return (l | 1) * 64; }
 
 bool bad_matrix(long long rows, long long cols, long long stride) { return rows > 1 && stride < cols; }
 
@@ -134,16 +134,17 @@ long long tiles_of(Shape s, long long m, long long n) { return ((m + kDims[s].tm
 // 65536 122 / 156, 32 x 4096 x 32000 52 / 53; 256 x 256 against 128 x 128, 1024 x 1024 x 8192 (128 tiles of 256) 35 / 29, 2048 x
 // 1024 x 5000 (160) 36 / 39; 128 x 128 against 64 x 64, 1024 x 2048 x 2048 (128 tiles of 128) 30 / 24.  No tile is wider than the
 // classes need.
-Shape pick_logits(long long m, long long n, bool grad)
+Shape pick_logits(long long m, long long n, bool grad, long long stride)
 {
     if (!grad && n <= 32) return TROW;
-    if (m > 128 && tiles_of(T256, m, n) >= 150) return T256;
+    // (a tile's rows lie within 2^32 bytes: 128 rows of 2^22 float32 features do)
+    if (m > 128 && tiles_of(T256, m, n) >= 150 && 256 * 2 * stride < 1LL << 32) return T256;
     if (m > 64 && tiles_of(T128, m, n) >= 200) return T128;
     return tiles_of(T64, m, n) <= kFewTiles ? T64FEW : T64;
 }
 // Tile of the gradients' products, which share a launch, and the splits of their sums, by an estimate in microseconds: the
 // launch takes its stages at the rate of the whole card or as long as its longest workgroup, whichever is more, and splits
-// cost a join.  Per stage and tile (measured at 16 bits; float32 half as much again): 256 x 256 1.0 with a CU to itself,
+// cost a join.  Per stage and tile (measured): 256 x 256 1.0 with a CU to itself,
 // 128 x 128 0.30 a CU's share and 0.6 from start to end, 64 x 64 0.16 and 0.45, with longer rings 0.35.
 struct GradPick { Shape shape; int splits_x, kper_x, splits_w, kper_w; };
 GradPick pick_grads(long long n, long long h, long long v, long long kx, long long kw, bool want_x, bool want_w)
@@ -180,16 +181,17 @@ GradPick pick_grads(long long n, long long h, long long v, long long kx, long lo
 }
 
 struct Plan {
-    bool small, few, split, forward, backward, pack_w, pack_x, keep;      // keep: the forward pass leaves exponentials for the backward pass
+    bool small, few, forward, backward, keep;                 // keep: the forward pass leaves exponentials for the backward pass
+    bool pack_w, pack_x, grad_w, grad_x;                      // images of W and X for the logits; of their own for the gradients
     long long n, H, V, vp, pieces;
-    long long kimg, ldk, ldd;                                 // image elements along the features; row strides of the images of X, W and D
-    int per, ks;                                              // image elements an element takes, k of a stage
+    long long kimg, ldl, ldg, ldd;                            // columns of the images of W and X; row strides of these and of D's
+    int lparts, gparts;                                       // parts of an element in the logits' and the gradients' products
     Shape lshape;
     int large_m, behind_m;                                    // the loss alone: tiles of 256 and, behind them, of 128 classes (0: none)
     long long spans;                                          // of a piece
     GradPick g;
     int fix_rows;
-    size_t xmax, wmax, ximg, wimg, part, part_e, part_t, tlogit, stats, ent, rowg, sums, factor, d, dbpart, dxacc, dwacc, logits, count, total;
+    size_t ximg, wimg, gximg, gwimg, part, part_e, part_t, tlogit, stats, ent, rowg, sums, factor, d, dbpart, dxacc, dwacc, logits, count, total;
 };
 
 bool aligned16(const void *p, long long stride, long long cols, long long rows)
@@ -199,16 +201,16 @@ bool aligned16(const void *p, long long stride, long long cols, long long rows)
 
 int make_plan(const azg_linear_ce_args *a, Plan *p)
 {
-    p->split = a->dtype == AZG_F32;
-    p->per = p->split ? 2 : 1;
-    p->ks = p->split ? 32 : 64;
+    const bool f32 = a->dtype == AZG_F32;
+    p->lparts = f32 ? OpF32::Logits::parts : 1;
+    p->gparts = f32 ? OpF32::Grad::parts : a->dtype == AZG_F16 ? OpF16::Grad::parts : OpBF16::Grad::parts;
     p->forward = a->loss != nullptr;
     p->backward = a->dx || a->dw || a->db;
     p->n = a->n; p->H = a->hidden; p->V = a->classes;
     // A forward pass whose stats are kept takes the path of the backward pass to come: the logits that are made again there have to
     // be the same bits (every tile adds up k in one order), or a large logit's exponential leaves [0, 1].
     const bool differentiable = p->backward || a->stats;
-    p->small = takes_small(p->split, differentiable, p->n, p->H, p->V);
+    p->small = takes_small(f32, differentiable, p->n, p->H, p->V);
     if (p->small) {
         Take t;
         p->logits = t((size_t)p->n * p->V * 4);
@@ -218,16 +220,20 @@ int make_plan(const azg_linear_ce_args *a, Plan *p)
         p->total = t.off;
         return AZG_OK;
     }
-    p->kimg = up_to(p->H, p->ks) * p->per;
-    p->ldk = image_stride(p->kimg);
+    p->kimg = up_to(p->H, 64);
+    p->ldl = image_stride(p->H, p->lparts);
+    p->ldg = image_stride(p->H, p->gparts);
     // (dW multiplies the rows that count for nothing by zero: they are copied as zeros, whatever they hold)
-    p->pack_x = p->split || !aligned16(a->x, a->x_stride, a->hidden, a->n) || (a->dw && a->target);
-    p->pack_w = p->split || !aligned16(a->w, a->w_stride, a->hidden, a->classes);
+    const bool shared = p->lparts == p->gparts;               // the gradients' products take the same images
+    p->pack_x = p->lparts > 1 || !aligned16(a->x, a->x_stride, a->hidden, a->n) || (shared && a->dw && a->target);
+    p->pack_w = p->lparts > 1 || !aligned16(a->w, a->w_stride, a->hidden, a->classes);
+    p->grad_x = !shared && a->dw;
+    p->grad_w = !shared && a->dx;
     p->few = !differentiable && p->n <= 32 && p->pack_w;
     if (p->few) p->pack_x = p->pack_w = false;
     // bytes a class of a piece costs
-    long long cost = p->pack_w ? p->ldk * 2 : 0;
-    if (p->backward) cost += p->n * p->per * 2;
+    long long cost = (p->pack_w ? p->ldl * 2 : 0) + (p->grad_w ? p->ldg * 2 : 0);
+    if (p->backward) cost += p->n * p->gparts * 2;
     p->vp = p->V;
     if (cost) p->vp = std::min<long long>(p->V, std::max<long long>(1024, kPieceBytes / cost / 256 * 256));
     p->pieces = (p->V + p->vp - 1) / p->vp;
@@ -236,9 +242,10 @@ int make_plan(const azg_linear_ce_args *a, Plan *p)
         p->pieces = (p->V + p->vp - 1) / p->vp;
     }
     p->keep = p->forward && p->backward && p->pieces == 1;
-    p->ldd = image_stride(up_to(p->vp, p->ks) * p->per);
-    p->lshape = pick_logits(p->vp, p->n, p->backward || p->split);   // (float32 has no tile for few rows)
-    p->g = pick_grads(p->n, p->H, p->vp, (p->vp + p->ks - 1) / p->ks, (p->n + p->ks - 1) / p->ks, a->dx != nullptr, a->dw != nullptr);
+    p->ldd = image_stride(p->vp, p->gparts);
+    p->lshape = pick_logits(p->vp, p->n, p->backward || f32, p->lparts > 1 ? p->ldl : 0);   // (float32 has no tile for few rows)
+    const int pairs = p->gparts * (p->gparts + 1) / 2;
+    p->g = pick_grads(p->n, p->H, p->vp, (p->vp + 63) / 64 * pairs, (p->n + 63) / 64 * pairs, a->dx != nullptr, a->dw != nullptr);
     // rows a workgroup turns into D: up to 64, fewer while they would not give four workgroups a CU
     // (more for very many rows: db is joined from one sum a run of rows, one after the other)
     p->fix_rows = 64;
@@ -262,14 +269,14 @@ int make_plan(const azg_linear_ce_args *a, Plan *p)
     }
     if (p->few) p->spans = (p->V + kSmallTile - 1) / kSmallTile;
     Take t;
-    p->xmax = t(p->split ? kMaxParts * 4 : 0);
-    p->wmax = t(p->split ? kMaxParts * 4 : 0);
-    p->ximg = t(p->pack_x ? (size_t)p->n * p->ldk * 2 : 0);
-    p->wimg = t(p->pack_w ? (size_t)p->vp * p->ldk * 2 : 0);
+    p->ximg = t(p->pack_x ? (size_t)p->n * p->ldl * 2 : 0);
+    p->wimg = t(p->pack_w ? (size_t)p->vp * p->ldl * 2 : 0);
+    p->gximg = t(p->grad_x ? (size_t)p->n * p->ldg * 2 : 0);
+    p->gwimg = t(p->grad_w ? (size_t)p->vp * p->ldg * 2 : 0);
     const size_t entries = (size_t)p->pieces * p->spans * p->n;
     p->part = t(p->forward ? entries * 8 : 0);
     p->part_e = t(p->forward && a->entropy ? entries * 4 : 0);
-    p->part_t = t(p->forward && a->probs ? entries * 16 : 0);
+    p->part_t = t(p->forward && a->probs ? entries * 8 : 0);
     p->tlogit = t((size_t)p->n * 4);
     p->stats = t((size_t)p->n * 16);
     p->ent = t((size_t)p->n * 4);
@@ -323,7 +330,7 @@ int launch_logits(Shape shape, const CeArgs &c, hipStream_t s)
     case T64: return launch_logits_shape<Op, 64, 64, 2, 2, GRAD>(c, s);
     case T64FEW: return launch_logits_shape<Op, 64, 64, 1, 4, GRAD>(c, s);
     default:
-        if constexpr (!GRAD && !Op::split) return launch_logits_shape<Op, 128, 32, 4, 1, false>(c, s);
+        if constexpr (!GRAD && Op::Logits::parts == 1) return launch_logits_shape<Op, 128, 32, 4, 1, false>(c, s);
         return fail(AZG_EINVAL, "azg_linear_ce: internal: no such tile");
     }
 }
@@ -379,14 +386,17 @@ int launch_joins(JoinList l, int count, hipStream_t s)
     OPS_HIP(hipGetLastError());
     return AZG_OK;
 }
-// one image or two (null: none)
-template <typename Op>
-int launch_packs(const PackArgs *p, const PackArgs *q, hipStream_t s)
+// the images of a list, `count` of them
+template <typename In>
+int launch_packs(PackList l, int count, hipStream_t s)
 {
-    if (!p) std::swap(p, q);
-    if (!p) return AZG_OK;
-    auto wgs = [](const PackArgs &a) { return (unsigned)std::min<long long>((a.rows * (a.icols / (Op::split ? 16 : 8)) + 255) / 256, 1 << 16); };
-    hipLaunchKernelGGL((pack_kernel<Op>), dim3(wgs(*p) + (q ? wgs(*q) : 0)), dim3(256), 0, s, *p, q ? *q : *p, wgs(*p));
+    unsigned grid = 0;
+    for (int i = 0; i < count; i++) {
+        l.p[i].wgs = (unsigned)std::min<long long>((l.p[i].rows * (l.p[i].icols / 8) + 255) / 256, 1 << 16);
+        grid += l.p[i].wgs;
+    }
+    if (!grid) return AZG_OK;
+    hipLaunchKernelGGL((pack_kernel<In>), dim3(grid), dim3(256), 0, s, l);
     OPS_HIP(hipGetLastError());
     return AZG_OK;
 }
@@ -403,30 +413,39 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
     const In *W = static_cast<const In *>(a->w);
     const ShapeDim dim = kDims[p.lshape];
 
-    PackArgs px{};
-    px.src = a->x; px.ld = a->x_stride; px.rows = a->n; px.cols = a->hidden; px.target = target; px.ignore = a->ignore_index;
-    px.maxpart = f32(p.xmax); px.img = ws + p.ximg; px.ldi = p.ldk; px.icols = p.kimg;
-    PackArgs pw{};
-    pw.src = W; pw.ld = a->w_stride; pw.rows = a->classes; pw.cols = a->hidden; pw.maxpart = f32(p.wmax); pw.img = ws + p.wimg; pw.ldi = p.ldk; pw.icols = p.kimg;
-    if (Op::split && !p.few) hipLaunchKernelGGL(absmax_kernel, dim3(2 * kMaxParts), dim3(512), 0, s, px, pw);
-    bool x_packed = !p.pack_x;
+    bool x_packed = false;
     CeArgs c{};
-    c.x = p.pack_x ? Operand{ws + p.ximg, p.ldk, a->n, p.kimg} : Operand{a->x, a->x_stride, a->n, a->hidden};
-    c.ktiles = (int)((p.H + p.ks - 1) / p.ks);
+    const int lblock = p.lparts * 64, gblock = p.gparts * 64;
+    c.x = p.pack_x ? Operand{ws + p.ximg, p.ldl, a->n, p.kimg, lblock} : Operand{a->x, a->x_stride, a->n, a->hidden, lblock};
+    const Operand grad_x_op = p.grad_x ? Operand{ws + p.gximg, p.ldg, a->n, p.kimg, gblock} : c.x;
+    Operand grad_w_op{};
+    c.ktiles = (int)((p.H + 63) / 64) * Op::Logits::pairs;
     c.n = a->n; c.target = target; c.ignore = a->ignore_index; c.ldp = a->probs_stride;
-    c.xmax = f32(p.xmax); c.wmax = f32(p.wmax);
 
-    auto piece = [&](long long i, bool pack) -> int {
+    // a piece of the classes, its images, and before the first piece X's; `grads`: the gradients' products are going to follow
+    auto piece = [&](long long i, bool grads) -> int {
         const long long v0 = i * p.vp, vn = std::min(p.vp, a->classes - v0);
         c.v0 = v0; c.classes = vn;
         c.bias = a->bias ? static_cast<const In *>(a->bias) + v0 : nullptr;
         c.probs = a->probs ? a->probs + v0 : nullptr;
         c.ldd = p.ldd;
-        c.dcols = up_to(vn, p.ks);
-        pw.src = W + v0 * a->w_stride; pw.rows = vn;
-        if (pack) OPS_TRY(launch_packs<Op>(x_packed ? nullptr : &px, p.pack_w ? &pw : nullptr, s));
+        c.dcols = up_to(vn, 64);
+        const In *w = W + v0 * a->w_stride;
+        PackList list{};
+        int count = 0;
+        auto image = [&](const void *src, long long ld, long long rows, size_t at, long long ldi, int parts, const long long *rows_of) {
+            PackArgs &q = list.p[count++];
+            q.src = src; q.ld = ld; q.rows = rows; q.cols = a->hidden; q.img = ws + at; q.ldi = ldi; q.icols = p.kimg; q.parts = parts;
+            q.target = rows_of; q.ignore = a->ignore_index;
+        };
+        if (!x_packed && p.pack_x) image(a->x, a->x_stride, a->n, p.ximg, p.ldl, p.lparts, target);
+        if (!x_packed && p.grad_x) image(a->x, a->x_stride, a->n, p.gximg, p.ldg, p.gparts, target);
+        if (p.pack_w) image(w, a->w_stride, vn, p.wimg, p.ldl, p.lparts, nullptr);
+        if (p.grad_w && grads) image(w, a->w_stride, vn, p.gwimg, p.ldg, p.gparts, nullptr);
+        OPS_TRY(launch_packs<In>(list, count, s));
         x_packed = true;
-        c.w = p.pack_w ? Operand{ws + p.wimg, p.ldk, vn, p.kimg} : Operand{W + v0 * a->w_stride, a->w_stride, vn, a->hidden};
+        c.w = p.pack_w ? Operand{ws + p.wimg, p.ldl, vn, p.kimg, lblock} : Operand{w, a->w_stride, vn, a->hidden, lblock};
+        grad_w_op = p.grad_w ? Operand{ws + p.gwimg, p.ldg, vn, p.kimg, gblock} : c.w;
         return AZG_OK;
     };
 
@@ -438,14 +457,14 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
             f.x = a->x; f.w = a->w; f.bias = a->bias; f.xs = a->x_stride; f.ws = a->w_stride;
             f.n = (int)a->n; f.H = (int)a->hidden; f.V = (int)a->classes; f.target = target; f.probs = a->probs; f.ldp = a->probs_stride;
             f.part = reinterpret_cast<float2 *>(ws + p.part); f.part_e = a->entropy ? f32(p.part_e) : nullptr;
-            f.part_t = a->probs ? reinterpret_cast<float4 *>(ws + p.part_t) : nullptr; f.tlogit = f32(p.tlogit);
+            f.part_t = a->probs ? reinterpret_cast<float2 *>(ws + p.part_t) : nullptr; f.tlogit = f32(p.tlogit);
             hipLaunchKernelGGL((few_rows_kernel<In>), dim3((unsigned)full), dim3(kSmallWaves * 64), 0, s, f);
             spans = full;
         } else for (long long i = 0; i < p.pieces; i++) {
-            OPS_TRY(piece(i, true));
+            OPS_TRY(piece(i, p.keep));
             c.part = reinterpret_cast<float2 *>(ws + p.part) + i * full * a->n;
             c.part_e = a->entropy ? f32(p.part_e) + i * full * a->n : nullptr;
-            c.part_t = a->probs ? reinterpret_cast<float4 *>(ws + p.part_t) + i * full * a->n : nullptr;
+            c.part_t = a->probs ? reinterpret_cast<float2 *>(ws + p.part_t) + i * full * a->n : nullptr;
             c.tlogit = f32(p.tlogit);
             c.d = p.keep ? ws + p.d : nullptr;
             if (p.behind_m) {
@@ -460,7 +479,7 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
         RowArgs r{};
         r.n = a->n; r.classes = a->classes; r.spans = (int)spans;
         r.part = reinterpret_cast<float2 *>(ws + p.part); r.part_e = a->entropy ? f32(p.part_e) : nullptr;
-        r.part_t = a->probs ? reinterpret_cast<float4 *>(ws + p.part_t) : nullptr; r.tlogit = f32(p.tlogit);
+        r.part_t = a->probs ? reinterpret_cast<float2 *>(ws + p.part_t) : nullptr; r.tlogit = f32(p.tlogit);
         r.target = target; r.ignore = a->ignore_index; r.stats = stats; r.ent = a->entropy ? f32(p.ent) : nullptr;
         if (a->reduction == AZG_REDUCE_NONE) { r.loss_out = a->loss; r.ent_out = a->entropy; }
         hipLaunchKernelGGL(rows_kernel, dim3((unsigned)((a->n + 3) / 4)), dim3(256), 0, s, r);
@@ -476,19 +495,18 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
     const bool ride = p.keep && target && a->reduction != AZG_REDUCE_NONE && (a->n <= kOneTotal || p.V >= 4096);
     if (ride) t.rowg = nullptr;
     else if (p.backward || a->reduction != AZG_REDUCE_NONE) {
-        unsigned grid = 1;
-        if (a->n > kOneTotal) {
+        const bool many = a->n > kOneTotal;
+        if (many && a->reduction != AZG_REDUCE_NONE) {
             t.sums = reinterpret_cast<RowSums *>(ws + p.sums);
             hipLaunchKernelGGL(sums_kernel, dim3(kMaxSums), dim3(256), 0, s, t);
-            grid = 64;
         }
-        hipLaunchKernelGGL(totals_kernel, dim3(grid), dim3(1024), 0, s, t);
+        hipLaunchKernelGGL(totals_kernel, dim3(many ? 64 : 1), dim3(1024), 0, s, t);
     }
     OPS_HIP(hipGetLastError());
     if (!p.backward) return AZG_OK;
 
     for (long long i = 0; i < p.pieces; i++) {
-        if (!p.keep) OPS_TRY(piece(i, !(p.forward && p.pieces == 1)));
+        if (!p.keep) OPS_TRY(piece(i, true));
         const long long vn = c.classes;
         int dbparts;
         if (p.keep) {
@@ -511,26 +529,26 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
         GradArgs gx{}, gw{};
         JoinList joins{};
         int count = 0;
-        const Operand d{ws + p.d, c.ldd, a->n, c.dcols * p.per};
+        const Operand d{ws + p.d, c.ldd, a->n, c.dcols, gblock};
         if (a->dx) {
-            gx.a = Operand{c.w.p, c.w.ld, vn, c.w.cols}; gx.b = d;
-            gx.ktiles = (int)((vn + p.ks - 1) / p.ks); gx.kper = p.g.kper_x; gx.splits = p.g.splits_x; gx.m = a->hidden; gx.n = a->n;
-            gx.amax = f32(p.wmax); gx.factor = f32(p.factor);
+            gx.a = grad_w_op; gx.b = d;
+            gx.ktiles = (int)((vn + 63) / 64) * Op::Grad::pairs; gx.kper = p.g.kper_x; gx.splits = p.g.splits_x; gx.m = a->hidden; gx.n = a->n;
+            gx.factor = f32(p.factor);
             const bool acc = p.g.splits_x > 1 || p.pieces > 1;
             gx.acc = acc ? f32(p.dxacc) : nullptr; gx.add = i > 0;
             gx.out = a->dx; gx.ldo = a->dx_stride;
-            if (acc && i == p.pieces - 1) joins.j[count++] = {gx.acc, gx.splits, gx.n, gx.m, gx.out, gx.ldo, gx.amax, gx.factor, kDScale, 0};
+            if (acc && i == p.pieces - 1) joins.j[count++] = {gx.acc, gx.splits, gx.n, gx.m, gx.out, gx.ldo, gx.factor, 0};
         }
         if (a->dw) {
-            gw.a = c.x; gw.b = d;
-            gw.ktiles = (int)((a->n + p.ks - 1) / p.ks); gw.kper = p.g.kper_w; gw.splits = p.g.splits_w; gw.m = a->hidden; gw.n = vn;
-            gw.amax = f32(p.xmax); gw.factor = f32(p.factor);
+            gw.a = grad_x_op; gw.b = d;
+            gw.ktiles = (int)((a->n + 63) / 64) * Op::Grad::pairs; gw.kper = p.g.kper_w; gw.splits = p.g.splits_w; gw.m = a->hidden; gw.n = vn;
+            gw.factor = f32(p.factor);
             gw.acc = p.g.splits_w > 1 ? f32(p.dwacc) : nullptr; gw.add = false;
             gw.out = static_cast<In *>(a->dw) + i * p.vp * a->dw_stride; gw.ldo = a->dw_stride;
-            if (gw.acc) joins.j[count++] = {gw.acc, gw.splits, gw.n, gw.m, gw.out, gw.ldo, gw.amax, gw.factor, kDScale, 0};
+            if (gw.acc) joins.j[count++] = {gw.acc, gw.splits, gw.n, gw.m, gw.out, gw.ldo, gw.factor, 0};
         }
         if (a->dx || a->dw) OPS_TRY(launch_grads<Op>(p.g.shape, gx, gw, s));
-        if (a->db) joins.j[count++] = {f32(p.dbpart), dbparts, 1, vn, static_cast<In *>(a->db) + i * p.vp, vn, nullptr, f32(p.factor), 1.f, 0};
+        if (a->db) joins.j[count++] = {f32(p.dbpart), dbparts, 1, vn, static_cast<In *>(a->db) + i * p.vp, vn, f32(p.factor), 0};
         OPS_TRY(launch_joins<Op>(joins, count, s));
     }
     return AZG_OK;

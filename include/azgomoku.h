@@ -319,8 +319,8 @@ int azg_dropout(const azg_dropout_args *a);
 
 /* Softmax cross entropy of the projection l = x w^T + bias (x [n,hidden], w [classes,hidden], bias [classes] or NULL, one
  * type), against class numbers or against probabilities (any real weights), and its gradients.  The logits of a large problem
- * are not stored: a backward pass keeps one array of 2 bytes (AZG_F32: 4) an element, of at most 1 GiB together with the
- * copies of x and w that it needs or of 1024 classes, and takes more classes than fit piece by piece.  Small problems keep at
+ * are not stored: a backward pass keeps one array of 2 bytes (AZG_F16: 4, AZG_F32: 6) an element, of at most 1 GiB together with
+ * the copies of w that it needs or of 1024 classes, and takes more classes than fit piece by piece.  Small problems keep at
  * most 16 MB of float32 logits.  n < 2^26, classes < 2^27, hidden and the row
  * strides of x and w at most 2^22.  For every row
  *   loss = lse - l[target]                        target int64 [n]; rows whose target is ignore_index count for nothing,
@@ -333,9 +333,11 @@ int azg_dropout(const azg_dropout_args *a);
  * Gradients are those of sum_i dloss_i loss_i (NONE, dloss [n]) or dloss loss ([1]), times grad_scale; dloss NULL = 1.
  * One call does the forward pass (loss not NULL), the backward pass (any of dx, dw, db not NULL), or both.  A backward pass
  * by itself takes the stats [n][4] (float32, 16-byte aligned, the caller's) that the forward pass of the same inputs wrote.
- * Sums, statistics and accumulators are float32 or wider; the gradient at the logits is rounded to x's type (float32: to 22
- * bits) before the two products that use it, and where one call makes loss and gradients its softmax to 11 bits before that
- * (float32: not).  Results do not depend on anything but the arguments and the alignment of x and w: the same bits every time.
+ * Sums, statistics and accumulators are float32 or wider and have float32's range, whatever the other rows and classes hold; a
+ * product of two float32 numbers is made to 2^-23 of itself.  Infinities in x or w: the logits they reach are infinite or NaN.  The
+ * gradient at the logits is rounded before the two products that use it, to 24 bits (AZG_F32), 16 (AZG_F16) or 8 (AZG_BF16), all
+ * with float32's range; where one call makes loss and gradients in AZG_BF16 its softmax is rounded to 11 bits, or by 2^-25 of the
+ * largest among the 128 classes around it, before that.  Results do not depend on anything but the arguments and the alignment of x and w: the same bits every time.
  * azg_linear_ce_workspace: bytes of workspace (256-byte aligned) the call needs with these very arguments, pointers included
  * (workspace, workspace_bytes and stream are not looked at), or AZG_E*. */
 #define AZG_REDUCE_NONE  0

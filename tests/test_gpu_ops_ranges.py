@@ -16,11 +16,11 @@ def ops():
     return o
 
 
-def autograd(ops, x, w, t, b, **kw):
-    """(loss, d_hidden, d_weight, d_bias): a forward pass and a backward pass by itself."""
+def autograd(ops, x, w, t, b, scale=1.0, **kw):
+    """(loss, d_hidden, d_weight, d_bias): a forward pass and a backward pass by itself, of scale times the sum of the losses."""
     leaves = [q.clone().requires_grad_() for q in (x, w, b)]
     loss = ops.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], **kw)
-    loss.sum().backward()
+    (scale * loss.sum()).backward()
     return (loss.detach(),) + tuple(q.grad for q in leaves)
 
 
@@ -134,3 +134,140 @@ def test_loss_and_entropy_of_exact_logits(ops, dtype, n, h, v, offset, peak):
             assert float(loss.min()) >= 0 and float(entropy.min()) >= 0
             assert bool(((loss.double() - want).abs() <= bound).all()), float(((loss.double() - want).abs() / bound.clamp_min(1e-300)).max())
             assert bool(((entropy.double() - ent).abs() <= b_ent).all()), float(((entropy.double() - ent).abs() / b_ent.clamp_min(1e-300)).max())
+
+
+# ---------------------------------------------------------------- operands, probabilities and weights far apart
+def elementwise(x, w, b, t, g, kept=0.0):
+    """{name: (value in float64, bound)} of loss rows, d_hidden, d_weight and d_bias under sum g_i loss_i, every bound an
+    element's own: products and sums of (H + 8) f sum|x w| in a logit (float32 leaves out 2 f of it); a probability by what its logit
+    and the others' (weighted by their probabilities) may be off, by (2 |l - max| + 100) f of itself, and by `kept` of itself where one call keeps
+    exponentials in 16 bits; the gradient at the logits D by its rounding (bfloat16 half a step, half precision 2^-17); the products by what they
+    leave out (float32 2 f, half precision 2^-16), (K + 40) f, and the result's rounding."""
+    dt = x.dtype
+    n, h = x.shape
+    v = w.shape[0]
+    by_index = t.dtype == torch.int64
+    xd, wd = x.double(), w.double()
+    l = xd @ wd.t() + (0 if b is None else b.double())
+    dl = (h + 8) * F * (xd.abs() @ wd.abs().t()) + F * l.abs()
+    q = torch.zeros_like(l) if by_index else t.double()
+    if by_index:
+        q[torch.arange(n), t] = 1.0
+    m = l.max(1, keepdim=True).values
+    lse = torch.logsumexp(l, 1, keepdim=True)
+    p = torch.exp(l - lse)
+    el = (p * dl).sum(1, keepdim=True)
+    own = p * ((2 * (l - m).abs() + 100) * F + kept)
+    up = torch.exp((l - lse + dl + el).clamp(max=0.0))               # a row with one class left: the others' bounds are what it may lose
+    top = l == m
+    low = torch.maximum(torch.exp(l - lse - dl - el), torch.where(top, 1 - torch.where(top, 0.0, up).sum(1, keepdim=True), 0.0))
+    bp = torch.maximum(up - p, p - low) * (1 + 2.0 ** -10) + own
+    qs = q.sum(1, keepdim=True)
+    gd = g.double()[:, None]
+    D = gd * (p * qs - q)
+    bD0 = gd.abs() * (bp * qs.abs() + 4 * F * (p * qs.abs() + q.abs()))
+    bD = bD0 + {torch.float32: F, torch.bfloat16: half_step(dt), torch.float16: 2.0 ** -17}[dt] * D.abs()
+    out, u = (2.0 ** -25 if dt == torch.float16 else 0.0), half_step(dt)
+    op = {torch.float32: 2 * F, torch.bfloat16: 0.0, torch.float16: 2.0 ** -16}[dt]
+
+    def product(a, ba, c, k):
+        r = a @ c
+        return r, (ba @ c.abs() + ((k + 40) * F + op) * (a.abs() @ c.abs())) * (1 + 2 * u) + u * r.abs() * (1 + 1e-6) + out
+    loss = ((m - l) * q).sum(1) + torch.log(torch.exp(l - m).sum(1)) * qs[:, 0]
+    b_loss = (q.abs() * dl).sum(1) + qs.abs()[:, 0] * (el[:, 0] + 100 * F) + 8 * F * ((q.abs() * (m - l)).sum(1) + loss.abs())
+    db = D.sum(0)
+    return {"loss": (loss, b_loss), "d_hidden": product(D, bD, wd, v), "d_weight": product(D.t(), bD.t(), xd, n),
+            "d_bias": (db, (bD0.sum(0) + (n + 40) * F * D.abs().sum(0)) * (1 + 2 * u) + u * db.abs() * (1 + 1e-6) + out)}
+
+
+def within(name, got, want, bound, rows=slice(None)):
+    err = (got.double() - want).abs()[rows]
+    bad = ~(err <= bound[rows])
+    assert not bool(bad.any()), "%s: %d of %d off, worst %.3g times its bound" % (name, int(bad.sum()), bad.numel(), float((err / bound[rows].clamp_min(1e-300)).max()))
+
+
+FAR = PATHS + [(7, 100, 5003), (300, 130, 2050), (1500, 64, 6000), (300, 33, 34000)]
+
+
+@pytest.mark.parametrize("n,h,v", FAR)
+@pytest.mark.parametrize("size", [1e6, 1e8, 1e12])
+@pytest.mark.parametrize("where", ["row", "class", "feature"])
+def test_one_large_row_or_class_spoils_no_other(ops, n, h, v, size, where):
+    """float32: a row, or a class, `size` times the others (a class that is so far below that no row has it), or one feature
+    that is large in one row and that no class looks at.  All the other rows' and classes' results keep their own bounds."""
+    x, w, b, t = make(n, h, v, "f32", "index", seed=n + h + v)
+    rest = torch.ones(n, dtype=torch.bool, device="cuda")
+    if where == "row":
+        x[2] *= size
+        rest[2] = False                                             # (whose logits are known to no better than size * f)
+    elif where == "class":
+        x[:, 0] = 1.0
+        w[:, 0] = 0.0
+        w[v // 2] = 0.0
+        w[v // 2, 0] = -size
+        t[t == v // 2] = 0
+    else:
+        w[:, 1] = 0.0
+        x[2, 1] = size
+    ref = elementwise(x, w, b, t, torch.ones(n, device="cuda"))
+    for dx, dw, db, loss in ((lambda r: r[2:] + (r[0],))(ops.linear_cross_entropy_grad(x, w, t, b, reduction="none")),
+                             (lambda r: r[1:] + (r[0],))(autograd(ops, x, w, t, b, reduction="none"))):
+        within("loss", loss, *ref["loss"], rest)
+        within("d_hidden", dx, *ref["d_hidden"], rest)
+        within("d_weight", dw, *ref["d_weight"])
+        within("d_bias", db, *ref["d_bias"])
+    within("loss alone", ops.linear_cross_entropy(x, w, t, b, reduction="none"), *ref["loss"], rest)
+
+
+@pytest.mark.parametrize("n,h,v", FAR)
+def test_operands_of_every_magnitude(ops, n, h, v):
+    """float32: rows of 2^-60 to 1 and classes of 2^-20 to 1 of the ordinary size, an empty row, and a row that holds the largest
+    number, where no class looks at it, and 2^-100, which every class raises to 1 or -1."""
+    x, w, b, t = make(n, h, v, "f32", "index", seed=n + h + v)
+    x *= torch.exp2(torch.linspace(-60, 0, n, device="cuda").round())[:, None]
+    w *= torch.exp2(torch.linspace(0, -20, v, device="cuda").round())[:, None]
+    x[0], x[1], x[:, 1] = 0.0, 0.0, 0.0
+    x[1, 0], x[1, 1], w[:, 0], w[:, 1] = 3.4028234e38, 2.0 ** -100, 0.0, 2.0 ** 100 * torch.sign(w[:, 1])
+    ref = elementwise(x, w, b, t, torch.ones(n, device="cuda"))
+    r = ops.linear_cross_entropy_grad(x, w, t, b, reduction="none")
+    for name, got in (("loss", r.loss), ("d_hidden", r.d_hidden), ("d_weight", r.d_weight), ("d_bias", r.d_bias)):
+        within(name, got, *ref[name])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("kind", ["index", "probs"])
+@pytest.mark.parametrize("n,h,v", FAR)
+def test_gradients_of_classes_that_are_hardly_ever_taken(ops, dtype, kind, n, h, v):
+    """Classes of probability 1e-5 to 1e-25 in every row, next to ordinary ones: their rows of d_weight keep their digits, in one call
+    and in two.  (Half precision with its gradients raised by 2^14; what falls below its own numbers counts as theirs.)"""
+    x, w, b, t = make(n, h, v, dtype, kind, seed=n + h + v)
+    rare = torch.arange(3, v, 7, device="cuda")
+    b[rare] = -torch.linspace(5.0, 50.0 if dtype == "f32" else 24.0, len(rare), device="cuda").to(b.dtype)
+    if kind == "index":
+        t = torch.where(t % 7 == 3, t - 1, t)
+    else:
+        t[:, rare] = 0.0
+    scale = 16384.0 if dtype == "f16" else 1.0
+    ref = elementwise(x, w, b, t, torch.full((n,), scale, device="cuda"))
+    for dw, db in (ops.linear_cross_entropy_grad(x, w, t, b, reduction="sum", grad_loss=scale)[3:],
+                   autograd(ops, x, w, t, b, scale, reduction="sum")[2:]):
+        within("d_weight", dw, *ref["d_weight"], rare)
+        within("d_bias", db, *ref["d_bias"], rare)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("kind", ["index", "probs"])
+@pytest.mark.parametrize("n,h,v", PATHS + [(300, 130, 2050), (1500, 64, 6000), (9000, 24, 500)])
+def test_rows_of_very_different_weight(ops, dtype, kind, n, h, v):
+    """reduction='none' with weights from 1e-30 (half precision: 1e-6) to 1: every row of d_hidden against its own size."""
+    x, w, b, t = make(n, h, v, dtype, kind, seed=n + h + v)
+    g = torch.logspace(-30 if dtype != "f16" else -6, 0, n, device="cuda")
+    g[::2] *= -1.0
+    if kind == "probs":
+        t = t * torch.logspace(0, -6, n, device="cuda")[:, None]
+    if dtype == "f16":
+        g *= 4096.0
+    ref = elementwise(x, w, b, t, g)
+    r = ops.linear_cross_entropy_grad(x, w, t, b, reduction="none", grad_loss=g)
+    for name, got in (("loss", r.loss), ("d_hidden", r.d_hidden), ("d_weight", r.d_weight), ("d_bias", r.d_bias)):
+        within(name, got, *ref[name])
