@@ -505,9 +505,24 @@ __device__ inline Pack<float, 4> four_of(const float *row, long long v, long lon
     return p;
 }
 
-// exp(l - the span's maximum) on its way to becoming D in the same place: half precision (11 bits; what lies below 2^-24 of
-// the span's largest probability is off by 2^-25 of that) where D will be 16 bits, float32 where D will be parts
-template <typename Op> using Expo = std::conditional_t<Op::Grad::parts == 1, _Float16, float>;
+// exp(l - the span's maximum) on its way to becoming D in the same place: float32 where D will be parts.  Where D will be 16
+// bits it is a code of 16 bits, which D's own rounding to 8 bits lets it be, with float32's range: a number from 2^-39 to 1
+// keeps ten bits after its first (off by 2^-11 of itself at most), one below keeps eight (2^-9); the codes of both run on from
+// each other.  (Half precision, which this was, has nothing below 2^-24.)
+template <typename Op> using Expo = std::conditional_t<Op::Grad::parts == 1, uint16_t, float>;
+constexpr uint32_t kFine = 88u << 23, kFineCodes = (kFine >> 13) - (kFine >> 15);        // 2^-39
+template <typename E>
+__device__ inline E expo(float x)                             // 0 <= x <= 1; a NaN: any code (the row's factor is NaN)
+{
+    if constexpr (sizeof(E) == 4) return x;
+    const uint32_t b = __builtin_bit_cast(uint32_t, x);
+    return (E)(b >= kFine ? ((b + (1u << 12)) >> 13) - kFineCodes : (b + (1u << 14)) >> 15);
+}
+__device__ inline float expo_of(float e) { return e; }
+__device__ inline float expo_of(uint16_t e)
+{
+    return __builtin_bit_cast(float, e >= kFine >> 15 ? ((uint32_t)e + kFineCodes) << 13 : (uint32_t)e << 15);
+}
 // where the image of D (the exponentials on their way there: counted in their own size) holds column c
 template <typename Op, typename T>
 __device__ inline T *place(void *d, long long row, long long ldd, long long c)
@@ -613,7 +628,7 @@ __device__ inline void logits_tile(const CeArgs &a, long long m_first, int span_
                 for (int i = 0; i < 4; i++) {
                     const float x = __builtin_amdgcn_exp2f((acc[mt][nt][i] - base) * kLog2e);
                     s += x;
-                    keep.v[i] = (E)x;
+                    keep.v[i] = expo<E>(x);
                 }
                 if (a.d && live && vw + mt * 16 < dpad) *reinterpret_cast<Pack<E, 4> *>(place<Op, E>(a.d, row, a.ldd, vw + mt * 16)) = keep;
             }
@@ -959,7 +974,7 @@ __global__ __launch_bounds__(256) void fix_kernel(FixArgs a)
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const bool out = c + i >= a.classes;
-            float q = (float)v[i] * f;
+            float q = expo_of((E)v[i]) * f;
             if (a.probs) q -= pv.v[i];
             else if (t == i) q -= 1.f;
             q = g == 0.f || out ? 0.f : q * g;                                  // a row that counts for nothing: zero whatever it holds

@@ -137,11 +137,11 @@ def test_loss_and_entropy_of_exact_logits(ops, dtype, n, h, v, offset, peak):
 
 
 # ---------------------------------------------------------------- operands, probabilities and weights far apart
-def elementwise(x, w, b, t, g, kept=0.0):
+def elementwise(x, w, b, t, g, kept=False):
     """{name: (value in float64, bound)} of loss rows, d_hidden, d_weight and d_bias under sum g_i loss_i, every bound an
     element's own: products and sums of (H + 8) f sum|x w| in a logit (float32 leaves out 2 f of it); a probability by what its logit
-    and the others' (weighted by their probabilities) may be off, by (2 |l - max| + 100) f of itself, and by `kept` of itself where one call keeps
-    exponentials in 16 bits; the gradient at the logits D by its rounding (bfloat16 half a step, half precision 2^-17); the products by what they
+    and the others' (weighted by their probabilities) may be off, by (2 |l - max| + 100) f of itself, and where one call keeps
+    exponentials in 16 bits (`kept`) by 2^-11, or below 2^-39 of its neighbours' largest 2^-9, of itself; the gradient at the logits D by its rounding (bfloat16 half a step, half precision 2^-17); the products by what they
     leave out (float32 2 f, half precision 2^-16), (K + 40) f, and the result's rounding."""
     dt = x.dtype
     n, h = x.shape
@@ -157,7 +157,7 @@ def elementwise(x, w, b, t, g, kept=0.0):
     lse = torch.logsumexp(l, 1, keepdim=True)
     p = torch.exp(l - lse)
     el = (p * dl).sum(1, keepdim=True)
-    own = p * ((2 * (l - m).abs() + 100) * F + kept)
+    own = p * ((2 * (l - m).abs() + 100) * F + (torch.where(p < 2.0 ** -38 * p.max(1, keepdim=True).values, 2.0 ** -9, 2.0 ** -11) if kept else 0.0))
     up = torch.exp((l - lse + dl + el).clamp(max=0.0))               # a row with one class left: the others' bounds are what it may lose
     top = l == m
     low = torch.maximum(torch.exp(l - lse - dl - el), torch.where(top, 1 - torch.where(top, 0.0, up).sum(1, keepdim=True), 0.0))
@@ -268,6 +268,42 @@ def test_rows_of_very_different_weight(ops, dtype, kind, n, h, v):
     if dtype == "f16":
         g *= 4096.0
     ref = elementwise(x, w, b, t, g)
+    r = ops.linear_cross_entropy_grad(x, w, t, b, reduction="none", grad_loss=g)
+    for name, got in (("loss", r.loss), ("d_hidden", r.d_hidden), ("d_weight", r.d_weight), ("d_bias", r.d_bias)):
+        within(name, got, *ref[name])
+
+
+@pytest.mark.parametrize("kind", ["index", "probs"])
+@pytest.mark.parametrize("n,h,v", FAR + [(64, 72, 4100)])
+def test_bfloat16_gradients_of_classes_that_are_hardly_ever_taken(ops, kind, n, h, v):
+    """As above in bfloat16, down to 1e-34: classes next to ordinary ones, and a run of 600 of them with one ordinary class in it."""
+    x, w, b, t = make(n, h, v, "bf16", kind, seed=n + h + v)
+    rare = torch.arange(3, v, 7, device="cuda")
+    b[rare] = -torch.linspace(5.0, 70.0, len(rare), device="cuda").to(b.dtype)
+    if v > 2000:
+        b[1001:1600] = -30.0
+        rare = torch.cat([rare, torch.arange(1001, 1600, device="cuda")])
+    common = torch.ones(v, dtype=torch.bool, device="cuda")
+    common[rare] = False
+    if kind == "index":
+        t = common.nonzero()[:, 0][t % int(common.sum())]
+    else:
+        t[:, rare] = 0.0
+    g = torch.ones(n, device="cuda")
+    for kept, (dw, db) in ((True, ops.linear_cross_entropy_grad(x, w, t, b, reduction="sum")[3:]), (False, autograd(ops, x, w, t, b, reduction="sum")[2:])):
+        ref = elementwise(x, w, b, t, g, kept)
+        within("d_weight", dw, *ref["d_weight"])
+        within("d_bias", db, *ref["d_bias"])
+        assert bool((dw[rare] != 0).any(1).all())
+
+
+@pytest.mark.parametrize("kind", ["index", "probs"])
+@pytest.mark.parametrize("n,h,v", PATHS + [(300, 130, 2050), (1500, 64, 6000), (9000, 24, 500)])
+def test_bfloat16_rows_of_very_different_weight(ops, kind, n, h, v):
+    x, w, b, t = make(n, h, v, "bf16", kind, seed=n + h + v)
+    g = torch.logspace(-30, 0, n, device="cuda")
+    g[::2] *= -1.0
+    ref = elementwise(x, w, b, t, g, True)
     r = ops.linear_cross_entropy_grad(x, w, t, b, reduction="none", grad_loss=g)
     for name, got in (("loss", r.loss), ("d_hidden", r.d_hidden), ("d_weight", r.d_weight), ("d_bias", r.d_bias)):
         within(name, got, *ref[name])
