@@ -50,7 +50,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropoutArgs a, long long b
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
         const long long row = a.rows == 1 ? 0 : i / blocks_per_row, j = i - row * blocks_per_row;
         const unsigned long long e0 = a.first + (unsigned long long)row * a.step;
-        const unsigned long long blk = (e0 >> 3) + (unsigned long long)j;
+        const unsigned long long blk = ((e0 >> 3) + (unsigned long long)j) & ((1ull << 61) - 1);   // (numbers are modulo 2^64)
         const long long col0 = (long long)(blk * 8 - e0);                   // column of the block's first element: -7 .. cols
         if (col0 >= a.cols) continue;
         uint32_t c[4] = {(uint32_t)blk, (uint32_t)(blk >> 32), (uint32_t)off, (uint32_t)(off >> 32)};

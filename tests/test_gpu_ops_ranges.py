@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_ops import DT, F, PATHS, half_step, make
+from test_gpu_ops import DT, F, PATHS, half_step, make, philox
 
 pytestmark = pytest.mark.gpu
 
@@ -307,3 +307,23 @@ def test_bfloat16_rows_of_very_different_weight(ops, kind, n, h, v):
     r = ops.linear_cross_entropy_grad(x, w, t, b, reduction="none", grad_loss=g)
     for name, got in (("loss", r.loss), ("d_hidden", r.d_hidden), ("d_weight", r.d_weight), ("d_bias", r.d_bias)):
         within(name, got, *ref[name])
+
+
+# ---------------------------------------------------------------- dropout's element numbers
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("cols,first,step", [(16, (1 << 60) - 2, 1), (7, ((1 << 64) - 2) // 7 - 1, 1), (13, (1 << 64) - 3, 1), (13, (1 << 64) - 3, 5),
+                                             (100, (1 << 64) - 1, (1 << 64) - 1), (8, (1 << 61) - 1, 1)])
+def test_dropout_numbers_elements_modulo_2_to_the_64(ops, dtype, cols, first, step):
+    """Element (r, c) is number ((first + r step) cols + c) modulo 2^64, whatever the layout of the rows."""
+    rows, seed, offset = 6, 77, 5
+    x = (torch.rand(rows, cols, device="cuda") + 1).to(DT[dtype])
+    keep = torch.empty(rows, cols, dtype=torch.bool)
+    for r in range(rows):
+        for c in range(cols):
+            at = ((first + r * step) * cols + c) % (1 << 64)
+            keep[r, c] = bool(philox(at - at % 8, 8, seed, offset)[at % 8] >= 32768)
+    far = torch.zeros(rows, cols + 3, dtype=x.dtype, device="cuda")
+    far[:, :cols] = x
+    for view in (x, far[:, :cols]):
+        y = ops.dropout(view, 0.5, seed, offset, first_row=first, row_step=step)
+        assert torch.equal(y, torch.where(keep.cuda(), 2 * x, torch.zeros_like(x)))
