@@ -5,11 +5,12 @@ azg_linear_ce).  They run on the tensors' device and its current stream, like Py
 dropout() and linear_cross_entropy() take part in autograd.  dropout_grad() and linear_cross_entropy_grad() are
 the same without it -- loss and gradients in one call, no graph of nodes -- and are what to capture into a HIP
 graph; the autograd forms refuse to be captured when an input wants a gradient (accumulating into leaves that
-an eager graph also holds cannot be captured)."""
+an eager graph also holds cannot be captured).  Forward-mode differentiation and second derivatives are refused."""
 import ctypes as C
 from collections import namedtuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -23,6 +24,8 @@ LinearCrossEntropyGrad = namedtuple("LinearCrossEntropyGrad", "loss entropy d_hi
 def _check_tensor(name, t, dtype=None, device=None):
     if not torch.is_tensor(t):
         raise TypeError("%s must be a tensor" % name)
+    if getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None:   # (its tangent would be lost)
+        raise NotImplementedError("%s carries a forward-mode tangent: these operators have no forward-mode derivative" % name)
     if not t.is_cuda:
         raise ValueError("%s must be a CUDA tensor: the operators have no CPU form" % name)
     if dtype is None:

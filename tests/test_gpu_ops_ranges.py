@@ -327,3 +327,26 @@ def test_dropout_numbers_elements_modulo_2_to_the_64(ops, dtype, cols, first, st
     for view in (x, far[:, :cols]):
         y = ops.dropout(view, 0.5, seed, offset, first_row=first, row_step=step)
         assert torch.equal(y, torch.where(keep.cuda(), 2 * x, torch.zeros_like(x)))
+
+
+# ---------------------------------------------------------------- derivatives that are not there
+def test_forward_mode_and_second_derivatives_are_refused(ops):
+    import torch.autograd.forward_ad as fw
+    x, w, b, t = make(8, 16, 9, "f32")
+    p = torch.rand(8, 9, device="cuda")
+    g = torch.ones(8, device="cuda")
+    with fw.dual_level():
+        def dual(q):
+            return fw.make_dual(q, torch.ones_like(q))
+        for call in (lambda: ops.dropout(dual(x), 0.1, 1), lambda: ops.dropout(x, 0.1, 1, residual=dual(x)), lambda: ops.dropout_grad(dual(x), 0.1, 1),
+                     lambda: ops.linear_cross_entropy(dual(x), w, t, b), lambda: ops.linear_cross_entropy(x, dual(w), t, b),
+                     lambda: ops.linear_cross_entropy(x, w, t, dual(b)), lambda: ops.linear_cross_entropy(x, w, dual(p), b),
+                     lambda: ops.linear_cross_entropy(x.clone().requires_grad_(), dual(w), t, b),
+                     lambda: ops.linear_cross_entropy_grad(x, w, t, b, reduction="none", grad_loss=dual(g))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        ops.linear_cross_entropy(x, w, t, b)                        # without a tangent inside a dual level: as ever
+    leaf = x.clone().requires_grad_()
+    first, = torch.autograd.grad(ops.linear_cross_entropy(leaf, w, t, b), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        first.sum().backward()

@@ -106,3 +106,18 @@ def test_python_forms_need_a_gpu():
     if not torch.cuda.is_available():                               # an error code, not a crash
         from alphazero_gomoku_amd import _lib
         assert _lib.load().azg_dropout(C.byref(dropout_args(_lib))) == -2
+
+
+def test_forward_mode_is_refused_without_a_gpu():
+    import torch.autograd.forward_ad as fw
+    from alphazero_gomoku_amd import ops
+    x, w, t = torch.randn(4, 8), torch.randn(5, 8), torch.zeros(4, dtype=torch.int64)
+    with fw.dual_level():
+        d = fw.make_dual(x, torch.ones_like(x))
+        assert not d.requires_grad
+        for call in (lambda: ops.dropout(d, 0.1, 1), lambda: ops.dropout_grad(d, 0.1, 1), lambda: ops.linear_cross_entropy(d, w, t),
+                     lambda: ops.linear_cross_entropy_grad(d, w, t)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda q: ops.dropout(q, 0.1, 1), (x,), (x,))
