@@ -102,11 +102,13 @@ def train_step_tensors(module, optimizer, s, p, z, lr, reduce_fn=None, dropout=N
 
 class PolicyValueNet(object):
     def __init__(self, board_width, board_height, model_file=None, use_gpu=True, device=0, native_train=True,
-                 dropout=0.0, dropout_seed=0):
+                 dropout=0.0, dropout_seed=0, dropout_step=0):
         if not 0.0 <= float(dropout) < 1.0:
             raise ValueError("dropout must lie in [0, 1)")
         if not 0 <= int(dropout_seed) < 1 << 64:
             raise ValueError("dropout_seed must be an integer from 0 to 2**64 - 1")
+        if not 0 <= int(dropout_step) < 1 << 62:
+            raise ValueError("dropout_step must be an integer from 0 to 2**62 - 1")
         if board_width != board_height:
             raise ValueError("only square boards are supported by the HIP engine")
         if not torch.cuda.is_available():
@@ -125,12 +127,14 @@ class PolicyValueNet(object):
         # (the two keep separate optimiser states: use one or the other on a net)
         self.native_train = bool(native_train)
         # dropout: probability with which train_step drops the features that the heads' fully connected layers read (0: the
-        # reference's step); the mask is a function of dropout_seed, the step's number and the position in the mini-batch
+        # reference's step); the mask is a function of dropout_seed, the step's number and the position in the mini-batch.
+        # A weight file holds no step number: a run that goes on from one with its old seed gives dropout_step (the property of
+        # the net that was saved), or it draws its first masks again.
         self.dropout, self.dropout_seed = float(dropout), int(dropout_seed)
         self._adam = None            # (grad, m, v) flat float32 vectors in state_dict order, step count
         self._ptr_cache = None
         self._adam_step = 0
-        self._dropout_step = 0       # training steps done either way: what the masks are numbered by
+        self._dropout_step = int(dropout_step)       # training steps done either way: what the masks are numbered by
         self._eval_engine = None
         self._eval_version = -1
 
@@ -241,6 +245,11 @@ class PolicyValueNet(object):
             ts = [p.data for p in (dict(self.policy_value_net.named_parameters())[k] for k in PARAM_ORDER)]
             self._ptr_cache = ((C.c_void_p * 16)(*[t.data_ptr() for t in ts]), ts)
         return self._ptr_cache
+
+    @property
+    def dropout_step(self):
+        """Training steps done so far, those before dropout_step= among them: what to save beside the weights to go on with."""
+        return self._dropout_step
 
     def _dropout_args(self, step):
         """(p, seed, offset, first_row, row_step) of a training step; ranks hold every world-th row of the mini-batch."""

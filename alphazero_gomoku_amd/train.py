@@ -58,7 +58,9 @@ class TrainPipeline:
                       learning rate follow each other on a net that has not moved yet; with this and the
                       ceiling of 1, twenty of twenty differently seeded runs learned.
     dropout           probability with which a training step drops the features of the two heads (PolicyValueNet's
-                      dropout, seeded with seed0), for a net created here; 0 is the reference's step."""
+                      dropout, seeded with seed0), for a net created here; 0 is the reference's step
+    dropout_step      training steps that a net read from init_model has behind it (PolicyValueNet.dropout_step of the
+                      run it goes on from): the masks go on from there instead of repeating."""
 
     @staticmethod
     def controller_defaults(play_batch_size, max_lr_multiplier=None, zero_head_biases=None):
@@ -76,7 +78,7 @@ class TrainPipeline:
                  play_batch_size=1, epochs=5, kl_targ=0.02, check_freq=50, game_batch_num=1500,
                  n_parallel=1024, device=0, seed0=0, policy_value_net=None, pure_mcts_playout_num=1000,
                  updates_per_batch=1, continuous=False, rng=None, max_lr_multiplier=None, zero_head_biases=None,
-                 dropout=0.0):
+                 dropout=0.0, dropout_step=0):
         import torch
         from .net import PolicyValueNet
         self.board_width, self.board_height, self.n_in_row = board_width, board_height, n_in_row
@@ -94,10 +96,11 @@ class TrainPipeline:
         self.best_win_ratio = 0.2                                            # train.py:88
         self.pure_mcts_playout_num = pure_mcts_playout_num
         fresh = policy_value_net is None and not init_model
-        if policy_value_net is not None and dropout:
-            raise ValueError("dropout is for a net created here: give the net passed in its own")
+        if policy_value_net is not None and (dropout or dropout_step):
+            raise ValueError("dropout and dropout_step are for a net created here: give the net passed in its own")
         self.policy_value_net = policy_value_net or PolicyValueNet(board_width, board_height, model_file=init_model,
-                                                                   device=device, dropout=dropout, dropout_seed=seed0 % (1 << 64))
+                                                                   device=device, dropout=dropout, dropout_seed=seed0 % (1 << 64),
+                                                                   dropout_step=dropout_step)
         self.zeroed_head_biases = bool(fresh and want_zero)      # reported by the training program
         if self.zeroed_head_biases:
             self.policy_value_net.zero_head_biases()
@@ -513,6 +516,7 @@ def main(argv=None):
                           "win_ratio_vs_rollout_player": final, "rollout_playouts": tp.pure_mcts_playout_num,
                           "lr_multiplier": tp.lr_multiplier, "max_lr_multiplier": tp.max_lr_multiplier,
                           "zero_head_biases": tp.zeroed_head_biases, "dropout": args.dropout,
+                          "dropout_step": tp.policy_value_net.dropout_step,
                           "reference_controller": tp.max_lr_multiplier == 10.0 and not tp.zeroed_head_biases,
                           "best_win_ratio": tp.best_win_ratio,
                           "evaluations_batch_playouts_win_ratio": tp.eval_history,
