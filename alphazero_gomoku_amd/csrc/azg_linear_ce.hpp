@@ -465,7 +465,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackList list)
             for (int k = 0; k < N; k++) *reinterpret_cast<bx8 *>(o + k * 64) = h[k];
         };
         if constexpr (sizeof(In) == 4) in_parts(std::integral_constant<int, 3>{});
-        else if (a.parts == 2) in_parts(std::integral_constant<int, 2>{});
+        else if (std::is_same_v<In, _Float16> && a.parts == 2) in_parts(std::integral_constant<int, 2>{});
         else *reinterpret_cast<Pack<In, 8> *>(static_cast<In *>(a.img) + r * a.ldi + c) = *reinterpret_cast<const Pack<In, 8> *>(v);
     }
 }
@@ -623,14 +623,18 @@ __device__ inline void logits_tile(const CeArgs &a, long long m_first, int span_
                     }
 #pragma unroll
             for (int mt = 0; mt < S::MT; mt++) {
-                Pack<E, 4> keep;
+                float x[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float x = __builtin_amdgcn_exp2f((acc[mt][nt][i] - base) * kLog2e);
-                    s += x;
-                    keep.v[i] = expo<E>(x);
+                    x[i] = __builtin_amdgcn_exp2f((acc[mt][nt][i] - base) * kLog2e);
+                    s += x[i];
                 }
-                if (a.d && live && vw + mt * 16 < dpad) *reinterpret_cast<Pack<E, 4> *>(place<Op, E>(a.d, row, a.ldd, vw + mt * 16)) = keep;
+                if (a.d && live && vw + mt * 16 < dpad) {
+                    Pack<E, 4> keep;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) keep.v[i] = expo<E>(x[i]);
+                    *reinterpret_cast<Pack<E, 4> *>(place<Op, E>(a.d, row, a.ldd, vw + mt * 16)) = keep;
+                }
             }
             if (a.probs) {
                 const float *pr = a.probs + min(row, a.n - 1) * a.ldp;
