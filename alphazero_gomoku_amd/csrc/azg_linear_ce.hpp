@@ -8,7 +8,7 @@
 //
 // Loss and gradients in one call, one piece: the logits' kernel also stores exp(l - the span's maximum), 16 bits an element
 // (float32: 4 bytes), and a pass in place turns that into the image of D once the rows' sums are known.  That costs two
-// passes over the image and saves a product: 4096 rows of 2048 features against 32000 classes (bfloat16) take 1.45 ms so, 1.79 ms
+// passes over the image and saves a product: 4096 rows of 2048 features against 32000 classes (bfloat16) take 1.40 ms so, 1.72 ms
 // with the logits made a second time.  A backward pass by itself, or of more than one piece, makes the logits again and
 // stores D at once.
 //
@@ -20,9 +20,12 @@
 // rounding of what the ones before it leave.  Eight bits a part and its sign hold all 24 bits of x, and every part has
 // float32's range of exponents, so nothing is scaled and what the other elements are does not matter.  A product of two
 // elements is the six products of parts i, j with i + j < 3; what is left out is at most 2^-24 of it (|x1| <= 2^-8 |x|,
-// |x2| <= 2^-17 |x|).  Gradients of half precision take two parts -- all of an operand's 11 bits; the gradient at the logits is
+// |x2| <= 2^-17 |x|).  That is twice the matrix work of two half-precision parts, which have neither the range nor, below 2^-17 of
+// their tensor's largest element, the bits (2048 x 1024 x 32000 with gradients: 2.1 ms, 1.15 so).  Gradients of half precision take two parts -- all of an operand's 11 bits; the gradient at the logits is
 // off by 2^-17 of itself -- and three products, which leave out 2^-16: half precision itself has not the range for
-// probabilities.  bfloat16 is one part.  An image row holds blocks of 64 columns, 64 elements of part 0, then of part 1, ...; a
+// probabilities (2048 x 1024 x 32000: 1.0 ms, 0.44 with one half-precision number, which loses classes below 2^-39).  bfloat16
+// is one part: its gradient at the logits has the type's own 8 bits, half a step of which the results are rounded by anyway, and
+// float32's range; a second part would make three products of each of the gradients' two.  An image row holds blocks of 64 columns, 64 elements of part 0, then of part 1, ...; a
 // product walks over the pairs of parts of one block of k and then over the blocks, every pair a stage of its own.
 #pragma once
 #include <hip/hip_runtime.h>
@@ -64,8 +67,9 @@ template <> struct Frag<__bf16> {
 
 // ---------------------------------------------------------------- the tile product
 // Bound by the matrix cores and, behind them, by the latency of loads: at 8192 x 4096 x 65536 in bfloat16 the two gradients run
-// at 1.36 PFLOP/s and the logits, with their epilogue, at 1.24 (a library's plain product of this size: 1.45); counters at
-// 4096 x 2048 x 32000: matrix cores busy 69 % and 64 % of the time, no bank conflict in LDS.  Measured and not taken: 128 x 128
+// at 1.35 PFLOP/s and the logits, with their epilogue, at 1.22 (a library's plain product of this size: 1.45); counters at
+// 4096 x 2048 x 32000: matrix cores busy 68 % and 61 % of the time, no bank conflict in LDS.  In float32, 2048 x 1024 x 32000, the
+// products of parts run at 1.25 and 1.39 PFLOP/s, busy 68 % and 71 %.  Measured and not taken: 128 x 128
 // tiles for the logits, two workgroups a CU (the whole call 5 % slower there, scores of 2048 x 1024 x 50001 14 %), four waves with 128 x 128 each (the accumulators
 // spill into copies), stages of 32 k with longer rings, workgroups that keep their CU and walk over tiles (no overlap gained:
 // all waves reach their epilogue together).
@@ -91,7 +95,7 @@ struct TileShape {
     static constexpr int MT = TM / WM / 16, NT = TN / WN / 16;
     // stages of A and of B in LDS: the 256 x 256 tile takes all of a CU's 160 KB, 128 x 128 leaves room for a second
     // workgroup; the tile for few rows, and 64 x 64 where there are few of them (one wave across m), do little but wait for
-    // memory and keep more in flight (550 x 3717 x 488 float32 with gradients 101 -> 78 us; where three workgroups fit a CU
+    // memory and keep more in flight (550 x 3717 x 488 with gradients, float32 190 -> 159 us, bfloat16 65 -> 55; where three workgroups fit a CU
     // they hide each other's waits, and longer rings cost 8 %: 974 x 2924 x 2167)
     static constexpr int ring_a = TN <= 32 ? 5 : TN == 64 && WM == 1 ? 4 : 3, ring_b = TN <= 32 ? 5 : TN == 64 && WM == 1 ? 4 : 2;
     static constexpr int bytes_a = TM * 128, bytes_b = TN * 128, lds_bytes = ring_a * bytes_a + ring_b * bytes_b;
@@ -427,7 +431,8 @@ __device__ inline void split_parts(float x, __bf16 (&part)[N])
     }
 }
 
-// Images of up to four matrices, zeros in the padding: a thread eight columns of a row.
+// Images of up to four matrices, zeros in the padding: a thread eight columns of a row.  Bound by memory: 139 MB of float32
+// read and 209 MB of parts written in 53 us, 6.5 TB/s.
 template <typename In>
 __global__ __launch_bounds__(256) void pack_kernel(PackList list)
 {
@@ -532,8 +537,8 @@ __device__ inline T *place(void *d, long long row, long long ldd, long long c)
 
 // A tile of logits; a lane holds four classes of a row next to each other (classes are the tile's m), sixteen rows a fragment.
 // Forward (GRAD false): span statistics and, where asked for, the exponentials; GRAD: D from the rows' statistics.  A 256 x 256
-// tile takes 9.7 us around one stage of 64 features (49152 classes of 64 features: 58 us, six rounds; with a bias 11): filling the
-// rings and this epilogue, an exponential an element on top of the maximum, the sum and the stores; and 1.4 us a stage more.
+// tile takes 10 us around one stage of 64 features (2048 x 64 x 49152: 60 us, six rounds; with a bias 10.7): filling the
+// rings and this epilogue, an exponential an element on top of the maximum, the sum and the stores; and 1.1 us a stage more.
 template <typename Op, int TM, int TN, int WM, int WN, bool GRAD>
 __device__ inline void logits_tile(const CeArgs &a, long long m_first, int span_first, int mtiles, int ntiles, unsigned wg, char *lds)
 {
@@ -746,7 +751,7 @@ __global__ __launch_bounds__(WM * WN * 64) void logits_kernel(CeArgs a)
     logits_tile<Op, TM, TN, WM, WN, GRAD>(a, 0, 0, a.mtiles, a.ntiles, blockIdx.x, lds);
 }
 // The loss alone, where 256 x 256 tiles of all classes would leave the last round of the CUs mostly empty: whole rounds of them,
-// and 128 x 128 tiles of the classes behind.  2048 x 1024 x 50001: 1536 and 112 tiles, 199 us instead of 210.
+// and 128 x 128 tiles of the classes behind.  2048 x 1024 x 50001: 1536 and 112 tiles, 206 us instead of 218.
 template <typename Op>
 __global__ __launch_bounds__(512) void logits_mixed_kernel(CeArgs a)
 {
@@ -767,7 +772,7 @@ struct RowArgs {
     float *ent;                   // [n] or null
 };
 // One wave per row: join the spans' sums, each relative to its span's maximum m_j, in a fixed order; relative to m they are
-// s_j f, (e_j + (m_j - m) s_j) f and t_j + (m_j - m) sum pi, f = exp(m_j - m).  Latency: 8 us for 2048 rows of 392 spans, 7 us for
+// s_j f, (e_j + (m_j - m) s_j) f and t_j + (m_j - m) sum pi, f = exp(m_j - m).  Latency: 9 us for 2048 rows of 392 spans, 8 us for
 // one row of 2048.
 __device__ inline void shift(float m, float base, float &s, float &e, float &tl, float ts)
 {
@@ -1061,7 +1066,7 @@ __device__ inline void grad_tile(const GradArgs &a, unsigned wg, char *lds)
 
 // dX = D W (D as it lies) by the first wgs_x workgroups, dW = D^T X (D transposed) by the others; the other factor, W or X,
 // is transposed in both.  One launch, so that the workgroups of the one fill the CUs that the other leaves at its end: 4096 rows,
-// 2048 features, 32000 classes 0.87 ms, 1.22 PFLOP/s (1128 workgroups, four and a half rounds of the CUs).
+// 2048 features, 32000 classes 0.82 ms, 1.31 PFLOP/s (1128 workgroups, four and a half rounds of the CUs).
 template <typename Op, int TM, int TN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64) void grads_kernel(GradArgs x, GradArgs w, unsigned wgs_x)
 {

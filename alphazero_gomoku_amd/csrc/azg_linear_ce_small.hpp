@@ -9,7 +9,7 @@
 // join through LDS.  Operands come straight from memory (L2) into the fragments of v_mfma_f32_16x16x4_f32: a lane of group
 // g = lane / 16 holds k = 4 g + j for the j-th of four instructions, so that where k is contiguous the four are one load.
 // Bound by latency, of launches and of loads from the L2: 512 positions on 8 x 8 (256 features, 64 classes) take 5 + 4 + 8 us, on
-// 15 x 15 (900, 225) 11 + 5 + 17 us; the tiled path takes 32 us and 44 us for them.
+// 15 x 15 (900, 225) 11 + 5 + 17 us; the tiled path takes 33 us and 58 us for them.
 #pragma once
 #include "azg_linear_ce.hpp"
 
@@ -231,8 +231,8 @@ __global__ __launch_bounds__(kSmallWaves * 64) void small_logits_kernel(SmallArg
 
 // The loss alone of at most 32 rows over many classes, for operands that the tiled path would have to copy first (float32, rows
 // that do not start at 16 bytes): the weights are read once, as they lie, and a tile's logits leave it as the statistics of a span
-// of 32 classes (rows_kernel joins them).  4 x 1892 x 50047 half precision: 44 us, 106 with a copy; 27 x 711 x 26667 float32:
-// 37 us, 72 with a copy in two parts.
+// of 32 classes (rows_kernel joins them).  4 x 1892 x 50047 half precision: 50 us, 112 with a copy; 27 x 711 x 26667 float32:
+// 40 us, 81 with a copy in parts.
 struct FewArgs {
     const void *x, *w, *bias;
     long long xs, ws;

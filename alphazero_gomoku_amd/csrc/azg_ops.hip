@@ -99,13 +99,14 @@ extern "C" int azg_dropout(const azg_dropout_args *a)
 namespace {
 
 // Which problems the three-launch float32 path takes.  Measured, the tiled path against it, microseconds of GPU time:
-//   float32, loss and gradients: 512 x 256 x 64 (rows, features, classes) 32 / 17, 512 x 900 x 225 44 / 32, 256 x 1024 x 1024
-//     53 / 51, then 2048 x 1024 x 256 62 / 94; with long sums or few tiles it falls behind: 32 x 1024 x 4096 56 / 71,
-//     4096 x 64 x 64 35 / 79;
-//   float32, the loss alone: 512 x 1024 x 256 33 / 18, 512 x 2048 x 512 51 / 29, 4096 x 64 x 64 22 / 16, then 16384 x 64 x 64
-//     35 / 47, 8 x 64 x 32768 29 / 58;
-//   16 bits, whose matrix instructions are sixteen times as fast as float32's: 128 x 256 x 1024 25 / 21, 512 x 256 x 64 22 / 17,
-//     then 512 x 1024 x 256 27 / 33, 16 x 512 x 4096 24 / 48 (the loss alone 13 / 11, 13 / 10, 16 / 17, 13 / 17).
+//   float32, loss and gradients: 512 x 256 x 64 (rows, features, classes) 33 / 17, 512 x 900 x 225 58 / 31, 256 x 1024 x 1024
+//     67 / 49, then 2048 x 1024 x 256 80 / 96; with long sums or few tiles it falls behind: 32 x 1024 x 4096 67 / 70,
+//     4096 x 64 x 64 34 / 79;
+//   float32, the loss alone: 512 x 1024 x 256 41 / 17, 512 x 2048 x 512 68 / 29, 4096 x 64 x 64 20 / 16, then 16384 x 64 x 64
+//     29 / 45, 40 x 64 x 32768 28 / 63;
+//   16 bits, whose matrix instructions are sixteen times as fast as float32's (bfloat16; half precision is a little slower
+//     tiled): 128 x 256 x 1024 26 / 21, 512 x 256 x 64 26 / 18, then 512 x 1024 x 256 28 / 33, 16 x 512 x 4096 25 / 47
+//     (the loss alone 13 / 11, 13 / 10, 16 / 17, 13 / 17).
 constexpr long long kSmallLogits = 1LL << 22;                 // 16 MB of float32
 bool takes_small(bool f32, bool backward, long long n, long long h, long long v)
 {

@@ -1,6 +1,10 @@
 """Operators of the training heads as functions of CUDA tensors: dropout whose mask is never stored, and the
-softmax cross entropy of a projection whose logits are never stored (include/azgomoku.h: azg_dropout,
-azg_linear_ce).  They run on the tensors' device and its current stream, like PyTorch's own operators.
+softmax cross entropy of a projection whose logits are not kept (include/azgomoku.h: azg_dropout, azg_linear_ce).
+While a call makes gradients it holds one array of rows x classes in place of the logits -- bfloat16 2 bytes an
+element, half precision 4, float32 6 -- of at most 1 GiB together with the copies of the weights that it needs, or
+of 1024 classes; beyond that it takes the classes in pieces and makes their logits twice.  A loss alone holds
+none; small problems hold at most 16 MB of float32 logits.  The operators run on the tensors' device and its
+current stream, like PyTorch's own.
 
 dropout() and linear_cross_entropy() take part in autograd.  dropout_grad() and linear_cross_entropy_grad() are
 the same without it -- loss and gradients in one call, no graph of nodes -- and are what to capture into a HIP
@@ -288,7 +292,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
 
 
 def linear_cross_entropy(hidden, weight, target, bias=None, *, reduction="mean", ignore_index=-100, return_entropy=False):
-    """Softmax cross entropy of hidden @ weight.T + bias against target, without storing the logits.
+    """Softmax cross entropy of hidden @ weight.T + bias against target; what a call holds meanwhile: see the module.
 
     hidden    float32, bfloat16 or float16 [..., features]; weight [classes, features] and bias [classes] of its type.
     target    int64 [...]: class numbers; rows with ignore_index count for nothing.  Or float32 [..., classes]:

@@ -297,9 +297,9 @@ int azg_train_epoch(azg_handle *h, int n, const float *states, const float *mcts
 #define AZG_BF16  1
 #define AZG_F16   2
 
-/* out = residual + (keep ? x * s : 0), rounded once: dropout with a mask that is a function of (seed, offset, element
+/* out = residual + (keep ? x * s : 0), in float32 and then rounded to the type: dropout with a mask that is a function of (seed, offset, element
  * number) and never stored.  T = round(65536 p); an element is kept when its 16 random bits are >= T; s = 65536 / (65536 - T)
- * (T = 65536 drops everything).  Element (r, c) has number (first_row + r * row_step) * cols + c modulo 2^64, so ranks that
+ * as a float32 (T = 65536 drops everything).  Element (r, c) has number (first_row + r * row_step) * cols + c modulo 2^64, so ranks that
  * hold rows of one batch draw one mask.  Bits: Philox4x32-10, counter = (number div 8, offset [+ *offset_dev]), key = seed;
  * element number mod 8 = q takes half-word q, low halves first.  The gradient at x is the same map of the gradient at out,
  * without residual.  A dropped element contributes exact zero whatever it holds.  out may be x or residual itself. */
@@ -334,7 +334,7 @@ int azg_dropout(const azg_dropout_args *a);
  * One call does the forward pass (loss not NULL), the backward pass (any of dx, dw, db not NULL), or both.  A backward pass
  * by itself takes the stats [n][4] (float32, 16-byte aligned, the caller's) that the forward pass of the same inputs wrote.
  * Sums, statistics and accumulators are float32 or wider and have float32's range, whatever the other rows and classes hold; a
- * product of two float32 numbers is made to 2^-23 of itself.  Infinities in x or w: the logits they reach are infinite or NaN.  The
+ * product of two float32 numbers is made to 2^-23 of itself (numbers below 2^-102: to 2^-126).  Infinities in x or w: the logits they reach are infinite or NaN.  The
  * gradient at the logits is rounded before the two products that use it, to 24 bits (AZG_F32), 16 (AZG_F16) or 8 (AZG_BF16), all
  * with float32's range; where one call makes loss and gradients in AZG_BF16 its softmax is rounded to 11 bits before that, to 9 where it
  * is below 2^-39 of the largest among the 128 classes around it.  Results do not depend on anything but the arguments and the alignment of x and w: the same bits every time.
