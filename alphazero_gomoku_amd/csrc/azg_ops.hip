@@ -242,7 +242,9 @@ int make_plan(const azg_linear_ce_args *a, Plan *p)
         p->vp = std::min<long long>(p->V, up_to((p->V + p->pieces - 1) / p->pieces, 256));
         p->pieces = (p->V + p->vp - 1) / p->vp;
     }
-    p->keep = p->forward && p->backward && p->pieces == 1;
+    // (against probabilities D is the difference of two numbers that training brings together: exponentials of 16 bits would leave
+    // little of it, and the logits are made again)
+    p->keep = p->forward && p->backward && p->pieces == 1 && !(a->probs && p->gparts == 1);
     p->ldd = image_stride(p->vp, p->gparts);
     p->lshape = pick_logits(p->vp, p->n, p->backward || f32, p->lparts > 1 ? p->ldl : 0);   // (float32 has no tile for few rows)
     const int pairs = p->gparts * (p->gparts + 1) / 2;
@@ -462,7 +464,7 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
             hipLaunchKernelGGL((few_rows_kernel<In>), dim3((unsigned)full), dim3(kSmallWaves * 64), 0, s, f);
             spans = full;
         } else for (long long i = 0; i < p.pieces; i++) {
-            OPS_TRY(piece(i, p.keep));
+            OPS_TRY(piece(i, p.backward && p.pieces == 1));
             c.part = reinterpret_cast<float2 *>(ws + p.part) + i * full * a->n;
             c.part_e = a->entropy ? f32(p.part_e) + i * full * a->n : nullptr;
             c.part_t = a->probs ? reinterpret_cast<float2 *>(ws + p.part_t) + i * full * a->n : nullptr;
@@ -507,7 +509,7 @@ int run_ce(const azg_linear_ce_args *a, const Plan &p)
     if (!p.backward) return AZG_OK;
 
     for (long long i = 0; i < p.pieces; i++) {
-        if (!p.keep) OPS_TRY(piece(i, true));
+        if (!p.forward || p.pieces > 1) OPS_TRY(piece(i, true));            // (else its images are there)
         const long long vn = c.classes;
         int dbparts;
         if (p.keep) {

@@ -336,7 +336,7 @@ int azg_dropout(const azg_dropout_args *a);
  * Sums, statistics and accumulators are float32 or wider and have float32's range, whatever the other rows and classes hold; a
  * product of two float32 numbers is made to 2^-23 of itself (numbers below 2^-102: to 2^-126).  Infinities in x or w: the logits they reach are infinite or NaN.  The
  * gradient at the logits is rounded before the two products that use it, to 24 bits (AZG_F32), 16 (AZG_F16) or 8 (AZG_BF16), all
- * with float32's range; where one call makes loss and gradients in AZG_BF16 its softmax is rounded to 11 bits before that, to 9 where it
+ * with float32's range; where one call makes loss and gradients against class numbers in AZG_BF16 its softmax is rounded to 11 bits before that, to 9 where it
  * is below 2^-39 of the largest among the 128 classes around it.  Results do not depend on anything but the arguments and the alignment of x and w: the same bits every time.
  * azg_linear_ce_workspace: bytes of workspace (256-byte aligned) the call needs with these very arguments, pointers included
  * (workspace, workspace_bytes and stream are not looked at), or AZG_E*. */

@@ -290,7 +290,7 @@ def test_bfloat16_gradients_of_classes_that_are_hardly_ever_taken(ops, kind, n, 
     else:
         t[:, rare] = 0.0
     g = torch.ones(n, device="cuda")
-    for kept, (dw, db) in ((True, ops.linear_cross_entropy_grad(x, w, t, b, reduction="sum")[3:]), (False, autograd(ops, x, w, t, b, reduction="sum")[2:])):
+    for kept, (dw, db) in ((kind == "index", ops.linear_cross_entropy_grad(x, w, t, b, reduction="sum")[3:]), (False, autograd(ops, x, w, t, b, reduction="sum")[2:])):
         ref = elementwise(x, w, b, t, g, kept)
         within("d_weight", dw, *ref["d_weight"])
         within("d_bias", db, *ref["d_bias"])
@@ -303,10 +303,27 @@ def test_bfloat16_rows_of_very_different_weight(ops, kind, n, h, v):
     x, w, b, t = make(n, h, v, "bf16", kind, seed=n + h + v)
     g = torch.logspace(-30, 0, n, device="cuda")
     g[::2] *= -1.0
-    ref = elementwise(x, w, b, t, g, True)
+    ref = elementwise(x, w, b, t, g, kind == "index")
     r = ops.linear_cross_entropy_grad(x, w, t, b, reduction="none", grad_loss=g)
     for name, got in (("loss", r.loss), ("d_hidden", r.d_hidden), ("d_weight", r.d_weight), ("d_bias", r.d_bias)):
         within(name, got, *ref[name])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,h,v", [(1, 24, 5003), (2, 24, 65), (2, 24, 5003), (3, 8, 20000), (40, 24, 3000)])
+@pytest.mark.parametrize("apart", [0.1, 0.01, 0.001])
+def test_probabilities_that_are_nearly_met(ops, dtype, n, h, v, apart):
+    """Target probabilities within `apart` of the softmax: the gradient at the logits is the small difference, rounded as such."""
+    x, w, b, t = make(n, h, v, dtype, "index", seed=n + h + v)
+    p = torch.softmax(x.double() @ w.double().t() + b.double(), 1)
+    t = (p * (1 + apart * torch.randn(n, v, device="cuda"))).float()
+    scale = 1024.0 if dtype == "f16" else 1.0
+    ref = elementwise(x, w, b, t, torch.full((n,), scale, device="cuda"))
+    one = ops.linear_cross_entropy_grad(x, w, t, b, reduction="sum", grad_loss=scale)
+    for dx, dw, db in (one[2:], autograd(ops, x, w, t, b, scale, reduction="sum")[1:]):
+        within("d_hidden", dx, *ref["d_hidden"])
+        within("d_weight", dw, *ref["d_weight"])
+        within("d_bias", db, *ref["d_bias"])
 
 
 # ---------------------------------------------------------------- dropout's element numbers
